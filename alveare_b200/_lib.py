@@ -75,6 +75,11 @@ SIGNATURES = {
     "alv_llama_reset": (_i, [_vp, _u32, _vp]),
     "alv_llama_info": (_i, [_vp, _u32, _vp]),
     "alv_llama_prefill": (_i, [_vp, _u32, _i, _i, _vp]),
+    "alv_qk_norm_rope": (_i, [_vp, _vp, _vp, _vp]),
+    "alv_paged_attention": (_i, [_vp, _vp, _vp, _vp]),
+    "alv_pages_update": (_i, [_vp, _vp, _vp, _i, _vp, _i, _vp, _i, _vp, _vp]),
+    "alv_pages_compact": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "alv_sample": (_i, [_vp, _vp, _vp]),
 }
 
 _lock = threading.Lock()

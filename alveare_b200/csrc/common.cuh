@@ -17,6 +17,7 @@ enum : uint32_t {
   kStatusGridTimeout = 1u << 1,   // a grid-wide barrier wait gave up
   kStatusBadLaunch   = 1u << 2,   // kernel saw an inconsistent launch shape
   kStatusPeerTimeout = 1u << 3,   // a barrier across tensor-parallel ranks gave up
+  kStatusBadIndex    = 1u << 4,   // a page, length, slot or position in device memory was out of range (skipped)
 };
 
 // One second: every spin-wait in these kernels gives up after this long.

@@ -71,6 +71,8 @@ int check_status(alv_ctx* ctx, cudaStream_t st) {
     if (t && w->world > 1) w->broken = true;
     s |= t;
   }
+  if (s == kStatusBadIndex)
+    return fail(ctx, ALV_ERR_ARG, "a page, length, slot or position in device memory was out of range (its work was skipped)");
   if (s) {
     char buf[128];
     std::snprintf(buf, sizeof(buf), "device-side wait timed out (status 0x%x)", s);

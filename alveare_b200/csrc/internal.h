@@ -1,5 +1,6 @@
 // Host-side internals shared by the translation units of the C ABI
-// (core.cu, gemv.cu, ffn.cu, stack.cu, gemm.cu, decode.cu): the context, the
+// (core.cu, gemv.cu, ffn.cu, stack.cu, gemm.cu, decode.cu, paged_*.cu,
+// pages.cu, sample.cu): the context, the
 // weight registry, status handling and launch helpers.  Not part of the ABI.
 #pragma once
 
@@ -7,6 +8,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -266,5 +268,10 @@ inline size_t stack_sync_bytes(const Weight* w) {
 }
 
 void free_weight_memory(Weight* w);
+
+// Check a paged-cache description and make the kernels' view of it (`who`
+// names the entry point in the error).  Defined in paged_rope.cu.
+struct PagedView;
+int make_paged_view(alv_ctx* ctx, const char* who, const alv_paged* p, PagedView* out);
 
 }  // namespace alv

@@ -1,0 +1,114 @@
+// Attention of new tokens over a paged cache, for row blocks of up to 16
+// query rows (a row = one query head of one new token; the heads of a kv
+// group share its keys, so they share a block).
+//
+//   o_r = sum_j p_rj v_j,   p_r = softmax_j(scale q_r . k_j)   over visible j:
+//   j <= pos_r and (no window, or j > pos_r - window, or j < sinks)
+//
+// One pass with a running maximum m and sum l (base 2, fp32):
+//   m' = max(m, max_j s_j),  l' = l 2^(m-m') + sum_j 2^(s_j-m'),
+//   O' = O 2^(m-m') + sum_j 2^(s_j-m') v_j
+// The positions are cut into slices of 16 (a slice never crosses a page: page
+// sizes are multiples of 16).  Every warp takes slices of its own, streams
+// their k and v rows through a private cp.async ring (no barrier between
+// warps in the loop) and keeps its own m, l and O in registers; the warps'
+// states are joined at the end.  The products run on mma.sync m16n8k16: the
+// work is bound by the cache's bytes, and 16 rows are all there is to a block.
+// p is rounded to bf16 for the product with v (the tensor core's operand type;
+// the result is rounded to bf16 anyway), l sums the unrounded fp32 p.
+#pragma once
+
+#include "paged.cuh"
+
+namespace alv {
+
+struct AttnArgs {
+  PagedView c;
+  const uint16_t* q;
+  int64_t q_tok, q_head;  // elements
+  uint16_t* out;
+  int64_t o_tok, o_head;
+  int nq, group;
+  int window, sinks;      // window 0: none
+  float scale_log2;       // scale * log2(e)
+};
+
+constexpr int kRowsPerBlock = 16;
+constexpr int kSlice = 16;
+constexpr int kRowWarps = 8;
+
+// Half-slices (16 rows of k or of v) in a warp's ring: 192 KB over 8 warps.
+template <int HD>
+struct RowRing {
+  static constexpr int kSlots = 192 * 1024 / kRowWarps / (kSlice * HD * 2);
+  static constexpr uint32_t kSlotBytes = kSlice * HD * 2;
+  static constexpr uint32_t kRingBytes = kRowWarps * kSlots * kSlotBytes;
+  static constexpr uint32_t kQBytes = kRowsPerBlock * HD * 2;
+  // joining the warps: m and l of every warp and row, then O
+  static constexpr uint32_t kJoinBytes = kRowWarps * kRowsPerBlock * (HD + 2) * 4;
+  static constexpr uint32_t kBytes = kQBytes + (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes);
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t src_bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+// 2^x (x <= 0 here; -inf gives 0).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf2_rn(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ bool bf2_nonfinite(uint32_t x) {
+  return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
+}
+
+// Which positions a row at position `pos` sees.
+__device__ __forceinline__ bool sees(int j, int pos, int window, int sinks) {
+  return j <= pos && (window == 0 || j > pos - window || j < sinks);
+}
+
+// The slices that any row at positions [p0, p1] sees: [0, n_sink) and
+// [first, first + n_main), with [0, n_sink) ending at or before `first`.
+struct SliceRange {
+  int n_sink, first, n_main;
+  int lo, hi;  // visible to some row: j < hi and (j >= lo or j < sinks)
+  __device__ __forceinline__ int count() const { return n_sink + n_main; }
+  __device__ __forceinline__ int slice(int i) const { return i < n_sink ? i : first + (i - n_sink); }
+};
+template <int TILE>
+__device__ __forceinline__ SliceRange slice_range(int p0, int p1, int window, int sinks) {
+  SliceRange r{0, 0, 0, 0, 0};
+  if (p1 < 0) return r;
+  r.hi = p1 + 1;
+  r.lo = window == 0 || p0 < window ? 0 : p0 - window + 1;
+  r.first = r.lo / TILE;
+  r.n_main = (p1 / TILE + 1) - r.first;
+  const int seen = sinks < r.lo ? sinks : r.lo;
+  const int ns = seen / TILE + (seen % TILE != 0);
+  r.n_sink = ns < r.first ? ns : r.first;
+  return r;
+}
+
+}  // namespace alv

@@ -1,0 +1,207 @@
+// Host side of the C ABI, part 7: per-head q/k norm, rotation and cache
+// append of a ragged batch of new tokens, in one pass over [q | k | v].
+//
+//   h  = x w / sqrt(mean(x^2) + eps)          (only where a norm weight is given)
+//   y_i        = h_i cos_i - h_{i+r/2} sin_i
+//   y_{i+r/2}  = h_{i+r/2} cos_i + h_i sin_i  (i < r/2; dims >= r pass through)
+//
+// q goes to q_out, k and v to the token's slot of the paged cache.  fp32
+// throughout, one rounding to bf16 at the stores.  Bound: HBM (each value of
+// qkv is read once and written once).
+#include "internal.h"
+#include "paged.cuh"
+
+namespace alv {
+namespace {
+
+constexpr int kRopeThreads = 256;
+
+struct RopeArgs {
+  PagedView c;
+  const void* qkv;
+  int64_t qkv_stride;      // elements per token
+  uint16_t* q_out;
+  int64_t q_tok, q_head;   // elements
+  const void* table;       // [max_pos][2 rot]: cos (rot) | sin (rot)
+  int max_pos, rot, nq, hd;
+  const float *qw, *kw;
+  float eps;
+};
+
+// Eight consecutive values as fp32.
+template <bool F32>
+__device__ __forceinline__ void load8(const void* base, int64_t at, float (&v)[8]) {
+  if (F32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+    const float4 a = p[0], b = p[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = bf16_bits_to_f32(w[i] & 0xFFFFu);
+      v[2 * i + 1] = bf16_bits_to_f32(w[i] >> 16);
+    }
+  }
+}
+
+__device__ __forceinline__ void store8(uint16_t* dst, const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack_bf2(bf16_bits_rn(v[2 * i]), bf16_bits_rn(v[2 * i + 1]));
+  *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The sequence that token t belongs to: the last b with q_start[b] <= t.
+__device__ __forceinline__ int seq_of(const PagedView& c, int t) {
+  int lo = 0, hi = c.batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (c.q_start[mid] <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// One (token, head) per group of hd / 16 lanes.  Each lane holds two groups of
+// eight values: a rotation pair's two halves, or 16 that pass through.
+template <bool F32, bool TF32>
+__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeArgs a) {
+  const PagedView& c = a.c;
+  const int heads = a.nq + 2 * c.nkv, lph = a.hd / 16;
+  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kRopeThreads + threadIdx.x) / lph;
+  const int l = threadIdx.x % lph;
+  const int t = static_cast<int>(unit / heads), head = static_cast<int>(unit % heads);
+  const bool real = t < c.tokens;
+  const bool is_q = head < a.nq, is_k = !is_q && head < a.nq + c.nkv;
+  const int pairs = a.rot / 16;
+  const bool turn = l < pairs && !(!is_q && !is_k);
+  const int d0 = l < pairs ? 8 * l : a.rot + 16 * (l - pairs);
+  const int d1 = l < pairs ? a.rot / 2 + 8 * l : d0 + 8;
+  float x0[8] = {}, x1[8] = {};
+  if (real) {
+    const int64_t at = t * a.qkv_stride + static_cast<int64_t>(head) * a.hd;
+    load8<F32>(a.qkv, at + d0, x0);
+    load8<F32>(a.qkv, at + d1, x1);
+  }
+  const float* w = is_q ? a.qw : (is_k ? a.kw : nullptr);
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss += x0[i] * x0[i] + x1[i] * x1[i];
+  for (int o = lph / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (!real) return;
+  if (w) {
+    const float inv = 1.0f / sqrtf(ss / static_cast<float>(a.hd) + a.eps);
+    float w0[8], w1[8];
+    load8<true>(w, d0, w0);
+    load8<true>(w, d1, w1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x0[i] = x0[i] * inv * w0[i];
+      x1[i] = x1[i] * inv * w1[i];
+    }
+  }
+  const int b = seq_of(c, t);
+  const SeqSpan s = seq_span(c, b);
+  const int pos = s.kv - s.qlen + (t - s.q0);
+  if (t < s.q0 || t >= s.q0 + s.qlen || pos < 0 || pos >= a.max_pos) {
+    atomicOr(c.status, kStatusBadIndex);
+    return;
+  }
+  if (turn) {
+    float cs[8], sn[8];
+    const int64_t at = static_cast<int64_t>(pos) * 2 * a.rot + d0;
+    load8<TF32>(a.table, at, cs);
+    load8<TF32>(a.table, at + a.rot, sn);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y0 = x0[i] * cs[i] - x1[i] * sn[i], y1 = x1[i] * cs[i] + x0[i] * sn[i];
+      x0[i] = y0;
+      x1[i] = y1;
+    }
+  }
+  uint16_t* dst;
+  if (is_q) {
+    dst = a.q_out + t * a.q_tok + head * a.q_head;
+  } else {
+    const int page = page_of(c, b, pos);
+    if (page < 0) return;
+    const int kvh = head - a.nq - (is_k ? 0 : c.nkv);
+    dst = (is_k ? c.k : c.v) + page * c.page_stride + kvh * c.head_stride + (pos % c.page_size) * c.row_stride;
+  }
+  store8(dst + d0, x0);
+  store8(dst + d1, x1);
+}
+
+}  // namespace
+
+int make_paged_view(alv_ctx* ctx, const char* who, const alv_paged* p, PagedView* out) {
+  const std::string w(who);
+  if (!p || p->batch < 0 || p->tokens < 0 || !p->k || !p->v || !p->table || !p->q_start || !p->kv_lens)
+    return fail(ctx, ALV_ERR_ARG, w + ": null pointer or negative size in the paged cache");
+  if (p->pages < 1 || p->kv_heads < 1 || p->page_size < 1 || p->table_width < 1 || p->table_stride < p->table_width)
+    return fail(ctx, ALV_ERR_ARG, w + ": pages, kv_heads, page_size and table_width must be positive");
+  if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+    return fail(ctx, ALV_ERR_SHAPE, w + ": head_dim must be 64, 128 or 256");
+  if (p->page_size % 16) return fail(ctx, ALV_ERR_SHAPE, w + ": page_size must be a multiple of 16");
+  if (static_cast<int64_t>(p->table_width) * p->page_size > INT_MAX)
+    return fail(ctx, ALV_ERR_UNSUPPORTED, w + ": a sequence may hold at most 2^31 - 1 positions");
+  if (p->row_stride < p->head_dim || p->head_stride < 0 || p->page_stride < 0 || p->row_stride % 8 ||
+      p->head_stride % 8 || p->page_stride % 8 || ((reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v)) & 15))
+    return fail(ctx, ALV_ERR_ARG, w + ": k, v must be 16-byte aligned with strides of whole 16 bytes");
+  int rc = ensure_scratch(ctx, 0);
+  if (rc) return rc;
+  *out = PagedView{p->k,         p->v,           p->page_stride, p->head_stride, p->row_stride, p->pages, p->page_size,
+                   p->kv_heads,  p->table,       p->table_stride, p->table_width, p->q_start,   p->kv_lens, p->batch,
+                   p->tokens,    status_ptr(ctx)};
+  return ALV_OK;
+}
+
+}  // namespace alv
+
+using namespace alv;
+
+extern "C" int alv_qk_norm_rope(alv_ctx* ctx, const alv_paged* cache, const alv_qk_norm_rope_args* args, void* stream) {
+  if (!ctx || !cache || !args) return fail(ctx, ALV_ERR_ARG, "qk_norm_rope: bad argument");
+  int rc = set_device(ctx);
+  if (rc) return rc;
+  RopeArgs a{};
+  if ((rc = make_paged_view(ctx, "qk_norm_rope", cache, &a.c))) return rc;
+  const int hd = cache->head_dim, heads = args->heads + 2 * cache->kv_heads;
+  if ((cache->tokens && (!args->qkv || !args->q_out)) || !args->rope || !valid_dtype(args->qkv_dtype) || !valid_dtype(args->rope_dtype) ||
+      args->heads < 1 || args->max_pos < 1 || !(args->eps >= 0.f))
+    return fail(ctx, ALV_ERR_ARG, "qk_norm_rope: bad argument");
+  if (args->rot < 16 || args->rot > hd || args->rot % 16)
+    return fail(ctx, ALV_ERR_SHAPE, "qk_norm_rope: the rotated dims must be a multiple of 16, at most head_dim");
+  if (args->qkv_stride < static_cast<int64_t>(heads) * hd || args->qkv_stride % 8 || args->q_token_stride % 8 ||
+      args->q_head_stride % 8 || args->q_token_stride < 0 || args->q_head_stride < 0 ||
+      ((reinterpret_cast<uintptr_t>(args->qkv) | reinterpret_cast<uintptr_t>(args->q_out) |
+        reinterpret_cast<uintptr_t>(args->rope) | reinterpret_cast<uintptr_t>(args->q_weight) |
+        reinterpret_cast<uintptr_t>(args->k_weight)) & 15))
+    return fail(ctx, ALV_ERR_ARG, "qk_norm_rope: buffers must be 16-byte aligned with strides of whole 16 bytes");
+  a.qkv = args->qkv;
+  a.qkv_stride = args->qkv_stride;
+  a.q_out = args->q_out;
+  a.q_tok = args->q_token_stride;
+  a.q_head = args->q_head_stride;
+  a.table = args->rope;
+  a.max_pos = args->max_pos;
+  a.rot = args->rot;
+  a.nq = args->heads;
+  a.hd = hd;
+  a.qw = args->q_weight;
+  a.kw = args->k_weight;
+  a.eps = args->eps;
+  const int64_t threads = static_cast<int64_t>(cache->tokens) * heads * (hd / 16);
+  const int64_t grid = (threads + kRopeThreads - 1) / kRopeThreads;
+  if (grid == 0 || cache->batch == 0) return ALV_OK;
+  if (grid > INT_MAX) return fail(ctx, ALV_ERR_UNSUPPORTED, "qk_norm_rope: too many tokens for one call");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool xf = args->qkv_dtype == ALV_F32, tf = args->rope_dtype == ALV_F32;
+  auto k = xf ? (tf ? qk_norm_rope_kernel<true, true> : qk_norm_rope_kernel<true, false>)
+              : (tf ? qk_norm_rope_kernel<false, true> : qk_norm_rope_kernel<false, false>);
+  k<<<static_cast<unsigned>(grid), kRopeThreads, 0, st>>>(a);
+  ALV_CUDA(ctx, cudaGetLastError());
+  return ALV_OK;
+}

@@ -1,0 +1,518 @@
+// Host side of the C ABI, part 9: page bookkeeping of a shared cache pool
+// (drop, fork, extend with copy-on-write, compaction) and the page copies it
+// asks for.
+//
+// One CTA does the bookkeeping: it is a few dependent passes over small
+// integer arrays, bound by latency.  It leaves a list of (from, to) pages in
+// the scratch arena; a second launch copies them, in every layer, with the
+// whole GPU (bound by HBM: each moved byte is read once and written once).
+// Counts change by integer atomics, so their order does not matter.
+#include "internal.h"
+
+namespace alv {
+namespace {
+
+constexpr int kPageThreads = 1024;
+
+struct PagesArgs {
+  int *table, *lens, *refs;
+  int64_t table_stride;
+  int pages, page_size, slots, width;
+  const int *free_ids, *fork, *extend;
+  int n_free, n_fork, n_extend;
+  int* info;
+  uint32_t* status;
+  // scratch: number of moves, moves (from, to), free page ids
+  int* n_moves;
+  int2* moves;
+  int* avail;
+  int* cow;  // [n_extend] the shared last page an extend copies, or -1
+};
+
+// Exclusive prefix sum over the CTA; `total` in every thread.
+__device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t* total, int64_t* sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) sh[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int64_t w = sh[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    sh[lane] = w;
+  }
+  __syncthreads();
+  *total = sh[31];
+  return x - v + (warp ? sh[warp - 1] : 0);
+}
+
+__device__ __forceinline__ int pages_for(int64_t len, int ps) { return static_cast<int>((len + ps - 1) / ps); }
+
+// Entries of a slot's row that may hold pages.
+__device__ __forceinline__ int row_entries(const PagesArgs& a, int slot) {
+  return min(a.width, pages_for(max(a.lens[slot], 0), a.page_size));
+}
+
+__device__ __forceinline__ bool slot_ok(const PagesArgs& a, int slot) {
+  if (slot >= 0 && slot < a.slots) return true;
+  atomicOr(a.status, kStatusBadIndex);
+  return false;
+}
+
+__device__ __forceinline__ void count(const PagesArgs& a, int page, int by) {
+  if (page >= 0 && page < a.pages) atomicAdd(a.refs + page, by);
+  else if (page >= a.pages) atomicOr(a.status, kStatusBadIndex);
+}
+
+// Whether ids[0 .. n) (stride apart) repeat a slot, by a bitmap in shared
+// memory; with `others`, also whether one of those is among them.
+__device__ bool ids_clash(const PagesArgs& a, uint32_t* bits, const int* ids, int n, int stride, const int* others) {
+  if (n < 2) return false;
+  for (int i = threadIdx.x; i < (a.slots + 31) / 32; i += blockDim.x) bits[i] = 0;
+  __syncthreads();
+  int clash = 0;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int s = ids[static_cast<int64_t>(i) * stride];
+    if (s < 0 || s >= a.slots) continue;
+    clash |= (atomicOr(bits + s / 32, 1u << (s % 32)) >> (s % 32)) & 1;
+  }
+  __syncthreads();
+  if (others)
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int s = others[static_cast<int64_t>(i) * stride];
+      if (s >= 0 && s < a.slots && s != ids[static_cast<int64_t>(i) * stride]) clash |= (bits[s / 32] >> (s % 32)) & 1;
+    }
+  return __syncthreads_or(clash);
+}
+
+// Slots free_ids[i0 .. i1): one warp per slot.
+__device__ void drop_slots(const PagesArgs& a, int i0, int i1) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  for (int i = i0 + warp; i < i1; i += nw) {
+    const int slot = a.free_ids[i];
+    if (!slot_ok(a, slot)) continue;
+    int* row = a.table + slot * a.table_stride;
+    const int n = row_entries(a, slot);
+    __syncwarp();
+    for (int e = lane; e < n; e += 32) {
+      count(a, row[e], -1);
+      row[e] = -1;
+    }
+    if (lane == 0) a.lens[slot] = 0;
+  }
+}
+
+__device__ void fork_slots(const PagesArgs& a, int i0, int i1) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  for (int i = i0 + warp; i < i1; i += nw) {
+    const int par = a.fork[2 * i], kid = a.fork[2 * i + 1];
+    if (!slot_ok(a, par) || !slot_ok(a, kid) || par == kid) continue;
+    const int* from = a.table + par * a.table_stride;
+    int* to = a.table + kid * a.table_stride;
+    const int np = row_entries(a, par), nk = row_entries(a, kid);
+    __syncwarp();
+    for (int e = lane; e < max(np, nk); e += 32) {
+      const int page = e < np ? from[e] : -1;
+      if (e < nk) count(a, to[e], -1);
+      count(a, page, 1);
+      to[e] = page;
+    }
+    if (lane == 0) a.lens[kid] = a.lens[par];
+  }
+}
+
+struct Need {
+  int slot, len, have, want, cow;  // cow: the shared, partly filled last page, or -1
+  bool ok;
+};
+__device__ __forceinline__ Need need_of(const PagesArgs& a, int i) {
+  Need n{a.extend[2 * i], 0, 0, 0, -1, false};
+  const int more = a.extend[2 * i + 1];
+  if (!slot_ok(a, n.slot) || more < 0) {
+    if (more < 0) atomicOr(a.status, kStatusBadIndex);
+    n.slot = -1;
+    n.ok = true;  // skipped: needs nothing
+    return n;
+  }
+  n.len = max(a.lens[n.slot], 0);
+  n.have = pages_for(n.len, a.page_size);
+  const int64_t want = (static_cast<int64_t>(n.len) + more + a.page_size - 1) / a.page_size;
+  n.ok = want <= a.width && static_cast<int64_t>(n.len) + more <= INT_MAX && n.have <= a.width;
+  if (!n.ok) return n;
+  n.want = static_cast<int>(want);
+  if (more > 0 && n.len % a.page_size) {
+    const int last = a.table[n.slot * a.table_stride + n.have - 1];
+    if (last >= 0 && last < a.pages && a.refs[last] > 1) n.cow = last;
+  }
+  return n;
+}
+
+// Extends i0 .. i1 (no slot twice).  Returns the index of the first that does
+// not fit, or i1.  `used` and `moves` accumulate the call's totals.
+__device__ int extend_slots(const PagesArgs& a, int i0, int i1, int64_t* used, int* moves, int64_t* sh) {
+  // pages wanted by the whole list (an entry past the table's width ends it);
+  // which last pages are shared is decided before any count changes
+  int64_t total = 0, t;
+  int stop = i1;
+  for (int base = i0; base < i1; base += blockDim.x) {
+    const int i = base + threadIdx.x;
+    int64_t want = 0;
+    int bad = INT_MAX;
+    if (i < i1) {
+      const Need n = need_of(a, i);
+      if (!n.ok) bad = i;
+      else want = n.slot < 0 ? 0 : n.want - n.have + (n.cow >= 0);
+      a.cow[i] = n.cow;
+    }
+    cta_scan(want, &t, sh);
+    total += t;
+    bad = __reduce_min_sync(0xffffffffu, bad);
+    __shared__ int first_bad;
+    if (threadIdx.x == 0) first_bad = INT_MAX;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0 && bad != INT_MAX) atomicMin(&first_bad, bad);
+    __syncthreads();
+    if (first_bad < stop) stop = first_bad;
+    __syncthreads();
+  }
+  // free pages in ascending order, as many as wanted
+  int64_t have = 0;
+  for (int base = 0; base < a.pages; base += blockDim.x) {
+    const int p = base + threadIdx.x;
+    const bool is_free = p < a.pages && a.refs[p] == 0;
+    const int64_t r = have + cta_scan(is_free ? 1 : 0, &t, sh);
+    if (is_free && r < total) a.avail[r] = p;
+    have += t;
+  }
+  __syncthreads();
+  // hand them out in list order
+  int64_t at = 0;
+  int n_moves = *moves;
+  int fail = stop;
+  for (int base = i0; base < stop; base += blockDim.x) {
+    const int i = base + threadIdx.x;
+    Need n{-1, 0, 0, 0, -1, true};
+    int64_t want = 0;
+    if (i < stop) {
+      n = need_of(a, i);
+      n.cow = a.cow[i];
+      want = n.slot < 0 ? 0 : n.want - n.have + (n.cow >= 0);
+    }
+    const int64_t first = at + cta_scan(want, &t, sh);
+    const bool fits = i < stop && first + want <= have;
+    __shared__ int first_fail;
+    __shared__ int64_t given;
+    if (threadIdx.x == 0) {
+      first_fail = INT_MAX;
+      given = at;
+    }
+    __syncthreads();
+    if (i < stop && !fits) atomicMin(&first_fail, i);
+    __syncthreads();
+    const bool apply = fits && i < first_fail && n.slot >= 0;
+    if (apply) atomicMax(reinterpret_cast<unsigned long long*>(&given), static_cast<unsigned long long>(first + want));
+    int64_t moved;
+    const int64_t mv = n_moves + cta_scan(apply && n.cow >= 0 ? 1 : 0, &moved, sh);
+    if (apply) {
+      int* row = a.table + n.slot * a.table_stride;
+      int64_t next = first;
+      if (n.cow >= 0) {
+        const int dst = a.avail[next++];
+        a.moves[mv] = make_int2(n.cow, dst);
+        atomicSub(a.refs + n.cow, 1);
+        a.refs[dst] = 1;
+        row[n.have - 1] = dst;
+      }
+      for (int e = n.have; e < n.want; ++e) {
+        const int page = a.avail[next++];
+        a.refs[page] = 1;
+        row[e] = page;
+      }
+      a.lens[n.slot] = n.len + a.extend[2 * i + 1];
+    }
+    __syncthreads();
+    n_moves += static_cast<int>(moved);
+    at = given;
+    const int ff = first_fail;
+    __syncthreads();
+    if (ff != INT_MAX) {
+      fail = ff;
+      break;
+    }
+  }
+  *moves = n_moves;
+  *used += at;
+  return fail;
+}
+
+__global__ void __launch_bounds__(kPageThreads, 1) pages_update_kernel(const PagesArgs a) {
+  extern __shared__ uint32_t bits[];
+  __shared__ int64_t sh[32];
+  pdl_trigger();
+  // A list that names a slot twice is taken one entry at a time.
+  bool one = ids_clash(a, bits, a.free_ids, a.n_free, 1, nullptr);
+  for (int i = 0; i < a.n_free; i = one ? i + 1 : a.n_free) {
+    drop_slots(a, i, one ? i + 1 : a.n_free);
+    __syncthreads();
+  }
+  one = ids_clash(a, bits, a.fork + 1, a.n_fork, 2, a.fork);
+  for (int i = 0; i < a.n_fork; i = one ? i + 1 : a.n_fork) {
+    fork_slots(a, i, one ? i + 1 : a.n_fork);
+    __syncthreads();
+  }
+  one = ids_clash(a, bits, a.extend, a.n_extend, 2, nullptr);
+  int moves = 0, done = 0;
+  int64_t used = 0;
+  while (done < a.n_extend) {
+    const int end = one ? done + 1 : a.n_extend;
+    done = extend_slots(a, done, end, &used, &moves, sh);
+    __syncthreads();
+    if (done < end) break;
+  }
+  if (threadIdx.x == 0) {
+    *a.n_moves = moves;
+    if (a.info) {
+      a.info[1] = static_cast<int>(used);
+      a.info[2] = moves;
+      a.info[3] = done < a.n_extend ? done : -1;
+    }
+  }
+  if (a.info) {  // a page whose last holder copied it counts as free
+    int64_t n = 0, t;
+    for (int p = threadIdx.x; p < a.pages; p += blockDim.x) n += a.refs[p] == 0;
+    cta_scan(n, &t, sh);
+    if (threadIdx.x == 0) a.info[0] = static_cast<int>(t);
+  }
+}
+
+struct CompactArgs {
+  const int *refs;
+  int* refs_out;
+  int pages;
+  int* info;
+  int* n_moves;
+  int2* moves;
+  int* to;      // [pages] new id of every page
+  int* holes;   // [pages]
+};
+
+__global__ void __launch_bounds__(kPageThreads, 1) pages_compact_kernel(const CompactArgs a) {
+  __shared__ int64_t sh[32];
+  pdl_trigger();
+  int64_t t, n = 0;
+  for (int p = threadIdx.x; p < a.pages; p += blockDim.x) n += a.refs[p] > 0;
+  cta_scan(n, &t, sh);
+  const int live = static_cast<int>(t);
+  int64_t nh = 0, nm = 0;
+  for (int base = 0; base < a.pages; base += blockDim.x) {
+    const int p = base + threadIdx.x;
+    const bool used = p < a.pages && a.refs[p] > 0;
+    const bool hole = p < live && !used, mover = p >= live && used;
+    // holes in the low, movers in the high half of the sum
+    const int64_t r = cta_scan((hole ? 1 : 0) + (static_cast<int64_t>(mover) << 32), &t, sh);
+    if (hole) a.holes[nh + (r & 0xFFFFFFFF)] = p;
+    if (mover) a.moves[nm + (r >> 32)].x = p;
+    if (p < a.pages) a.to[p] = p;
+    nh += t & 0xFFFFFFFF;
+    nm += t >> 32;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nm; i += blockDim.x) {
+    const int src = a.moves[i].x, dst = a.holes[i];
+    a.moves[i].y = dst;
+    a.to[src] = dst;
+  }
+  __syncthreads();
+  for (int p = threadIdx.x; p < live; p += blockDim.x)
+    if (a.refs[p] > 0) a.refs_out[p] = a.refs[p];
+  __syncthreads();
+  for (int i = threadIdx.x; i < nm; i += blockDim.x) a.refs_out[a.moves[i].y] = a.refs[a.moves[i].x];
+  __syncthreads();
+  for (int p = live + threadIdx.x; p < a.pages; p += blockDim.x) a.refs_out[p] = 0;
+  if (threadIdx.x == 0) {
+    *a.n_moves = static_cast<int>(nm);
+    if (a.info) {
+      a.info[0] = live;
+      a.info[1] = static_cast<int>(nm);
+    }
+  }
+}
+
+struct CopyArgs {
+  uint8_t *k, *v;
+  int64_t layer_stride, page_stride, page_bytes;
+  int layers;
+  const int* n_moves;
+  const int2* moves;
+  // compaction also renumbers the table
+  const int* table;
+  int* table_out;
+  int64_t table_stride;
+  int slots, width, pages;
+  const int* to;
+  uint32_t* status;
+};
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyVec = 8;  // 16-byte loads in flight per thread
+
+__global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const CopyArgs a) {
+  pdl_wait();
+  const int n = *a.n_moves;
+  if (a.table_out) {
+    const int64_t entries = static_cast<int64_t>(a.slots) * a.width;
+    for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < entries;
+         e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+      int page = a.table[e / a.width * a.table_stride + e % a.width];
+      if (page >= a.pages) atomicOr(a.status, kStatusBadIndex);
+      else if (page >= 0) page = a.to[page];
+      a.table_out[e] = page;
+    }
+  }
+  // work unit: kCopyThreads * kCopyVec * 16 bytes of one page of one layer's k or v
+  constexpr int64_t kUnit = kCopyThreads * kCopyVec * 16;
+  const int64_t per_page = (a.page_bytes + kUnit - 1) / kUnit;
+  const int64_t units = n * per_page * a.layers * 2;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t part = u % per_page, blk = u / per_page;
+    const int kv = static_cast<int>(blk & 1);
+    const int64_t ml = blk >> 1;
+    const int layer = static_cast<int>(ml % a.layers);
+    const int2 mv = a.moves[ml / a.layers];
+    uint8_t* base = (kv ? a.v : a.k) + layer * a.layer_stride;
+    const uint4* src = reinterpret_cast<const uint4*>(base + mv.x * a.page_stride);
+    uint4* dst = reinterpret_cast<uint4*>(base + mv.y * a.page_stride);
+    const int64_t n16 = a.page_bytes / 16, i0 = part * (kUnit / 16) + threadIdx.x;
+    uint4 r[kCopyVec];
+#pragma unroll
+    for (int i = 0; i < kCopyVec; ++i)
+      if (i0 + i * kCopyThreads < n16) r[i] = __ldcs(src + i0 + i * kCopyThreads);
+#pragma unroll
+    for (int i = 0; i < kCopyVec; ++i)
+      if (i0 + i * kCopyThreads < n16) __stcs(dst + i0 + i * kCopyThreads, r[i]);
+  }
+}
+
+int check_pages(alv_ctx* ctx, const char* who, const alv_pages* p) {
+  const std::string w(who);
+  if (!p->k || !p->v || !p->table || !p->refs)
+    return fail(ctx, ALV_ERR_ARG, w + ": null pointer in the page pool");
+  if (p->layers < 1 || p->pages < 1 || p->page_size < 1 || p->slots < 1 || p->table_width < 1 ||
+      p->table_stride < p->table_width || p->page_bytes < 16)
+    return fail(ctx, ALV_ERR_ARG, w + ": every size of the page pool must be positive");
+  if (p->page_bytes % 16 || p->page_stride % 16 || p->layer_stride % 16 || p->page_stride < p->page_bytes ||
+      p->layer_stride < 0 || ((reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v)) & 15))
+    return fail(ctx, ALV_ERR_ARG, w + ": pages must be 16-byte aligned blocks of whole 16 bytes");
+  if (p->slots > 1 << 20) return fail(ctx, ALV_ERR_UNSUPPORTED, w + ": at most 1,048,576 slots");
+  return ALV_OK;
+}
+
+CopyArgs copy_args(alv_ctx* ctx, const alv_pages* p) {
+  CopyArgs c{};
+  c.k = static_cast<uint8_t*>(p->k);
+  c.v = static_cast<uint8_t*>(p->v);
+  c.layer_stride = p->layer_stride;
+  c.page_stride = p->page_stride;
+  c.page_bytes = p->page_bytes;
+  c.layers = p->layers;
+  c.pages = p->pages;
+  c.status = status_ptr(ctx);
+  return c;
+}
+
+int launch_copy(alv_ctx* ctx, const CopyArgs& c, cudaStream_t st) {
+  return launch_ex(ctx, pages_copy_kernel, dim3(ctx->num_sms * 4), dim3(kCopyThreads), 0, st, true, c);
+}
+
+}  // namespace
+}  // namespace alv
+
+using namespace alv;
+
+extern "C" int alv_pages_update(alv_ctx* ctx, const alv_pages* p, const int32_t* free, int n_free, const int32_t* fork,
+                                int n_fork, const int32_t* extend, int n_extend, int32_t* info, void* stream) {
+  if (!ctx || !p) return fail(ctx, ALV_ERR_ARG, "pages_update: bad argument");
+  int rc = check_pages(ctx, "pages_update", p);
+  if (rc) return rc;
+  if (n_free < 0 || n_fork < 0 || n_extend < 0 || !p->lens || (n_free && !free) || (n_fork && !fork) || (n_extend && !extend))
+    return fail(ctx, ALV_ERR_ARG, "pages_update: a list is missing");
+  if ((rc = set_device(ctx))) return rc;
+  const size_t o_moves = 256, o_cow = o_moves + align_up(static_cast<size_t>(n_extend) * 8, 256),
+               o_avail = o_cow + align_up(static_cast<size_t>(n_extend) * 4, 256);
+  if ((rc = ensure_scratch(ctx, o_avail + static_cast<size_t>(p->pages) * 4))) return rc;
+  uint8_t* ws = work_ptr(ctx);
+  PagesArgs a{};
+  a.table = p->table;
+  a.lens = p->lens;
+  a.refs = p->refs;
+  a.table_stride = p->table_stride;
+  a.pages = p->pages;
+  a.page_size = p->page_size;
+  a.slots = p->slots;
+  a.width = p->table_width;
+  a.free_ids = free;
+  a.n_free = n_free;
+  a.fork = fork;
+  a.n_fork = n_fork;
+  a.extend = extend;
+  a.n_extend = n_extend;
+  a.info = info;
+  a.status = status_ptr(ctx);
+  a.n_moves = reinterpret_cast<int*>(ws);
+  a.moves = reinterpret_cast<int2*>(ws + o_moves);
+  a.cow = reinterpret_cast<int*>(ws + o_cow);
+  a.avail = reinterpret_cast<int*>(ws + o_avail);
+  const size_t smem = static_cast<size_t>((p->slots + 31) / 32) * 4;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = prepare_kernel(ctx, pages_update_kernel, smem))) return rc;
+  if ((rc = launch_ex(ctx, pages_update_kernel, dim3(1), dim3(kPageThreads), smem, st, false, a))) return rc;
+  if (n_extend == 0) return ALV_OK;
+  CopyArgs c = copy_args(ctx, p);
+  c.n_moves = a.n_moves;
+  c.moves = a.moves;
+  return launch_copy(ctx, c, st);
+}
+
+extern "C" int alv_pages_compact(alv_ctx* ctx, const alv_pages* p, int32_t* table_out, int32_t* refs_out, int32_t* info,
+                                 void* stream) {
+  if (!ctx || !p || !table_out || !refs_out) return fail(ctx, ALV_ERR_ARG, "pages_compact: bad argument");
+  int rc = check_pages(ctx, "pages_compact", p);
+  if (rc) return rc;
+  if (table_out == p->table && p->table_stride != p->table_width)
+    return fail(ctx, ALV_ERR_ARG, "pages_compact: a table renumbered in place must be contiguous");
+  if ((rc = set_device(ctx))) return rc;
+  const size_t np = static_cast<size_t>(p->pages), o_moves = 256, o_to = o_moves + align_up(np * 8, 256),
+               o_holes = o_to + align_up(np * 4, 256);
+  if ((rc = ensure_scratch(ctx, o_holes + np * 4))) return rc;
+  uint8_t* ws = work_ptr(ctx);
+  CompactArgs a{};
+  a.refs = p->refs;
+  a.refs_out = refs_out;
+  a.pages = p->pages;
+  a.info = info;
+  a.n_moves = reinterpret_cast<int*>(ws);
+  a.moves = reinterpret_cast<int2*>(ws + o_moves);
+  a.to = reinterpret_cast<int*>(ws + o_to);
+  a.holes = reinterpret_cast<int*>(ws + o_holes);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = launch_ex(ctx, pages_compact_kernel, dim3(1), dim3(kPageThreads), 0, st, false, a))) return rc;
+  CopyArgs c = copy_args(ctx, p);
+  c.n_moves = a.n_moves;
+  c.moves = a.moves;
+  c.table = p->table;
+  c.table_out = table_out;
+  c.table_stride = p->table_stride;
+  c.slots = p->slots;
+  c.width = p->table_width;
+  c.to = a.to;
+  return launch_copy(ctx, c, st);
+}

@@ -311,6 +311,133 @@ int alv_llama_reset(alv_ctx* ctx, alv_handle model, void* stream);
  * in the reference. */
 int alv_llama_info(alv_ctx* ctx, alv_handle model, int64_t* info);
 
+/* ---- paged serving --------------------------------------------------------
+ * Many sequences over one pool of cache pages: per-head q/k norm + rotation +
+ * cache append, attention of a ragged batch of new tokens, page bookkeeping
+ * and token sampling.  The reference serves one sequence from a contiguous
+ * cache (runtime/cpp/src/model.cpp:315-370: QK-norm, RoPE, KV write, sliding
+ * and global attention on the host; runtime/py/sampler.py:3-50: sampling).
+ * Lengths, page tables and reference counts are device memory, read when the
+ * kernel runs: no call reads them on the host, and a captured call may be
+ * replayed while they change.  An index found out of range there is skipped,
+ * never followed, and makes the next alv_sync_status report ALV_ERR_ARG. */
+
+/* One layer's cache and a ragged batch of new tokens.  k and v hold bf16 pages
+ * reached by strides in elements (row_stride: between positions of a page);
+ * sequence b's position j is row j % page_size of page table[b * table_stride
+ * + j / page_size].  Its new tokens are rows q_start[b] .. q_start[b + 1] - 1
+ * of the call's token tensors and the last positions of kv_lens[b] (which
+ * counts them).  head_dim 64, 128 or 256; page_size a multiple of 16; k, v
+ * 16-byte aligned and strides multiples of 8 elements. */
+typedef struct {
+  uint16_t *k, *v;
+  int64_t page_stride, head_stride, row_stride;
+  int32_t pages, kv_heads, page_size, head_dim;
+  const int32_t* table;   /* (batch, table_width) */
+  int64_t table_stride;
+  const int32_t* q_start; /* batch + 1 */
+  const int32_t* kv_lens; /* batch */
+  int32_t table_width, batch, tokens, reserved;
+} alv_paged;
+
+/* q, k = rotate(rmsnorm(.) * weight) per head, then q -> q_out, and k, v ->
+ * the tokens' cache slots, in one pass over qkv = [q | k | v] (tokens rows of
+ * (heads + 2 kv_heads) * head_dim, ALV_F32 or ALV_BF16).  q_weight / k_weight
+ * (head_dim fp32; NULL: no norm); rope: (max_pos, 2 * rot) rows of cos (rot) |
+ * sin (rot), ALV_F32 or ALV_BF16 (the first rot / 2 of each are read); dims
+ * past rot pass through unrotated.  fp32 arithmetic, one rounding to bf16. */
+typedef struct {
+  const void* qkv;
+  int64_t qkv_stride;
+  uint16_t* q_out;
+  int64_t q_token_stride, q_head_stride;
+  const void* rope;
+  const float *q_weight, *k_weight;
+  int32_t qkv_dtype, rope_dtype, heads, rot, max_pos;
+  float eps;
+} alv_qk_norm_rope_args;
+int alv_qk_norm_rope(alv_ctx* ctx, const alv_paged* cache, const alv_qk_norm_rope_args* args, void* stream);
+
+/* out = softmax(scale q k^T) v for every new token and head: the token at
+ * position p sees positions j <= p that also have j > p - window (window 0:
+ * all) or j < sinks.  heads a multiple of kv_heads (consecutive heads share a
+ * kv head).  A token that sees nothing gives zeros; what a token does not see
+ * never reaches its output, whatever it holds.  q, out bf16 (tokens, heads,
+ * head_dim) by strides; max_q_len: no sequence has more new tokens (rows past
+ * it are not computed). */
+typedef struct {
+  const uint16_t* q;
+  int64_t q_token_stride, q_head_stride;
+  uint16_t* out;
+  int64_t out_token_stride, out_head_stride;
+  int32_t heads, max_q_len, window, sinks;
+  float scale;
+  int32_t reserved;
+} alv_attention_args;
+int alv_paged_attention(alv_ctx* ctx, const alv_paged* cache, const alv_attention_args* args, void* stream);
+
+/* The pool's pages over all layers and its bookkeeping, all device memory:
+ * k, v: layers x pages blocks of page_bytes contiguous bytes (a multiple of
+ * 16) at byte strides; table (slots, table_width) page ids, -1 where a slot
+ * has none; lens (slots): positions held; refs (pages): table entries naming
+ * the page. */
+typedef struct {
+  void *k, *v;
+  int64_t layer_stride, page_stride, page_bytes; /* bytes */
+  int32_t *table, *lens, *refs;
+  int64_t table_stride;
+  int32_t layers, pages, page_size, slots, table_width, reserved;
+} alv_pages;
+
+/* One scheduler turn, in this order: drop the slots in `free` (n_free ids);
+ * make slot fork[i][1] a copy of fork[i][0] that shares its pages (n_fork
+ * pairs; what the child held is dropped); give slot extend[i][0] room for
+ * extend[i][1] more positions (n_extend pairs).  A partly filled last page
+ * that others share is first copied to a page of the slot's own, in every
+ * layer.  New pages are the free ones of lowest id, in list order.  The first
+ * extend that does not fit (no free page, or past table_width) and all after
+ * it change nothing.  Lists are device int32; info (4 int32 or NULL) receives
+ * free pages left, pages handed out, pages copied, and the index of the first
+ * extend that did not fit or -1. */
+int alv_pages_update(alv_ctx* ctx, const alv_pages* p, const int32_t* free, int n_free, const int32_t* fork, int n_fork,
+                     const int32_t* extend, int n_extend, int32_t* info, void* stream);
+
+/* Move the n pages in use to ids 0 .. n - 1: the i-th page in use past them
+ * goes to the i-th free id below n.  Writes the renumbered table (contiguous
+ * (slots, table_width)) and counts to table_out and refs_out, which may be
+ * p->table (then table_stride must be table_width) and p->refs; lens is not
+ * used.
+ * Pages that move keep their old copy.  info as 2 int32 or NULL: pages in use,
+ * pages moved. */
+int alv_pages_compact(alv_ctx* ctx, const alv_pages* p, int32_t* table_out, int32_t* refs_out, int32_t* info,
+                      void* stream);
+
+/* One token per row of logits (rows, vocab; ALV_F32 or ALV_BF16) from given
+ * uniform numbers u in [0, 1):
+ *   s = logits / temperature;  w = exp(s - max s) in steps of 2^-40
+ *   keep the top_k largest (ties: lowest index first; <= 0 or >= vocab: all),
+ *   of these the shortest prefix that holds top_p of their mass (>= 1: all),
+ *   and of these the tokens with w >= min_p;
+ *   token = the first, in index order, whose running mass passes u * total.
+ * Masses are summed as integers, so the result does not depend on any order.
+ * Per-row parameters are device arrays where the pointer is given, else the
+ * scalar applies to all.  temperature 0: the largest logit (lowest index).
+ * NaN counts as -inf.  A row with nothing above -inf gives token -1.  logprobs
+ * (fp32, may be NULL): log of the token's share of the kept mass. */
+typedef struct {
+  const void* logits;
+  int64_t logits_stride; /* elements per row */
+  const float* u;
+  int32_t* tokens;
+  float* logprobs;
+  const float *temperature_rows, *top_p_rows, *min_p_rows;
+  const int32_t* top_k_rows;
+  int32_t logits_dtype, rows, vocab, top_k;
+  float temperature, top_p, min_p;
+  int32_t reserved;
+} alv_sample_args;
+int alv_sample(alv_ctx* ctx, const alv_sample_args* args, void* stream);
+
 /* Allocation-free gemv: same arithmetic and arguments as alv_gemv, for
  * callers that must not allocate device memory while they run (a decode
  * loop with a fixed GPU memory budget, a host runtime that owns the device
