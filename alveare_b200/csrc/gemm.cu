@@ -5,16 +5,8 @@
 #include "gemm_tc.cuh"
 #include "launch.h"
 
-using namespace alv;
-
-namespace {
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 // The driver's tensor-map encoder, looked up once through the runtime.
-int tensor_map_encoder(alv_ctx* ctx, EncodeTiledFn* out) {
+int alv::tensor_map_encoder(alv_ctx* ctx, EncodeTiledFn* out) {
   static std::mutex mu;
   static EncodeTiledFn fn = nullptr;
   std::lock_guard<std::mutex> lock(mu);
@@ -23,12 +15,16 @@ int tensor_map_encoder(alv_ctx* ctx, EncodeTiledFn* out) {
     cudaDriverEntryPointQueryResult q;
     ALV_CUDA(ctx, cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q));
     if (q != cudaDriverEntryPointSuccess || !f)
-      return fail(ctx, ALV_ERR_CUDA, "gemm: cuTensorMapEncodeTiled is not available");
+      return fail(ctx, ALV_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     fn = reinterpret_cast<EncodeTiledFn>(f);
   }
   *out = fn;
   return ALV_OK;
 }
+
+using namespace alv;
+
+namespace {
 
 template <int NT, bool FAST>
 int launch_gemm_t(alv_ctx* ctx, const GemmParams& p, const CUtensorMap& map, cudaStream_t st) {

@@ -24,7 +24,14 @@
 
 #include "stream.cuh"
 
+struct alv_ctx;
+
 namespace alv {
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int tensor_map_encoder(alv_ctx* ctx, EncodeTiledFn* out);  // defined in gemm.cu
 
 constexpr int kTcM = 128;        // weight rows per tile: 8 unit rows of 16
 constexpr int kTcStages = 4;

@@ -22,8 +22,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) paged_rows_kernel(const Att
   const int kvh = blockIdx.y, b = blockIdx.z;
   const SeqSpan s = seq_span(a.c, b);
   const int r0 = blockIdx.x * kRowsPerBlock;
-  const int nrow = min(kRowsPerBlock, s.qlen * a.group - r0);
-  if (nrow <= 0) return;
+  const int64_t rows = static_cast<int64_t>(s.qlen) * a.group;
+  const int nrow = static_cast<int>(min(static_cast<int64_t>(kRowsPerBlock), rows - r0));
+  if (nrow <= 0 || rows > a.row_max) return;
   const int pfirst = s.kv - s.qlen;  // position of the sequence's first new token
   const int p0 = pfirst + r0 / a.group, p1 = pfirst + (r0 + nrow - 1) / a.group;
   const SliceRange sr = slice_range<kSlice>(p0, p1, a.window, a.sinks);
@@ -221,7 +222,7 @@ int launch_rows(alv_ctx* ctx, const AttnArgs& a, int max_q_len, cudaStream_t st)
   const size_t smem = RowRing<HD>::kBytes;
   int rc = prepare_kernel(ctx, k, smem);
   if (rc) return rc;
-  const int64_t rows = static_cast<int64_t>(max_q_len) * a.group;
+  const int64_t rows = std::min<int64_t>(static_cast<int64_t>(max_q_len) * a.group, a.row_max);
   const dim3 grid(static_cast<unsigned>((rows + kRowsPerBlock - 1) / kRowsPerBlock), a.c.nkv, a.c.batch);
   k<<<grid, kRowWarps * 32, smem, st>>>(a);
   ALV_CUDA(ctx, cudaGetLastError());
@@ -262,6 +263,15 @@ extern "C" int alv_paged_attention(alv_ctx* ctx, const alv_paged* cache, const a
   a.sinks = args->sinks;
   a.scale_log2 = static_cast<float>(static_cast<double>(args->scale) * 1.4426950408889634);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Sequences of more than 16 rows go to the tensor-core form; a batch may hold
+  // both kinds (the lengths are on the device).
+  a.row_max = INT_MAX;
+  if (static_cast<int64_t>(args->max_q_len) * a.group > kRowsPerBlock && chunk_takes(a)) {
+    a.row_max = kRowsPerBlock;
+    if ((rc = launch_chunk(ctx, a, cache->head_dim, kRowsPerBlock + 1, st))) return rc;
+    // all sequences as long as the longest: none is left for the row blocks
+    if (static_cast<int64_t>(cache->batch) * args->max_q_len == cache->tokens) return ALV_OK;
+  }
   switch (cache->head_dim) {
     case 64: return launch_rows<64>(ctx, a, args->max_q_len, st);
     case 128: return launch_rows<128>(ctx, a, args->max_q_len, st);

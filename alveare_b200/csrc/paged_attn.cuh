@@ -18,6 +18,7 @@
 // the result is rounded to bf16 anyway), l sums the unrounded fp32 p.
 #pragma once
 
+#include "internal.h"
 #include "paged.cuh"
 
 namespace alv {
@@ -31,7 +32,13 @@ struct AttnArgs {
   int nq, group;
   int window, sinks;      // window 0: none
   float scale_log2;       // scale * log2(e)
+  int row_max;            // row-block kernel: sequences with more rows are not its
 };
+
+// The tensor-core form for chunks (paged_chunk.cu): sequences with at least
+// row_min rows (new tokens x heads of a kv group).
+bool chunk_takes(const AttnArgs& a);
+int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int row_min, cudaStream_t st);
 
 constexpr int kRowsPerBlock = 16;
 constexpr int kSlice = 16;

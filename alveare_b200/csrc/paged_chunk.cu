@@ -1,0 +1,772 @@
+// Attention of chunks of new tokens over a paged cache on the tensor cores
+// (tcgen05, TMEM).  Same mathematics as paged_attn.cuh, tiles of 128 query
+// rows (tokens x the heads of a kv group) against tiles of BN positions:
+//
+//   S = Q K^T          tcgen05.mma, Q and K tiles in shared memory, S in TMEM
+//   P = 2^(S c - m)    softmax warps: one thread per row, TMEM -> registers;
+//                      P goes back to TMEM as bf16 over S's own columns
+//   O += P V           tcgen05.mma with P from TMEM, O stays in TMEM
+//
+// Head sizes 64 and 128: two query tiles per CTA (TMEM: 2 x (S 128 + O HD)
+// columns), each with its own softmax warpgroup, so the tensor cores work for
+// one tile while the other's softmax runs.  Head size 256: O alone takes 256
+// columns, so one query tile with two S buffers of 64 positions.
+//
+// The running maximum only moves when a row's new maximum exceeds the one in
+// use by 2^8 (p stays below 2^8 then, exact in fp32 sums and in range of
+// bf16), so O is rescaled in TMEM on the first few tiles and hardly ever
+// after; rows take p = 2^(s - m) of whatever m they use, and l sums the same.
+//
+// Work: a unit is one BN-position tile of one item (sequence, kv head, query
+// tiles).  The units of all items, in order, are cut into equal runs, one per
+// CTA, so that a short chunk over a long past fills the GPU and ragged batches
+// balance; an item cut between CTAs leaves unnormalised parts (O, m, l) that a
+// second launch joins in a fixed order.
+#include <cuda.h>
+
+#include "gemm_tc.cuh"
+#include "internal.h"
+#include "paged_attn.cuh"
+
+namespace alv {
+namespace {
+
+constexpr int kChunkRows = 128;
+constexpr int kMinUnits = 4;  // units of a CTA's run at least: a part costs about as much as two tiles
+
+template <int HD>
+struct Chunk {
+  static constexpr int kNQ = HD == 256 ? 1 : 2;    // query tiles per item
+  static constexpr int kBN = HD == 256 ? 64 : 128; // positions per tile
+  static constexpr int kSB = HD == 256 ? 2 : 1;    // S buffers per query tile
+  static constexpr int kStages = HD == 64 ? 3 : 2; // K and V stages each
+  static constexpr uint32_t kQTile = kChunkRows * HD * 2;
+  static constexpr uint32_t kKV = kBN * HD * 2;
+  static constexpr uint32_t kBytes = kNQ * kQTile + 2 * kStages * kKV + 1024;
+  static constexpr int kSoftWarps = 4 * kNQ;
+  static constexpr int kThreads = (kSoftWarps + 2) * 32;
+  static constexpr uint32_t kSCol = 0;      // S (and P) of tile q, buffer b: (q + b) * kBN
+  static constexpr uint32_t kOCol = 256;    // O of tile q: 256 + q * HD
+};
+
+struct ChunkArgs {
+  AttnArgs a;
+  int tpt;        // tokens per query tile: 128 / group
+  int box;        // positions per tensor copy
+  int head_first; // cache tensor map order: (hd, head, row, page) instead of (hd, row, head, page)
+  int row_min;    // sequences with at least this many rows are this kernel's
+  float* parts;   // [2 * grid][kNQ * 128][HD + 2]
+  int4* cuts;     // [grid]: item (b, kvh, pair), units before the cut (x = -1: none)
+  int64_t* total; // [1] units of all items
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Shared-memory descriptor of an operand whose M/N index is contiguous
+// (128-byte swizzle): 64 values per 128-byte row, rows along K; `chunk` bytes
+// from one 64-value column to the next, 1024 bytes from 8 rows to the next 8.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr, uint32_t chunk) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(chunk >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+#define ALV_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define ALV_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// 32 consecutive columns of this thread's TMEM lane (complete after tmem_wait_ld).
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : ALV_R8(r, 0), ALV_R8(r, 8), ALV_R8(r, 16), ALV_R8(r, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::ALV_I8(r, 0),
+      ALV_I8(r, 8), ALV_I8(r, 16), ALV_I8(r, 24), "r"(addr)
+      : "memory");
+}
+#undef ALV_R8
+#undef ALV_I8
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One run of units: items (b, kvh, pair) in order, pair fastest.
+template <int HD>
+struct Walk {
+  using C = Chunk<HD>;
+  int b, kvh, pair, pairs;
+  SeqSpan s;
+  SliceRange r;      // tiles of the current item
+  int p0, p1;        // positions of the item's first and last new token
+
+  __device__ __forceinline__ int pairs_of(const ChunkArgs& c, const SeqSpan& q) const {
+    if (q.qlen <= 0 || static_cast<int64_t>(q.qlen) * c.a.group < c.row_min) return 0;
+    return (q.qlen + C::kNQ * c.tpt - 1) / (C::kNQ * c.tpt);
+  }
+  __device__ __forceinline__ SliceRange range_of(const ChunkArgs& c, const SeqSpan& q, int pr, int* lo, int* hi) const {
+    const int first = q.kv - q.qlen + pr * C::kNQ * c.tpt;
+    const int last = min(first + C::kNQ * c.tpt, q.kv) - 1;
+    *lo = first;
+    *hi = last;
+    SliceRange x = slice_range<C::kBN>(first, last, c.a.window, c.a.sinks);
+    // an item that sees nothing still has one (masked) tile: it writes zeros
+    if (x.count() == 0) x.n_main = 1;
+    return x;
+  }
+  // Units of one kv head of sequence q.
+  __device__ __forceinline__ int64_t units_of(const ChunkArgs& c, const SeqSpan& q) const {
+    const int n = pairs_of(c, q);
+    int64_t u = 0;
+    int lo, hi;
+    for (int i = 0; i < n; ++i) u += range_of(c, q, i, &lo, &hi).count();
+    return u;
+  }
+  __device__ __forceinline__ void load(const ChunkArgs& c) { r = range_of(c, s, pair, &p0, &p1); }
+  __device__ __forceinline__ void next(const ChunkArgs& c) {
+    if (++pair == pairs) {
+      pair = 0;
+      if (++kvh == c.a.c.nkv) {
+        kvh = 0;
+        do {
+          if (++b >= c.a.c.batch) return;
+          s = seq_span(c.a.c, b);
+          pairs = pairs_of(c, s);
+        } while (pairs == 0);
+      }
+    }
+    load(c);
+  }
+};
+
+template <int HD>
+struct ChunkShared {
+  using C = Chunk<HD>;
+  uint64_t kfull[C::kStages], kempty[C::kStages], vfull[C::kStages], vempty[C::kStages];
+  uint64_t qfull, qempty, sfull[C::kNQ][C::kSB], pfull[C::kNQ][C::kSB], odone[C::kNQ], pvdone;
+  uint32_t tmem;
+  volatile uint32_t failed;
+  // redo[i & 1] = i + 1: item i of the run has masked values that are not
+  // finite (see slow_row; a warpgroup is at most one item ahead of the other)
+  volatile uint32_t redo[2];
+  // the CTA's run
+  int64_t sums[C::kThreads / 32 + 1];
+  int64_t u0, u1, total;
+  int start_b;
+  int64_t start_before;  // units before start_b
+};
+
+// One row from the cache, one warp, plain arithmetic: for the rare item in
+// which a v value that some row must not see is not finite (the tensor cores
+// would multiply it by that row's p = 0).
+template <int HD>
+__device__ __noinline__ void slow_row(const ChunkArgs& c, int b, int kvh, int pos, const SliceRange& r, int t0, int t1,
+                                      const uint16_t* q, float (&o)[HD / 32], float* m_out, float* l_out) {
+  const int lane = threadIdx.x & 31;
+  float qv[HD / 32];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) {
+    qv[i] = bf16_bits_to_f32(q[lane + 32 * i]);
+    o[i] = 0.f;
+  }
+  for (int t = t0; t < t1; ++t) {
+    const int j0 = r.slice(t) * Chunk<HD>::kBN;
+    for (int j = j0; j < j0 + Chunk<HD>::kBN; ++j) {
+      if (!sees(j, pos, c.a.window, c.a.sinks)) continue;
+      const int page = page_of(c.a.c, b, j);
+      if (page < 0) continue;
+      const int64_t at = page * c.a.c.page_stride + kvh * c.a.c.head_stride + (j % c.a.c.page_size) * c.a.c.row_stride;
+      float dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) dot += qv[i] * bf16_bits_to_f32(c.a.c.k[at + lane + 32 * i]);
+#pragma unroll
+      for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
+      const float sc = dot * c.a.scale_log2, mn = fmaxf(m, sc);
+      const float base = mn == -INFINITY ? 0.f : mn;
+      const float f = exp2_fast(m - base), p = exp2_fast(sc - base);
+      l = l * f + p;
+      m = mn;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) o[i] = o[i] * f + p * bf16_bits_to_f32(c.a.c.v[at + lane + 32 * i]);
+    }
+  }
+  *m_out = m;
+  *l_out = l;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
+    paged_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap, const ChunkArgs c) {
+  using C = Chunk<HD>;
+  constexpr int NQ = C::kNQ, BN = C::kBN, ST = C::kStages;
+  extern __shared__ uint8_t smem_dyn[];
+  __shared__ ChunkShared<HD> sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+  const uint32_t q_sm = base, k_sm = base + NQ * C::kQTile, v_sm = k_sm + ST * C::kKV;
+  pdl_trigger();
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&sh.kfull[i], 1);
+      mbar_init(&sh.kempty[i], 1);
+      mbar_init(&sh.vfull[i], 1);
+      mbar_init(&sh.vempty[i], 1);
+    }
+    mbar_init(&sh.qfull, 1);
+    mbar_init(&sh.qempty, 1);
+    for (int q = 0; q < NQ; ++q) {
+      for (int i = 0; i < C::kSB; ++i) {
+        mbar_init(&sh.sfull[q][i], 1);
+        // per S buffer: with two, a warp may be a tile ahead of its fellows
+        mbar_init(&sh.pfull[q][i], 4);
+      }
+      mbar_init(&sh.odone[q], 1);
+    }
+    mbar_init(&sh.pvdone, 1);
+    fence_mbar_init();
+    sh.failed = 0;
+    sh.redo[0] = sh.redo[1] = 0;
+  }
+  // query rows past tpt * group are never loaded: keep them zero
+  for (uint32_t i = threadIdx.x; i < NQ * C::kQTile / 16; i += C::kThreads)
+    *reinterpret_cast<uint4*>(smem_dyn + (base - smem_u32(smem_dyn)) + i * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+
+  // ---- the CTA's run of units: thread t sums the sequences of its range, a
+  // scan over the threads finds where the run starts
+  Walk<HD> w{};
+  const int per = (c.a.c.batch + C::kThreads - 1) / C::kThreads;
+  const int b0 = threadIdx.x * per, b1 = min(b0 + per, c.a.c.batch);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += w.units_of(c, seq_span(c.a.c, b)) * c.a.c.nkv;
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) sh.sums[warp] = incl;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int64_t t = 0;
+    for (int i = 0; i < C::kThreads / 32; ++i) {
+      const int64_t x = sh.sums[i];
+      sh.sums[i] = t;
+      t += x;
+    }
+    int64_t g = (t + kMinUnits - 1) / kMinUnits;  // CTAs that get work
+    if (g > gridDim.x) g = gridDim.x;
+    sh.total = t;
+    sh.u0 = blockIdx.x < g ? t * blockIdx.x / g : t;
+    sh.u1 = blockIdx.x < g ? t * (blockIdx.x + 1) / g : t;
+    if (blockIdx.x == 0) *c.total = t;
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  __syncthreads();
+  const int64_t u0 = sh.u0, u1 = sh.u1;
+  const int64_t before = sh.sums[warp] + incl - mine;
+  if (u0 < u1 && before <= u0 && u0 < before + mine) {  // this thread's range holds the start
+    int64_t at = before;
+    for (int b = b0; b < b1; ++b) {
+      const int64_t u = w.units_of(c, seq_span(c.a.c, b)) * c.a.c.nkv;
+      if (u0 < at + u) {
+        sh.start_b = b;
+        sh.start_before = at;
+        break;
+      }
+      at += u;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  int first_tile = 0;
+  if (u0 < u1) {  // locate the start inside its sequence
+    w.b = sh.start_b;
+    w.s = seq_span(c.a.c, w.b);
+    w.pairs = w.pairs_of(c, w.s);
+    const int64_t per_head = w.units_of(c, w.s), off = u0 - sh.start_before;
+    w.kvh = static_cast<int>(off / per_head);
+    int64_t rem = off - w.kvh * per_head;
+    w.pair = 0;
+    w.load(c);
+    while (rem >= w.r.count()) {
+      rem -= w.r.count();
+      ++w.pair;
+      w.load(c);
+    }
+    first_tile = static_cast<int>(rem);
+  }
+  if (threadIdx.x == 0)
+    c.cuts[blockIdx.x] = first_tile > 0 ? make_int4(w.b, w.kvh, w.pair, first_tile) : make_int4(-1, 0, 0, 0);
+
+  auto fail_now = [&] {
+    atomicOr(c.a.c.status, kStatusMbarTimeout);
+    sh.failed = 1;
+  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    if (mbar_wait_bounded_s(smem_u32(bar), parity)) return true;
+    fail_now();
+    return false;
+  };
+
+  if (warp == C::kSoftWarps) {
+    // ---- copies: lane i fetches box i of a tile's k and v
+    const int boxes = BN / c.box;
+    uint32_t it = 0, item = 0;
+    int64_t u = u0;
+    int t = first_tile;
+    bool ok = true;
+    while (ok && u < u1) {
+      const int n = static_cast<int>(min(static_cast<int64_t>(w.r.count() - t), u1 - u));
+      const int tok = w.pair * NQ * c.tpt;
+      if (item > 0) ok = __all_sync(0xffffffffu, wait(&sh.qempty, (item - 1) & 1));
+      if (!ok) break;
+      const int nq = NQ == 2 && tok + c.tpt < w.s.qlen ? 2 : 1;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&sh.qfull, nq * c.tpt * c.a.group * HD * 2);
+        for (int q = 0; q < nq; ++q)
+          for (int d = 0; d < HD / 64; ++d)
+            tma_load_3d(q_sm + q * C::kQTile + d * (kChunkRows * 128), &qmap, d * 64, w.kvh * c.a.group,
+                        w.s.q0 + tok + q * c.tpt, smem_u32(&sh.qfull));
+      }
+      for (int i = 0; i < n && ok && !sh.failed; ++i, ++it) {
+        const int j = w.r.slice(t + i) * BN + lane * c.box;
+        // boxes that no row sees are not fetched (their pages may be gone)
+        const bool live = lane < boxes && j < w.r.hi && (j + c.box > w.r.lo || j < c.a.sinks);
+        int page = c.a.c.pages;  // past the end: the copy reads zeros
+        if (live) {
+          const int p = page_of(c.a.c, w.b, j);
+          if (p >= 0) page = p;
+        }
+        const uint32_t n_live = __popc(__ballot_sync(0xffffffffu, live));
+        const int row = j % c.a.c.page_size;
+        const uint32_t stage = it % ST, ph = (it / ST) & 1;
+        for (int kv = 0; kv < 2; ++kv) {
+          uint64_t* full = kv ? &sh.vfull[stage] : &sh.kfull[stage];
+          uint64_t* empty = kv ? &sh.vempty[stage] : &sh.kempty[stage];
+          if (it >= ST) ok = __all_sync(0xffffffffu, wait(empty, ph ^ 1));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(full, n_live * c.box * HD * 2);
+          __syncwarp();
+          if (live) {
+            const uint32_t dst = (kv ? v_sm : k_sm) + stage * C::kKV + lane * c.box * 128;
+            const CUtensorMap* map = kv ? &vmap : &kmap;
+            for (int d = 0; d < HD / 64; ++d) {
+              if (c.head_first) tma_load_4d(dst + d * (BN * 128), map, d * 64, w.kvh, row, page, smem_u32(full));
+              else tma_load_4d(dst + d * (BN * 128), map, d * 64, row, w.kvh, page, smem_u32(full));
+            }
+          }
+          __syncwarp();
+        }
+      }
+      u += n;
+      t = 0;
+      ++item;
+      if (u < u1) w.next(c);
+    }
+    // every armed stage lands before the CTA may exit
+    for (uint32_t k = it > ST ? it - ST : 0; k < it; ++k) {
+      mbar_wait_bounded_s(smem_u32(&sh.kfull[k % ST]), (k / ST) & 1);
+      mbar_wait_bounded_s(smem_u32(&sh.vfull[k % ST]), (k / ST) & 1);
+    }
+    if (item > 0) mbar_wait_bounded_s(smem_u32(&sh.qfull), (item - 1) & 1);
+  } else if (warp == C::kSoftWarps + 1) {
+    // ---- tensor-core issue (one thread)
+    if (lane == 0) {
+      const uint32_t s_idesc = umma_idesc_bf16_f32(kChunkRows, BN);
+      const uint32_t o_idesc = umma_idesc_bf16_f32(kChunkRows, HD) | (1u << 16);  // B's N index contiguous
+      uint32_t it = 0, item = 0, pph[NQ][C::kSB] = {};
+      int64_t u = u0;
+      int t = first_tile;
+      bool ok = true;
+      auto qk = [&](int q, int buf, uint32_t k) {
+        const uint32_t ks = k_sm + (k % ST) * C::kKV, qs = q_sm + q * C::kQTile;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d)
+          umma_bf16(tmem + C::kSCol + (q + buf) * BN, umma_desc_sw128(qs + (d / 4) * (kChunkRows * 128)) + 2 * (d % 4),
+                    umma_desc_sw128(ks + (d / 4) * (BN * 128)) + 2 * (d % 4), s_idesc, d != 0);
+        umma_commit(smem_u32(&sh.sfull[q][buf]));
+      };
+      auto pv = [&](int q, int buf, uint32_t k, bool acc) {
+        const uint32_t vs = v_sm + (k % ST) * C::kKV;
+#pragma unroll
+        for (int j = 0; j < BN / 16; ++j)
+          umma_bf16_ts(tmem + C::kOCol + q * HD, tmem + C::kSCol + (q + buf) * BN + 8 * j,
+                       umma_desc_mn_sw128(vs + j * 2048, BN * 128), o_idesc, acc || j != 0);
+      };
+      while (ok && u < u1 && !sh.failed) {
+        const int n = static_cast<int>(min(static_cast<int64_t>(w.r.count() - t), u1 - u));
+        const int nq = NQ == 2 && w.pair * NQ * c.tpt + c.tpt < w.s.qlen ? 2 : 1;
+        ok = wait(&sh.qfull, item & 1) && wait(&sh.kfull[it % ST], (it / ST) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        for (int q = 0; q < nq; ++q) qk(q, 0, it);
+        umma_commit(smem_u32(&sh.kempty[it % ST]));
+        if (n == 1) umma_commit(smem_u32(&sh.qempty));
+        for (int i = 0; i < n && ok; ++i) {
+          const uint32_t k = it + i;
+          const bool more = i + 1 < n;
+          if (NQ == 1 && more) {  // the next scores before this tile's P V
+            if (!(ok = wait(&sh.kfull[(k + 1) % ST], ((k + 1) / ST) & 1))) break;
+            tc_fence_after();
+            qk(0, (i + 1) & 1, k + 1);
+            umma_commit(smem_u32(&sh.kempty[(k + 1) % ST]));
+            if (i + 2 == n) umma_commit(smem_u32(&sh.qempty));
+          }
+          for (int q = 0; q < nq && ok; ++q) {
+            const int buf = C::kSB == 2 ? i & 1 : 0;
+            ok = wait(&sh.pfull[q][buf], pph[q][buf] & 1) && (q > 0 || wait(&sh.vfull[k % ST], (k / ST) & 1));
+            if (!ok) break;
+            ++pph[q][buf];
+            tc_fence_after();
+            pv(q, buf, k, i > 0);
+            if (NQ == 1) umma_commit(smem_u32(&sh.pvdone));
+            if (q == nq - 1) umma_commit(smem_u32(&sh.vempty[k % ST]));
+            if (!more) umma_commit(smem_u32(&sh.odone[q]));
+            if (NQ == 2 && more) {
+              if (q == 0 && !(ok = wait(&sh.kfull[(k + 1) % ST], ((k + 1) / ST) & 1))) break;
+              tc_fence_after();
+              qk(q, 0, k + 1);
+              if (q == nq - 1) {
+                umma_commit(smem_u32(&sh.kempty[(k + 1) % ST]));
+                if (i + 2 == n) umma_commit(smem_u32(&sh.qempty));
+              }
+            }
+          }
+        }
+        it += n;
+        u += n;
+        t = 0;
+        ++item;
+        if (u < u1) w.next(c);
+      }
+    }
+  } else {
+    // ---- softmax: thread = row of query tile q
+    const int q = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lane_addr = tmem + (((warp & 3) * 32) << 16);
+    const uint32_t o_addr = lane_addr + C::kOCol + q * HD;
+    const float scale = c.a.scale_log2;
+    uint32_t sph = 0, oph = 0, it = 0, item = 0;  // S tiles seen, items stored, tiles and items of the run
+    int64_t u = u0;
+    int t = first_tile;
+    bool ok = true;
+    while (ok && u < u1 && !sh.failed) {
+      const int n = static_cast<int>(min(static_cast<int64_t>(w.r.count() - t), u1 - u));
+      const int tok0 = (w.pair * NQ + q) * c.tpt, tok = tok0 + row / c.a.group;
+      const bool active = q == 0 || tok0 < w.s.qlen;
+      const bool real = row < c.tpt * c.a.group && tok < w.s.qlen;
+      const int pfirst = w.s.kv - w.s.qlen;
+      const int pos = real ? pfirst + tok : -1;
+      const int pmin = pfirst + tok0, pmax = min(pmin + c.tpt, w.s.kv) - 1;
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; active && i < n; ++i) {
+        const int j0 = w.r.slice(t + i) * BN;
+        const uint32_t buf = C::kSB == 2 ? (i & 1) : 0, k = it + i;
+        if (!(ok = __all_sync(0xffffffffu, wait(&sh.sfull[q][buf], C::kSB == 2 ? (sph >> buf) & 1 : sph & 1)))) break;
+        if (C::kSB == 2) sph ^= 1u << buf;
+        else ++sph;
+        tc_fence_after();
+        // values of v that no row may see: zero the rows no one sees, and look
+        // for values that are not finite where only some rows see them
+        const bool whole_item = j0 + BN - 1 <= w.p0 && (c.a.window == 0 || j0 > w.p1 - c.a.window || j0 + BN <= c.a.sinks);
+        if (q == 0 && !whole_item) {
+          if (!(ok = __all_sync(0xffffffffu, wait(&sh.vfull[k % ST], (k / ST) & 1)))) break;
+          const uint32_t vs = v_sm + (k % ST) * C::kKV;
+          bool odd = false;
+          for (int e = row; e < BN * (HD / 8); e += kChunkRows) {
+            const int r = e % BN, ch = e / BN, j = j0 + r;
+            const uint32_t at = vs + (ch / 8) * (BN * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4);
+            if (j >= w.r.hi || (j < w.r.lo && j >= c.a.sinks)) {
+              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0) : "memory");
+            } else {
+              const uint4 x = lds128_at<0>(at);
+              odd |= bf2_nonfinite(x.x) | bf2_nonfinite(x.y) | bf2_nonfinite(x.z) | bf2_nonfinite(x.w);
+            }
+          }
+          if (odd) sh.redo[item & 1] = item + 1;
+          fence_proxy_async_smem();
+        }
+        uint32_t s[BN];
+#pragma unroll
+        for (int e = 0; e < BN / 32; ++e) tmem_ld32(lane_addr + C::kSCol + (q + buf) * BN + 32 * e, s + 32 * e);
+        tmem_wait_ld();
+        const bool whole = j0 + BN - 1 <= pmin && (c.a.window == 0 || j0 > pmax - c.a.window || j0 + BN <= c.a.sinks);
+        if (!whole) {
+          const int hi = pos - j0, lo = c.a.window ? pos - c.a.window - j0 : -BN - 1, sk = c.a.window ? c.a.sinks - j0 : 0;
+#pragma unroll
+          for (int e = 0; e < BN; ++e)
+            if (!(e <= hi && (e > lo || e < sk))) s[e] = 0xFF800000u;  // -inf
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < BN; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+        const bool move = mt > m + 8.f;  // also from -inf
+        if (__any_sync(0xffffffffu, move)) {
+          const float f = move ? (m == -INFINITY ? 0.f : exp2_fast(m - mt)) : 1.f;
+          if (move) m = mt;
+          l *= f;
+          if (i > 0) {
+            if (NQ == 1) {  // O must hold the last product (with two tiles S's arrival says so)
+              if (!(ok = __all_sync(0xffffffffu, wait(&sh.pvdone, (it + i - 1) & 1)))) break;
+              tc_fence_after();
+            }
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) {
+              uint32_t o[32];
+              tmem_ld32(o_addr + 32 * e, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st32(o_addr + 32 * e, o);
+            }
+          }
+        }
+        const float sub = m == -INFINITY ? 0.f : m;
+        float sum[4] = {};
+#pragma unroll
+        for (int e = 0; e < BN; e += 2) {
+          const float p0 = exp2_fast(fmaf(__uint_as_float(s[e]), scale, -sub));
+          const float p1 = exp2_fast(fmaf(__uint_as_float(s[e + 1]), scale, -sub));
+          sum[e & 2] += p0;
+          sum[(e & 2) + 1] += p1;
+          s[e / 2] = pack_bf2_rn(p0, p1);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int e = 0; e < BN / 64; ++e) tmem_st32(lane_addr + C::kSCol + (q + buf) * BN + 32 * e, s + 32 * e);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.pfull[q][buf]);
+      }
+      if (!ok) break;
+      // ---- the item's rows (or this CTA's part of them)
+      if (active) {
+        if (!(ok = __all_sync(0xffffffffu, wait(&sh.odone[q], oph & 1)))) break;
+        ++oph;
+        tc_fence_after();
+        const bool part = t > 0 || n < w.r.count();
+        const int head = w.kvh * c.a.group + row % c.a.group;
+        uint16_t* dst = c.a.out + static_cast<int64_t>(w.s.q0 + tok) * c.a.o_tok + head * c.a.o_head;
+        float* pd = c.parts + ((static_cast<int64_t>(blockIdx.x) * 2 + (t > 0 ? 0 : 1)) * NQ * kChunkRows + q * kChunkRows +
+                               row) * (HD + 2);
+        if (sh.redo[item & 1] == item + 1) {
+          for (int rr = 0; rr < 32; ++rr) {
+            const int p = __shfl_sync(0xffffffffu, pos, rr);
+            if (!__shfl_sync(0xffffffffu, static_cast<int>(real), rr)) continue;
+            const int tk = __shfl_sync(0xffffffffu, tok, rr), hd_ = __shfl_sync(0xffffffffu, head, rr);
+            float o[HD / 32], sm, sl;
+            slow_row<HD>(c, w.b, w.kvh, p, w.r, t, t + n,
+                         c.a.q + static_cast<int64_t>(w.s.q0 + tk) * c.a.q_tok + hd_ * c.a.q_head, o, &sm, &sl);
+            uint16_t* d = c.a.out + static_cast<int64_t>(w.s.q0 + tk) * c.a.o_tok + hd_ * c.a.o_head;
+            float* ps = pd + (rr - lane) * (HD + 2);
+            const float inv = sm == -INFINITY ? 0.f : 1.f / sl;
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) {
+              if (part) ps[2 + lane + 32 * e] = o[e];
+              else d[lane + 32 * e] = bf16_bits_rn(o[e] * inv);
+            }
+            if (part && lane == 0) ps[0] = sm, ps[1] = sl;
+          }
+        } else {
+          const float inv = m == -INFINITY ? 0.f : 1.f / l;  // a row that sees nothing gives zeros
+          if (part && real) pd[0] = m, pd[1] = l;
+#pragma unroll 1
+          for (int e = 0; e < HD / 32; ++e) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + 32 * e, o);
+            tmem_wait_ld();
+            if (real && part) {
+#pragma unroll
+              for (int x = 0; x < 32; x += 2)
+                *reinterpret_cast<float2*>(pd + 2 + 32 * e + x) = make_float2(__uint_as_float(o[x]), __uint_as_float(o[x + 1]));
+            } else if (real) {
+#pragma unroll
+              for (int x = 0; x < 32; x += 8) {
+                uint32_t p[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                  p[y] = pack_bf2_rn(__uint_as_float(o[x + 2 * y]) * inv, __uint_as_float(o[x + 2 * y + 1]) * inv);
+                *reinterpret_cast<uint4*>(dst + 32 * e + x) = make_uint4(p[0], p[1], p[2], p[3]);
+              }
+            }
+            __syncwarp();
+          }
+        }
+        tc_fence_before();
+      }
+      it += n;
+      u += n;
+      t = 0;
+      ++item;
+      if (u < u1) w.next(c);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// Join the parts of items cut between CTAs: block (c, y) joins rows 32 y ..
+// 32 y + 31 of the item that cut c is the first inside, a warp per row.
+template <int HD>
+__global__ void __launch_bounds__(256) paged_join_kernel(const ChunkArgs c, int grid) {
+  using C = Chunk<HD>;
+  pdl_wait();
+  const int cut = blockIdx.x + 1;
+  const int4 it = c.cuts[cut];
+  if (it.x < 0) return;
+  const int64_t total = *c.total;
+  int64_t g = (total + kMinUnits - 1) / kMinUnits;
+  if (g > grid) g = grid;
+  if (cut >= g) return;
+  const int64_t at = total * cut / g, g0 = at - it.w;  // the item's first unit
+  if (total * (cut - 1) / g > g0) return;              // an earlier cut is inside the item
+  Walk<HD> w{};
+  w.b = it.x;
+  w.kvh = it.y;
+  w.pair = it.z;
+  w.s = seq_span(c.a.c, w.b);
+  w.load(c);
+  const int64_t g1 = g0 + w.r.count();
+  const int lane = threadIdx.x & 31;
+  for (int r = blockIdx.y * 32 + (threadIdx.x >> 5); r < min(C::kNQ * kChunkRows, static_cast<int>(blockIdx.y) * 32 + 32); r += 8) {
+    const int q = r / kChunkRows, row = r % kChunkRows;
+    const int tok = (w.pair * C::kNQ + q) * c.tpt + row / c.a.group;
+    if (row >= c.tpt * c.a.group || tok >= w.s.qlen) continue;
+    auto part = [&](int cta) {  // the CTA's part: its last run's (slot 1) where the item starts, else its first
+      return c.parts + ((static_cast<int64_t>(cta) * 2 + (cta < cut ? 1 : 0)) * C::kNQ * kChunkRows + r) * (HD + 2);
+    };
+    float m = -INFINITY, l = 0.f, o[HD / 32] = {};
+    for (int cta = cut - 1; cta < g && total * cta / g < g1; ++cta) {
+      const float* p = part(cta);
+      const float pm = p[0], mn = fmaxf(m, pm), base = mn == -INFINITY ? 0.f : mn;
+      const float f0 = exp2_fast(m - base), f1 = exp2_fast(pm - base);
+      l = l * f0 + p[1] * f1;
+#pragma unroll
+      for (int e = 0; e < HD / 32; ++e) o[e] = o[e] * f0 + p[2 + lane + 32 * e] * f1;
+      m = mn;
+    }
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    const int head = w.kvh * c.a.group + row % c.a.group;
+    uint16_t* dst = c.a.out + static_cast<int64_t>(w.s.q0 + tok) * c.a.o_tok + head * c.a.o_head;
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) dst[lane + 32 * e] = bf16_bits_rn(o[e] * inv);
+  }
+}
+
+int encode(alv_ctx* ctx, CUtensorMap* map, uint32_t rank, const void* p, const cuuint64_t* dims, const cuuint64_t* strides,
+           const cuuint32_t* box) {
+  EncodeTiledFn enc = nullptr;
+  int rc = tensor_map_encoder(ctx, &enc);
+  if (rc) return rc;
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  const CUresult cr = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(p), dims, strides, box, one,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (cr != CUDA_SUCCESS)
+    return fail(ctx, ALV_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed (" + std::to_string(cr) + ")");
+  return ALV_OK;
+}
+
+template <int HD>
+int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int row_min, cudaStream_t st) {
+  using C = Chunk<HD>;
+  ChunkArgs c{};
+  c.a = a;
+  c.tpt = kChunkRows / a.group;
+  c.row_min = row_min;
+  c.box = 16;
+  while (c.box < C::kBN && a.c.page_size % (2 * c.box) == 0) c.box *= 2;
+  c.head_first = a.c.head_stride < a.c.row_stride;
+  CUtensorMap qmap, kmap, vmap;
+  {
+    const cuuint64_t dims[3] = {HD, static_cast<cuuint64_t>(a.nq), static_cast<cuuint64_t>(a.c.tokens)};
+    const cuuint64_t str[2] = {static_cast<cuuint64_t>(a.q_head) * 2, static_cast<cuuint64_t>(a.q_tok) * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(c.tpt)};
+    const int rc = encode(ctx, &qmap, 3, a.q, dims, str, box);
+    if (rc) return rc;
+  }
+  for (int kv = 0; kv < 2; ++kv) {
+    const cuuint64_t rows = a.c.page_size, heads = a.c.nkv, rs = a.c.row_stride * 2, hs = a.c.head_stride * 2,
+                     ps = a.c.page_stride * 2;
+    const cuuint32_t bx = static_cast<cuuint32_t>(c.box);
+    const cuuint64_t dims[4] = {HD, c.head_first ? heads : rows, c.head_first ? rows : heads,
+                                static_cast<cuuint64_t>(a.c.pages)};
+    const cuuint64_t str[3] = {c.head_first ? hs : rs, c.head_first ? rs : hs, ps};
+    const cuuint32_t box[4] = {64, c.head_first ? 1 : bx, c.head_first ? bx : 1, 1};
+    const int rc = encode(ctx, kv ? &vmap : &kmap, 4, kv ? a.c.v : a.c.k, dims, str, box);
+    if (rc) return rc;
+  }
+  const int grid = ctx->num_sms;
+  const size_t o_cuts = 256, o_parts = o_cuts + align_up(static_cast<size_t>(grid) * sizeof(int4), 256);
+  int rc = ensure_scratch(ctx, o_parts + static_cast<size_t>(grid) * 2 * C::kNQ * kChunkRows * (HD + 2) * 4);
+  if (rc) return rc;
+  c.total = reinterpret_cast<int64_t*>(work_ptr(ctx));
+  c.cuts = reinterpret_cast<int4*>(work_ptr(ctx) + o_cuts);
+  c.parts = reinterpret_cast<float*>(work_ptr(ctx) + o_parts);
+  c.a.c.status = status_ptr(ctx);
+  auto k = paged_chunk_kernel<HD>;
+  if ((rc = prepare_kernel(ctx, k, C::kBytes))) return rc;
+  if ((rc = launch_ex(ctx, k, dim3(grid), dim3(C::kThreads), C::kBytes, st, false, qmap, kmap, vmap, c))) return rc;
+  if (grid < 2) return ALV_OK;
+  return launch_ex(ctx, paged_join_kernel<HD>, dim3(grid - 1, C::kNQ * kChunkRows / 32), dim3(256), 0, st, true, c, grid);
+}
+
+}  // namespace
+
+// The tensor-core form takes whole kv groups as rows of one tile, a positive
+// scale (masked scores are -inf before the scale), and strides a tensor map
+// can hold; anything else runs on the row-block kernel.
+bool chunk_takes(const AttnArgs& a) {
+  constexpr int64_t kMaxStride = int64_t{1} << 39;  // elements: a tensor map's strides are below 2^40 bytes
+  return a.group <= kChunkRows && a.scale_log2 > 0.f && a.q_head > 0 && a.q_tok > 0 && a.c.head_stride > 0 &&
+         a.c.page_stride > 0 && a.q_tok < kMaxStride && a.c.page_stride < kMaxStride && a.c.head_stride < kMaxStride &&
+         a.c.row_stride < kMaxStride;
+}
+
+int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int row_min, cudaStream_t st) {
+  switch (hd) {
+    case 64: return launch_chunk_t<64>(ctx, a, row_min, st);
+    case 128: return launch_chunk_t<128>(ctx, a, row_min, st);
+    default: return launch_chunk_t<256>(ctx, a, row_min, st);
+  }
+}
+
+}  // namespace alv
