@@ -107,10 +107,57 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
       ALV_I8(r, 8), ALV_I8(r, 16), ALV_I8(r, 24), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::ALV_I8(r, 0),
+      ALV_I8(r, 8), "r"(addr)
+      : "memory");
+}
 #undef ALV_R8
 #undef ALV_I8
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two fp32 values in a register pair.
+__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ float lo_f2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float hi_f2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Scores of 32 columns that the row does not see -> -inf.
+__device__ __forceinline__ void mask32(uint32_t (&s)[32], int hi, int lo, int sinks) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    if (!(e <= hi && (e > lo || e < sinks))) s[e] = 0xFF800000u;
+}
+// p = 2^(s scale - m) of 32 scores, added to the sums, as 16 packed bf16 pairs in s[0 .. 16).
+__device__ __forceinline__ void probs32(uint32_t (&s)[32], uint64_t scale2, uint64_t sub2, uint64_t (&sum)[2]) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) {
+    const uint64_t x = fma_f2(pack_f2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, sub2);
+    const float p0 = exp2_fast(lo_f2(x)), p1 = exp2_fast(hi_f2(x));
+    sum[e / 2 & 1] = add_f2(sum[e / 2 & 1], pack_f2(p0, p1));
+    s[e / 2] = pack_bf2_rn(p0, p1);
+  }
+}
 
 // One run of units: items (b, kvh, pair) in order, pair fastest.
 template <int HD>
@@ -167,9 +214,10 @@ struct ChunkShared {
   uint64_t qfull, qempty, sfull[C::kNQ][C::kSB], pfull[C::kNQ][C::kSB], odone[C::kNQ], pvdone;
   uint32_t tmem;
   volatile uint32_t failed;
-  // redo[i & 1] = i + 1: item i of the run has masked values that are not
-  // finite (see slow_row; a warpgroup is at most one item ahead of the other)
-  volatile uint32_t redo[2];
+  // odd[i & 1] = i + 1: item i of the run has v values that are not finite in
+  // a tile that only some rows see whole (a warpgroup with work in an item is
+  // at most one item ahead of the other)
+  volatile uint32_t odd[2];
   // the CTA's run
   int64_t sums[C::kThreads / 32 + 1];
   int64_t u0, u1, total;
@@ -177,43 +225,31 @@ struct ChunkShared {
   int64_t start_before;  // units before start_b
 };
 
-// One row from the cache, one warp, plain arithmetic: for the rare item in
-// which a v value that some row must not see is not finite (the tensor cores
-// would multiply it by that row's p = 0).
+// Whether every row of the item sees the whole tile of positions j0 ...
 template <int HD>
-__device__ __noinline__ void slow_row(const ChunkArgs& c, int b, int kvh, int pos, const SliceRange& r, int t0, int t1,
-                                      const uint16_t* q, float (&o)[HD / 32], float* m_out, float* l_out) {
-  const int lane = threadIdx.x & 31;
-  float qv[HD / 32];
-  float m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < HD / 32; ++i) {
-    qv[i] = bf16_bits_to_f32(q[lane + 32 * i]);
-    o[i] = 0.f;
-  }
+__device__ __forceinline__ bool sees_all(const AttnArgs& a, const Walk<HD>& w, int j0) {
+  constexpr int BN = Chunk<HD>::kBN;
+  return j0 + BN - 1 <= w.p0 && (a.window == 0 || j0 > w.p1 - a.window || j0 + BN <= a.sinks);
+}
+
+// Add to 32 of a row's sums the values that are not finite and were left out
+// of its products: those it sees in tiles that not every row sees whole.
+template <int HD>
+__device__ __forceinline__ void add_odd(const ChunkArgs& c, const Walk<HD>& w, int t0, int t1, int pos, int d0, uint32_t (&o)[32]) {
   for (int t = t0; t < t1; ++t) {
-    const int j0 = r.slice(t) * Chunk<HD>::kBN;
+    const int j0 = w.r.slice(t) * Chunk<HD>::kBN;
+    if (sees_all(c.a, w, j0)) continue;
     for (int j = j0; j < j0 + Chunk<HD>::kBN; ++j) {
       if (!sees(j, pos, c.a.window, c.a.sinks)) continue;
-      const int page = page_of(c.a.c, b, j);
+      const int page = page_of(c.a.c, w.b, j);
       if (page < 0) continue;
-      const int64_t at = page * c.a.c.page_stride + kvh * c.a.c.head_stride + (j % c.a.c.page_size) * c.a.c.row_stride;
-      float dot = 0.f;
+      const uint16_t* v = c.a.c.v + page * c.a.c.page_stride + w.kvh * c.a.c.head_stride +
+                          (j % c.a.c.page_size) * c.a.c.row_stride + d0;
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) dot += qv[i] * bf16_bits_to_f32(c.a.c.k[at + lane + 32 * i]);
-#pragma unroll
-      for (int k = 16; k > 0; k >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
-      const float sc = dot * c.a.scale_log2, mn = fmaxf(m, sc);
-      const float base = mn == -INFINITY ? 0.f : mn;
-      const float f = exp2_fast(m - base), p = exp2_fast(sc - base);
-      l = l * f + p;
-      m = mn;
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i) o[i] = o[i] * f + p * bf16_bits_to_f32(c.a.c.v[at + lane + 32 * i]);
+      for (int x = 0; x < 32; ++x)
+        if ((v[x] & 0x7F80u) == 0x7F80u) o[x] = __float_as_uint(__uint_as_float(o[x]) + bf16_bits_to_f32(v[x]));
     }
   }
-  *m_out = m;
-  *l_out = l;
 }
 
 template <int HD>
@@ -249,7 +285,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     mbar_init(&sh.pvdone, 1);
     fence_mbar_init();
     sh.failed = 0;
-    sh.redo[0] = sh.redo[1] = 0;
+    sh.odd[0] = sh.odd[1] = 0;
   }
   // query rows past tpt * group are never loaded: keep them zero
   for (uint32_t i = threadIdx.x; i < NQ * C::kQTile / 16; i += C::kThreads)
@@ -498,40 +534,56 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         if (C::kSB == 2) sph ^= 1u << buf;
         else ++sph;
         tc_fence_after();
-        // values of v that no row may see: zero the rows no one sees, and look
-        // for values that are not finite where only some rows see them
-        const bool whole_item = j0 + BN - 1 <= w.p0 && (c.a.window == 0 || j0 > w.p1 - c.a.window || j0 + BN <= c.a.sinks);
-        if (q == 0 && !whole_item) {
+        // A row's p is 0 where it does not see, but 0 * inf is not: zero the v
+        // rows no one sees and the values that are not finite (the rows that
+        // see those take them in the end).
+        if (q == 0 && !sees_all(c.a, w, j0)) {
           if (!(ok = __all_sync(0xffffffffu, wait(&sh.vfull[k % ST], (k / ST) & 1)))) break;
           const uint32_t vs = v_sm + (k % ST) * C::kKV;
           bool odd = false;
           for (int e = row; e < BN * (HD / 8); e += kChunkRows) {
             const int r = e % BN, ch = e / BN, j = j0 + r;
             const uint32_t at = vs + (ch / 8) * (BN * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4);
-            if (j >= w.r.hi || (j < w.r.lo && j >= c.a.sinks)) {
-              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0) : "memory");
-            } else {
-              const uint4 x = lds128_at<0>(at);
-              odd |= bf2_nonfinite(x.x) | bf2_nonfinite(x.y) | bf2_nonfinite(x.z) | bf2_nonfinite(x.w);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (j < w.r.hi && (j >= w.r.lo || j < c.a.sinks)) {
+              x = lds128_at<0>(at);
+              uint32_t* const xs[4] = {&x.x, &x.y, &x.z, &x.w};
+              bool here = false;
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                if ((*xs[y] & 0x7F80u) == 0x7F80u) *xs[y] &= 0xFFFF0000u, here = true;
+                if ((*xs[y] & 0x7F800000u) == 0x7F800000u) *xs[y] &= 0xFFFFu, here = true;
+              }
+              if (!here) continue;
+              odd = true;
             }
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
           }
-          if (odd) sh.redo[item & 1] = item + 1;
+          if (odd) sh.odd[item & 1] = item + 1;
           fence_proxy_async_smem();
         }
-        uint32_t s[BN];
-#pragma unroll
-        for (int e = 0; e < BN / 32; ++e) tmem_ld32(lane_addr + C::kSCol + (q + buf) * BN + 32 * e, s + 32 * e);
-        tmem_wait_ld();
+        // The scores, 32 at a time: the upper half first, so that the lower half
+        // is still in registers when its p (which overwrite it) are due.
+        const uint32_t s_addr = lane_addr + C::kSCol + (q + buf) * BN;
         const bool whole = j0 + BN - 1 <= pmin && (c.a.window == 0 || j0 > pmax - c.a.window || j0 + BN <= c.a.sinks);
-        if (!whole) {
-          const int hi = pos - j0, lo = c.a.window ? pos - c.a.window - j0 : -BN - 1, sk = c.a.window ? c.a.sinks - j0 : 0;
-#pragma unroll
-          for (int e = 0; e < BN; ++e)
-            if (!(e <= hi && (e > lo || e < sk))) s[e] = 0xFF800000u;  // -inf
-        }
+        const int hi = pos - j0, lo = c.a.window ? pos - c.a.window - j0 : -BN - 1, sk = c.a.window ? c.a.sinks - j0 : 0;
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t sa[32], sb[32];
 #pragma unroll
-        for (int e = 0; e < BN; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
+        for (int half = BN / 64 - 1; half >= 0; --half) {
+          tmem_ld32(s_addr + 64 * half, sa);
+          tmem_ld32(s_addr + 64 * half + 32, sb);
+          tmem_wait_ld();
+          if (!whole) {
+            mask32(sa, hi - 64 * half, lo - 64 * half, sk - 64 * half);
+            mask32(sb, hi - 64 * half - 32, lo - 64 * half - 32, sk - 64 * half - 32);
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            mx[e / 2 & 1] = max3(mx[e / 2 & 1], __uint_as_float(sa[e]), __uint_as_float(sa[e + 1]));
+            mx[2 + (e / 2 & 1)] = max3(mx[2 + (e / 2 & 1)], __uint_as_float(sb[e]), __uint_as_float(sb[e + 1]));
+          }
+        }
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
         const bool move = mt > m + 8.f;  // also from -inf
         if (__any_sync(0xffffffffu, move)) {
@@ -555,18 +607,27 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
           }
         }
         const float sub = m == -INFINITY ? 0.f : m;
-        float sum[4] = {};
-#pragma unroll
-        for (int e = 0; e < BN; e += 2) {
-          const float p0 = exp2_fast(fmaf(__uint_as_float(s[e]), scale, -sub));
-          const float p1 = exp2_fast(fmaf(__uint_as_float(s[e + 1]), scale, -sub));
-          sum[e & 2] += p0;
-          sum[(e & 2) + 1] += p1;
-          s[e / 2] = pack_bf2_rn(p0, p1);
+        const uint64_t scale2 = pack_f2(scale, scale), sub2 = pack_f2(-sub, -sub);
+        uint64_t sum[2] = {};
+        probs32(sa, scale2, sub2, sum);
+        tmem_st16(s_addr, sa);
+        if constexpr (BN == 128) tmem_ld32(s_addr + 64, sa);
+        probs32(sb, scale2, sub2, sum);
+        tmem_st16(s_addr + 16, sb);
+        if constexpr (BN == 128) {
+          tmem_ld32(s_addr + 96, sb);
+          tmem_wait_ld();
+          if (!whole) {
+            mask32(sa, hi - 64, lo - 64, sk - 64);
+            mask32(sb, hi - 96, lo - 96, sk - 96);
+          }
+          probs32(sa, scale2, sub2, sum);
+          tmem_st16(s_addr + 32, sa);
+          probs32(sb, scale2, sub2, sum);
+          tmem_st16(s_addr + 48, sb);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-        for (int e = 0; e < BN / 64; ++e) tmem_st32(lane_addr + C::kSCol + (q + buf) * BN + 32 * e, s + 32 * e);
+        const uint64_t sums = add_f2(sum[0], sum[1]);
+        l += lo_f2(sums) + hi_f2(sums);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -583,25 +644,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         uint16_t* dst = c.a.out + static_cast<int64_t>(w.s.q0 + tok) * c.a.o_tok + head * c.a.o_head;
         float* pd = c.parts + ((static_cast<int64_t>(blockIdx.x) * 2 + (t > 0 ? 0 : 1)) * NQ * kChunkRows + q * kChunkRows +
                                row) * (HD + 2);
-        if (sh.redo[item & 1] == item + 1) {
-          for (int rr = 0; rr < 32; ++rr) {
-            const int p = __shfl_sync(0xffffffffu, pos, rr);
-            if (!__shfl_sync(0xffffffffu, static_cast<int>(real), rr)) continue;
-            const int tk = __shfl_sync(0xffffffffu, tok, rr), hd_ = __shfl_sync(0xffffffffu, head, rr);
-            float o[HD / 32], sm, sl;
-            slow_row<HD>(c, w.b, w.kvh, p, w.r, t, t + n,
-                         c.a.q + static_cast<int64_t>(w.s.q0 + tk) * c.a.q_tok + hd_ * c.a.q_head, o, &sm, &sl);
-            uint16_t* d = c.a.out + static_cast<int64_t>(w.s.q0 + tk) * c.a.o_tok + hd_ * c.a.o_head;
-            float* ps = pd + (rr - lane) * (HD + 2);
-            const float inv = sm == -INFINITY ? 0.f : 1.f / sl;
-#pragma unroll
-            for (int e = 0; e < HD / 32; ++e) {
-              if (part) ps[2 + lane + 32 * e] = o[e];
-              else d[lane + 32 * e] = bf16_bits_rn(o[e] * inv);
-            }
-            if (part && lane == 0) ps[0] = sm, ps[1] = sl;
-          }
-        } else {
+        {
           const float inv = m == -INFINITY ? 0.f : 1.f / l;  // a row that sees nothing gives zeros
           if (part && real) pd[0] = m, pd[1] = l;
 #pragma unroll 1
@@ -609,6 +652,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
             uint32_t o[32];
             tmem_ld32(o_addr + 32 * e, o);
             tmem_wait_ld();
+            if (sh.odd[item & 1] == item + 1) add_odd<HD>(c, w, t, t + n, pos, 32 * e, o);
             if (real && part) {
 #pragma unroll
               for (int x = 0; x < 32; x += 2)
