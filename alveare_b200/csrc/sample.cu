@@ -6,19 +6,34 @@
 //   min-p: of those, w_i >= min_p;
 //   token: the first, in index order, whose running mass passes floor(u * total).
 //
-// The masses are integers (w is exact to 2^-40 below 1, a vocabulary of 2^20
-// sums to at most 2^60), so sums of any order and atomics give one result.
-// The prefix's end is found by radix selection on s's bits (mapped so that
-// unsigned order is s's order): a histogram of counts and masses per digit,
-// the digit where the k-th element (or the wanted mass) falls, then the next
-// digit among its elements.  Elements equal to the last one kept enter in
-// index order.
+// The masses are integers (a vocabulary of 2^20 sums to at most 2^60), so sums
+// of any order and atomics give one result.
+//
+// A cluster of CTAs takes a row and keeps it in its shared memory, so the
+// logits are read once; the CTAs exchange sums and histograms through
+// distributed shared memory.  The end of a prefix is found by a histogram over
+// max - s (2048 even bins; counts for top-k, masses for top-p), the bin where
+// the k-th element (or the wanted mass) falls, and then among that bin's
+// elements, gathered in one CTA, by comparing each with each; a bin with too
+// many elements is cut again by the bits of s.  Elements equal to the last one
+// kept enter in index order.  For top-p only elements that can be in the
+// prefix enter the histogram: those below e = (1 - p) total / (2 n) weigh less
+// than (1 - p) total together.
+#include <cooperative_groups.h>
+
 #include "internal.h"
 
 namespace alv {
 namespace {
 
-constexpr int kSampleThreads = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int kSampleThreads = 512;
+constexpr int kSampleWarps = kSampleThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kCand = kSampleThreads;  // elements of the last bin compared each with each
+constexpr int kMaxCluster = 8;
+constexpr float kMaxDist = 27.75f;     // exp(-27.75) < 2^-40: no mass beyond
 typedef unsigned long long u64;
 
 struct SampleArgs {
@@ -29,27 +44,47 @@ struct SampleArgs {
   float* logprobs;
   const float *t_rows, *p_rows, *m_rows;
   const int* k_rows;
-  int vocab, k;
+  int vocab, k, slice;  // slice: elements of the row per CTA
   float t, p, m;
 };
 
-// s's bits, ordered: key(a) < key(b) exactly when a < b (-0 counts as +0, NaN as -inf).
+// Bits of s in an order that unsigned comparison follows.
 __device__ __forceinline__ uint32_t key_of(float s) {
-  if (s != s) s = -INFINITY;
-  const uint32_t b = __float_as_uint(s + 0.0f == 0.0f ? 0.0f : s);
+  const uint32_t b = __float_as_uint(s);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// w of the element with key k when the row's largest value is `top`.
-__device__ __forceinline__ float weight(uint32_t k, float top) {
-  const float s = key_value(k);
-  if (top == INFINITY) return s == INFINITY ? 1.f : 0.f;
-  return expf(s - top);
+// floor(w 2^40) for w in [0, 1], by two additions that round down: at 8 a
+// float's step is 2^-20, at 2^-17 it is 2^-40.
+__device__ __forceinline__ u64 mass_of(float w) {
+  const float a = __fadd_rz(w, 8.0f);
+  const float rest = __fsub_rn(w, __fsub_rn(a, 8.0f));
+  const float b = __fadd_rz(rest, 7.62939453125e-06f);
+  return (static_cast<u64>(__float_as_uint(a) - 0x41000000u) << 20) + (__float_as_uint(b) - 0x37000000u);
 }
-__device__ __forceinline__ u64 mass_of(float w) { return static_cast<u64>(w * 1099511627776.0f); }
+
+struct Cut {  // kept: s > last, and the first `ties` (in index order) of s == last
+  float last;
+  uint32_t ties, of;  // of: how many equal `last`
+};
+
+struct SampleShared {
+  uint32_t lo[kBins], hi[kBins];  // counts, or masses in two words
+  uint32_t ckey[kCand], cidx[kCand];
+  u64 cmass[kCand];
+  uint32_t n_cand;
+  u64 scan[32];
+  // what this CTA shows the others, one slot per use
+  u64 sum[5];
+  uint32_t best_key, best_idx, kmin, kmax;
+  // what a CTA tells all
+  struct { int bin; u64 before; uint32_t last_key, ties, of; } found;
+  uint32_t wties[kSampleWarps];
+  u64 wmass[kSampleWarps];
+};
 
 // Inclusive prefix sum over the CTA; *total in every thread.
 __device__ __forceinline__ u64 cta_scan(u64 v, u64* total, u64* sh) {
@@ -63,176 +98,395 @@ __device__ __forceinline__ u64 cta_scan(u64 v, u64* total, u64* sh) {
   __syncthreads();
   if (lane == 31) sh[warp] = x;
   __syncthreads();
-  if (warp == 0) {
-    u64 w = sh[lane];
+  u64 before = 0, all = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    sh[lane] = w;
+  for (int w = 0; w < kSampleWarps; ++w) {
+    const u64 y = sh[w];
+    if (w < warp) before += y;
+    all += y;
   }
-  __syncthreads();
-  *total = sh[31];
-  return x + (warp ? sh[warp - 1] : 0);
+  *total = all;
+  return x + before;
 }
 
-struct Cut {  // kept: key > key_last, and the first `ties` (in index order) of key == key_last
-  uint32_t key;
-  u64 ties;
-  u64 mass;  // of everything kept
-};
-
-template <bool BF16>
+// The row's values, in shared memory (RES) or read again where they do not fit.
+template <bool BF16, bool RES>
 struct Row {
-  const void* base;
-  int vocab;
+  const void* base;  // this CTA's slice
+  float* vals;
+  int n, first;      // elements of the slice, index of its first
   float temp;
-  bool greedy;
-  __device__ __forceinline__ uint32_t key(int i) const {
-    float x = BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(base)[i]) : static_cast<const float*>(base)[i];
-    if (!greedy) x = __fdiv_rn(x, temp);
-    return key_of(x);
+  bool greedy, infinite;  // infinite: the largest value is +inf, only those count
+  __device__ __forceinline__ float value(float x) const {
+    if (!greedy && temp != 1.0f) x = __fdiv_rn(x, temp);
+    if (x != x) x = -INFINITY;
+    return x == 0.0f ? 0.0f : x;  // -0 counts as +0
+  }
+  __device__ __forceinline__ float raw(int i) const {
+    return BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(base)[i]) : static_cast<const float*>(base)[i];
+  }
+  __device__ __forceinline__ float at(int i) const {
+    float x = RES ? vals[i] : value(raw(i));
+    if (infinite) x = x == INFINITY ? 0.f : -INFINITY;
+    return x;
+  }
+  // f(i, value) for every element of the slice, 16-byte loads where aligned.
+  template <class F>
+  __device__ __forceinline__ void load(F f) const {
+    constexpr int V = BF16 ? 8 : 4;
+    int i0 = 0;
+    if ((reinterpret_cast<uintptr_t>(base) & 15) == 0) {
+      const uint4* p = static_cast<const uint4*>(base);
+      const int nv = n / V;
+#pragma unroll 4
+      for (int c = threadIdx.x; c < nv; c += kSampleThreads) {
+        const uint4 x = p[c];
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (BF16) {
+            f(c * V + 2 * e, value(bf16_bits_to_f32(w[e] & 0xFFFFu)));
+            f(c * V + 2 * e + 1, value(bf16_bits_to_f32(w[e] >> 16)));
+          } else {
+            f(c * V + e, value(__uint_as_float(w[e])));
+          }
+        }
+      }
+      i0 = nv * V;
+    }
+    for (int i = i0 + threadIdx.x; i < n; i += kSampleThreads) f(i, value(raw(i)));
   }
 };
 
-// The prefix of the row (in (s descending, index ascending) order) that ends
-// where the count reaches `want_n`, or (by_mass) the mass reaches `want_m`.
-template <bool BF16>
-__device__ Cut select(const Row<BF16>& row, float top, bool by_mass, u64 want_n, u64 want_m, unsigned* hn, u64* hm) {
-  __shared__ uint32_t pick;
-  __shared__ u64 before_n, before_m, in_n, in_m;
-  uint32_t prefix = 0;
-  u64 acc_n = 0, acc_m = 0, cnt = 0, ms = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int d = threadIdx.x; d < 256; d += blockDim.x) hn[d] = 0, hm[d] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < row.vocab; i += blockDim.x) {
-      const uint32_t k = row.key(i);
-      if (shift < 24 && (k >> (shift + 8)) != prefix) continue;
-      atomicAdd(hn + ((k >> shift) & 255), 1u);
-      atomicAdd(hm + ((k >> shift) & 255), mass_of(weight(k, top)));
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      u64 n = acc_n, m = acc_m;
-      int d = 255;
-      for (; d > 0; --d) {
-        if (by_mass ? m + hm[d] >= want_m : n + hn[d] >= want_n) break;
-        n += hn[d];
-        m += hm[d];
-      }
-      pick = d;
-      before_n = n;
-      before_m = m;
-      in_n = hn[d];
-      in_m = hm[d];
-    }
-    __syncthreads();
-    prefix = (prefix << 8) | pick;
-    acc_n = before_n;
-    acc_m = before_m;
-    cnt = in_n;
-    ms = in_m;
-    __syncthreads();
-  }
-  // every element left equals the key; each holds the same mass
-  const u64 each = cnt ? ms / cnt : 0;
-  u64 ties = by_mass ? (each && want_m > acc_m ? (want_m - acc_m + each - 1) / each : 1) : want_n - acc_n;
-  if (ties > cnt) ties = cnt;
-  return {prefix, ties, acc_m + ties * each};
+// Sum over the cluster of v (a thread's share), through slot `slot`.
+__device__ __forceinline__ u64 cluster_sum(cg::cluster_group& cl, SampleShared& sh, u64 v, int slot) {
+  u64 t;
+  cta_scan(v, &t, sh.scan);
+  if (threadIdx.x == 0) sh.sum[slot] = t;
+  cl.sync();
+  u64 all = 0;
+  for (unsigned r = 0; r < cl.num_blocks(); ++r) all += cl.map_shared_rank(&sh, r)->sum[slot];
+  return all;
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleArgs a) {
-  __shared__ unsigned hn[256];
-  __shared__ u64 hm[256], sh[32];
-  __shared__ uint32_t wk[32];
-  __shared__ int wi[32], chosen;
-  __shared__ u64 chosen_mass;
-  const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Row<BF16> row;
-  row.base = static_cast<const char*>(a.logits) + r * a.stride * (BF16 ? 2 : 4);
-  row.vocab = a.vocab;
+// The prefix of the row, in (s descending, index ascending) order, that ends
+// with the element where the count (or, MASS, the mass) reaches `want`; the
+// elements are those with top - s <= dist and s >= floor_s, and they reach it.
+template <bool MASS, bool BF16, bool RES>
+__device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, float top, float dist,
+                      float floor_s, u64 want) {
+  const unsigned rank = cl.block_rank(), nb = cl.num_blocks();
+  const float scale = static_cast<float>(kBins) / dist;
+  uint32_t kmin = 0, kmax = 0;  // after the first round: the keys of the bin that is cut again
+  int shift = 0;
+  u64 acc = 0;
+  for (int round = 0;; ++round) {
+    auto bin_of = [&](float s) -> int {  // -1: not in question
+      if (round == 0) {
+        const float d = top - s;
+        return d <= dist && s >= floor_s ? min(static_cast<int>(d * scale), kBins - 1) : -1;
+      }
+      const uint32_t k = key_of(s);
+      return k >= kmin && k <= kmax ? static_cast<int>((kmax - k) >> shift) : -1;
+    };
+    for (int b = threadIdx.x; b < kBins; b += kSampleThreads) sh.lo[b] = sh.hi[b] = 0;
+    if (threadIdx.x == 0) {
+      sh.n_cand = 0;
+      sh.kmin = 0xFFFFFFFFu;
+      sh.kmax = 0;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
+      const float s = row.at(i);
+      const int b = bin_of(s);
+      if (b < 0) continue;
+      if (MASS) {
+        const u64 m = mass_of(expf(s - top));
+        const uint32_t ml = static_cast<uint32_t>(m), old = atomicAdd(&sh.lo[b], ml);
+        const uint32_t mh = static_cast<uint32_t>(m >> 32) + (old + ml < old);
+        if (mh) atomicAdd(&sh.hi[b], mh);
+      } else {
+        atomicAdd(&sh.lo[b], 1u);
+      }
+    }
+    cl.sync();
+    // CTA r adds up bins [r, r + 1) * kBins / nb of all CTAs
+    const int per = kBins / nb, tp = (per + kSampleThreads - 1) / kSampleThreads;
+    u64 bins[kBins / kSampleThreads] = {}, mine = 0;
+    for (int e = 0; e < tp; ++e) {
+      const int b = threadIdx.x * tp + e;
+      if (b < per)
+        for (unsigned r = 0; r < nb; ++r) {
+          const SampleShared* o = cl.map_shared_rank(&sh, r);
+          bins[e] += o->lo[rank * per + b] + (static_cast<u64>(o->hi[rank * per + b]) << 32);
+        }
+      mine += bins[e];
+    }
+    u64 t;
+    u64 upto = cta_scan(mine, &t, sh.scan) - mine;
+    if (threadIdx.x == 0) sh.sum[round & 1] = t;
+    cl.sync();
+    u64 before = acc;
+    for (unsigned r = 0; r < rank; ++r) before += cl.map_shared_rank(&sh, r)->sum[round & 1];
+    upto += before;
+    for (int e = 0; e < tp; ++e) {
+      if (upto < want && want <= upto + bins[e])
+        for (unsigned r = 0; r < nb; ++r) {
+          SampleShared* o = cl.map_shared_rank(&sh, r);
+          o->found.bin = static_cast<int>(rank) * per + threadIdx.x * tp + e;
+          o->found.before = upto;
+        }
+      upto += bins[e];
+    }
+    cl.sync();
+    const int bin = sh.found.bin;
+    acc = sh.found.before;
+    // gather the bin's elements in CTA 0
+    SampleShared* lead = cl.map_shared_rank(&sh, 0);
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
+      const float s = row.at(i);
+      if (bin_of(s) != bin) continue;
+      const uint32_t k = key_of(s), at = atomicAdd(&lead->n_cand, 1u);
+      lo = min(lo, k);
+      hi = max(hi, k);
+      if (at < kCand) {
+        lead->ckey[at] = k;
+        lead->cidx[at] = row.first + i;
+      }
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if ((threadIdx.x & 31) == 0 && hi >= lo) {
+      atomicMin(&lead->kmin, lo);
+      atomicMax(&lead->kmax, hi);
+    }
+    cl.sync();
+    const uint32_t n = lead->n_cand;
+    kmin = lead->kmin;
+    kmax = lead->kmax;
+    if (kmin == kmax) {  // all equal
+      const u64 each = MASS ? mass_of(expf(key_value(kmin) - top)) : 1;
+      const u64 need = (want - acc + each - 1) / each;
+      cl.sync();  // CTA 0 stays until its words are read
+      return {key_value(kmin), static_cast<uint32_t>(need), n};
+    }
+    if (n <= kCand) {
+      if (rank == 0) {
+        const int i = threadIdx.x;
+        uint32_t k = 0, idx = 0;
+        u64 m = 0;
+        if (i < n) {
+          k = sh.ckey[i];
+          idx = sh.cidx[i];
+          m = MASS ? mass_of(expf(key_value(k) - top)) : 1;
+          sh.cmass[i] = m;
+        }
+        __syncthreads();
+        if (i < n) {
+          u64 pre = acc;
+          uint32_t ties = 1, of = 0;
+          for (uint32_t j = 0; j < n; ++j) {
+            const uint32_t kj = sh.ckey[j];
+            const bool earlier = kj == k && sh.cidx[j] < idx;
+            if (kj > k || earlier) pre += sh.cmass[j];
+            ties += earlier;
+            of += kj == k;
+          }
+          if (pre < want && want <= pre + m)
+            for (unsigned r = 0; r < nb; ++r) {
+              SampleShared* o = cl.map_shared_rank(&sh, r);
+              o->found.last_key = k;
+              o->found.ties = ties;
+              o->found.of = of;
+            }
+        }
+      }
+      cl.sync();
+      return {key_value(sh.found.last_key), sh.found.ties, sh.found.of};
+    }
+    shift = 0;
+    while (((kmax - kmin) >> shift) >= kBins) ++shift;
+    cl.sync();  // CTA 0's words are read before the next round clears them
+  }
+}
+
+template <bool BF16, bool RES>
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleArgs a) {
+  extern __shared__ __align__(16) uint8_t dyn[];
+  SampleShared& sh = *reinterpret_cast<SampleShared*>(dyn);
+  cg::cluster_group cl = cg::this_cluster();
+  const unsigned rank = cl.block_rank(), nb = cl.num_blocks();
+  const int r = blockIdx.x / nb, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Row<BF16, RES> row;
+  row.first = min(static_cast<int>(rank) * a.slice, a.vocab);
+  row.n = min(a.slice, a.vocab - row.first);
+  row.base = static_cast<const char*>(a.logits) + (r * a.stride + row.first) * (BF16 ? 2 : 4);
+  row.vals = reinterpret_cast<float*>(dyn + (sizeof(SampleShared) + 15) / 16 * 16);
   row.temp = a.t_rows ? a.t_rows[r] : a.t;
   row.greedy = !(row.temp > 0.f);
+  row.infinite = false;
   const int k = a.k_rows ? a.k_rows[r] : a.k;
   const float p = a.p_rows ? a.p_rows[r] : a.p, min_p = fminf(a.m_rows ? a.m_rows[r] : a.m, 1.f);
 
-  // the largest value and its first index
-  uint32_t best = 0;
+  // ---- the row into shared memory; its largest value and that one's first index
+  float best = -INFINITY;
   int bi = INT_MAX;
-  for (int i = threadIdx.x; i < a.vocab; i += blockDim.x) {
-    const uint32_t key = row.key(i);
-    if (key > best) best = key, bi = i;
+  row.load([&](int i, float s) {
+    if (RES) row.vals[i] = s;
+    if (s > best || (s == best && i < bi)) best = s, bi = i;
+  });
+  uint32_t bk = key_of(best), idx = bi == INT_MAX ? 0xFFFFFFFFu : static_cast<uint32_t>(row.first + bi);
+  {
+    const uint32_t wk = __reduce_max_sync(0xffffffffu, bk);
+    idx = __reduce_min_sync(0xffffffffu, bk == wk ? idx : 0xFFFFFFFFu);
+    if (lane == 0) sh.wties[warp] = wk, sh.wmass[warp] = idx;
+    __syncthreads();
+    bk = 0;
+    for (int w = 0; w < kSampleWarps; ++w) {
+      const uint32_t x = sh.wties[w], y = static_cast<uint32_t>(sh.wmass[w]);
+      if (x > bk || (x == bk && y < idx)) bk = x, idx = y;
+    }
+    if (threadIdx.x == 0) sh.best_key = bk, sh.best_idx = idx;
+    cl.sync();
+    for (unsigned o = 0; o < nb; ++o) {
+      const SampleShared* q = cl.map_shared_rank(&sh, o);
+      const uint32_t x = q->best_key, y = q->best_idx;
+      if (x > bk || (x == bk && y < idx)) bk = x, idx = y;
+    }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint32_t ok = __shfl_xor_sync(0xffffffffu, best, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-    if (ok > best || (ok == best && oi < bi)) best = ok, bi = oi;
-  }
-  if (lane == 0) wk[warp] = best, wi[warp] = bi;
-  __syncthreads();
-  for (int w = 0; w < 32; ++w)
-    if (wk[w] > best || (wk[w] == best && wi[w] < bi)) best = wk[w], bi = wi[w];
-  const float top = key_value(best);
-  if (row.greedy || top == -INFINITY) {
-    if (threadIdx.x == 0) {
-      a.tokens[r] = top == -INFINITY ? -1 : bi;
+  float top = key_value(bk);
+  if (row.greedy || top == -INFINITY) {  // the same in every CTA of the cluster
+    if (rank == 0 && threadIdx.x == 0) {
+      a.tokens[r] = top == -INFINITY ? -1 : static_cast<int>(idx);
       if (a.logprobs) a.logprobs[r] = top == -INFINITY ? -INFINITY : 0.f;
     }
+    cl.sync();  // no CTA leaves while another reads its words
     return;
   }
-  Cut cut{0, ~0ull, 0};
-  const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.f;
-  if (by_k) cut = select(row, top, false, static_cast<u64>(k), 0, hn, hm);
-  if (by_p) {
-    if (!by_k) {
-      u64 m = 0;
-      for (int i = threadIdx.x; i < a.vocab; i += blockDim.x) m += mass_of(weight(row.key(i), top));
-      cta_scan(m, &cut.mass, sh);
+  row.infinite = top == INFINITY;
+  if (row.infinite) top = 0.f;
+
+  // ---- where the kept prefix ends
+  Cut cut{-INFINITY, 0, 0};
+  bool all = true;
+  uint32_t n_kept = a.vocab;
+  if (k > 0 && k < a.vocab) {
+    // elements without mass do not matter: if fewer than k have some, all do
+    u64 n = 0;
+    for (int i = threadIdx.x; i < row.n; i += kSampleThreads) n += top - row.at(i) <= kMaxDist;
+    n = cluster_sum(cl, sh, n, 2);
+    if (n > static_cast<u64>(k)) {
+      cut = select<false>(cl, sh, row, top, kMaxDist, -INFINITY, static_cast<u64>(k));
+      all = false;
     }
-    const double goal = ceil(static_cast<double>(cut.mass) * static_cast<double>(p));
-    cut = select(row, top, true, 0, goal >= 1.0 ? static_cast<u64>(goal) : 1, hn, hm);
+    n_kept = k;
   }
-  // two walks in index order: the kept mass, then the token
-  u64 total = 0;
-  for (int walk = 0; walk < 2; ++walk) {
-    u64 goal = 0;
-    if (walk) {
-      const u64 x = static_cast<u64>(fmax(floor(static_cast<double>(a.u[r]) * static_cast<double>(total)), 0.0));
-      goal = x < total ? x : total - 1;
-      if (threadIdx.x == 0) chosen = INT_MAX;
-      __syncthreads();
+  if (p < 1.f) {
+    u64 m = 0;
+    for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
+      const float s = row.at(i);
+      if (all || s > cut.last) m += mass_of(expf(s - top));
     }
-    u64 ties = 0, run = 0, t;
-    for (int base = 0; base < a.vocab; base += blockDim.x) {
-      const int i = base + threadIdx.x;
-      const uint32_t key = i < a.vocab ? row.key(i) : 0;
-      const bool tie = i < a.vocab && key == cut.key;
-      const u64 rank = ties + cta_scan(tie ? 1 : 0, &t, sh);
-      ties += t;
-      u64 mass = 0;
-      if (i < a.vocab && (key > cut.key || (tie && rank <= cut.ties))) {
-        const float w = weight(key, top);
-        if (w >= min_p) mass = mass_of(w);
-      }
-      const u64 upto = run + cta_scan(mass, &t, sh);
-      run += t;
-      if (walk && upto > goal && upto - mass <= goal) {
-        chosen = i;
-        chosen_mass = mass;
-      }
-    }
-    total = run;
-    __syncthreads();
+    m = cluster_sum(cl, sh, m, 3);
+    if (!all) m += cut.ties * mass_of(expf(cut.last - top));
+    const double goal = ceil(static_cast<double>(m) * static_cast<double>(p));
+    const double eps = 0.5 * (1.0 - static_cast<double>(p)) * (static_cast<double>(m) / 1099511627776.0) / n_kept;
+    const float dist = fminf(0.01f - logf(fmaxf(static_cast<float>(eps), 1e-30f)), kMaxDist);
+    cut = select<true>(cl, sh, row, top, fmaxf(dist, 0.01f), cut.last, goal >= 1.0 ? static_cast<u64>(goal) : 1);
+    all = false;
   }
+
+  // ---- the kept mass of every warp's run of the slice, then the token
+  const int seg = (row.n + kSampleWarps * 32 - 1) / (kSampleWarps * 32) * 32;
+  const int i0 = min(warp * seg, row.n), i1 = min(i0 + seg, row.n);
+  const bool ranked = !all && cut.ties < cut.of;  // only some of the equals are kept
+  uint32_t tie0 = 0;
+  if (ranked) {
+    uint32_t n = 0;
+    for (int i = i0 + lane; i < i1; i += 32) n += row.at(i) == cut.last;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) sh.wties[warp] = n;
+    cl.sync();
+    for (unsigned o = 0; o <= rank; ++o) {
+      const SampleShared* q = cl.map_shared_rank(&sh, o);
+      for (int w = 0; w < (o == rank ? warp : kSampleWarps); ++w) tie0 += q->wties[w];
+    }
+  }
+  uint32_t ties = tie0;
+  auto kept_mass = [&](int i) -> u64 {  // lanes take consecutive elements; `ties` counts the equals so far
+    const float s = i < i1 ? row.at(i) : -INFINITY;
+    bool keep = i < i1 && (all || s >= cut.last);
+    if (ranked) {
+      const uint32_t eq = __ballot_sync(0xffffffffu, i < i1 && s == cut.last);
+      if (i < i1 && s == cut.last) keep = ties + __popc(eq & ((1u << lane) - 1)) < cut.ties;
+      ties += __popc(eq);
+    }
+    if (!keep) return 0;
+    const float w = expf(s - top);
+    return w >= min_p ? mass_of(w) : 0;
+  };
+  u64 m = 0;
+  for (int b = i0; b < i1; b += 32) m += kept_mass(b + lane);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+  if (lane == 0) sh.wmass[warp] = m;
+  __syncthreads();
   if (threadIdx.x == 0) {
-    a.tokens[r] = chosen;
-    if (a.logprobs)
-      a.logprobs[r] = static_cast<float>(log(static_cast<double>(chosen_mass) / static_cast<double>(total)));
+    u64 t = 0;
+    for (int w = 0; w < kSampleWarps; ++w) t += sh.wmass[w];
+    sh.sum[4] = t;
   }
+  cl.sync();
+  u64 total = 0, before = 0;
+  for (unsigned o = 0; o < nb; ++o) {
+    const u64 t = cl.map_shared_rank(&sh, o)->sum[4];
+    if (o < rank) before += t;
+    total += t;
+  }
+  for (int w = 0; w < warp; ++w) before += sh.wmass[w];
+  const u64 x = static_cast<u64>(fmax(floor(static_cast<double>(a.u[r]) * static_cast<double>(total)), 0.0));
+  const u64 goal = x < total ? x : total - 1;
+  if (before <= goal && goal < before + m) {  // this warp's run holds the token
+    ties = tie0;
+    for (int b = i0; b < i1; b += 32) {
+      const u64 e = kept_mass(b + lane);
+      u64 upto = e;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      if (before + upto > goal && before + upto - e <= goal) {
+        a.tokens[r] = row.first + b + lane;
+        if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(e) / static_cast<double>(total)));
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+      if (before > goal) break;
+    }
+  }
+  cl.sync();  // no CTA leaves while another reads its words
+}
+
+template <bool BF16, bool RES>
+int launch_sample(alv_ctx* ctx, const SampleArgs& a, int rows, int cluster, cudaStream_t st) {
+  auto k = sample_kernel<BF16, RES>;
+  const size_t smem = (sizeof(SampleShared) + 15) / 16 * 16 + (RES ? static_cast<size_t>(a.slice) * 4 : 0);
+  int rc = prepare_kernel(ctx, k, smem);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * cluster);
+  cfg.blockDim = dim3(kSampleThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  ALV_CUDA(ctx, cudaLaunchKernelEx(&cfg, k, a));
+  return ALV_OK;
 }
 
 }  // namespace
@@ -269,8 +523,19 @@ extern "C" int alv_sample(alv_ctx* ctx, const alv_sample_args* s, void* stream) 
   a.t = s->temperature;
   a.p = s->top_p;
   a.m = s->min_p;
-  auto k = s->logits_dtype == ALV_BF16 ? sample_kernel<true> : sample_kernel<false>;
-  k<<<s->rows, kSampleThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  ALV_CUDA(ctx, cudaGetLastError());
-  return ALV_OK;
+  // CTAs per row: as few as keep a CTA's slice at 16 K elements (64 KB: two
+  // CTAs of other rows share the SM); more, down to slices of 2 K, while the
+  // rows alone leave SMs idle.
+  int cluster = 1;
+  auto slice_of = [&](int c) { return static_cast<int>(align_up((s->vocab + c - 1) / c, 8)); };
+  while (cluster < kMaxCluster &&
+         (slice_of(cluster) > 16384 || (static_cast<int64_t>(s->rows) * cluster * 2 <= ctx->num_sms && slice_of(cluster) > 2048)))
+    cluster *= 2;
+  if (static_cast<int64_t>(s->rows) * cluster > INT_MAX) return fail(ctx, ALV_ERR_UNSUPPORTED, "sample: too many rows");
+  a.slice = slice_of(cluster);
+  const bool fits = a.slice <= 45056;  // 176 KB; a longer slice is read again in every pass
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (s->logits_dtype == ALV_BF16)
+    return fits ? launch_sample<true, true>(ctx, a, s->rows, cluster, st) : launch_sample<true, false>(ctx, a, s->rows, cluster, st);
+  return fits ? launch_sample<false, true>(ctx, a, s->rows, cluster, st) : launch_sample<false, false>(ctx, a, s->rows, cluster, st);
 }
