@@ -150,8 +150,7 @@ _contexts: dict[int, Context] = {}
 
 def context(device: int = 0) -> Context:
     """Process-wide context for `device` (created on first use)."""
-    with _lock:
-        ctx = _contexts.get(device)
+    ctx = _contexts.get(device)
     if ctx is None:
         ctx = Context(device)
         with _lock:

@@ -6,225 +6,450 @@
 namespace alv {
 namespace {
 
-// One warp's online-softmax state over the slices it takes.
-template <int HD>
-struct RowState {
-  float o[HD / 8][4];  // C fragments: rows g, g + 8 (g = lane / 4), dims 8n + 2t, +1 (t = lane % 4)
-  float m[2], l[2];
+struct RowArgs {
+  AttnArgs a;
+  float* parts;    // [2 * grid][kPart]: slot 0 where a run starts inside a block, 1 where it ends inside one
+  uint32_t* done;  // [grid]: finished parts of the block that cut c is the first inside; zero between launches
+};
+
+// Blocks (sequence, kv head, 16 rows) in order, rows fastest.
+struct RowWalk {
+  int b, kvh, blk, blks;
+  SeqSpan s;
+  SliceRange r;  // slices of the current block
+  int p0, p1, nrow;
+
+  __device__ __forceinline__ int blocks_of(const AttnArgs& a, const SeqSpan& q) const {
+    const int64_t rows = static_cast<int64_t>(q.qlen) * a.group;
+    return rows > a.row_max ? 0 : static_cast<int>((rows + kRowsPerBlock - 1) / kRowsPerBlock);
+  }
+  __device__ __forceinline__ void load(const AttnArgs& a) {
+    const int64_t r0 = static_cast<int64_t>(blk) * kRowsPerBlock;
+    nrow = static_cast<int>(min(static_cast<int64_t>(kRowsPerBlock), static_cast<int64_t>(s.qlen) * a.group - r0));
+    p0 = s.kv - s.qlen + static_cast<int>(r0 / a.group);
+    p1 = s.kv - s.qlen + static_cast<int>((r0 + nrow - 1) / a.group);
+    r = slice_range<kSlice>(p0, p1, a.window, a.sinks);
+  }
+  // A block that sees nothing still has one (empty) unit: it writes zeros.
+  __device__ __forceinline__ int units() const { return max(1, (r.count() + kRowWarps - 1) / kRowWarps); }
+  __device__ __forceinline__ int64_t units_of(const AttnArgs& a, const SeqSpan& q) {  // of one kv head
+    s = q;
+    const int n = blocks_of(a, q);
+    int64_t u = 0;
+    for (blk = 0; blk < n; ++blk) {
+      load(a);
+      u += units();
+    }
+    return u;
+  }
+  __device__ __forceinline__ void next(const AttnArgs& a) {
+    if (++blk == blks) {
+      blk = 0;
+      if (++kvh == a.c.nkv) {
+        kvh = 0;
+        do {
+          if (++b >= a.c.batch) return;
+          s = seq_span(a.c, b);
+          blks = blocks_of(a, s);
+        } while (blks == 0);
+      }
+    }
+    load(a);
+  }
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kRowWarps * 32, 1) paged_rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const RowArgs ra) {
   using R = RowRing<HD>;
   constexpr int NS = R::kSlots, CH = HD / 8;  // 16-byte chunks per row
+  const AttnArgs& a = ra.a;
   extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ int64_t sums[kRowWarps];
+  __shared__ int64_t start_before;
+  __shared__ int start_b;
+  __shared__ uint32_t arrived;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kvh = blockIdx.y, b = blockIdx.z;
-  const SeqSpan s = seq_span(a.c, b);
-  const int r0 = blockIdx.x * kRowsPerBlock;
-  const int64_t rows = static_cast<int64_t>(s.qlen) * a.group;
-  const int nrow = static_cast<int>(min(static_cast<int64_t>(kRowsPerBlock), rows - r0));
-  if (nrow <= 0 || rows > a.row_max) return;
-  const int pfirst = s.kv - s.qlen;  // position of the sequence's first new token
-  const int p0 = pfirst + r0 / a.group, p1 = pfirst + (r0 + nrow - 1) / a.group;
-  const SliceRange sr = slice_range<kSlice>(p0, p1, a.window, a.sinks);
 
-  // q rows (row r = token r / group, head kvh * group + r % group)
-  uint8_t* qs = smem;
-  const uint32_t q_sm = smem_u32(smem), ring = q_sm + R::kQBytes + warp * NS * R::kSlotBytes;
-  for (int e = threadIdx.x; e < kRowsPerBlock * CH; e += blockDim.x) {
-    const int r = e / CH, c = e % CH;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < nrow) {
-      const int tok = s.q0 + (r0 + r) / a.group, head = kvh * a.group + (r0 + r) % a.group;
-      v = *reinterpret_cast<const uint4*>(a.q + tok * a.q_tok + head * a.q_head + c * 8);
+  // ---- this CTA's run of units
+  RowWalk w{};
+  int64_t total, u0, u1;
+  int G;  // CTAs that get a run
+  {
+    const int per = (a.c.batch + kRowWarps * 32 - 1) / (kRowWarps * 32);
+    const int b0 = threadIdx.x * per, b1 = min(b0 + per, a.c.batch);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += w.units_of(a, seq_span(a.c, b)) * a.c.nkv;
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
     }
-    *reinterpret_cast<uint4*>(qs + r * HD * 2 + ((c ^ (r & 7)) << 4)) = v;
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    int64_t before = incl - mine;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < kRowWarps; ++i) {
+      if (i < warp) before += sums[i];
+      total += sums[i];
+    }
+    G = static_cast<int>(min((total + R::kMinUnits - 1) / R::kMinUnits, static_cast<int64_t>(gridDim.x)));
+    if (blockIdx.x >= G) return;
+    u0 = mul_div(total, blockIdx.x, G);
+    u1 = mul_div(total, blockIdx.x + 1, G);
+    if (before <= u0 && u0 < before + mine) {
+      int64_t at = before;
+      for (int b = b0; b < b1; ++b) {
+        const int64_t u = w.units_of(a, seq_span(a.c, b)) * a.c.nkv;
+        if (u0 < at + u) {
+          start_b = b;
+          start_before = at;
+          break;
+        }
+        at += u;
+      }
+    }
+    __syncthreads();
   }
-  __syncthreads();
+  int t0;  // first unit of the run inside its block
+  {
+    const SeqSpan q = seq_span(a.c, start_b);
+    const int64_t per_head = w.units_of(a, q);
+    int64_t rem = u0 - start_before;
+    w.b = start_b;
+    w.blks = w.blocks_of(a, q);
+    w.kvh = 0;
+    if (rem >= per_head) {
+      w.kvh = static_cast<int>(mul_div(rem, 1, static_cast<int>(min(per_head, static_cast<int64_t>(INT_MAX)))));
+      rem -= w.kvh * per_head;
+    }
+    w.blk = 0;
+    w.load(a);
+    while (rem >= w.units()) {
+      rem -= w.units();
+      ++w.blk;
+      w.load(a);
+    }
+    t0 = static_cast<int>(rem);
+    if (t0 > 0 && w.units() <= R::kWhole) {  // a block that is not cut belongs to the run its first unit is in
+      u0 += w.units() - t0;
+      t0 = 0;
+      if (u0 >= u1) return;
+      w.next(a);
+    }
+  }
 
-  const int n_mine = (sr.count() - warp + kRowWarps - 1) / kRowWarps;  // slices warp, warp + 8, ...
-  // Start the copy of half h (k of slice h / 2, or v) into its slot.
-  auto copy = [&](int h) {
-    if (h < 2 * n_mine) {
-      const int j0 = sr.slice(warp + (h >> 1) * kRowWarps) * kSlice;
-      const int page = page_of(a.c, b, j0);
-      const uint16_t* base = ((h & 1) ? a.c.v : a.c.k) + max(page, 0) * a.c.page_stride + kvh * a.c.head_stride +
-                             (j0 % a.c.page_size) * a.c.row_stride;
-      const uint32_t dst = ring + (h % NS) * R::kSlotBytes;
-#pragma unroll
-      for (int e = lane; e < kSlice * CH; e += 32) {
-        const int r = e / CH, c = e % CH, j = j0 + r;
-        const bool ok = page >= 0 && j < sr.hi && (j >= sr.lo || j < a.sinks);  // else zeros: never read
-        cp_async16(dst + r * HD * 2 + ((c ^ (r & 7)) << 4), base + (ok ? r * a.c.row_stride + c * 8 : 0), ok ? 16u : 0u);
+  // the run that holds unit x: the last c with total * c / G <= x
+  auto run_of = [&](int64_t x) { return static_cast<int>(((x + 1) * G - 1) / total); };
+  const uint32_t q_sm = smem_u32(smem), ring = q_sm + R::kQBytes + warp * NS * R::kSlotBytes;
+  // this lane's part of a half-slice copy: rows lane / CH + i * 32 / CH, chunk lane % CH
+  const int64_t lane_off = lane / CH * a.c.row_stride + lane % CH * 8;
+  for (int64_t u = u0; u < u1;) {
+    const SeqSpan& s = w.s;
+    const int r0 = w.blk * kRowsPerBlock, nrow = w.nrow;
+    const int n_units = w.units() <= R::kWhole ? w.units() : static_cast<int>(min(static_cast<int64_t>(w.units() - t0), u1 - u));
+    const int pfirst = s.kv - s.qlen, p0 = w.p0, p1 = w.p1;
+    // q rows (row r = token r / group, head kvh * group + r % group)
+    for (int e = threadIdx.x; e < kRowsPerBlock * CH; e += kRowWarps * 32) {
+      const int r = e / CH, c = e % CH;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < nrow) {
+        const int tok = s.q0 + (r0 + r) / a.group, head = w.kvh * a.group + (r0 + r) % a.group;
+        v = *reinterpret_cast<const uint4*>(a.q + tok * a.q_tok + head * a.q_head + c * 8);
       }
+      *reinterpret_cast<uint4*>(smem + r * HD * 2 + ((c ^ (r & 7)) << 4)) = v;
     }
-    cp_async_commit();
-  };
-  RowState<HD> st;
-#pragma unroll
-  for (int n = 0; n < HD / 8; ++n) st.o[n][0] = st.o[n][1] = st.o[n][2] = st.o[n][3] = 0.f;
-  st.m[0] = st.m[1] = -INFINITY;
-  st.l[0] = st.l[1] = 0.f;
-  // positions of this lane's two rows
-  const int pr[2] = {pfirst + (r0 + g) / a.group, pfirst + (r0 + g + 8) / a.group};
-  const bool one_token = p0 == p1;
-  for (int h = 0; h < NS - 1; ++h) copy(h);
-  for (int i = 0; i < n_mine; ++i) {
-    const int j0 = sr.slice(warp + i * kRowWarps) * kSlice;
-    // scores of the slice: two n-tiles of 8 positions
-    cp_async_wait<NS - 2>();
-    __syncwarp();
-    copy(2 * i + NS - 1);
-    float sc[2][4] = {};
-    const uint32_t ks = ring + ((2 * i) % NS) * R::kSlotBytes;
-#pragma unroll
-    for (int k = 0; k < HD / 16; ++k) {
-      uint32_t qa[4], kb[4];
-      const int qr = lane & 15, qc = 2 * k + (lane >> 4);
-      ldsm4(q_sm + qr * HD * 2 + ((qc ^ (qr & 7)) << 4), qa);
-      const int kr = (lane & 7) + ((lane >> 4) << 3), kc = 2 * k + ((lane >> 3) & 1);
-      ldsm4(ks + kr * HD * 2 + ((kc ^ (kr & 7)) << 4), kb);
-      mma_16816(sc[0], qa[0], qa[1], qa[2], qa[3], kb[0], kb[1]);
-      mma_16816(sc[1], qa[0], qa[1], qa[2], qa[3], kb[2], kb[3]);
-    }
-    // every row sees the whole slice?
-    const bool whole = j0 + kSlice - 1 <= p0 && (a.window == 0 || j0 > p1 - a.window || j0 + kSlice <= a.sinks);
-    const bool paged = page_of(a.c, b, j0) >= 0;
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = j0 + 8 * n + 2 * t + (e & 1);
-        sc[n][e] = paged && (whole || sees(j, pr[e >> 1], a.window, a.sinks)) ? sc[n][e] * a.scale_log2 : -INFINITY;
+
+    // slices warp, warp + 4, ... of the run's units
+    const int first = t0 * kRowWarps + warp;
+    const int n_mine = max(0, (min(w.r.count(), (t0 + n_units) * kRowWarps) - first + kRowWarps - 1) / kRowWarps);
+    auto j_of = [&](int i) { return w.r.slice(first + i * kRowWarps) * kSlice; };
+    // Where slices start in the cache, 32 at a time (lane l holds slice
+    // 32 k + l); -1: no valid page.
+    int64_t where = -1;
+    auto look_up = [&](int i) {
+      where = -1;
+      if (i + lane < n_mine) {
+        const int j = j_of(i + lane), page = page_of(a.c, w.b, j);
+        if (page >= 0)
+          where = page * a.c.page_stride + w.kvh * a.c.head_stride + (j % a.c.page_size) * a.c.row_stride;
       }
-    float f[2];
+    };
+    uint32_t paged = 0;  // bit i % 32: slice i (of the copies under way) has a page
+    // Start the copy of half h (k of slice h / 2, then v) into its slot.
+    auto copy = [&](int h) {
+      const int i = h >> 1;
+      if (i < n_mine) {
+        if (!(h & 1) && (i & 31) == 0) look_up(i);
+        const int64_t at = __shfl_sync(0xffffffffu, where, i & 31);
+        if (!(h & 1)) paged = (paged & ~(1u << (i & 31))) | (at >= 0 ? 1u << (i & 31) : 0u);
+        const int j0 = j_of(i);
+        const bool edge = at < 0 || j0 + kSlice > w.r.hi || (j0 < w.r.lo && j0 + kSlice > a.sinks);
+        const uint16_t* src = ((h & 1) ? a.c.v : a.c.k) + at + lane_off;
+        const uint32_t dst = ring + (h % NS) * R::kSlotBytes;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float mx = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      mx = fmaxf(mx, st.m[r]);
-      const float base = mx == -INFINITY ? 0.f : mx;
-      f[r] = exp2_fast(st.m[r] - base);
-      st.m[r] = mx;
-      float sum = 0.f;
+        for (int e = 0; e < kSlice * CH / 32; ++e) {
+          const int r = lane / CH + e * 32 / CH, c = lane % CH, j = j0 + r;
+          // rows no one sees are not read: zeros
+          const bool ok = !edge || (at >= 0 && j < w.r.hi && (j >= w.r.lo || j < a.sinks));
+          cp_async16(dst + r * HD * 2 + ((c ^ (r & 7)) << 4), ok ? src + e * (32 / CH) * a.c.row_stride : a.c.k, ok ? 16u : 0u);
+        }
+      }
+      cp_async_commit();
+    };
+    float o[HD / 8][4];  // C fragments: rows g, g + 8, dims 8n + 2t, +1
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    const int pr[2] = {pfirst + (r0 + g) / a.group, pfirst + (r0 + g + 8) / a.group};  // positions of this lane's rows
+    const bool one_token = p0 == p1;
+    for (int h = 0; h < NS - 1; ++h) copy(h);
+    __syncthreads();  // q
+    for (int i = 0; i < n_mine; ++i) {
+      const int j0 = j_of(i);
+      // scores of the slice: two n-tiles of 8 positions
+      cp_async_wait<NS - 2>();
+      __syncwarp();
+      copy(2 * i + NS - 1);
+      const bool has_page = paged >> (i & 31) & 1;
+      float sc[2][4] = {};
+      const uint32_t ks = ring + ((2 * i) % NS) * R::kSlotBytes;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        uint32_t qa[4], kb[4];
+        const int qr = lane & 15, qc = 2 * k + (lane >> 4);
+        ldsm4(q_sm + qr * HD * 2 + ((qc ^ (qr & 7)) << 4), qa);
+        const int kr = (lane & 7) + ((lane >> 4) << 3), kc = 2 * k + ((lane >> 3) & 1);
+        ldsm4(ks + kr * HD * 2 + ((kc ^ (kr & 7)) << 4), kb);
+        mma_16816(sc[0], qa[0], qa[1], qa[2], qa[3], kb[0], kb[1]);
+        mma_16816(sc[1], qa[0], qa[1], qa[2], qa[3], kb[2], kb[3]);
+      }
+      // every row sees the whole slice?
+      const bool whole = j0 + kSlice - 1 <= p0 && (a.window == 0 || j0 > p1 - a.window || j0 + kSlice <= a.sinks);
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float p = exp2_fast(sc[n][2 * r + e] - base);
-          sc[n][2 * r + e] = p;
-          sum += p;
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + 8 * n + 2 * t + (e & 1);
+          sc[n][e] = has_page && (whole || sees(j, pr[e >> 1], a.window, a.sinks)) ? sc[n][e] * a.scale_log2 : -INFINITY;
         }
-      st.l[r] = st.l[r] * f[r] + sum;  // this lane's four columns; lanes are added at the end
-    }
-    if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+      float f[2];
 #pragma unroll
-      for (int n = 0; n < HD / 8; ++n) {
-        st.o[n][0] *= f[0];
-        st.o[n][1] *= f[0];
-        st.o[n][2] *= f[1];
-        st.o[n][3] *= f[1];
+      for (int r = 0; r < 2; ++r) {
+        float mx = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        mx = fmaxf(mx, m[r]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        f[r] = exp2_fast(m[r] - base);
+        m[r] = mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float p = exp2_fast(sc[n][2 * r + e] - base);
+            sc[n][2 * r + e] = p;
+            sum += p;
+          }
+        l[r] = l[r] * f[r] + sum;  // this lane's four columns; lanes are added at the end
+      }
+      if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {
+          o[n][0] *= f[0];
+          o[n][1] *= f[0];
+          o[n][2] *= f[1];
+          o[n][3] *= f[1];
+        }
+      }
+      const uint32_t pa[4] = {pack_bf2_rn(sc[0][0], sc[0][1]), pack_bf2_rn(sc[0][2], sc[0][3]),
+                              pack_bf2_rn(sc[1][0], sc[1][1]), pack_bf2_rn(sc[1][2], sc[1][3])};
+      cp_async_wait<NS - 2>();
+      __syncwarp();
+      copy(2 * i + NS);
+      const uint32_t vs = ring + ((2 * i + 1) % NS) * R::kSlotBytes;
+      const bool mixed = !whole && !one_token;
+#pragma unroll
+      for (int n = 0; n < HD / 16; ++n) {
+        uint32_t vb[4];
+        const int vr = lane & 15, vc = 2 * n + (lane >> 4);
+        ldsm4_t(vs + vr * HD * 2 + ((vc ^ (vr & 7)) << 4), vb);
+        // A value that is not finite must not reach the rows that do not see
+        // its position (0 * inf): then each token's rows take their own product.
+        if (mixed && __any_sync(0xffffffffu, bf2_nonfinite(vb[0]) | bf2_nonfinite(vb[1]) | bf2_nonfinite(vb[2]) |
+                                                 bf2_nonfinite(vb[3]))) {
+          for (int pt = p0; pt <= p1; ++pt) {
+            uint32_t mk[2];
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              const int j = j0 + 8 * hh + 2 * t;
+              mk[hh] = (sees(j, pt, a.window, a.sinks) ? 0xFFFFu : 0u) |
+                       (sees(j + 1, pt, a.window, a.sinks) ? 0xFFFF0000u : 0u);
+            }
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              float tmp[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) tmp[e] = o[2 * n + hh][e];
+              mma_16816(tmp, pa[0], pa[1], pa[2], pa[3], vb[2 * hh] & mk[0], vb[2 * hh + 1] & mk[1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (pr[e >> 1] == pt) o[2 * n + hh][e] = tmp[e];
+            }
+          }
+        } else {
+          mma_16816(o[2 * n], pa[0], pa[1], pa[2], pa[3], vb[0], vb[1]);
+          mma_16816(o[2 * n + 1], pa[0], pa[1], pa[2], pa[3], vb[2], vb[3]);
+        }
       }
     }
-    const uint32_t pa[4] = {pack_bf2_rn(sc[0][0], sc[0][1]), pack_bf2_rn(sc[0][2], sc[0][3]),
-                            pack_bf2_rn(sc[1][0], sc[1][1]), pack_bf2_rn(sc[1][2], sc[1][3])};
-    cp_async_wait<NS - 2>();
-    __syncwarp();
-    copy(2 * i + NS);
-    const uint32_t vs = ring + ((2 * i + 1) % NS) * R::kSlotBytes;
-    const bool mixed = !whole && !one_token;
+    cp_async_wait<0>();
 #pragma unroll
-    for (int n = 0; n < HD / 16; ++n) {
-      uint32_t vb[4];
-      const int vr = lane & 15, vc = 2 * n + (lane >> 4);
-      ldsm4_t(vs + vr * HD * 2 + ((vc ^ (vr & 7)) << 4), vb);
-      // A value that is not finite must not reach the rows that do not see
-      // its position (0 * inf): then each token's rows take their own product.
-      if (mixed && __any_sync(0xffffffffu, bf2_nonfinite(vb[0]) | bf2_nonfinite(vb[1]) | bf2_nonfinite(vb[2]) |
-                                               bf2_nonfinite(vb[3]))) {
-        for (int pt = p0; pt <= p1; ++pt) {
-          uint32_t mk[2];
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+    // ---- join the warps in warp order
+    __syncthreads();
+    float* jm = reinterpret_cast<float*>(smem + R::kQBytes);
+    float* jl = jm + kRowWarps * kRowsPerBlock;
+    float* jo = jl + kRowWarps * kRowsPerBlock;
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            const int j = j0 + 8 * hh + 2 * t;
-            mk[hh] = (sees(j, pt, a.window, a.sinks) ? 0xFFFFu : 0u) |
-                     (sees(j + 1, pt, a.window, a.sinks) ? 0xFFFF0000u : 0u);
-          }
+    for (int r = 0; r < 2; ++r) {
+      const int row = warp * kRowsPerBlock + g + 8 * r;
+      if (t == 0) {
+        jm[row] = m[r];
+        jl[row] = l[r];
+      }
+      if (g + 8 * r < nrow) {
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            float tmp[4];
+        for (int n = 0; n < HD / 8; ++n)
+          *reinterpret_cast<float2*>(jo + row * HD + 8 * n + 2 * t) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+      }
+    }
+    __syncthreads();
+    const bool part = t0 > 0 || n_units < w.units();
+    float* mypart = ra.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * R::kPart;
+    auto store = [&](int r, int d, float x, float y) {  // two dims of a finished row
+      const int tok = s.q0 + (r0 + r) / a.group, head = w.kvh * a.group + (r0 + r) % a.group;
+      *reinterpret_cast<uint32_t*>(a.out + tok * a.o_tok + head * a.o_head + d) = pack_bf2_rn(x, y);
+    };
+    for (int e = threadIdx.x; e < nrow * (HD / 2); e += kRowWarps * 32) {
+      const int r = e / (HD / 2), d = (e % (HD / 2)) * 2;
+      float mm = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) tmp[e] = st.o[2 * n + hh][e];
-            mma_16816(tmp, pa[0], pa[1], pa[2], pa[3], vb[2 * hh] & mk[0], vb[2 * hh + 1] & mk[1]);
+      for (int x = 0; x < kRowWarps; ++x) mm = fmaxf(mm, jm[x * kRowsPerBlock + r]);
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (pr[e >> 1] == pt) st.o[2 * n + hh][e] = tmp[e];
-          }
-        }
+      for (int k = 0; k < kRowWarps; ++k) {
+        const int row = k * kRowsPerBlock + r;
+        const float f = exp2_fast(jm[row] - base);
+        const float2 v = *reinterpret_cast<const float2*>(jo + row * HD + d);
+        ll += f * jl[row];
+        x += f * v.x;
+        y += f * v.y;
+      }
+      if (part) {
+        if (d == 0) mypart[r] = mm, mypart[kRowsPerBlock + r] = ll;
+        *reinterpret_cast<float2*>(mypart + 2 * kRowsPerBlock + r * HD + d) = make_float2(x, y);
       } else {
-        mma_16816(st.o[2 * n], pa[0], pa[1], pa[2], pa[3], vb[0], vb[1]);
-        mma_16816(st.o[2 * n + 1], pa[0], pa[1], pa[2], pa[3], vb[2], vb[3]);
+        const float inv = mm == -INFINITY ? 0.f : 1.f / ll;  // a row that sees nothing gives zeros
+        store(r, d, x * inv, y * inv);
       }
     }
-  }
-  cp_async_wait<0>();
+    if (part) {
+      // CTAs c0 .. c1 hold the block's parts; the last to finish joins them
+      const int64_t g0 = u - t0, g1 = g0 + w.units();
+      const int c0 = run_of(g0), c1 = run_of(g1 - 1);
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        __threadfence();
+        arrived = atomicAdd(ra.done + c0 + 1, 1u);
+      }
+      __syncthreads();
+      if (arrived == static_cast<uint32_t>(c1 - c0)) {
+        __threadfence();
+        if (threadIdx.x == 0) ra.done[c0 + 1] = 0;
+        // warp w joins parts w, w + 4, ... (m, l in registers of its lanes as
+        // row = lane; O summed in shared memory), then the warps are joined
+        auto part_at = [&](int c) {
+          return ra.parts + (static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * R::kPart;
+        };
+        float wm = -INFINITY, wl = 0.f;
+        if (lane < nrow)
+          for (int c = c0 + warp; c <= c1; c += kRowWarps) wm = fmaxf(wm, __ldcg(part_at(c) + lane));
+        const float base = wm == -INFINITY ? 0.f : wm;
+        if (lane < nrow)
+          for (int c = c0 + warp; c <= c1; c += kRowWarps)
+            wl += exp2_fast(__ldcg(part_at(c) + lane) - base) * __ldcg(part_at(c) + kRowsPerBlock + lane);
+        if (lane < kRowsPerBlock) {
+          jm[warp * kRowsPerBlock + lane] = wm;
+          jl[warp * kRowsPerBlock + lane] = wl;
+        }
+        __syncwarp();
+        for (int e = lane; e < nrow * (HD / 4); e += 32) {
+          const int r = e / (HD / 4), d = (e % (HD / 4)) * 4;
+          const float rm = jm[warp * kRowsPerBlock + r], rb = rm == -INFINITY ? 0.f : rm;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int c = c0 + warp; c <= c1; c += kRowWarps) {
+            const float f = exp2_fast(__ldcg(part_at(c) + r) - rb);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part_at(c) + 2 * kRowsPerBlock + r * HD + d));
+            acc.x += f * v.x;
+            acc.y += f * v.y;
+            acc.z += f * v.z;
+            acc.w += f * v.w;
+          }
+          *reinterpret_cast<float4*>(jo + (warp * kRowsPerBlock + r) * HD + d) = acc;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < nrow * (HD / 2); e += kRowWarps * 32) {
+          const int r = e / (HD / 2), d = (e % (HD / 2)) * 2;
+          float mm = -INFINITY;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 1);
-    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 2);
-  }
-  // join the warps in warp order
-  __syncthreads();
-  float* jm = reinterpret_cast<float*>(smem + R::kQBytes);
-  float* jl = jm + kRowWarps * kRowsPerBlock;
-  float* jo = jl + kRowWarps * kRowsPerBlock;
+          for (int x = 0; x < kRowWarps; ++x) mm = fmaxf(mm, jm[x * kRowsPerBlock + r]);
+          const float b2 = mm == -INFINITY ? 0.f : mm;
+          float ll = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = warp * kRowsPerBlock + g + 8 * r;
-    if (t == 0) {
-      jm[row] = st.m[r];
-      jl[row] = st.l[r];
+          for (int k = 0; k < kRowWarps; ++k) {
+            const int row = k * kRowsPerBlock + r;
+            const float f = exp2_fast(jm[row] - b2);
+            const float2 v = *reinterpret_cast<const float2*>(jo + row * HD + d);
+            ll += f * jl[row];
+            x += f * v.x;
+            y += f * v.y;
+          }
+          const float inv = mm == -INFINITY ? 0.f : 1.f / ll;
+          store(r, d, x * inv, y * inv);
+        }
+      }
     }
-    if (g + 8 * r < nrow) {
-#pragma unroll
-      for (int n = 0; n < HD / 8; ++n)
-        *reinterpret_cast<float2*>(jo + row * HD + 8 * n + 2 * t) = make_float2(st.o[n][2 * r], st.o[n][2 * r + 1]);
+    u += n_units;
+    t0 = 0;
+    if (u < u1) {
+      w.next(a);
+      __syncthreads();  // q and the join's words are free
     }
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < nrow * (HD / 2); e += blockDim.x) {
-    const int r = e / (HD / 2), d = (e % (HD / 2)) * 2;
-    float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) m = fmaxf(m, jm[w * kRowsPerBlock + r]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) {
-      const int row = w * kRowsPerBlock + r;
-      const float f = exp2_fast(jm[row] - base);
-      const float2 o = *reinterpret_cast<const float2*>(jo + row * HD + d);
-      l += f * jl[row];
-      x += f * o.x;
-      y += f * o.y;
-    }
-    const float inv = m == -INFINITY ? 0.f : 1.f / l;  // a row that sees nothing gives zeros
-    const int tok = s.q0 + (r0 + r) / a.group, head = kvh * a.group + (r0 + r) % a.group;
-    *reinterpret_cast<uint32_t*>(a.out + tok * a.o_tok + head * a.o_head + d) = pack_bf2_rn(x * inv, y * inv);
   }
 }
 
 template <int HD>
-int launch_rows(alv_ctx* ctx, const AttnArgs& a, int max_q_len, cudaStream_t st) {
+int launch_rows(alv_ctx* ctx, const AttnArgs& a, cudaStream_t st) {
+  using R = RowRing<HD>;
   auto k = paged_rows_kernel<HD>;
-  const size_t smem = RowRing<HD>::kBytes;
-  int rc = prepare_kernel(ctx, k, smem);
+  int rc = prepare_kernel(ctx, k, R::kBytes);
   if (rc) return rc;
-  const int64_t rows = std::min<int64_t>(static_cast<int64_t>(max_q_len) * a.group, a.row_max);
-  const dim3 grid(static_cast<unsigned>((rows + kRowsPerBlock - 1) / kRowsPerBlock), a.c.nkv, a.c.batch);
-  k<<<grid, kRowWarps * 32, smem, st>>>(a);
+  const int grid = ctx->num_sms * 2;
+  if ((rc = ensure_scratch(ctx, static_cast<size_t>(grid) * 2 * R::kPart * 4))) return rc;
+  RowArgs ra{};
+  ra.a = a;
+  ra.a.c.status = status_ptr(ctx);
+  ra.parts = reinterpret_cast<float*>(work_ptr(ctx));
+  ra.done = counters_ptr(ctx);
+  k<<<grid, kRowWarps * 32, R::kBytes, st>>>(ra);
   ALV_CUDA(ctx, cudaGetLastError());
   return ALV_OK;
 }
@@ -248,8 +473,6 @@ extern "C" int alv_paged_attention(alv_ctx* ctx, const alv_paged* cache, const a
       args->q_head_stride % 8 || args->out_token_stride % 8 || args->out_head_stride % 8 || args->q_token_stride < 0 ||
       args->q_head_stride < 0 || args->out_token_stride < 0 || args->out_head_stride < 0)
     return fail(ctx, ALV_ERR_ARG, "paged_attention: q and out must be 16-byte aligned with strides of whole 16 bytes");
-  if (cache->batch > 65535 || cache->kv_heads > 65535)
-    return fail(ctx, ALV_ERR_UNSUPPORTED, "paged_attention: at most 65,535 sequences and kv heads in one call");
   if (cache->batch == 0 || cache->tokens == 0 || args->max_q_len == 0) return ALV_OK;
   a.q = args->q;
   a.q_tok = args->q_token_stride;
@@ -273,8 +496,8 @@ extern "C" int alv_paged_attention(alv_ctx* ctx, const alv_paged* cache, const a
     if (static_cast<int64_t>(cache->batch) * args->max_q_len == cache->tokens) return ALV_OK;
   }
   switch (cache->head_dim) {
-    case 64: return launch_rows<64>(ctx, a, args->max_q_len, st);
-    case 128: return launch_rows<128>(ctx, a, args->max_q_len, st);
-    default: return launch_rows<256>(ctx, a, args->max_q_len, st);
+    case 64: return launch_rows<64>(ctx, a, st);
+    case 128: return launch_rows<128>(ctx, a, st);
+    default: return launch_rows<256>(ctx, a, st);
   }
 }

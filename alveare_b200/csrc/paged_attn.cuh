@@ -9,13 +9,19 @@
 //   m' = max(m, max_j s_j),  l' = l 2^(m-m') + sum_j 2^(s_j-m'),
 //   O' = O 2^(m-m') + sum_j 2^(s_j-m') v_j
 // The positions are cut into slices of 16 (a slice never crosses a page: page
-// sizes are multiples of 16).  Every warp takes slices of its own, streams
-// their k and v rows through a private cp.async ring (no barrier between
-// warps in the loop) and keeps its own m, l and O in registers; the warps'
-// states are joined at the end.  The products run on mma.sync m16n8k16: the
-// work is bound by the cache's bytes, and 16 rows are all there is to a block.
-// p is rounded to bf16 for the product with v (the tensor core's operand type;
-// the result is rounded to bf16 anyway), l sums the unrounded fp32 p.
+// sizes are multiples of 16), four slices to a unit, one for each warp of a
+// CTA.  Every warp streams its slices' k and v rows through a private cp.async
+// ring (no barrier between warps in the loop) and keeps its own m, l and O in
+// registers; the warps' states are joined at the end.  The products run on
+// mma.sync m16n8k16: the work is bound by the cache's bytes, and 16 rows are
+// all there is to a block.  p is rounded to bf16 for the product with v (the
+// tensor core's operand type; the result is rounded to bf16 anyway), l sums
+// the unrounded fp32 p.
+//
+// The units of all blocks (sequence, kv head, 16 rows), in order, are cut into
+// equal runs, one per CTA (two CTAs per SM: one joins while the other
+// streams).  A block cut between CTAs leaves parts (m, l, O); the CTA that
+// finishes last joins them in a fixed order.
 #pragma once
 
 #include "internal.h"
@@ -42,18 +48,25 @@ int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int row_min, cudaStrea
 
 constexpr int kRowsPerBlock = 16;
 constexpr int kSlice = 16;
-constexpr int kRowWarps = 8;
+constexpr int kRowWarps = 4;
+constexpr int kUnit = kSlice * kRowWarps;  // positions of a unit
 
-// Half-slices (16 rows of k or of v) in a warp's ring: 192 KB over 8 warps.
+// Half-slices (16 rows of k or of v) in a warp's ring: 96 KB over 4 warps.
 template <int HD>
 struct RowRing {
-  static constexpr int kSlots = 192 * 1024 / kRowWarps / (kSlice * HD * 2);
+  static constexpr int kSlots = 96 * 1024 / kRowWarps / (kSlice * HD * 2);
   static constexpr uint32_t kSlotBytes = kSlice * HD * 2;
   static constexpr uint32_t kRingBytes = kRowWarps * kSlots * kSlotBytes;
   static constexpr uint32_t kQBytes = kRowsPerBlock * HD * 2;
   // joining the warps: m and l of every warp and row, then O
   static constexpr uint32_t kJoinBytes = kRowWarps * kRowsPerBlock * (HD + 2) * 4;
   static constexpr uint32_t kBytes = kQBytes + (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes);
+  static constexpr int kPart = kRowsPerBlock * (HD + 2);  // floats of a part: m[16], l[16], O[16][HD]
+  // A run is at least kMinUnits, and blocks of up to kWhole units are not cut:
+  // joining parts costs about 4 us, a unit a CTA alone about 0.3 us (64-wide
+  // heads) to 0.8 us (256-wide).
+  static constexpr int kMinUnits = HD == 256 ? 2 : 4;
+  static constexpr int kWhole = HD == 256 ? 6 : 12;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t src_bytes) {
@@ -94,6 +107,12 @@ __device__ __forceinline__ bool bf2_nonfinite(uint32_t x) {
 // Which positions a row at position `pos` sees.
 __device__ __forceinline__ bool sees(int j, int pos, int window, int sinks) {
   return j <= pos && (window == 0 || j > pos - window || j < sinks);
+}
+
+// x * y / z for x < 2^40 and y, z <= 2^16: in 32 bits where it fits.
+__device__ __forceinline__ int64_t mul_div(int64_t x, int y, int z) {
+  if (x < (1 << 21) && y < (1 << 10)) return static_cast<uint32_t>(x) * static_cast<uint32_t>(y) / static_cast<uint32_t>(z);
+  return x * y / z;
 }
 
 // The slices that any row at positions [p0, p1] sees: [0, n_sink) and

@@ -24,8 +24,8 @@ next ``context(device).sync_status()``.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 from ._lib import BF16, F32, context
 
@@ -34,79 +34,51 @@ try:
 except Exception:  # pragma: no cover
     torch = None
 
-_i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
+_INT_MAX = 2 ** 31 - 1
 
-
-class _Paged(ctypes.Structure):
-    """alv_paged"""
-    _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _i64), ("head_stride", _i64), ("row_stride", _i64),
-                ("pages", _i32), ("kv_heads", _i32), ("page_size", _i32), ("head_dim", _i32), ("table", _vp),
-                ("table_stride", _i64), ("q_start", _vp), ("kv_lens", _vp), ("table_width", _i32), ("batch", _i32),
-                ("tokens", _i32), ("reserved", _i32)]
-
-
-class _NormRope(ctypes.Structure):
-    """alv_qk_norm_rope_args"""
-    _fields_ = [("qkv", _vp), ("qkv_stride", _i64), ("q_out", _vp), ("q_token_stride", _i64), ("q_head_stride", _i64),
-                ("rope", _vp), ("q_weight", _vp), ("k_weight", _vp), ("qkv_dtype", _i32), ("rope_dtype", _i32),
-                ("heads", _i32), ("rot", _i32), ("max_pos", _i32), ("eps", _f32)]
-
-
-class _Attention(ctypes.Structure):
-    """alv_attention_args"""
-    _fields_ = [("q", _vp), ("q_token_stride", _i64), ("q_head_stride", _i64), ("out", _vp),
-                ("out_token_stride", _i64), ("out_head_stride", _i64), ("heads", _i32), ("max_q_len", _i32),
-                ("window", _i32), ("sinks", _i32), ("scale", _f32), ("reserved", _i32)]
-
-
-class _Pages(ctypes.Structure):
-    """alv_pages"""
-    _fields_ = [("k", _vp), ("v", _vp), ("layer_stride", _i64), ("page_stride", _i64), ("page_bytes", _i64),
-                ("table", _vp), ("lens", _vp), ("refs", _vp), ("table_stride", _i64), ("layers", _i32),
-                ("pages", _i32), ("page_size", _i32), ("slots", _i32), ("table_width", _i32), ("reserved", _i32)]
-
-
-class _Sample(ctypes.Structure):
-    """alv_sample_args"""
-    _fields_ = [("logits", _vp), ("logits_stride", _i64), ("u", _vp), ("tokens", _vp), ("logprobs", _vp),
-                ("temperature_rows", _vp), ("top_p_rows", _vp), ("min_p_rows", _vp), ("top_k_rows", _vp),
-                ("logits_dtype", _i32), ("rows", _i32), ("vocab", _i32), ("top_k", _i32), ("temperature", _f32),
-                ("top_p", _f32), ("min_p", _f32), ("reserved", _i32)]
+# The C structures, packed (a call costs a few microseconds of host time; the
+# ctypes.Structure form alone would take as long again).
+_PAGED = struct.Struct("@PPqqqiiiiPqPPiiii")             # alv_paged
+_NORM_ROPE = struct.Struct("@PqPqqPPPiiiiif")            # alv_qk_norm_rope_args
+_ATTENTION = struct.Struct("@PqqPqqiiiifi")              # alv_attention_args
+_PAGES = struct.Struct("@PPqqqPPPqiiiiii")               # alv_pages
+_SAMPLE = struct.Struct("@PqPPPPPPPiiiifffi")            # alv_sample_args
 
 
 # ---------------------------------------------------------------------------
 # checks
 # ---------------------------------------------------------------------------
-def _need(t, name: str, device: int, dtype, ndim: int):
+def _need(t, name: str, device: int, dtype, ndim: int) -> None:
     """A CUDA tensor of this type and rank on the call's device."""
+    try:
+        if t.get_device() == device and t.dtype is dtype and t.dim() == ndim and device >= 0:
+            return
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a torch CUDA tensor")
-    if t.device.index != device:
-        raise ValueError(f"{name} is on cuda:{t.device.index}, the call is on cuda:{device}")
-    if t.dtype != dtype:
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on cuda:{t.get_device()}, the call is on cuda:{device}")
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
-    if t.dim() != ndim:
-        raise ValueError(f"{name} must have {ndim} dimensions, not {t.dim()}")
+    raise ValueError(f"{name} must have {ndim} dimensions, not {t.dim()}")
 
 
 def _device(t, name: str) -> int:
     if torch is None or not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a torch CUDA tensor")
-    return t.device.index
+    return t.get_device()
 
 
-def _rows(t, name: str, device: int, ndim: int):
-    """A tensor of any supported activation type; the type's code."""
-    code = F32 if t.dtype == torch.float32 else BF16 if t.dtype == torch.bfloat16 else None
+def _rows(t, name: str, device: int, ndim: int) -> int:
+    """A tensor of either activation type; the type's code."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch CUDA tensor")
+    code = F32 if t.dtype is torch.float32 else BF16 if t.dtype is torch.bfloat16 else None
     if code is None:
         raise TypeError(f"{name} must be float32 or bfloat16, not {t.dtype}")
     _need(t, name, device, t.dtype, ndim)
     return code
-
-
-def _unit(t, name: str) -> None:
-    if t.stride(-1) != 1:
-        raise ValueError(f"{name} must be contiguous in its last dimension")
 
 
 def _vector(t, name: str, device: int, dtype, n: int) -> int:
@@ -121,24 +93,32 @@ def _stream(device: int) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def _paged(device: int, k_pages, v_pages, page_table, q_start, kv_lens, tokens: int) -> _Paged:
-    _need(k_pages, "k_pages", device, torch.bfloat16, 4)
-    _need(v_pages, "v_pages", device, torch.bfloat16, 4)
-    _need(page_table, "page_table", device, torch.int32, 2)
-    _need(q_start, "q_start", device, torch.int32, 1)
-    _need(kv_lens, "kv_lens", device, torch.int32, 1)
+if torch is not None and hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    _stream = torch._C._cuda_getCurrentRawStream  # noqa: F811  (the same handle, without the Stream object)
+
+
+def _paged(device: int, k_pages, v_pages, page_table, q_start, kv_lens, tokens: int):
+    """alv_paged, the kv heads and the head size."""
+    bf16, i32 = torch.bfloat16, torch.int32
+    _need(k_pages, "k_pages", device, bf16, 4)
+    _need(v_pages, "v_pages", device, bf16, 4)
+    _need(page_table, "page_table", device, i32, 2)
+    _need(q_start, "q_start", device, i32, 1)
+    _need(kv_lens, "kv_lens", device, i32, 1)
     shape, strides = k_pages.shape, k_pages.stride()
     if v_pages.shape != shape or v_pages.stride() != strides:
         raise ValueError("k_pages and v_pages must have the same shape and strides")
     batch = kv_lens.shape[0]
-    if page_table.shape[0] != batch or q_start.shape[0] != batch + 1:
+    rows, width = page_table.shape
+    if rows != batch or q_start.shape[0] != batch + 1:
         raise ValueError(f"page_table and q_start must have {batch} and {batch + 1} rows (kv_lens has {batch})")
-    if strides[3] != 1 or page_table.stride(1) != 1 or not q_start.is_contiguous() or not kv_lens.is_contiguous():
+    ts = page_table.stride()
+    if strides[3] != 1 or ts[1] != 1 or not q_start.is_contiguous() or not kv_lens.is_contiguous():
         raise ValueError("pages and page_table must be contiguous in their last dimension, q_start and kv_lens whole")
-    width = page_table.shape[1]
-    return _Paged(k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], strides[2], shape[0], shape[1],
-                  shape[2], shape[3], page_table.data_ptr(), max(page_table.stride(0), width), q_start.data_ptr(),
-                  kv_lens.data_ptr(), width, batch, tokens, 0)
+    pages, heads, ps, hd = shape
+    return _PAGED.pack(k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], strides[2], pages, heads, ps, hd,
+                       page_table.data_ptr(), max(ts[0], width), q_start.data_ptr(), kv_lens.data_ptr(), width, batch,
+                       tokens, 0), heads, hd
 
 
 # ---------------------------------------------------------------------------
@@ -164,20 +144,25 @@ def qk_norm_rope(qkv, q_out, k_pages, v_pages, page_table, q_start, kv_lens, rop
     _need(q_out, "q_out", device, torch.bfloat16, 3)
     rd = _rows(rope, "rope", device, 2)
     tokens, heads, hd = q_out.shape
-    c = _paged(device, k_pages, v_pages, page_table, q_start, kv_lens, tokens)
-    if c.head_dim != hd or qkv.shape != (tokens, (heads + 2 * c.kv_heads) * hd):
-        raise ValueError(f"qkv must be ({tokens}, {(heads + 2 * c.kv_heads) * c.head_dim}) for q_out "
-                         f"{tuple(q_out.shape)} and {c.kv_heads} kv heads of {c.head_dim}")
-    if rope.shape[1] % 2 or not rope.is_contiguous():
+    c, kv_heads, cache_hd = _paged(device, k_pages, v_pages, page_table, q_start, kv_lens, tokens)
+    cols = (heads + 2 * kv_heads) * hd
+    if cache_hd != hd or qkv.shape[0] != tokens or qkv.shape[1] != cols:
+        raise ValueError(f"qkv must be ({tokens}, {(heads + 2 * kv_heads) * cache_hd}) for q_out "
+                         f"{tuple(q_out.shape)} and {kv_heads} kv heads of {cache_hd}")
+    max_pos, width = rope.shape
+    if width % 2 or not rope.is_contiguous():
         raise ValueError("rope must be contiguous rows of cos | sin")
-    _unit(qkv, "qkv")
-    _unit(q_out, "q_out")
-    qw = None if q_weight is None else _vector(q_weight, "q_weight", device, torch.float32, hd)
-    kw = None if k_weight is None else _vector(k_weight, "k_weight", device, torch.float32, hd)
-    a = _NormRope(qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
-                  rope.data_ptr(), qw, kw, qd, rd, heads, rope.shape[1] // 2, rope.shape[0], eps)
+    xs, qs = qkv.stride(), q_out.stride()
+    if xs[1] != 1 or qs[2] != 1:
+        raise ValueError("qkv and q_out must be contiguous in their last dimension")
+    qw = 0 if q_weight is None else _vector(q_weight, "q_weight", device, torch.float32, hd)
+    kw = 0 if k_weight is None else _vector(k_weight, "k_weight", device, torch.float32, hd)
+    a = _NORM_ROPE.pack(qkv.data_ptr(), max(xs[0], cols), q_out.data_ptr(), qs[0], qs[1], rope.data_ptr(), qw, kw, qd,
+                        rd, heads, width // 2, max_pos, eps)
     ctx = context(device)
-    ctx.check(ctx.lib.alv_qk_norm_rope(ctx.ptr, ctypes.byref(c), ctypes.byref(a), _stream(device)), "alv_qk_norm_rope")
+    rc = ctx.lib.alv_qk_norm_rope(ctx.ptr, c, a, _stream(device))
+    if rc:
+        ctx.check(rc, "alv_qk_norm_rope")
 
 
 def paged_attention(q, out, k_pages, v_pages, page_table, q_start, kv_lens, *, max_q_len: int,
@@ -197,39 +182,41 @@ def paged_attention(q, out, k_pages, v_pages, page_table, q_start, kv_lens, *, m
     device = _device(q, "q")
     _need(q, "q", device, torch.bfloat16, 3)
     _need(out, "out", device, torch.bfloat16, 3)
-    tokens, heads, hd = q.shape
-    c = _paged(device, k_pages, v_pages, page_table, q_start, kv_lens, tokens)
-    if c.head_dim != hd or out.shape != q.shape:
-        raise ValueError(f"q and out must both be (tokens, heads, {c.head_dim})")
-    _unit(q, "q")
-    _unit(out, "out")
+    tokens, heads, hd = shape = q.shape
+    c, _, cache_hd = _paged(device, k_pages, v_pages, page_table, q_start, kv_lens, tokens)
+    if cache_hd != hd or out.shape != shape:
+        raise ValueError(f"q and out must both be (tokens, heads, {cache_hd})")
+    qs, os = q.stride(), out.stride()
+    if qs[2] != 1 or os[2] != 1:
+        raise ValueError("q and out must be contiguous in their last dimension")
     if window < 0 or sinks < 0 or max_q_len < 0:
         raise ValueError("window, sinks and max_q_len must not be negative")
-    a = _Attention(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), heads,
-                   min(max_q_len, tokens), window, sinks, 1.0 / math.sqrt(hd) if scale is None else scale, 0)
+    a = _ATTENTION.pack(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], heads, min(max_q_len, tokens),
+                        min(window, _INT_MAX), min(sinks, _INT_MAX), hd ** -0.5 if scale is None else scale, 0)
     ctx = context(device)
-    ctx.check(ctx.lib.alv_paged_attention(ctx.ptr, ctypes.byref(c), ctypes.byref(a), _stream(device)),
-              "alv_paged_attention")
+    rc = ctx.lib.alv_paged_attention(ctx.ptr, c, a, _stream(device))
+    if rc:
+        ctx.check(rc, "alv_paged_attention")
 
 
 # ---------------------------------------------------------------------------
 # page bookkeeping
 # ---------------------------------------------------------------------------
-def _pool(device: int, k_pool, v_pool, page_table, lens, refs) -> _Pages:
+def _pool(device: int, k_pool, v_pool, page_table, lens, refs) -> bytes:
     _need(k_pool, "k_pool", device, torch.bfloat16, 5)
     _need(v_pool, "v_pool", device, torch.bfloat16, 5)
     _need(page_table, "page_table", device, torch.int32, 2)
     layers, pages, nkv, ps, hd = k_pool.shape
-    st = k_pool.stride()
+    st, ts = k_pool.stride(), page_table.stride()
     if v_pool.shape != k_pool.shape or v_pool.stride() != st:
         raise ValueError("k_pool and v_pool must have the same shape and strides")
-    if st[2:] != (ps * hd, hd, 1) or page_table.stride(1) != 1:
+    if st[2:] != (ps * hd, hd, 1) or ts[1] != 1:
         raise ValueError("a page must be contiguous, and page_table in its last dimension")
     slots, width = page_table.shape
-    lp = None if lens is None else _vector(lens, "lens", device, torch.int32, slots)
-    return _Pages(k_pool.data_ptr(), v_pool.data_ptr(), st[0] * 2, st[1] * 2, nkv * ps * hd * 2, page_table.data_ptr(),
-                  lp, _vector(refs, "refs", device, torch.int32, pages), max(page_table.stride(0), width), layers,
-                  pages, ps, slots, width, 0)
+    lp = 0 if lens is None else _vector(lens, "lens", device, torch.int32, slots)
+    return _PAGES.pack(k_pool.data_ptr(), v_pool.data_ptr(), st[0] * 2, st[1] * 2, nkv * ps * hd * 2,
+                       page_table.data_ptr(), lp, _vector(refs, "refs", device, torch.int32, pages), max(ts[0], width),
+                       layers, pages, ps, slots, width, 0)
 
 
 def _list(t, name: str, device: int, pairs: bool):
@@ -270,8 +257,9 @@ def update_pages(k_pool, v_pool, page_table, lens, refs, *, free=None, fork=None
     ex, n_ex = _list(extend, "extend", device, True)
     ip = None if info is None else _vector(info, "info", device, torch.int32, 4)
     ctx = context(device)
-    ctx.check(ctx.lib.alv_pages_update(ctx.ptr, ctypes.byref(p), fr, n_fr, fo, n_fo, ex, n_ex, ip, _stream(device)),
-              "alv_pages_update")
+    rc = ctx.lib.alv_pages_update(ctx.ptr, p, fr, n_fr, fo, n_fo, ex, n_ex, ip, _stream(device))
+    if rc:
+        ctx.check(rc, "alv_pages_update")
 
 
 def compact_pages(k_pool, v_pool, page_table, refs, table_out, refs_out, *, info=None) -> None:
@@ -287,18 +275,19 @@ def compact_pages(k_pool, v_pool, page_table, refs, table_out, refs_out, *, info
     ro = _vector(refs_out, "refs_out", device, torch.int32, refs.shape[0])
     ip = None if info is None else _vector(info, "info", device, torch.int32, 2)
     ctx = context(device)
-    ctx.check(ctx.lib.alv_pages_compact(ctx.ptr, ctypes.byref(p), table_out.data_ptr(), ro, ip, _stream(device)),
-              "alv_pages_compact")
+    rc = ctx.lib.alv_pages_compact(ctx.ptr, p, table_out.data_ptr(), ro, ip, _stream(device))
+    if rc:
+        ctx.check(rc, "alv_pages_compact")
 
 
 # ---------------------------------------------------------------------------
 # sampling
 # ---------------------------------------------------------------------------
 def _param(v, name: str, device: int, dtype, rows: int, default):
-    """(pointer of per-row values or None, scalar)"""
+    """(pointer of per-row values or 0, scalar)"""
     if isinstance(v, torch.Tensor):
         return _vector(v, name, device, dtype, rows), default
-    return None, v
+    return 0, v
 
 
 def sample_tokens(logits, u, tokens, logprobs=None, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> None:
@@ -320,19 +309,23 @@ def sample_tokens(logits, u, tokens, logprobs=None, *, temperature=1.0, top_k=0,
     """
     device = _device(logits, "logits")
     ld = _rows(logits, "logits", device, 2)
-    _unit(logits, "logits")
     rows, vocab = logits.shape
+    stride = logits.stride()
+    if stride[1] != 1:
+        raise ValueError("logits must be contiguous in their last dimension")
     up = _vector(u, "u", device, torch.float32, rows)
     tp = _vector(tokens, "tokens", device, torch.int32, rows)
-    lp = None if logprobs is None else _vector(logprobs, "logprobs", device, torch.float32, rows)
+    lp = 0 if logprobs is None else _vector(logprobs, "logprobs", device, torch.float32, rows)
     t_rows, t = _param(temperature, "temperature", device, torch.float32, rows, 1.0)
     k_rows, k = _param(top_k, "top_k", device, torch.int32, rows, 0)
     p_rows, p = _param(top_p, "top_p", device, torch.float32, rows, 1.0)
     m_rows, m = _param(min_p, "min_p", device, torch.float32, rows, 0.0)
-    a = _Sample(logits.data_ptr(), max(logits.stride(0), vocab), up, tp, lp, t_rows, p_rows, m_rows, k_rows, ld, rows,
-                vocab, max(0, min(k, vocab)), t, p, m, 0)
+    a = _SAMPLE.pack(logits.data_ptr(), max(stride[0], vocab), up, tp, lp, t_rows, p_rows, m_rows, k_rows, ld, rows,
+                     vocab, max(0, min(k, vocab)), t, p, m, 0)
     ctx = context(device)
-    ctx.check(ctx.lib.alv_sample(ctx.ptr, ctypes.byref(a), _stream(device)), "alv_sample")
+    rc = ctx.lib.alv_sample(ctx.ptr, a, _stream(device))
+    if rc:
+        ctx.check(rc, "alv_sample")
 
 
 # ---------------------------------------------------------------------------

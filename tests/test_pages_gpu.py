@@ -252,10 +252,9 @@ def test_refusals():
         ab.compact_pages(p.k, p.v, p.table, p.refs, p.table[:2], p.refs)
     with pytest.raises(_lib.AlvError):   # renumbered in place, but not contiguous
         wide = torch.full((4, 9), -1, dtype=torch.int32, device="cuda")
-        rc = ab.paged._pool(0, p.k, p.v, wide[:, :4], None, p.refs)
-        import ctypes
+        pool = ab.paged._pool(0, p.k, p.v, wide[:, :4], None, p.refs)
         ctx = _lib.context(0)
-        ctx.check(ctx.lib.alv_pages_compact(ctx.ptr, ctypes.byref(rc), wide.data_ptr(), p.refs.data_ptr(), None, None),
+        ctx.check(ctx.lib.alv_pages_compact(ctx.ptr, pool, wide.data_ptr(), p.refs.data_ptr(), None, None),
                   "alv_pages_compact")
 
 
