@@ -15,6 +15,8 @@
 
 namespace alv {
 
+constexpr int64_t kMaxMapStride = int64_t{1} << 39;  // elements: a tensor map's strides are below 2^40 bytes
+
 struct PagedView {
   uint16_t* k;
   uint16_t* v;

@@ -8,12 +8,15 @@ namespace {
 
 struct RowArgs {
   AttnArgs a;
+  int box, head_first;  // positions per tensor copy, order of the cache's maps
   float* parts;    // [2 * grid][kPart]: slot 0 where a run starts inside a block, 1 where it ends inside one
   uint32_t* done;  // [grid]: finished parts of the block that cut c is the first inside; zero between launches
 };
 
 // Blocks (sequence, kv head, 16 rows) in order, rows fastest.
+template <int HD>
 struct RowWalk {
+  using R = RowRing<HD>;
   int b, kvh, blk, blks;
   SeqSpan s;
   SliceRange r;  // slices of the current block
@@ -28,17 +31,18 @@ struct RowWalk {
     nrow = static_cast<int>(min(static_cast<int64_t>(kRowsPerBlock), static_cast<int64_t>(s.qlen) * a.group - r0));
     p0 = s.kv - s.qlen + static_cast<int>(r0 / a.group);
     p1 = s.kv - s.qlen + static_cast<int>((r0 + nrow - 1) / a.group);
-    r = slice_range<kSlice>(p0, p1, a.window, a.sinks);
+    r = slice_range<R::kSlice>(p0, p1, a.window, a.sinks);
   }
   // A block that sees nothing still has one (empty) unit: it writes zeros.
   __device__ __forceinline__ int units() const { return max(1, (r.count() + kRowWarps - 1) / kRowWarps); }
-  __device__ __forceinline__ int64_t units_of(const AttnArgs& a, const SeqSpan& q) {  // of one kv head
+  __device__ __forceinline__ int length() const { return units() + R::kExtra; }
+  __device__ __forceinline__ int64_t length_of(const AttnArgs& a, const SeqSpan& q) {  // of one kv head's blocks
     s = q;
     const int n = blocks_of(a, q);
     int64_t u = 0;
     for (blk = 0; blk < n; ++blk) {
       load(a);
-      u += units();
+      u += length();
     }
     return u;
   }
@@ -59,26 +63,31 @@ struct RowWalk {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const RowArgs ra) {
+__global__ void __launch_bounds__(kRowWarps * 32, 2)
+    paged_rows_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const RowArgs ra) {
   using R = RowRing<HD>;
-  constexpr int NS = R::kSlots, CH = HD / 8;  // 16-byte chunks per row
+  constexpr int NS = R::kSlots, SL = R::kSlice, CH = HD / 8;  // CH: 16-byte chunks per row
   const AttnArgs& a = ra.a;
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ uint8_t smem_dyn[];
+  __shared__ __align__(8) uint64_t full[kRowWarps][NS];
   __shared__ int64_t sums[kRowWarps];
   __shared__ int64_t start_before;
   __shared__ int start_b;
   __shared__ uint32_t arrived;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* smem = smem_dyn + (((smem_u32(smem_dyn) + 1023u) & ~1023u) - smem_u32(smem_dyn));
+  if (lane < NS) mbar_init(&full[warp][lane], 1);
+  fence_mbar_init();
 
-  // ---- this CTA's run of units
-  RowWalk w{};
+  // ---- this CTA's run [u0, u1) of the blocks laid end to end
+  RowWalk<HD> w{};
   int64_t total, u0, u1;
   int G;  // CTAs that get a run
   {
     const int per = (a.c.batch + kRowWarps * 32 - 1) / (kRowWarps * 32);
     const int b0 = threadIdx.x * per, b1 = min(b0 + per, a.c.batch);
     int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += w.units_of(a, seq_span(a.c, b)) * a.c.nkv;
+    for (int b = b0; b < b1; ++b) mine += w.length_of(a, seq_span(a.c, b)) * a.c.nkv;
     int64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -101,7 +110,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Row
     if (before <= u0 && u0 < before + mine) {
       int64_t at = before;
       for (int b = b0; b < b1; ++b) {
-        const int64_t u = w.units_of(a, seq_span(a.c, b)) * a.c.nkv;
+        const int64_t u = w.length_of(a, seq_span(a.c, b)) * a.c.nkv;
         if (u0 < at + u) {
           start_b = b;
           start_before = at;
@@ -112,10 +121,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Row
     }
     __syncthreads();
   }
-  int t0;  // first unit of the run inside its block
+  int x;  // where the run is inside the current block
   {
     const SeqSpan q = seq_span(a.c, start_b);
-    const int64_t per_head = w.units_of(a, q);
+    const int64_t per_head = w.length_of(a, q);
     int64_t rem = u0 - start_before;
     w.b = start_b;
     w.blks = w.blocks_of(a, q);
@@ -126,30 +135,88 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Row
     }
     w.blk = 0;
     w.load(a);
-    while (rem >= w.units()) {
-      rem -= w.units();
+    while (rem >= w.length()) {
+      rem -= w.length();
       ++w.blk;
       w.load(a);
     }
-    t0 = static_cast<int>(rem);
-    if (t0 > 0 && w.units() <= R::kWhole) {  // a block that is not cut belongs to the run its first unit is in
-      u0 += w.units() - t0;
-      t0 = 0;
-      if (u0 >= u1) return;
-      w.next(a);
-    }
+    x = static_cast<int>(rem);
   }
 
-  // the run that holds unit x: the last c with total * c / G <= x
-  auto run_of = [&](int64_t x) { return static_cast<int>(((x + 1) * G - 1) / total); };
+  // the run that holds place x: the last c with total * c / G <= x
+  auto run_of = [&](int64_t at) { return static_cast<int>(((at + 1) * G - 1) / total); };
   const uint32_t q_sm = smem_u32(smem), ring = q_sm + R::kQBytes + warp * NS * R::kSlotBytes;
-  // this lane's part of a half-slice copy: rows lane / CH + i * 32 / CH, chunk lane % CH
-  const int64_t lane_off = lane / CH * a.c.row_stride + lane % CH * 8;
+  // the ring: next slot (and its barrier's phase) to fill and to use
+  int fill = 0, use = 0;
+  uint32_t phase = 0;
+  bool dead = false;  // a copy never came: report, copy and wait no more
   for (int64_t u = u0; u < u1;) {
     const SeqSpan& s = w.s;
-    const int r0 = w.blk * kRowsPerBlock, nrow = w.nrow;
-    const int n_units = w.units() <= R::kWhole ? w.units() : static_cast<int>(min(static_cast<int64_t>(w.units() - t0), u1 - u));
+    const int units = w.units(), r0 = w.blk * kRowsPerBlock, nrow = w.nrow;
+    int t0 = 0, t1 = units;  // units of this block that are this run's
+    if (units <= R::kWhole) {
+      if (x > 0) t1 = 0;  // a block that is not cut belongs to the run it begins in
+    } else {
+      t0 = max(0, x - R::kExtra);
+      t1 = max(0, static_cast<int>(min(static_cast<int64_t>(units + R::kExtra), x + (u1 - u))) - R::kExtra);
+    }
+    const int64_t g0 = u - x;  // where the block begins
+    u = g0 + units + R::kExtra;
+    x = 0;
+    if (t0 >= t1) {
+      if (u < u1) w.next(a);
+      continue;
+    }
     const int pfirst = s.kv - s.qlen, p0 = w.p0, p1 = w.p1;
+
+    // slices warp, warp + 4, ... of the run's units
+    const int first = t0 * kRowWarps + warp;
+    const int n_mine = max(0, (min(w.r.count(), t1 * kRowWarps) - first + kRowWarps - 1) / kRowWarps);
+    auto j_of = [&](int i) { return w.r.slice(first + i * kRowWarps) * SL; };
+    // Pages of the boxes to come: lane l holds box base + l (box b is part
+    // b % sub of slice b / sub).
+    const int sub = SL / ra.box;
+    int page = 0, row = 0;
+    auto look_up = [&](int i) {
+      const int bx = i * sub + lane, sl = bx / sub, j = sl < n_mine ? j_of(sl) + bx % sub * ra.box : w.r.hi;
+      page = a.c.pages;  // past the end: the copy reads zeros
+      row = 0;
+      if (j < w.r.hi && (j + ra.box > w.r.lo || j < a.sinks)) {
+        const int pg = page_of(a.c, w.b, j);
+        if (pg >= 0) page = pg, row = j % a.c.page_size;
+      }
+    };
+    // Copy k or v of slice i into the next slot: lane l fetches box l / (HD / 64), dims 64 (l % (HD / 64)) ...
+    auto copy = [&](int i, bool v) {
+      if (i < n_mine && !dead) {
+        const int per = 32 / sub;
+        if (!v && i % per == 0) look_up(i);
+        const int bx = lane / (HD / 64), d = lane % (HD / 64);
+        const int pg = __shfl_sync(0xffffffffu, page, (i % per) * sub + (bx < sub ? bx : 0));
+        const int rw = __shfl_sync(0xffffffffu, row, (i % per) * sub + (bx < sub ? bx : 0));
+        const uint32_t bar = smem_u32(&full[warp][fill]);
+        if (lane == 0) mbar_arrive_expect_tx_s(bar, R::kSlotBytes);
+        __syncwarp();
+        if (bx < sub) {
+          const uint32_t dst = ring + fill * R::kSlotBytes + d * (SL * 128) + bx * ra.box * 128;
+          if (ra.head_first) tma_load_4d(dst, v ? &vmap : &kmap, d * 64, w.kvh, rw, pg, bar);
+          else tma_load_4d(dst, v ? &vmap : &kmap, d * 64, rw, w.kvh, pg, bar);
+        }
+      }
+      if (i < n_mine) fill = fill + 1 == NS ? 0 : fill + 1;
+    };
+    auto arrive = [&]() {  // wait for the slot in use
+      if (!dead && !__all_sync(0xffffffffu, mbar_wait_bounded_s(smem_u32(&full[warp][use]), phase))) {
+        dead = true;
+        if (lane == 0) atomicOr(a.c.status, kStatusMbarTimeout);
+      }
+      __syncwarp();
+    };
+    auto release = [&]() {
+      __syncwarp();
+      if (++use == NS) use = 0, phase ^= 1;
+    };
+    for (int h = 0; h < NS - 1; ++h) copy(h >> 1, h & 1);
     // q rows (row r = token r / group, head kvh * group + r % group)
     for (int e = threadIdx.x; e < kRowsPerBlock * CH; e += kRowWarps * 32) {
       const int r = e / CH, c = e % CH;
@@ -160,100 +227,69 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Row
       }
       *reinterpret_cast<uint4*>(smem + r * HD * 2 + ((c ^ (r & 7)) << 4)) = v;
     }
-
-    // slices warp, warp + 4, ... of the run's units
-    const int first = t0 * kRowWarps + warp;
-    const int n_mine = max(0, (min(w.r.count(), (t0 + n_units) * kRowWarps) - first + kRowWarps - 1) / kRowWarps);
-    auto j_of = [&](int i) { return w.r.slice(first + i * kRowWarps) * kSlice; };
-    // Where slices start in the cache, 32 at a time (lane l holds slice
-    // 32 k + l); -1: no valid page.
-    int64_t where = -1;
-    auto look_up = [&](int i) {
-      where = -1;
-      if (i + lane < n_mine) {
-        const int j = j_of(i + lane), page = page_of(a.c, w.b, j);
-        if (page >= 0)
-          where = page * a.c.page_stride + w.kvh * a.c.head_stride + (j % a.c.page_size) * a.c.row_stride;
-      }
-    };
-    uint32_t paged = 0;  // bit i % 32: slice i (of the copies under way) has a page
-    // Start the copy of half h (k of slice h / 2, then v) into its slot.
-    auto copy = [&](int h) {
-      const int i = h >> 1;
-      if (i < n_mine) {
-        if (!(h & 1) && (i & 31) == 0) look_up(i);
-        const int64_t at = __shfl_sync(0xffffffffu, where, i & 31);
-        if (!(h & 1)) paged = (paged & ~(1u << (i & 31))) | (at >= 0 ? 1u << (i & 31) : 0u);
-        const int j0 = j_of(i);
-        const bool edge = at < 0 || j0 + kSlice > w.r.hi || (j0 < w.r.lo && j0 + kSlice > a.sinks);
-        const uint16_t* src = ((h & 1) ? a.c.v : a.c.k) + at + lane_off;
-        const uint32_t dst = ring + (h % NS) * R::kSlotBytes;
-#pragma unroll
-        for (int e = 0; e < kSlice * CH / 32; ++e) {
-          const int r = lane / CH + e * 32 / CH, c = lane % CH, j = j0 + r;
-          // rows no one sees are not read: zeros
-          const bool ok = !edge || (at >= 0 && j < w.r.hi && (j >= w.r.lo || j < a.sinks));
-          cp_async16(dst + r * HD * 2 + ((c ^ (r & 7)) << 4), ok ? src + e * (32 / CH) * a.c.row_stride : a.c.k, ok ? 16u : 0u);
-        }
-      }
-      cp_async_commit();
-    };
     float o[HD / 8][4];  // C fragments: rows g, g + 8, dims 8n + 2t, +1
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     const int pr[2] = {pfirst + (r0 + g) / a.group, pfirst + (r0 + g + 8) / a.group};  // positions of this lane's rows
     const bool one_token = p0 == p1;
-    for (int h = 0; h < NS - 1; ++h) copy(h);
     __syncthreads();  // q
+    // this lane's part of ldmatrix addresses: q and v rows lane % 16, k rows (lane & 7) + 8 (lane / 16)
+    const uint32_t lrow = lane & 15, lhi = lane >> 4, krow = (lane & 7) + ((lane >> 4) << 3), khi = (lane >> 3) & 1;
     for (int i = 0; i < n_mine; ++i) {
       const int j0 = j_of(i);
-      // scores of the slice: two n-tiles of 8 positions
-      cp_async_wait<NS - 2>();
-      __syncwarp();
-      copy(2 * i + NS - 1);
-      const bool has_page = paged >> (i & 31) & 1;
-      float sc[2][4] = {};
-      const uint32_t ks = ring + ((2 * i) % NS) * R::kSlotBytes;
+      // scores of the slice: n-tiles of 8 positions
+      arrive();
+      copy(i + (NS - 1) / 2, (NS - 1) & 1);
+      float sc[SL / 8][4] = {};
+      const uint32_t ks = ring + use * R::kSlotBytes;
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
-        uint32_t qa[4], kb[4];
-        const int qr = lane & 15, qc = 2 * k + (lane >> 4);
-        ldsm4(q_sm + qr * HD * 2 + ((qc ^ (qr & 7)) << 4), qa);
-        const int kr = (lane & 7) + ((lane >> 4) << 3), kc = 2 * k + ((lane >> 3) & 1);
-        ldsm4(ks + kr * HD * 2 + ((kc ^ (kr & 7)) << 4), kb);
-        mma_16816(sc[0], qa[0], qa[1], qa[2], qa[3], kb[0], kb[1]);
-        mma_16816(sc[1], qa[0], qa[1], qa[2], qa[3], kb[2], kb[3]);
-      }
-      // every row sees the whole slice?
-      const bool whole = j0 + kSlice - 1 <= p0 && (a.window == 0 || j0 > p1 - a.window || j0 + kSlice <= a.sinks);
+        uint32_t qa[4];
+        ldsm4(q_sm + lrow * (HD * 2) + (((2 * k + lhi) ^ (lrow & 7)) << 4), qa);
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = j0 + 8 * n + 2 * t + (e & 1);
-          sc[n][e] = has_page && (whole || sees(j, pr[e >> 1], a.window, a.sinks)) ? sc[n][e] * a.scale_log2 : -INFINITY;
+        for (int n = 0; n < SL / 16; ++n) {
+          uint32_t kb[4];
+          ldsm4(ks + (k / 4) * (SL * 128) + (16 * n + krow) * 128 + (((2 * (k % 4) + khi) ^ (krow & 7)) << 4), kb);
+          mma_16816(sc[2 * n], qa[0], qa[1], qa[2], qa[3], kb[0], kb[1]);
+          mma_16816(sc[2 * n + 1], qa[0], qa[1], qa[2], qa[3], kb[2], kb[3]);
         }
+      }
+      release();
+      // every row sees the whole slice?
+      const bool whole = j0 + SL - 1 <= p0 && (a.window == 0 || j0 > p1 - a.window || j0 + SL <= a.sinks);
+#pragma unroll
+      for (int n = 0; n < SL / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[n][e] *= a.scale_log2;
+      if (!whole) {
+#pragma unroll
+        for (int n = 0; n < SL / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!sees(j0 + 8 * n + 2 * t + (e & 1), pr[e >> 1], a.window, a.sinks)) sc[n][e] = -INFINITY;
+      }
       float f[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float mx = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+        float mx = m[r];
+#pragma unroll
+        for (int n = 0; n < SL / 8; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        mx = fmaxf(mx, m[r]);
         const float base = mx == -INFINITY ? 0.f : mx;
         f[r] = exp2_fast(m[r] - base);
         m[r] = mx;
         float sum = 0.f;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < SL / 8; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float p = exp2_fast(sc[n][2 * r + e] - base);
             sc[n][2 * r + e] = p;
             sum += p;
           }
-        l[r] = l[r] * f[r] + sum;  // this lane's four columns; lanes are added at the end
+        l[r] = l[r] * f[r] + sum;  // this lane's columns; lanes are added at the end
       }
       if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
@@ -264,48 +300,65 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Row
           o[n][3] *= f[1];
         }
       }
-      const uint32_t pa[4] = {pack_bf2_rn(sc[0][0], sc[0][1]), pack_bf2_rn(sc[0][2], sc[0][3]),
-                              pack_bf2_rn(sc[1][0], sc[1][1]), pack_bf2_rn(sc[1][2], sc[1][3])};
-      cp_async_wait<NS - 2>();
-      __syncwarp();
-      copy(2 * i + NS);
-      const uint32_t vs = ring + ((2 * i + 1) % NS) * R::kSlotBytes;
+      arrive();
+      copy(i + NS / 2, NS & 1);
+      const uint32_t vs = ring + use * R::kSlotBytes;
+      // positions no row sees hold anything: their v counts as zero
+      const bool edge = j0 + SL > w.r.hi || (j0 < w.r.lo && j0 + SL > a.sinks);
       const bool mixed = !whole && !one_token;
 #pragma unroll
-      for (int n = 0; n < HD / 16; ++n) {
-        uint32_t vb[4];
-        const int vr = lane & 15, vc = 2 * n + (lane >> 4);
-        ldsm4_t(vs + vr * HD * 2 + ((vc ^ (vr & 7)) << 4), vb);
-        // A value that is not finite must not reach the rows that do not see
-        // its position (0 * inf): then each token's rows take their own product.
-        if (mixed && __any_sync(0xffffffffu, bf2_nonfinite(vb[0]) | bf2_nonfinite(vb[1]) | bf2_nonfinite(vb[2]) |
-                                                 bf2_nonfinite(vb[3]))) {
-          for (int pt = p0; pt <= p1; ++pt) {
-            uint32_t mk[2];
+      for (int k = 0; k < SL / 16; ++k) {
+        uint32_t pa[4];
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              const int j = j0 + 8 * hh + 2 * t;
-              mk[hh] = (sees(j, pt, a.window, a.sinks) ? 0xFFFFu : 0u) |
-                       (sees(j + 1, pt, a.window, a.sinks) ? 0xFFFF0000u : 0u);
-            }
+        for (int e = 0; e < 4; ++e) pa[e] = pack_bf2_rn(sc[2 * k + (e >> 1)][2 * (e & 1)], sc[2 * k + (e >> 1)][2 * (e & 1) + 1]);
+        uint32_t live[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+        if (edge) {
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              float tmp[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) tmp[e] = o[2 * n + hh][e];
-              mma_16816(tmp, pa[0], pa[1], pa[2], pa[3], vb[2 * hh] & mk[0], vb[2 * hh + 1] & mk[1]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (pr[e >> 1] == pt) o[2 * n + hh][e] = tmp[e];
-            }
+          for (int hh = 0; hh < 2; ++hh) {
+            const int j = j0 + 16 * k + 8 * hh + 2 * t;
+            live[hh] = (j < w.r.hi && (j >= w.r.lo || j < a.sinks) ? 0xFFFFu : 0u) |
+                       (j + 1 < w.r.hi && (j + 1 >= w.r.lo || j + 1 < a.sinks) ? 0xFFFF0000u : 0u);
           }
-        } else {
-          mma_16816(o[2 * n], pa[0], pa[1], pa[2], pa[3], vb[0], vb[1]);
-          mma_16816(o[2 * n + 1], pa[0], pa[1], pa[2], pa[3], vb[2], vb[3]);
+        }
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) {
+          uint32_t vb[4];
+          ldsm4_t(vs + (n / 4) * (SL * 128) + (16 * k + lrow) * 128 + (((2 * (n % 4) + lhi) ^ (lrow & 7)) << 4), vb);
+          if (edge) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vb[e] &= live[e & 1];
+          }
+          // A value that is not finite must not reach the rows that do not see
+          // its position (0 * inf): then each token's rows take their own product.
+          if (mixed && __any_sync(0xffffffffu, bf2_nonfinite(vb[0]) | bf2_nonfinite(vb[1]) | bf2_nonfinite(vb[2]) |
+                                                   bf2_nonfinite(vb[3]))) {
+            for (int pt = p0; pt <= p1; ++pt) {
+              uint32_t mk[2];
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                const int j = j0 + 16 * k + 8 * hh + 2 * t;
+                mk[hh] = (sees(j, pt, a.window, a.sinks) ? 0xFFFFu : 0u) |
+                         (sees(j + 1, pt, a.window, a.sinks) ? 0xFFFF0000u : 0u);
+              }
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                float tmp[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) tmp[e] = o[2 * n + hh][e];
+                mma_16816(tmp, pa[0], pa[1], pa[2], pa[3], vb[2 * hh] & mk[0], vb[2 * hh + 1] & mk[1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (pr[e >> 1] == pt) o[2 * n + hh][e] = tmp[e];
+              }
+            }
+          } else {
+            mma_16816(o[2 * n], pa[0], pa[1], pa[2], pa[3], vb[0], vb[1]);
+            mma_16816(o[2 * n + 1], pa[0], pa[1], pa[2], pa[3], vb[2], vb[3]);
+          }
         }
       }
+      release();
     }
-    cp_async_wait<0>();
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -330,7 +383,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Row
       }
     }
     __syncthreads();
-    const bool part = t0 > 0 || n_units < w.units();
+    const bool part = t0 > 0 || t1 < units;
     float* mypart = ra.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * R::kPart;
     auto store = [&](int r, int d, float x, float y) {  // two dims of a finished row
       const int tok = s.q0 + (r0 + r) / a.group, head = w.kvh * a.group + (r0 + r) % a.group;
@@ -362,8 +415,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Row
     }
     if (part) {
       // CTAs c0 .. c1 hold the block's parts; the last to finish joins them
-      const int64_t g0 = u - t0, g1 = g0 + w.units();
-      const int c0 = run_of(g0), c1 = run_of(g1 - 1);
+      const int c0 = run_of(g0 + R::kExtra), c1 = run_of(g0 + R::kExtra + units - 1);
       __syncthreads();
       if (threadIdx.x == 0) {
         __threadfence();
@@ -427,11 +479,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Row
         }
       }
     }
-    u += n_units;
-    t0 = 0;
     if (u < u1) {
       w.next(a);
-      __syncthreads();  // q and the join's words are free
+      fence_proxy_async_smem();  // the join's words lie where copies will
+      __syncthreads();
     }
   }
 }
@@ -449,7 +500,10 @@ int launch_rows(alv_ctx* ctx, const AttnArgs& a, cudaStream_t st) {
   ra.a.c.status = status_ptr(ctx);
   ra.parts = reinterpret_cast<float*>(work_ptr(ctx));
   ra.done = counters_ptr(ctx);
-  k<<<grid, kRowWarps * 32, R::kBytes, st>>>(ra);
+  CUtensorMap kmap, vmap;
+  ra.box = box_rows(a.c.page_size, R::kSlice);
+  if ((rc = encode_cache(ctx, a.c, HD, ra.box, &kmap, &vmap, &ra.head_first))) return rc;
+  k<<<grid, kRowWarps * 32, R::kBytes, st>>>(kmap, vmap, ra);
   ALV_CUDA(ctx, cudaGetLastError());
   return ALV_OK;
 }

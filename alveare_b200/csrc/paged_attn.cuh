@@ -8,21 +8,24 @@
 // One pass with a running maximum m and sum l (base 2, fp32):
 //   m' = max(m, max_j s_j),  l' = l 2^(m-m') + sum_j 2^(s_j-m'),
 //   O' = O 2^(m-m') + sum_j 2^(s_j-m') v_j
-// The positions are cut into slices of 16 (a slice never crosses a page: page
-// sizes are multiples of 16), four slices to a unit, one for each warp of a
-// CTA.  Every warp streams its slices' k and v rows through a private cp.async
-// ring (no barrier between warps in the loop) and keeps its own m, l and O in
-// registers; the warps' states are joined at the end.  The products run on
-// mma.sync m16n8k16: the work is bound by the cache's bytes, and 16 rows are
-// all there is to a block.  p is rounded to bf16 for the product with v (the
-// tensor core's operand type; the result is rounded to bf16 anyway), l sums
-// the unrounded fp32 p.
+// The positions are cut into slices of 32 (16 for 256-wide heads), four slices
+// to a unit, one for each warp of a CTA.  Every warp streams its slices' k and
+// v rows through a private ring of tensor copies (128-byte swizzle; no barrier
+// between warps in the loop) and keeps its own m, l and O in registers; the
+// warps' states are joined at the end.  The products run on mma.sync
+// m16n8k16: the work is bound by the cache's bytes, and 16 rows are all there
+// is to a block.  p is rounded to bf16 for the product with v (the tensor
+// core's operand type; the result is rounded to bf16 anyway), l sums the
+// unrounded fp32 p.
 //
-// The units of all blocks (sequence, kv head, 16 rows), in order, are cut into
-// equal runs, one per CTA (two CTAs per SM: one joins while the other
+// The blocks (sequence, kv head, 16 rows), in order, are laid end to end, each
+// as long as its units and a few more for what a block costs by itself, and
+// cut into equal runs, one per CTA (two CTAs per SM: one joins while the other
 // streams).  A block cut between CTAs leaves parts (m, l, O); the CTA that
 // finishes last joins them in a fixed order.
 #pragma once
+
+#include <cuda.h>
 
 #include "internal.h"
 #include "paged.cuh"
@@ -47,36 +50,29 @@ bool chunk_takes(const AttnArgs& a);
 int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int row_min, cudaStream_t st);
 
 constexpr int kRowsPerBlock = 16;
-constexpr int kSlice = 16;
 constexpr int kRowWarps = 4;
-constexpr int kUnit = kSlice * kRowWarps;  // positions of a unit
 
-// Half-slices (16 rows of k or of v) in a warp's ring: 96 KB over 4 warps.
 template <int HD>
 struct RowRing {
-  static constexpr int kSlots = 96 * 1024 / kRowWarps / (kSlice * HD * 2);
+  static constexpr int kSlice = HD == 256 ? 16 : 32;  // positions
+  // half-slices (k or v rows of a slice) in a warp's ring: 96 KB over 4 warps
   static constexpr uint32_t kSlotBytes = kSlice * HD * 2;
+  static constexpr int kSlots = 96 * 1024 / kRowWarps / kSlotBytes;
   static constexpr uint32_t kRingBytes = kRowWarps * kSlots * kSlotBytes;
   static constexpr uint32_t kQBytes = kRowsPerBlock * HD * 2;
   // joining the warps: m and l of every warp and row, then O
   static constexpr uint32_t kJoinBytes = kRowWarps * kRowsPerBlock * (HD + 2) * 4;
-  static constexpr uint32_t kBytes = kQBytes + (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes);
+  static constexpr uint32_t kBytes = kQBytes + (kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes) + 1024;
   static constexpr int kPart = kRowsPerBlock * (HD + 2);  // floats of a part: m[16], l[16], O[16][HD]
-  // A run is at least kMinUnits, and blocks of up to kWhole units are not cut:
-  // joining parts costs about 4 us, a unit a CTA alone about 0.3 us (64-wide
-  // heads) to 0.8 us (256-wide).
-  static constexpr int kMinUnits = HD == 256 ? 2 : 4;
-  static constexpr int kWhole = HD == 256 ? 6 : 12;
+  // A unit is 32 KB (64-wide heads) or 64 KB of cache, 1.5 or 3 us of a CTA's
+  // share of the memory; starting and joining a block takes about 3 us, so a
+  // block counts kExtra units more.  A run is at least kMinUnits, and blocks
+  // of up to kWhole units are not cut: joining parts costs another 4 us.
+  static constexpr int kExtra = HD == 64 ? 2 : 1;
+  static constexpr int kMinUnits = 2;
+  static constexpr int kWhole = 6;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t src_bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -102,6 +98,24 @@ __device__ __forceinline__ uint32_t pack_bf2_rn(float lo, float hi) {
 }
 __device__ __forceinline__ bool bf2_nonfinite(uint32_t x) {
   return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+// Tensor maps of a layer's k and v pages with boxes of 64 dims x `box`
+// positions; *head_first: the map's order is (dim, head, row, page) instead of
+// (dim, row, head, page).
+int encode_cache(alv_ctx* ctx, const PagedView& c, int hd, int box, CUtensorMap* kmap, CUtensorMap* vmap, int* head_first);
+// The largest power of two that divides page sizes, at most `most`.
+inline int box_rows(int page_size, int most) {
+  int b = 16;
+  while (b < most && page_size % (2 * b) == 0) b *= 2;
+  return b;
 }
 
 // Which positions a row at position `pos` sees.

@@ -31,6 +31,20 @@
 namespace alv {
 namespace {
 
+int encode(alv_ctx* ctx, CUtensorMap* map, uint32_t rank, const void* p, const cuuint64_t* dims, const cuuint64_t* strides,
+           const cuuint32_t* box) {
+  EncodeTiledFn enc = nullptr;
+  int rc = tensor_map_encoder(ctx, &enc);
+  if (rc) return rc;
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  const CUresult cr = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(p), dims, strides, box, one,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (cr != CUDA_SUCCESS)
+    return fail(ctx, ALV_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed (" + std::to_string(cr) + ")");
+  return ALV_OK;
+}
+
 constexpr int kChunkRows = 128;
 constexpr int kMinUnits = 4;  // units of a CTA's run at least: a part costs about as much as two tiles
 
@@ -65,13 +79,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
           dst),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-          dst),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
       : "memory");
 }
 // D[tmem] (+)= A[tmem] B[smem]
@@ -735,20 +742,6 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const ChunkArgs c, int 
   }
 }
 
-int encode(alv_ctx* ctx, CUtensorMap* map, uint32_t rank, const void* p, const cuuint64_t* dims, const cuuint64_t* strides,
-           const cuuint32_t* box) {
-  EncodeTiledFn enc = nullptr;
-  int rc = tensor_map_encoder(ctx, &enc);
-  if (rc) return rc;
-  const cuuint32_t one[4] = {1, 1, 1, 1};
-  const CUresult cr = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(p), dims, strides, box, one,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (cr != CUDA_SUCCESS)
-    return fail(ctx, ALV_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed (" + std::to_string(cr) + ")");
-  return ALV_OK;
-}
-
 template <int HD>
 int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int row_min, cudaStream_t st) {
   using C = Chunk<HD>;
@@ -756,9 +749,7 @@ int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int row_min, cudaStream_t st
   c.a = a;
   c.tpt = kChunkRows / a.group;
   c.row_min = row_min;
-  c.box = 16;
-  while (c.box < C::kBN && a.c.page_size % (2 * c.box) == 0) c.box *= 2;
-  c.head_first = a.c.head_stride < a.c.row_stride;
+  c.box = box_rows(a.c.page_size, C::kBN);
   CUtensorMap qmap, kmap, vmap;
   {
     const cuuint64_t dims[3] = {HD, static_cast<cuuint64_t>(a.nq), static_cast<cuuint64_t>(a.c.tokens)};
@@ -767,17 +758,7 @@ int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int row_min, cudaStream_t st
     const int rc = encode(ctx, &qmap, 3, a.q, dims, str, box);
     if (rc) return rc;
   }
-  for (int kv = 0; kv < 2; ++kv) {
-    const cuuint64_t rows = a.c.page_size, heads = a.c.nkv, rs = a.c.row_stride * 2, hs = a.c.head_stride * 2,
-                     ps = a.c.page_stride * 2;
-    const cuuint32_t bx = static_cast<cuuint32_t>(c.box);
-    const cuuint64_t dims[4] = {HD, c.head_first ? heads : rows, c.head_first ? rows : heads,
-                                static_cast<cuuint64_t>(a.c.pages)};
-    const cuuint64_t str[3] = {c.head_first ? hs : rs, c.head_first ? rs : hs, ps};
-    const cuuint32_t box[4] = {64, c.head_first ? 1 : bx, c.head_first ? bx : 1, 1};
-    const int rc = encode(ctx, kv ? &vmap : &kmap, 4, kv ? a.c.v : a.c.k, dims, str, box);
-    if (rc) return rc;
-  }
+  if (const int rc = encode_cache(ctx, a.c, HD, c.box, &kmap, &vmap, &c.head_first)) return rc;
   const int grid = ctx->num_sms;
   const size_t o_cuts = 256, o_parts = o_cuts + align_up(static_cast<size_t>(grid) * sizeof(int4), 256);
   int rc = ensure_scratch(ctx, o_parts + static_cast<size_t>(grid) * 2 * C::kNQ * kChunkRows * (HD + 2) * 4);
@@ -795,14 +776,25 @@ int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int row_min, cudaStream_t st
 
 }  // namespace
 
+int encode_cache(alv_ctx* ctx, const PagedView& c, int hd, int box, CUtensorMap* kmap, CUtensorMap* vmap, int* head_first) {
+  const bool hf = c.head_stride < c.row_stride;
+  *head_first = hf;
+  const cuuint64_t rows = c.page_size, heads = c.nkv, rs = c.row_stride * 2, hs = c.head_stride * 2;
+  const cuuint32_t bx = static_cast<cuuint32_t>(box);
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), hf ? heads : rows, hf ? rows : heads,
+                              static_cast<cuuint64_t>(c.pages)};
+  const cuuint64_t str[3] = {hf ? hs : rs, hf ? rs : hs, static_cast<cuuint64_t>(c.page_stride) * 2};
+  const cuuint32_t bdim[4] = {64, hf ? 1 : bx, hf ? bx : 1, 1};
+  const int rc = encode(ctx, kmap, 4, c.k, dims, str, bdim);
+  return rc ? rc : encode(ctx, vmap, 4, c.v, dims, str, bdim);
+}
+
 // The tensor-core form takes whole kv groups as rows of one tile, a positive
-// scale (masked scores are -inf before the scale), and strides a tensor map
+// scale (masked scores are -inf before the scale), and q strides a tensor map
 // can hold; anything else runs on the row-block kernel.
 bool chunk_takes(const AttnArgs& a) {
-  constexpr int64_t kMaxStride = int64_t{1} << 39;  // elements: a tensor map's strides are below 2^40 bytes
-  return a.group <= kChunkRows && a.scale_log2 > 0.f && a.q_head > 0 && a.q_tok > 0 && a.c.head_stride > 0 &&
-         a.c.page_stride > 0 && a.q_tok < kMaxStride && a.c.page_stride < kMaxStride && a.c.head_stride < kMaxStride &&
-         a.c.row_stride < kMaxStride;
+  return a.group <= kChunkRows && a.scale_log2 > 0.f && a.q_head > 0 && a.q_tok > 0 && a.q_tok < kMaxMapStride &&
+         a.q_head < kMaxMapStride;
 }
 
 int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int row_min, cudaStream_t st) {

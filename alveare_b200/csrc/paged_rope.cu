@@ -147,8 +147,10 @@ int make_paged_view(alv_ctx* ctx, const char* who, const alv_paged* p, PagedView
   if (p->page_size % 16) return fail(ctx, ALV_ERR_SHAPE, w + ": page_size must be a multiple of 16");
   if (static_cast<int64_t>(p->table_width) * p->page_size > INT_MAX)
     return fail(ctx, ALV_ERR_UNSUPPORTED, w + ": a sequence may hold at most 2^31 - 1 positions");
-  if (p->row_stride < p->head_dim || p->head_stride < 0 || p->page_stride < 0 || p->row_stride % 8 ||
-      p->head_stride % 8 || p->page_stride % 8 || ((reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v)) & 15))
+  if (p->row_stride < p->head_dim || p->head_stride < 1 || p->page_stride < 1 || p->row_stride >= kMaxMapStride ||
+      p->head_stride >= kMaxMapStride || p->page_stride >= kMaxMapStride)
+    return fail(ctx, ALV_ERR_ARG, w + ": the pages' strides must be positive (no broadcast), rows of head_dim values apart");
+  if (p->row_stride % 8 || p->head_stride % 8 || p->page_stride % 8 || ((reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v)) & 15))
     return fail(ctx, ALV_ERR_ARG, w + ": k, v must be 16-byte aligned with strides of whole 16 bytes");
   int rc = ensure_scratch(ctx, 0);
   if (rc) return rc;
