@@ -3,13 +3,14 @@
 // rows (tokens x the heads of a kv group) against tiles of BN positions:
 //
 //   S = Q K^T          tcgen05.mma, Q and K tiles in shared memory, S in TMEM
-//   P = 2^(S c - m)    softmax warps: one thread per row, TMEM -> registers;
-//                      P goes back to TMEM as bf16 over S's own columns
+//   P = 2^(S c - m)    softmax warps: two threads per row, half of its columns
+//                      each, TMEM -> registers; P goes back to TMEM as bf16
+//                      over S's own columns
 //   O += P V           tcgen05.mma with P from TMEM, O stays in TMEM
 //
 // Head sizes 64 and 128: two query tiles per CTA (TMEM: 2 x (S 128 + O HD)
-// columns), each with its own softmax warpgroup, so the tensor cores work for
-// one tile while the other's softmax runs.  Head size 256: O alone takes 256
+// columns), each with its own softmax warps, so the tensor cores work for one
+// tile while the other's softmax runs.  Head size 256: O alone takes 256
 // columns, so one query tile with two S buffers of 64 positions.
 //
 // The running maximum only moves when a row's new maximum exceeds the one in
@@ -57,7 +58,8 @@ struct Chunk {
   static constexpr uint32_t kQTile = kChunkRows * HD * 2;
   static constexpr uint32_t kKV = kBN * HD * 2;
   static constexpr uint32_t kBytes = kNQ * kQTile + 2 * kStages * kKV + 1024;
-  static constexpr int kSoftWarps = 4 * kNQ;
+  static constexpr int kHalf = kBN / 2;            // columns of S a softmax thread takes
+  static constexpr int kSoftWarps = 8 * kNQ;
   static constexpr int kThreads = (kSoftWarps + 2) * 32;
   static constexpr uint32_t kSCol = 0;      // S (and P) of tile q, buffer b: (q + b) * kBN
   static constexpr uint32_t kOCol = 256;    // O of tile q: 256 + q * HD
@@ -107,12 +109,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
       : ALV_R8(r, 0), ALV_R8(r, 8), ALV_R8(r, 16), ALV_R8(r, 24)
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_ld16u(uint32_t addr, uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::ALV_I8(r, 0),
-      ALV_I8(r, 8), ALV_I8(r, 16), ALV_I8(r, 24), "r"(addr)
-      : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : ALV_R8(r, 0), ALV_R8(r, 8)
+      : "r"(addr));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
@@ -220,7 +221,9 @@ struct ChunkShared {
   uint64_t kfull[C::kStages], kempty[C::kStages], vfull[C::kStages], vempty[C::kStages];
   uint64_t qfull, qempty, sfull[C::kNQ][C::kSB], pfull[C::kNQ][C::kSB], odone[C::kNQ], pvdone;
   uint32_t tmem;
-  volatile uint32_t failed;
+  volatile uint32_t failed;  // a wait gave up: report, wait no more, run to the end
+  float mx[C::kNQ][2][2][kChunkRows];  // a row's maximum over each half, two tiles deep
+  float lx[C::kNQ][2][kChunkRows];
   // odd[i & 1] = i + 1: item i of the run has v values that are not finite in
   // a tile that only some rows see whole (a warpgroup with work in an item is
   // at most one item ahead of the other)
@@ -285,7 +288,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
       for (int i = 0; i < C::kSB; ++i) {
         mbar_init(&sh.sfull[q][i], 1);
         // per S buffer: with two, a warp may be a tile ahead of its fellows
-        mbar_init(&sh.pfull[q][i], 4);
+        mbar_init(&sh.pfull[q][i], 8);
       }
       mbar_init(&sh.odone[q], 1);
     }
@@ -373,14 +376,10 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
   if (threadIdx.x == 0)
     c.cuts[blockIdx.x] = first_tile > 0 ? make_int4(w.b, w.kvh, w.pair, first_tile) : make_int4(-1, 0, 0, 0);
 
-  auto fail_now = [&] {
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (sh.failed || mbar_wait_bounded_s(smem_u32(bar), parity)) return;
     atomicOr(c.a.c.status, kStatusMbarTimeout);
     sh.failed = 1;
-  };
-  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    if (mbar_wait_bounded_s(smem_u32(bar), parity)) return true;
-    fail_now();
-    return false;
   };
 
   if (warp == C::kSoftWarps) {
@@ -389,12 +388,10 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     uint32_t it = 0, item = 0;
     int64_t u = u0;
     int t = first_tile;
-    bool ok = true;
-    while (ok && u < u1) {
+    while (u < u1) {
       const int n = static_cast<int>(min(static_cast<int64_t>(w.r.count() - t), u1 - u));
       const int tok = w.pair * NQ * c.tpt;
-      if (item > 0) ok = __all_sync(0xffffffffu, wait(&sh.qempty, (item - 1) & 1));
-      if (!ok) break;
+      if (item > 0) wait(&sh.qempty, (item - 1) & 1);
       const int nq = NQ == 2 && tok + c.tpt < w.s.qlen ? 2 : 1;
       if (lane == 0) {
         mbar_arrive_expect_tx(&sh.qfull, nq * c.tpt * c.a.group * HD * 2);
@@ -403,7 +400,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
             tma_load_3d(q_sm + q * C::kQTile + d * (kChunkRows * 128), &qmap, d * 64, w.kvh * c.a.group,
                         w.s.q0 + tok + q * c.tpt, smem_u32(&sh.qfull));
       }
-      for (int i = 0; i < n && ok && !sh.failed; ++i, ++it) {
+      for (int i = 0; i < n; ++i, ++it) {
         const int j = w.r.slice(t + i) * BN + lane * c.box;
         // boxes that no row sees are not fetched (their pages may be gone)
         const bool live = lane < boxes && j < w.r.hi && (j + c.box > w.r.lo || j < c.a.sinks);
@@ -417,9 +414,8 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         const uint32_t stage = it % ST, ph = (it / ST) & 1;
         for (int kv = 0; kv < 2; ++kv) {
           uint64_t* full = kv ? &sh.vfull[stage] : &sh.kfull[stage];
-          uint64_t* empty = kv ? &sh.vempty[stage] : &sh.kempty[stage];
-          if (it >= ST) ok = __all_sync(0xffffffffu, wait(empty, ph ^ 1));
-          if (!ok) break;
+          if (it >= ST) wait(kv ? &sh.vempty[stage] : &sh.kempty[stage], ph ^ 1);
+          __syncwarp();
           if (lane == 0) mbar_arrive_expect_tx(full, n_live * c.box * HD * 2);
           __syncwarp();
           if (live) {
@@ -452,7 +448,6 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
       uint32_t it = 0, item = 0, pph[NQ][C::kSB] = {};
       int64_t u = u0;
       int t = first_tile;
-      bool ok = true;
       auto qk = [&](int q, int buf, uint32_t k) {
         const uint32_t ks = k_sm + (k % ST) * C::kKV, qs = q_sm + q * C::kQTile;
 #pragma unroll
@@ -465,32 +460,33 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         const uint32_t vs = v_sm + (k % ST) * C::kKV;
 #pragma unroll
         for (int j = 0; j < BN / 16; ++j)
-          umma_bf16_ts(tmem + C::kOCol + q * HD, tmem + C::kSCol + (q + buf) * BN + 8 * j,
+          umma_bf16_ts(tmem + C::kOCol + q * HD,
+                       tmem + C::kSCol + (q + buf) * BN + j / (C::kHalf / 16) * C::kHalf + j % (C::kHalf / 16) * 8,
                        umma_desc_mn_sw128(vs + j * 2048, BN * 128), o_idesc, acc || j != 0);
       };
-      while (ok && u < u1 && !sh.failed) {
+      while (u < u1) {
         const int n = static_cast<int>(min(static_cast<int64_t>(w.r.count() - t), u1 - u));
         const int nq = NQ == 2 && w.pair * NQ * c.tpt + c.tpt < w.s.qlen ? 2 : 1;
-        ok = wait(&sh.qfull, item & 1) && wait(&sh.kfull[it % ST], (it / ST) & 1);
-        if (!ok) break;
+        wait(&sh.qfull, item & 1);
+        wait(&sh.kfull[it % ST], (it / ST) & 1);
         tc_fence_after();
         for (int q = 0; q < nq; ++q) qk(q, 0, it);
         umma_commit(smem_u32(&sh.kempty[it % ST]));
         if (n == 1) umma_commit(smem_u32(&sh.qempty));
-        for (int i = 0; i < n && ok; ++i) {
+        for (int i = 0; i < n; ++i) {
           const uint32_t k = it + i;
           const bool more = i + 1 < n;
           if (NQ == 1 && more) {  // the next scores before this tile's P V
-            if (!(ok = wait(&sh.kfull[(k + 1) % ST], ((k + 1) / ST) & 1))) break;
+            wait(&sh.kfull[(k + 1) % ST], ((k + 1) / ST) & 1);
             tc_fence_after();
             qk(0, (i + 1) & 1, k + 1);
             umma_commit(smem_u32(&sh.kempty[(k + 1) % ST]));
             if (i + 2 == n) umma_commit(smem_u32(&sh.qempty));
           }
-          for (int q = 0; q < nq && ok; ++q) {
+          for (int q = 0; q < nq; ++q) {
             const int buf = C::kSB == 2 ? i & 1 : 0;
-            ok = wait(&sh.pfull[q][buf], pph[q][buf] & 1) && (q > 0 || wait(&sh.vfull[k % ST], (k / ST) & 1));
-            if (!ok) break;
+            wait(&sh.pfull[q][buf], pph[q][buf] & 1);
+            if (q == 0) wait(&sh.vfull[k % ST], (k / ST) & 1);
             ++pph[q][buf];
             tc_fence_after();
             pv(q, buf, k, i > 0);
@@ -498,7 +494,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
             if (q == nq - 1) umma_commit(smem_u32(&sh.vempty[k % ST]));
             if (!more) umma_commit(smem_u32(&sh.odone[q]));
             if (NQ == 2 && more) {
-              if (q == 0 && !(ok = wait(&sh.kfull[(k + 1) % ST], ((k + 1) / ST) & 1))) break;
+              if (q == 0) wait(&sh.kfull[(k + 1) % ST], ((k + 1) / ST) & 1);
               tc_fence_after();
               qk(q, 0, k + 1);
               if (q == nq - 1) {
@@ -516,16 +512,17 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
       }
     }
   } else {
-    // ---- softmax: thread = row of query tile q
-    const int q = warp >> 2, row = (warp & 3) * 32 + lane;
+    // ---- softmax: a thread has half of the columns of a row of query tile q
+    constexpr int HB = C::kHalf;
+    const int q = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
     const uint32_t lane_addr = tmem + (((warp & 3) * 32) << 16);
-    const uint32_t o_addr = lane_addr + C::kOCol + q * HD;
+    const uint32_t o_addr = lane_addr + C::kOCol + q * HD + half * (HD / 2);
     const float scale = c.a.scale_log2;
+    auto both_halves = [&] { asm volatile("bar.sync %0, 256;" ::"r"(1 + q) : "memory"); };
     uint32_t sph = 0, oph = 0, it = 0, item = 0;  // S tiles seen, items stored, tiles and items of the run
     int64_t u = u0;
     int t = first_tile;
-    bool ok = true;
-    while (ok && u < u1 && !sh.failed) {
+    while (u < u1) {
       const int n = static_cast<int>(min(static_cast<int64_t>(w.r.count() - t), u1 - u));
       const int tok0 = (w.pair * NQ + q) * c.tpt, tok = tok0 + row / c.a.group;
       const bool active = q == 0 || tok0 < w.s.qlen;
@@ -537,7 +534,8 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
       for (int i = 0; active && i < n; ++i) {
         const int j0 = w.r.slice(t + i) * BN;
         const uint32_t buf = C::kSB == 2 ? (i & 1) : 0, k = it + i;
-        if (!(ok = __all_sync(0xffffffffu, wait(&sh.sfull[q][buf], C::kSB == 2 ? (sph >> buf) & 1 : sph & 1)))) break;
+        wait(&sh.sfull[q][buf], C::kSB == 2 ? (sph >> buf) & 1 : sph & 1);
+        __syncwarp();
         if (C::kSB == 2) sph ^= 1u << buf;
         else ++sph;
         tc_fence_after();
@@ -545,10 +543,10 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         // rows no one sees and the values that are not finite (the rows that
         // see those take them in the end).
         if (q == 0 && !sees_all(c.a, w, j0)) {
-          if (!(ok = __all_sync(0xffffffffu, wait(&sh.vfull[k % ST], (k / ST) & 1)))) break;
+          wait(&sh.vfull[k % ST], (k / ST) & 1);
           const uint32_t vs = v_sm + (k % ST) * C::kKV;
           bool odd = false;
-          for (int e = row; e < BN * (HD / 8); e += kChunkRows) {
+          for (int e = half * kChunkRows + row; e < BN * (HD / 8); e += 2 * kChunkRows) {
             const int r = e % BN, ch = e / BN, j = j0 + r;
             const uint32_t at = vs + (ch / 8) * (BN * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4);
             uint4 x = make_uint4(0, 0, 0, 0);
@@ -568,30 +566,28 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
           }
           if (odd) sh.odd[item & 1] = item + 1;
           fence_proxy_async_smem();
+          __syncwarp();
         }
-        // The scores, 32 at a time: the upper half first, so that the lower half
-        // is still in registers when its p (which overwrite it) are due.
-        const uint32_t s_addr = lane_addr + C::kSCol + (q + buf) * BN;
+        // The scores, 32 at a time: the upper ones first, so that the lower are
+        // still in registers when their p (which overwrite them) are due.
+        const uint32_t s_addr = lane_addr + C::kSCol + (q + buf) * BN + half * HB;
         const bool whole = j0 + BN - 1 <= pmin && (c.a.window == 0 || j0 > pmax - c.a.window || j0 + BN <= c.a.sinks);
-        const int hi = pos - j0, lo = c.a.window ? pos - c.a.window - j0 : -BN - 1, sk = c.a.window ? c.a.sinks - j0 : 0;
+        const int jh = j0 + half * HB, hi = pos - jh;
+        const int lo = c.a.window ? pos - c.a.window - jh : -BN - 1, sk = c.a.window ? c.a.sinks - jh : 0;
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        uint32_t sa[32], sb[32];
+        uint32_t sa[32];
 #pragma unroll
-        for (int half = BN / 64 - 1; half >= 0; --half) {
-          tmem_ld32(s_addr + 64 * half, sa);
-          tmem_ld32(s_addr + 64 * half + 32, sb);
+        for (int part = HB / 32 - 1; part >= 0; --part) {
+          tmem_ld32(s_addr + 32 * part, sa);
           tmem_wait_ld();
-          if (!whole) {
-            mask32(sa, hi - 64 * half, lo - 64 * half, sk - 64 * half);
-            mask32(sb, hi - 64 * half - 32, lo - 64 * half - 32, sk - 64 * half - 32);
-          }
+          if (!whole) mask32(sa, hi - 32 * part, lo - 32 * part, sk - 32 * part);
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            mx[e / 2 & 1] = max3(mx[e / 2 & 1], __uint_as_float(sa[e]), __uint_as_float(sa[e + 1]));
-            mx[2 + (e / 2 & 1)] = max3(mx[2 + (e / 2 & 1)], __uint_as_float(sb[e]), __uint_as_float(sb[e + 1]));
-          }
+          for (int e = 0; e < 32; e += 2) mx[e / 2 & 3] = max3(mx[e / 2 & 3], __uint_as_float(sa[e]), __uint_as_float(sa[e + 1]));
         }
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+        const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        sh.mx[q][i & 1][half][row] = mine;
+        both_halves();
+        const float mt = fmaxf(mine, sh.mx[q][i & 1][half ^ 1][row]) * scale;
         const bool move = mt > m + 8.f;  // also from -inf
         if (__any_sync(0xffffffffu, move)) {
           const float f = move ? (m == -INFINITY ? 0.f : exp2_fast(m - mt)) : 1.f;
@@ -599,17 +595,18 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
           l *= f;
           if (i > 0) {
             if (NQ == 1) {  // O must hold the last product (with two tiles S's arrival says so)
-              if (!(ok = __all_sync(0xffffffffu, wait(&sh.pvdone, (it + i - 1) & 1)))) break;
+              wait(&sh.pvdone, (it + i - 1) & 1);
+              __syncwarp();
               tc_fence_after();
             }
-#pragma unroll
-            for (int e = 0; e < HD / 32; ++e) {
-              uint32_t o[32];
-              tmem_ld32(o_addr + 32 * e, o);
+#pragma unroll 1
+            for (int e = 0; e < HD / 2; e += 16) {
+              uint32_t o[16];
+              tmem_ld16u(o_addr + e, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-              tmem_st32(o_addr + 32 * e, o);
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st16(o_addr + e, o);
             }
           }
         }
@@ -618,20 +615,12 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         uint64_t sum[2] = {};
         probs32(sa, scale2, sub2, sum);
         tmem_st16(s_addr, sa);
-        if constexpr (BN == 128) tmem_ld32(s_addr + 64, sa);
-        probs32(sb, scale2, sub2, sum);
-        tmem_st16(s_addr + 16, sb);
-        if constexpr (BN == 128) {
-          tmem_ld32(s_addr + 96, sb);
+        if constexpr (HB == 64) {
+          tmem_ld32(s_addr + 32, sa);
           tmem_wait_ld();
-          if (!whole) {
-            mask32(sa, hi - 64, lo - 64, sk - 64);
-            mask32(sb, hi - 96, lo - 96, sk - 96);
-          }
+          if (!whole) mask32(sa, hi - 32, lo - 32, sk - 32);
           probs32(sa, scale2, sub2, sum);
-          tmem_st16(s_addr + 32, sa);
-          probs32(sb, scale2, sub2, sum);
-          tmem_st16(s_addr + 48, sb);
+          tmem_st16(s_addr + 16, sa);
         }
         const uint64_t sums = add_f2(sum[0], sum[1]);
         l += lo_f2(sums) + hi_f2(sums);
@@ -640,43 +629,46 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.pfull[q][buf]);
       }
-      if (!ok) break;
-      // ---- the item's rows (or this CTA's part of them)
+      // ---- the item's rows (or this CTA's part of them): half of the dims each
       if (active) {
-        if (!(ok = __all_sync(0xffffffffu, wait(&sh.odone[q], oph & 1)))) break;
+        wait(&sh.odone[q], oph & 1);
         ++oph;
+        sh.lx[q][half][row] = l;
+        both_halves();
+        l = sh.lx[q][0][row] + sh.lx[q][1][row];
         tc_fence_after();
         const bool part = t > 0 || n < w.r.count();
         const int head = w.kvh * c.a.group + row % c.a.group;
-        uint16_t* dst = c.a.out + static_cast<int64_t>(w.s.q0 + tok) * c.a.o_tok + head * c.a.o_head;
+        uint16_t* dst = c.a.out + static_cast<int64_t>(w.s.q0 + tok) * c.a.o_tok + head * c.a.o_head + half * (HD / 2);
         float* pd = c.parts + ((static_cast<int64_t>(blockIdx.x) * 2 + (t > 0 ? 0 : 1)) * NQ * kChunkRows + q * kChunkRows +
                                row) * (HD + 2);
-        {
-          const float inv = m == -INFINITY ? 0.f : 1.f / l;  // a row that sees nothing gives zeros
-          if (part && real) pd[0] = m, pd[1] = l;
+        const bool odd = sh.odd[item & 1] == item + 1;
+        const float inv = m == -INFINITY ? 0.f : 1.f / l;  // a row that sees nothing gives zeros
+        if (part && real && half == 0) pd[0] = m, pd[1] = l;
+        pd += 2 + half * (HD / 2);
 #pragma unroll 1
-          for (int e = 0; e < HD / 32; ++e) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + 32 * e, o);
-            tmem_wait_ld();
-            if (sh.odd[item & 1] == item + 1) add_odd<HD>(c, w, t, t + n, pos, 32 * e, o);
-            if (real && part) {
+        for (int e = 0; e < HD / 2; e += 32) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld32(o_addr + e, o);
+          tmem_wait_ld();
+          if (odd) add_odd<HD>(c, w, t, t + n, pos, half * (HD / 2) + e, o);
+          if (real && part) {
 #pragma unroll
-              for (int x = 0; x < 32; x += 2)
-                *reinterpret_cast<float2*>(pd + 2 + 32 * e + x) = make_float2(__uint_as_float(o[x]), __uint_as_float(o[x + 1]));
-            } else if (real) {
+            for (int x = 0; x < 32; x += 2)
+              *reinterpret_cast<float2*>(pd + e + x) = make_float2(__uint_as_float(o[x]), __uint_as_float(o[x + 1]));
+          } else if (real) {
 #pragma unroll
-              for (int x = 0; x < 32; x += 8) {
-                uint32_t p[4];
+            for (int x = 0; x < 32; x += 8) {
+              uint32_t p[4];
 #pragma unroll
-                for (int y = 0; y < 4; ++y)
-                  p[y] = pack_bf2_rn(__uint_as_float(o[x + 2 * y]) * inv, __uint_as_float(o[x + 2 * y + 1]) * inv);
-                *reinterpret_cast<uint4*>(dst + 32 * e + x) = make_uint4(p[0], p[1], p[2], p[3]);
-              }
+              for (int y = 0; y < 4; ++y)
+                p[y] = pack_bf2_rn(__uint_as_float(o[x + 2 * y]) * inv, __uint_as_float(o[x + 2 * y + 1]) * inv);
+              *reinterpret_cast<uint4*>(dst + e + x) = make_uint4(p[0], p[1], p[2], p[3]);
             }
-            __syncwarp();
           }
         }
+        __syncwarp();
         tc_fence_before();
       }
       it += n;
