@@ -126,6 +126,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -441,75 +447,103 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     }
     if (item > 0) mbar_wait_bounded_s(smem_u32(&sh.qfull), (item - 1) & 1);
   } else if (warp == C::kSoftWarps + 1) {
-    // ---- tensor-core issue (one thread)
-    if (lane == 0) {
-      const uint32_t s_idesc = umma_idesc_bf16_f32(kChunkRows, BN);
-      const uint32_t o_idesc = umma_idesc_bf16_f32(kChunkRows, HD) | (1u << 16);  // B's N index contiguous
-      uint32_t it = 0, item = 0, pph[NQ][C::kSB] = {};
-      int64_t u = u0;
-      int t = first_tile;
-      auto qk = [&](int q, int buf, uint32_t k) {
-        const uint32_t ks = k_sm + (k % ST) * C::kKV, qs = q_sm + q * C::kQTile;
+    // ---- tensor-core issue.  The whole warp walks the run and one lane
+    // issues: addresses and counters stay warp-uniform (scalar registers); with
+    // one lane in the loop every operand would be moved there one by one, 95
+    // cycles an instruction against the 64 it takes.
+    const bool leader = elect_one();
+    const uint32_t s_idesc = umma_idesc_bf16_f32(kChunkRows, BN);
+    const uint32_t o_idesc = umma_idesc_bf16_f32(kChunkRows, HD) | (1u << 16);  // B's N index contiguous
+    // stage of K (and of V), phases
+    uint32_t ks = 0, kph = 0, vs = 0, vph = 0, item = 0, pph = 0;
+    int64_t u = u0;
+    int t = first_tile;
+    auto qk = [&](int q, int buf) {
+      const uint64_t kd = umma_desc_sw128(k_sm + ks * C::kKV), qd = umma_desc_sw128(q_sm + q * C::kQTile);
+      const uint32_t d_addr = tmem + C::kSCol + (q + buf) * BN;
+      if (leader) {
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d)
-          umma_bf16(tmem + C::kSCol + (q + buf) * BN, umma_desc_sw128(qs + (d / 4) * (kChunkRows * 128)) + 2 * (d % 4),
-                    umma_desc_sw128(ks + (d / 4) * (BN * 128)) + 2 * (d % 4), s_idesc, d != 0);
+          umma_bf16(d_addr, qd + (d / 4) * (kChunkRows * 8) + 2 * (d % 4), kd + (d / 4) * (BN * 8) + 2 * (d % 4), s_idesc, d != 0);
         umma_commit(smem_u32(&sh.sfull[q][buf]));
-      };
-      auto pv = [&](int q, int buf, uint32_t k, bool acc) {
-        const uint32_t vs = v_sm + (k % ST) * C::kKV;
+      }
+      __syncwarp();
+    };
+    auto pv = [&](int q, int buf, bool acc) {
+      const uint64_t vd = umma_desc_mn_sw128(v_sm + vs * C::kKV, BN * 128);
+      const uint32_t d_addr = tmem + C::kOCol + q * HD, p_addr = tmem + C::kSCol + (q + buf) * BN;
+      if (leader) {
 #pragma unroll
         for (int j = 0; j < BN / 16; ++j)
-          umma_bf16_ts(tmem + C::kOCol + q * HD,
-                       tmem + C::kSCol + (q + buf) * BN + j / (C::kHalf / 16) * C::kHalf + j % (C::kHalf / 16) * 8,
-                       umma_desc_mn_sw128(vs + j * 2048, BN * 128), o_idesc, acc || j != 0);
-      };
-      while (u < u1) {
-        const int n = static_cast<int>(min(static_cast<int64_t>(w.r.count() - t), u1 - u));
-        const int nq = NQ == 2 && w.pair * NQ * c.tpt + c.tpt < w.s.qlen ? 2 : 1;
-        wait(&sh.qfull, item & 1);
-        wait(&sh.kfull[it % ST], (it / ST) & 1);
-        tc_fence_after();
-        for (int q = 0; q < nq; ++q) qk(q, 0, it);
-        umma_commit(smem_u32(&sh.kempty[it % ST]));
-        if (n == 1) umma_commit(smem_u32(&sh.qempty));
-        for (int i = 0; i < n; ++i) {
-          const uint32_t k = it + i;
-          const bool more = i + 1 < n;
-          if (NQ == 1 && more) {  // the next scores before this tile's P V
-            wait(&sh.kfull[(k + 1) % ST], ((k + 1) / ST) & 1);
+          umma_bf16_ts(d_addr, p_addr + j / (C::kHalf / 16) * C::kHalf + j % (C::kHalf / 16) * 8, vd + j * 128, o_idesc,
+                       acc || j != 0);
+      }
+      __syncwarp();
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (leader) umma_commit(smem_u32(bar));
+      __syncwarp();
+    };
+    auto next_k = [&] {
+      commit(&sh.kempty[ks]);
+      if (++ks == ST) ks = 0, kph ^= 1;
+    };
+    int items = 0;  // of the run: a first walk, so that the loop below is uniform
+    for (Walk<HD> w2 = w; u < u1; t = 0) {
+      u += min(static_cast<int64_t>(w2.r.count() - t), u1 - u);
+      ++items;
+      if (u < u1) w2.next(c);
+    }
+    u = u0;
+    t = first_tile;
+    items = __shfl_sync(0xffffffffu, items, 0);
+    for (int it = 0; it < items; ++it) {
+      const int n = __shfl_sync(0xffffffffu, static_cast<int>(min(static_cast<int64_t>(w.r.count() - t), u1 - u)), 0);
+      const int nq = NQ == 1 ? 1 : __shfl_sync(0xffffffffu, w.pair * NQ * c.tpt + c.tpt < w.s.qlen ? 2 : 1, 0);
+      wait(&sh.qfull, item & 1);
+      wait(&sh.kfull[ks], kph);
+      tc_fence_after();
+      qk(0, 0);
+      if (nq == 2) qk(NQ - 1, 0);
+      next_k();
+      if (n == 1) commit(&sh.qempty);
+      for (int i = 0; i < n; ++i) {
+        const bool more = i + 1 < n;
+        if (NQ == 1 && more) {  // the next scores before this tile's P V
+          wait(&sh.kfull[ks], kph);
+          tc_fence_after();
+          qk(0, (i + 1) & 1);
+          next_k();
+          if (i + 2 == n) commit(&sh.qempty);
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          if (q >= nq) break;
+          const int buf = C::kSB == 2 ? i & 1 : 0;
+          wait(&sh.pfull[q][buf], pph >> (2 * q + buf) & 1);
+          if (q == 0) wait(&sh.vfull[vs], vph);
+          pph ^= 1u << (2 * q + buf);
+          tc_fence_after();
+          pv(q, buf, i > 0);
+          if (NQ == 1) commit(&sh.pvdone);
+          if (!more) commit(&sh.odone[q]);
+          if (NQ == 2 && more) {
+            if (q == 0) wait(&sh.kfull[ks], kph);
             tc_fence_after();
-            qk(0, (i + 1) & 1, k + 1);
-            umma_commit(smem_u32(&sh.kempty[(k + 1) % ST]));
-            if (i + 2 == n) umma_commit(smem_u32(&sh.qempty));
-          }
-          for (int q = 0; q < nq; ++q) {
-            const int buf = C::kSB == 2 ? i & 1 : 0;
-            wait(&sh.pfull[q][buf], pph[q][buf] & 1);
-            if (q == 0) wait(&sh.vfull[k % ST], (k / ST) & 1);
-            ++pph[q][buf];
-            tc_fence_after();
-            pv(q, buf, k, i > 0);
-            if (NQ == 1) umma_commit(smem_u32(&sh.pvdone));
-            if (q == nq - 1) umma_commit(smem_u32(&sh.vempty[k % ST]));
-            if (!more) umma_commit(smem_u32(&sh.odone[q]));
-            if (NQ == 2 && more) {
-              if (q == 0) wait(&sh.kfull[(k + 1) % ST], ((k + 1) / ST) & 1);
-              tc_fence_after();
-              qk(q, 0, k + 1);
-              if (q == nq - 1) {
-                umma_commit(smem_u32(&sh.kempty[(k + 1) % ST]));
-                if (i + 2 == n) umma_commit(smem_u32(&sh.qempty));
-              }
-            }
+            qk(q, 0);
           }
         }
-        it += n;
-        u += n;
-        t = 0;
-        ++item;
-        if (u < u1) w.next(c);
+        commit(&sh.vempty[vs]);
+        if (++vs == ST) vs = 0, vph ^= 1;
+        if (NQ == 2 && more) {
+          next_k();
+          if (i + 2 == n) commit(&sh.qempty);
+        }
       }
+      u += n;
+      t = 0;
+      ++item;
+      if (u < u1) w.next(c);
     }
   } else {
     // ---- softmax: a thread has half of the columns of a row of query tile q
