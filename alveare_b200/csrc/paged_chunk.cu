@@ -162,14 +162,40 @@ __device__ __forceinline__ void mask32(uint32_t (&s)[32], int hi, int lo, int si
   for (int e = 0; e < 32; ++e)
     if (!(e <= hi && (e > lo || e < sinks))) s[e] = 0xFF800000u;
 }
-// p = 2^(s scale - m) of 32 scores, added to the sums, as 16 packed bf16 pairs in s[0 .. 16).
+// 2^x of two values x >= -126 on the FMA pipe: x = n + f with n the nearest
+// integer (the low bits of x + 1.5 2^23), 2^f by the cubic of least relative
+// error on [-1/2, 1/2] (7.5e-5: a fiftieth of p's rounding to bf16), n added to
+// the exponent.
+__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
+  const uint64_t magic = pack_f2(12582912.f, 12582912.f), minus_magic = pack_f2(-12582912.f, -12582912.f);
+  const uint64_t r = add_f2(x, magic);
+  const uint64_t f = fma_f2(add_f2(r, minus_magic), pack_f2(-1.f, -1.f), x);
+  uint64_t p = fma_f2(pack_f2(0.05517167f, 0.05517167f), f, pack_f2(0.24261113f, 0.24261113f));
+  p = fma_f2(p, f, pack_f2(0.69326097f, 0.69326097f));
+  p = fma_f2(p, f, pack_f2(0.99992806f, 0.99992806f));
+  const uint32_t lo = static_cast<uint32_t>(p) + (static_cast<uint32_t>(r) << 23);
+  const uint32_t hi = static_cast<uint32_t>(p >> 32) + (static_cast<uint32_t>(r >> 32) << 23);
+  return static_cast<uint64_t>(lo) | static_cast<uint64_t>(hi) << 32;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+// p = 2^(s scale - m) of 32 scores, added to the sums, as 16 packed bf16 pairs
+// in s[0 .. 16).  Where every score counts (POLY) a quarter of the
+// exponentials goes to the FMA pipe: the special-function unit's 16 a cycle
+// are as scarce as the tensor cores' cycles.
+template <bool POLY>
 __device__ __forceinline__ void probs32(uint32_t (&s)[32], uint64_t scale2, uint64_t sub2, uint64_t (&sum)[2]) {
 #pragma unroll
   for (int e = 0; e < 32; e += 2) {
     const uint64_t x = fma_f2(pack_f2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, sub2);
-    const float p0 = exp2_fast(lo_f2(x)), p1 = exp2_fast(hi_f2(x));
-    sum[e / 2 & 1] = add_f2(sum[e / 2 & 1], pack_f2(p0, p1));
-    s[e / 2] = pack_bf2_rn(p0, p1);
+    uint64_t p;
+    if (POLY && e % 8 == 6) p = exp2_poly2(pack_f2(max_nan(lo_f2(x), -126.f), max_nan(hi_f2(x), -126.f)));
+    else p = pack_f2(exp2_fast(lo_f2(x)), exp2_fast(hi_f2(x)));
+    sum[e / 2 & 1] = add_f2(sum[e / 2 & 1], p);
+    s[e / 2] = pack_bf2_rn(lo_f2(p), hi_f2(p));
   }
 }
 
@@ -230,6 +256,7 @@ struct ChunkShared {
   volatile uint32_t failed;  // a wait gave up: report, wait no more, run to the end
   float mx[C::kNQ][2][2][kChunkRows];  // a row's maximum over each half, two tiles deep
   float lx[C::kNQ][2][kChunkRows];
+  Walk<HD> walk[C::kSoftWarps];  // each softmax warp's place (its registers hold scores)
   // odd[i & 1] = i + 1: item i of the run has v values that are not finite in
   // a tile that only some rows see whole (a warpgroup with work in an item is
   // at most one item ahead of the other)
@@ -554,19 +581,23 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     const float scale = c.a.scale_log2;
     auto both_halves = [&] { asm volatile("bar.sync %0, 256;" ::"r"(1 + q) : "memory"); };
     uint32_t sph = 0, oph = 0, it = 0, item = 0;  // S tiles seen, items stored, tiles and items of the run
+    Walk<HD>& sw = sh.walk[warp];
+    if (lane == 0) sw = w;
+    __syncwarp();
     int64_t u = u0;
     int t = first_tile;
     while (u < u1) {
-      const int n = static_cast<int>(min(static_cast<int64_t>(w.r.count() - t), u1 - u));
-      const int tok0 = (w.pair * NQ + q) * c.tpt, tok = tok0 + row / c.a.group;
-      const bool active = q == 0 || tok0 < w.s.qlen;
-      const bool real = row < c.tpt * c.a.group && tok < w.s.qlen;
-      const int pfirst = w.s.kv - w.s.qlen;
+      const int n = static_cast<int>(min(static_cast<int64_t>(sw.r.count() - t), u1 - u));
+      const int tok0 = (sw.pair * NQ + q) * c.tpt, tok = tok0 + row / c.a.group;
+      const bool active = q == 0 || tok0 < sw.s.qlen;
+      const bool real = row < c.tpt * c.a.group && tok < sw.s.qlen;
+      const int pfirst = sw.s.kv - sw.s.qlen;
       const int pos = real ? pfirst + tok : -1;
-      const int pmin = pfirst + tok0, pmax = min(pmin + c.tpt, w.s.kv) - 1;
+      // every row of the item sees the whole tile at j0: j0 <= all_hi and (j0 > all_lo or j0 <= all_sink)
+      const int all_hi = sw.p0 - BN + 1, all_lo = c.a.window ? sw.p1 - c.a.window : -1, all_sink = c.a.sinks - BN;
       float m = -INFINITY, l = 0.f;
       for (int i = 0; active && i < n; ++i) {
-        const int j0 = w.r.slice(t + i) * BN;
+        const int j0 = sw.r.slice(t + i) * BN;
         const uint32_t buf = C::kSB == 2 ? (i & 1) : 0, k = it + i;
         wait(&sh.sfull[q][buf], C::kSB == 2 ? (sph >> buf) & 1 : sph & 1);
         __syncwarp();
@@ -576,7 +607,8 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         // A row's p is 0 where it does not see, but 0 * inf is not: zero the v
         // rows no one sees and the values that are not finite (the rows that
         // see those take them in the end).
-        if (q == 0 && !sees_all(c.a, w, j0)) {
+        const bool whole = j0 <= all_hi && (j0 > all_lo || j0 <= all_sink);
+        if (q == 0 && !whole) {
           wait(&sh.vfull[k % ST], (k / ST) & 1);
           const uint32_t vs = v_sm + (k % ST) * C::kKV;
           bool odd = false;
@@ -584,7 +616,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
             const int r = e % BN, ch = e / BN, j = j0 + r;
             const uint32_t at = vs + (ch / 8) * (BN * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4);
             uint4 x = make_uint4(0, 0, 0, 0);
-            if (j < w.r.hi && (j >= w.r.lo || j < c.a.sinks)) {
+            if (j < sw.r.hi && (j >= sw.r.lo || j < c.a.sinks)) {
               x = lds128_at<0>(at);
               uint32_t* const xs[4] = {&x.x, &x.y, &x.z, &x.w};
               bool here = false;
@@ -602,21 +634,22 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
           fence_proxy_async_smem();
           __syncwarp();
         }
-        // The scores, 32 at a time: the upper ones first, so that the lower are
-        // still in registers when their p (which overwrite them) are due.
         const uint32_t s_addr = lane_addr + C::kSCol + (q + buf) * BN + half * HB;
-        const bool whole = j0 + BN - 1 <= pmin && (c.a.window == 0 || j0 > pmax - c.a.window || j0 + BN <= c.a.sinks);
-        const int jh = j0 + half * HB, hi = pos - jh;
-        const int lo = c.a.window ? pos - c.a.window - jh : -BN - 1, sk = c.a.window ? c.a.sinks - jh : 0;
+        uint32_t sa[32], sb[32];
+        tmem_ld32(s_addr, sa);
+        if constexpr (HB == 64) tmem_ld32(s_addr + 32, sb);
+        tmem_wait_ld();
+        if (!whole) {
+          const int jh = j0 + half * HB, hi = pos - jh;
+          const int lo = c.a.window ? pos - c.a.window - jh : -BN - 1, sk = c.a.window ? c.a.sinks - jh : 0;
+          mask32(sa, hi, lo, sk);
+          if constexpr (HB == 64) mask32(sb, hi - 32, lo - 32, sk - 32);
+        }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        uint32_t sa[32];
 #pragma unroll
-        for (int part = HB / 32 - 1; part >= 0; --part) {
-          tmem_ld32(s_addr + 32 * part, sa);
-          tmem_wait_ld();
-          if (!whole) mask32(sa, hi - 32 * part, lo - 32 * part, sk - 32 * part);
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) mx[e / 2 & 3] = max3(mx[e / 2 & 3], __uint_as_float(sa[e]), __uint_as_float(sa[e + 1]));
+        for (int e = 0; e < 32; e += 2) {
+          mx[e / 2 & 1] = max3(mx[e / 2 & 1], __uint_as_float(sa[e]), __uint_as_float(sa[e + 1]));
+          if constexpr (HB == 64) mx[2 + (e / 2 & 1)] = max3(mx[2 + (e / 2 & 1)], __uint_as_float(sb[e]), __uint_as_float(sb[e + 1]));
         }
         const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         sh.mx[q][i & 1][half][row] = mine;
@@ -647,14 +680,20 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         const float sub = m == -INFINITY ? 0.f : m;
         const uint64_t scale2 = pack_f2(scale, scale), sub2 = pack_f2(-sub, -sub);
         uint64_t sum[2] = {};
-        probs32(sa, scale2, sub2, sum);
-        tmem_st16(s_addr, sa);
-        if constexpr (HB == 64) {
-          tmem_ld32(s_addr + 32, sa);
-          tmem_wait_ld();
-          if (!whole) mask32(sa, hi - 32, lo - 32, sk - 32);
-          probs32(sa, scale2, sub2, sum);
-          tmem_st16(s_addr + 16, sa);
+        if (whole) {
+          probs32<true>(sa, scale2, sub2, sum);
+          tmem_st16(s_addr, sa);
+          if constexpr (HB == 64) {
+            probs32<true>(sb, scale2, sub2, sum);
+            tmem_st16(s_addr + 16, sb);
+          }
+        } else {
+          probs32<false>(sa, scale2, sub2, sum);
+          tmem_st16(s_addr, sa);
+          if constexpr (HB == 64) {
+            probs32<false>(sb, scale2, sub2, sum);
+            tmem_st16(s_addr + 16, sb);
+          }
         }
         const uint64_t sums = add_f2(sum[0], sum[1]);
         l += lo_f2(sums) + hi_f2(sums);
@@ -671,9 +710,9 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         both_halves();
         l = sh.lx[q][0][row] + sh.lx[q][1][row];
         tc_fence_after();
-        const bool part = t > 0 || n < w.r.count();
-        const int head = w.kvh * c.a.group + row % c.a.group;
-        uint16_t* dst = c.a.out + static_cast<int64_t>(w.s.q0 + tok) * c.a.o_tok + head * c.a.o_head + half * (HD / 2);
+        const bool part = t > 0 || n < sw.r.count();
+        const int head = sw.kvh * c.a.group + row % c.a.group;
+        uint16_t* dst = c.a.out + static_cast<int64_t>(sw.s.q0 + tok) * c.a.o_tok + head * c.a.o_head + half * (HD / 2);
         float* pd = c.parts + ((static_cast<int64_t>(blockIdx.x) * 2 + (t > 0 ? 0 : 1)) * NQ * kChunkRows + q * kChunkRows +
                                row) * (HD + 2);
         const bool odd = sh.odd[item & 1] == item + 1;
@@ -686,7 +725,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
           __syncwarp();
           tmem_ld32(o_addr + e, o);
           tmem_wait_ld();
-          if (odd) add_odd<HD>(c, w, t, t + n, pos, half * (HD / 2) + e, o);
+          if (odd) add_odd<HD>(c, sw, t, t + n, pos, half * (HD / 2) + e, o);
           if (real && part) {
 #pragma unroll
             for (int x = 0; x < 32; x += 2)
@@ -709,7 +748,9 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
       u += n;
       t = 0;
       ++item;
-      if (u < u1) w.next(c);
+      __syncwarp();
+      if (lane == 0 && u < u1) sw.next(c);
+      __syncwarp();
     }
   }
   tc_fence_before();
