@@ -545,7 +545,7 @@ extern "C" int alv_paged_attention(alv_ctx* ctx, const alv_paged* cache, const a
   a.row_max = INT_MAX;
   if (static_cast<int64_t>(args->max_q_len) * a.group > kRowsPerBlock && chunk_takes(a)) {
     a.row_max = kRowsPerBlock;
-    if ((rc = launch_chunk(ctx, a, cache->head_dim, kRowsPerBlock + 1, st))) return rc;
+    if ((rc = launch_chunk(ctx, a, cache->head_dim, args->max_q_len, kRowsPerBlock + 1, st))) return rc;
     // all sequences as long as the longest: none is left for the row blocks
     if (static_cast<int64_t>(cache->batch) * args->max_q_len == cache->tokens) return ALV_OK;
   }

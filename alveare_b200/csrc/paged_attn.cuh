@@ -47,7 +47,7 @@ struct AttnArgs {
 // The tensor-core form for chunks (paged_chunk.cu): sequences with at least
 // row_min rows (new tokens x heads of a kv group).
 bool chunk_takes(const AttnArgs& a);
-int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int row_min, cudaStream_t st);
+int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int max_q_len, int row_min, cudaStream_t st);
 
 constexpr int kRowsPerBlock = 16;
 constexpr int kRowWarps = 4;

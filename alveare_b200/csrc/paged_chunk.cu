@@ -18,11 +18,12 @@
 // bf16), so O is rescaled in TMEM on the first few tiles and hardly ever
 // after; rows take p = 2^(s - m) of whatever m they use, and l sums the same.
 //
-// Work: a unit is one BN-position tile of one item (sequence, kv head, query
-// tiles).  The units of all items, in order, are cut into equal runs, one per
-// CTA, so that a short chunk over a long past fills the GPU and ragged batches
-// balance; an item cut between CTAs leaves unnormalised parts (O, m, l) that a
-// second launch joins in a fixed order.
+// Work: the items (sequence, query tiles, kv head), in order, are laid end to
+// end, each as long as its tiles and a few more for what an item costs by
+// itself, and cut into equal runs, one per CTA, so that a short chunk over a
+// long past fills the GPU and ragged batches balance; an item cut between CTAs
+// leaves unnormalised parts (O, m, l) that a second launch joins in a fixed
+// order.
 #include <cuda.h>
 
 #include "gemm_tc.cuh"
@@ -47,7 +48,8 @@ int encode(alv_ctx* ctx, CUtensorMap* map, uint32_t rank, const void* p, const c
 }
 
 constexpr int kChunkRows = 128;
-constexpr int kMinUnits = 4;  // units of a CTA's run at least: a part costs about as much as two tiles
+constexpr int kMinRun = 4;  // a CTA's run at least, in tiles: a part costs about as much as two
+constexpr int kExtra = 2;   // tiles an item counts for its start and end (query tile, first scores, store)
 
 template <int HD>
 struct Chunk {
@@ -60,7 +62,7 @@ struct Chunk {
   static constexpr uint32_t kBytes = kNQ * kQTile + 2 * kStages * kKV + 1024;
   static constexpr int kHalf = kBN / 2;            // columns of S a softmax thread takes
   static constexpr int kSoftWarps = 8 * kNQ;
-  static constexpr int kThreads = (kSoftWarps + 2) * 32;
+  static constexpr int kThreads = (kSoftWarps + 4) * 32;  // + copy, issue and two scan warps
   static constexpr uint32_t kSCol = 0;      // S (and P) of tile q, buffer b: (q + b) * kBN
   static constexpr uint32_t kOCol = 256;    // O of tile q: 256 + q * HD
 };
@@ -72,8 +74,9 @@ struct ChunkArgs {
   int head_first; // cache tensor map order: (hd, head, row, page) instead of (hd, row, head, page)
   int row_min;    // sequences with at least this many rows are this kernel's
   float* parts;   // [2 * grid][kNQ * 128][HD + 2]
-  int4* cuts;     // [grid]: item (b, kvh, pair), units before the cut (x = -1: none)
-  int64_t* total; // [1] units of all items
+  int4* cuts;     // [grid]: item (b, pair, kvh) that the run starts inside, and where (x = -1: none)
+  int64_t* total; // [1] length of all items
+  int max_pairs;  // query-tile pairs of the longest sequence
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -156,11 +159,15 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// Scores of 32 columns that the row does not see -> -inf.
+// The lowest n bits.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1; }
+// Scores of 32 columns that the row does not see (it sees e <= hi with e > lo
+// or e < sinks) -> -inf.
 __device__ __forceinline__ void mask32(uint32_t (&s)[32], int hi, int lo, int sinks) {
+  const uint32_t seen = low_bits(hi + 1) & (~low_bits(lo + 1) | low_bits(sinks));
 #pragma unroll
   for (int e = 0; e < 32; ++e)
-    if (!(e <= hi && (e > lo || e < sinks))) s[e] = 0xFF800000u;
+    if (!(seen & (1u << e))) s[e] = 0xFF800000u;
 }
 // 2^x of two values x >= -126 on the FMA pipe: x = n + f with n the nearest
 // integer (the low bits of x + 1.5 2^23), 2^f by the cubic of least relative
@@ -199,74 +206,103 @@ __device__ __forceinline__ void probs32(uint32_t (&s)[32], uint64_t scale2, uint
   }
 }
 
-// One run of units: items (b, kvh, pair) in order, pair fastest.
+// Items (b, pair, kvh) in order, kv heads fastest.
 template <int HD>
 struct Walk {
   using C = Chunk<HD>;
-  int b, kvh, pair, pairs;
+  int b, pair, kvh, pairs;
   SeqSpan s;
   SliceRange r;      // tiles of the current item
   int p0, p1;        // positions of the item's first and last new token
 
-  __device__ __forceinline__ int pairs_of(const ChunkArgs& c, const SeqSpan& q) const {
-    if (q.qlen <= 0 || static_cast<int64_t>(q.qlen) * c.a.group < c.row_min) return 0;
-    return (q.qlen + C::kNQ * c.tpt - 1) / (C::kNQ * c.tpt);
-  }
-  __device__ __forceinline__ SliceRange range_of(const ChunkArgs& c, const SeqSpan& q, int pr, int* lo, int* hi) const {
-    const int first = q.kv - q.qlen + pr * C::kNQ * c.tpt;
-    const int last = min(first + C::kNQ * c.tpt, q.kv) - 1;
-    *lo = first;
-    *hi = last;
-    SliceRange x = slice_range<C::kBN>(first, last, c.a.window, c.a.sinks);
+  __device__ __forceinline__ void load(const ChunkArgs& c) {
+    p0 = s.kv - s.qlen + pair * C::kNQ * c.tpt;
+    p1 = min(p0 + C::kNQ * c.tpt, s.kv) - 1;
+    r = slice_range<C::kBN>(p0, p1, c.a.window, c.a.sinks);
     // an item that sees nothing still has one (masked) tile: it writes zeros
-    if (x.count() == 0) x.n_main = 1;
-    return x;
+    if (r.count() == 0) r.n_main = 1;
   }
-  // Units of one kv head of sequence q.
-  __device__ __forceinline__ int64_t units_of(const ChunkArgs& c, const SeqSpan& q) const {
-    const int n = pairs_of(c, q);
-    int64_t u = 0;
-    int lo, hi;
-    for (int i = 0; i < n; ++i) u += range_of(c, q, i, &lo, &hi).count();
-    return u;
+  __device__ __forceinline__ int pairs_of(const ChunkArgs& c) const {
+    if (s.qlen <= 0 || static_cast<int64_t>(s.qlen) * c.a.group < c.row_min) return 0;
+    return min((s.qlen + C::kNQ * c.tpt - 1) / (C::kNQ * c.tpt), c.max_pairs);
   }
-  __device__ __forceinline__ void load(const ChunkArgs& c) { r = range_of(c, s, pair, &p0, &p1); }
+  // Sequence and pair number e of batch x max_pairs; false where there is none.
+  __device__ __forceinline__ bool at(const ChunkArgs& c, int64_t e) {
+    b = e <= INT_MAX ? static_cast<int>(static_cast<uint32_t>(e) / static_cast<uint32_t>(c.max_pairs))
+                     : static_cast<int>(e / c.max_pairs);
+    pair = static_cast<int>(e - static_cast<int64_t>(b) * c.max_pairs);
+    kvh = 0;
+    s = seq_span(c.a.c, b);
+    pairs = pairs_of(c);
+    if (pair >= pairs) return false;
+    load(c);
+    return true;
+  }
+  __device__ __forceinline__ int length() const { return r.count() + kExtra; }
   __device__ __forceinline__ void next(const ChunkArgs& c) {
+    if (++kvh < c.a.c.nkv) return;
+    kvh = 0;
     if (++pair == pairs) {
       pair = 0;
-      if (++kvh == c.a.c.nkv) {
-        kvh = 0;
-        do {
-          if (++b >= c.a.c.batch) return;
-          s = seq_span(c.a.c, b);
-          pairs = pairs_of(c, s);
-        } while (pairs == 0);
-      }
+      do {
+        if (++b >= c.a.c.batch) return;
+        s = seq_span(c.a.c, b);
+        pairs = pairs_of(c);
+      } while (pairs == 0);
     }
     load(c);
   }
+  // The next item of the run [u, u1), at place x of the current one, of which
+  // tiles [t, t + n) are this run's; false at the run's end.  After each item
+  // the caller moves on with next() if u < u1.
+  __device__ __forceinline__ bool take(const ChunkArgs& c, int64_t& u, int64_t u1, int& x, int& t, int& n) {
+    while (u < u1) {
+      const int len = length();
+      t = max(0, x - kExtra);
+      n = max(0, static_cast<int>(min(static_cast<int64_t>(len), x + (u1 - u))) - kExtra) - t;
+      u += len - x;
+      x = 0;
+      if (n > 0) return true;
+      if (u < u1) next(c);
+    }
+    return false;
+  }
 };
+// CTAs that get a run, and the run that holds a place: the last c with total * c / g <= place.
+__device__ __forceinline__ int runs_of(int64_t total, int grid) {
+  return static_cast<int>(min((total + kMinRun - 1) / kMinRun, static_cast<int64_t>(grid)));
+}
+__device__ __forceinline__ int run_of(int64_t place, int64_t total, int g) {
+  return static_cast<int>(((place + 1) * g - 1) / total);
+}
 
 template <int HD>
 struct ChunkShared {
   using C = Chunk<HD>;
-  uint64_t kfull[C::kStages], kempty[C::kStages], vfull[C::kStages], vempty[C::kStages];
+  uint64_t kfull[C::kStages], kempty[C::kStages], vfull[C::kStages], vempty[C::kStages], vscan[C::kStages];
   uint64_t qfull, qempty, sfull[C::kNQ][C::kSB], pfull[C::kNQ][C::kSB], odone[C::kNQ], pvdone;
   uint32_t tmem;
   volatile uint32_t failed;  // a wait gave up: report, wait no more, run to the end
   float mx[C::kNQ][2][2][kChunkRows];  // a row's maximum over each half, two tiles deep
   float lx[C::kNQ][2][kChunkRows];
   Walk<HD> walk[C::kSoftWarps];  // each softmax warp's place (its registers hold scores)
-  // odd[i & 1] = i + 1: item i of the run has v values that are not finite in
-  // a tile that only some rows see whole (a warpgroup with work in an item is
-  // at most one item ahead of the other)
-  volatile uint32_t odd[2];
+  // odd[i & 3] = i + 1: item i of the run has v values that are not finite in
+  // a tile that only some rows see whole (the scan is at most kStages items
+  // ahead of an item's store)
+  volatile uint32_t odd[4];
   // the CTA's run
   int64_t sums[C::kThreads / 32 + 1];
-  int64_t u0, u1, total;
-  int start_b;
-  int64_t start_before;  // units before start_b
+  int64_t u0, u1;
+  int64_t start_e;     // batch x pair number the run starts in
+  int64_t start_rest;  // and how far into its kv heads' items
 };
+
+// A CTA's part of a cut item: m, l of the rows of a query tile, then O as
+// [dims / 4][row][4].  Slot 0: the item its run starts inside, 1: the one it
+// ends inside.
+__device__ __forceinline__ float* part_of(const ChunkArgs& c, int cta, int slot, int floats) {
+  return c.parts + (static_cast<int64_t>(cta) * 2 + slot) * floats;
+}
 
 // Whether every row of the item sees the whole tile of positions j0 ...
 template <int HD>
@@ -314,6 +350,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
       mbar_init(&sh.kempty[i], 1);
       mbar_init(&sh.vfull[i], 1);
       mbar_init(&sh.vempty[i], 1);
+      mbar_init(&sh.vscan[i], 2);
     }
     mbar_init(&sh.qfull, 1);
     mbar_init(&sh.qempty, 1);
@@ -328,20 +365,21 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     mbar_init(&sh.pvdone, 1);
     fence_mbar_init();
     sh.failed = 0;
-    sh.odd[0] = sh.odd[1] = 0;
+    sh.odd[0] = sh.odd[1] = sh.odd[2] = sh.odd[3] = 0;
   }
   // query rows past tpt * group are never loaded: keep them zero
   for (uint32_t i = threadIdx.x; i < NQ * C::kQTile / 16; i += C::kThreads)
     *reinterpret_cast<uint4*>(smem_dyn + (base - smem_u32(smem_dyn)) + i * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
 
-  // ---- the CTA's run of units: thread t sums the sequences of its range, a
-  // scan over the threads finds where the run starts
+  // ---- the CTA's run: thread t adds up the lengths of its sequences and
+  // pairs, a scan over the threads finds where the run starts
   Walk<HD> w{};
-  const int per = (c.a.c.batch + C::kThreads - 1) / C::kThreads;
-  const int b0 = threadIdx.x * per, b1 = min(b0 + per, c.a.c.batch);
+  const int64_t n_e = static_cast<int64_t>(c.a.c.batch) * c.max_pairs, per = (n_e + C::kThreads - 1) / C::kThreads;
+  const int64_t e0 = threadIdx.x * per, e1 = min(e0 + per, n_e);
   int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += w.units_of(c, seq_span(c.a.c, b)) * c.a.c.nkv;
+  for (int64_t e = e0; e < e1; ++e)
+    if (w.at(c, e)) mine += static_cast<int64_t>(w.length()) * c.a.c.nkv;
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -349,39 +387,32 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     if (lane >= o) incl += y;
   }
   if (lane == 31) sh.sums[warp] = incl;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int64_t t = 0;
-    for (int i = 0; i < C::kThreads / 32; ++i) {
-      const int64_t x = sh.sums[i];
-      sh.sums[i] = t;
-      t += x;
-    }
-    int64_t g = (t + kMinUnits - 1) / kMinUnits;  // CTAs that get work
-    if (g > gridDim.x) g = gridDim.x;
-    sh.total = t;
-    sh.u0 = blockIdx.x < g ? t * blockIdx.x / g : t;
-    sh.u1 = blockIdx.x < g ? t * (blockIdx.x + 1) / g : t;
-    if (blockIdx.x == 0) *c.total = t;
-  }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   __syncthreads();
-  const int64_t u0 = sh.u0, u1 = sh.u1;
-  const int64_t before = sh.sums[warp] + incl - mine;
+  int64_t before = incl - mine, total = 0;
+  for (int i = 0; i < C::kThreads / 32; ++i) {
+    if (i < warp) before += sh.sums[i];
+    total += sh.sums[i];
+  }
+  const int g = runs_of(total, gridDim.x);
+  const int64_t u0 = static_cast<int>(blockIdx.x) < g ? mul_div(total, blockIdx.x, g) : total;
+  const int64_t u1 = static_cast<int>(blockIdx.x) < g ? mul_div(total, blockIdx.x + 1, g) : total;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *c.total = total;
   if (u0 < u1 && before <= u0 && u0 < before + mine) {  // this thread's range holds the start
     int64_t at = before;
-    for (int b = b0; b < b1; ++b) {
-      const int64_t u = w.units_of(c, seq_span(c.a.c, b)) * c.a.c.nkv;
-      if (u0 < at + u) {
-        sh.start_b = b;
-        sh.start_before = at;
+    for (int64_t e = e0; e < e1; ++e) {
+      if (!w.at(c, e)) continue;
+      const int64_t len = static_cast<int64_t>(w.length()) * c.a.c.nkv;
+      if (u0 < at + len) {
+        sh.start_e = e;
+        sh.start_rest = u0 - at;
         break;
       }
-      at += u;
+      at += len;
     }
   }
   tc_fence_before();
@@ -389,25 +420,16 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
-  int first_tile = 0;
-  if (u0 < u1) {  // locate the start inside its sequence
-    w.b = sh.start_b;
-    w.s = seq_span(c.a.c, w.b);
-    w.pairs = w.pairs_of(c, w.s);
-    const int64_t per_head = w.units_of(c, w.s), off = u0 - sh.start_before;
-    w.kvh = static_cast<int>(off / per_head);
-    int64_t rem = off - w.kvh * per_head;
-    w.pair = 0;
-    w.load(c);
-    while (rem >= w.r.count()) {
-      rem -= w.r.count();
-      ++w.pair;
-      w.load(c);
-    }
-    first_tile = static_cast<int>(rem);
+  int x0 = 0;  // where the run starts inside its first item
+  if (u0 < u1) {
+    w.at(c, sh.start_e);
+    w.kvh = static_cast<int>(sh.start_rest) / w.length();
+    x0 = static_cast<int>(sh.start_rest) - w.kvh * w.length();
   }
   if (threadIdx.x == 0)
-    c.cuts[blockIdx.x] = first_tile > 0 ? make_int4(w.b, w.kvh, w.pair, first_tile) : make_int4(-1, 0, 0, 0);
+    c.cuts[blockIdx.x] = x0 > kExtra ? make_int4(w.b, w.pair, w.kvh, x0) : make_int4(-1, 0, 0, 0);
+  int64_t u = u0;
+  int x = x0, t = 0, n = 0;
 
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (sh.failed || mbar_wait_bounded_s(smem_u32(bar), parity)) return;
@@ -419,10 +441,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     // ---- copies: lane i fetches box i of a tile's k and v
     const int boxes = BN / c.box;
     uint32_t it = 0, item = 0;
-    int64_t u = u0;
-    int t = first_tile;
-    while (u < u1) {
-      const int n = static_cast<int>(min(static_cast<int64_t>(w.r.count() - t), u1 - u));
+    while (w.take(c, u, u1, x, t, n)) {
       const int tok = w.pair * NQ * c.tpt;
       if (item > 0) wait(&sh.qempty, (item - 1) & 1);
       const int nq = NQ == 2 && tok + c.tpt < w.s.qlen ? 2 : 1;
@@ -462,8 +481,6 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
           __syncwarp();
         }
       }
-      u += n;
-      t = 0;
       ++item;
       if (u < u1) w.next(c);
     }
@@ -483,8 +500,6 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     const uint32_t o_idesc = umma_idesc_bf16_f32(kChunkRows, HD) | (1u << 16);  // B's N index contiguous
     // stage of K (and of V), phases
     uint32_t ks = 0, kph = 0, vs = 0, vph = 0, item = 0, pph = 0;
-    int64_t u = u0;
-    int t = first_tile;
     auto qk = [&](int q, int buf) {
       const uint64_t kd = umma_desc_sw128(k_sm + ks * C::kKV), qd = umma_desc_sw128(q_sm + q * C::kQTile);
       const uint32_t d_addr = tmem + C::kSCol + (q + buf) * BN;
@@ -516,16 +531,16 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
       if (++ks == ST) ks = 0, kph ^= 1;
     };
     int items = 0;  // of the run: a first walk, so that the loop below is uniform
-    for (Walk<HD> w2 = w; u < u1; t = 0) {
-      u += min(static_cast<int64_t>(w2.r.count() - t), u1 - u);
+    for (Walk<HD> w2 = w; w2.take(c, u, u1, x, t, n);) {
       ++items;
       if (u < u1) w2.next(c);
     }
     u = u0;
-    t = first_tile;
+    x = x0;
     items = __shfl_sync(0xffffffffu, items, 0);
     for (int it = 0; it < items; ++it) {
-      const int n = __shfl_sync(0xffffffffu, static_cast<int>(min(static_cast<int64_t>(w.r.count() - t), u1 - u)), 0);
+      w.take(c, u, u1, x, t, n);
+      n = __shfl_sync(0xffffffffu, n, 0);
       const int nq = NQ == 1 ? 1 : __shfl_sync(0xffffffffu, w.pair * NQ * c.tpt + c.tpt < w.s.qlen ? 2 : 1, 0);
       wait(&sh.qfull, item & 1);
       wait(&sh.kfull[ks], kph);
@@ -548,7 +563,10 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
           if (q >= nq) break;
           const int buf = C::kSB == 2 ? i & 1 : 0;
           wait(&sh.pfull[q][buf], pph >> (2 * q + buf) & 1);
-          if (q == 0) wait(&sh.vfull[vs], vph);
+          if (q == 0) {
+            wait(&sh.vfull[vs], vph);
+            wait(&sh.vscan[vs], vph);
+          }
           pph ^= 1u << (2 * q + buf);
           tc_fence_after();
           pv(q, buf, i > 0);
@@ -567,8 +585,49 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
           if (i + 2 == n) commit(&sh.qempty);
         }
       }
-      u += n;
-      t = 0;
+      ++item;
+      if (u < u1) w.next(c);
+    }
+  } else if (warp > C::kSoftWarps + 1) {
+    // ---- scan of v.  A row's p is 0 where it does not see, but 0 * inf is not:
+    // in tiles that not every row sees whole, zero the v rows no one sees and
+    // the values that are not finite (the rows that see those take them in the
+    // end).
+    uint32_t vs = 0, vph = 0, item = 0;
+    while (w.take(c, u, u1, x, t, n)) {
+      for (int i = 0; i < n; ++i) {
+        const int j0 = w.r.slice(t + i) * BN;
+        wait(&sh.vfull[vs], vph);
+        __syncwarp();
+        if (!sees_all(c.a, w, j0)) {
+          const uint32_t v = v_sm + vs * C::kKV;
+          bool odd = false;
+          // 64 threads: 64 rows of one 16-byte column at a time
+          for (int e = threadIdx.x - (C::kSoftWarps + 2) * 32; e < BN * (HD / 8); e += 64) {
+            const int r = e % BN, ch = e / BN, j = j0 + r;
+            const uint32_t at = v + (ch / 8) * (BN * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4);
+            uint4 val = make_uint4(0, 0, 0, 0);
+            if (j < w.r.hi && (j >= w.r.lo || j < c.a.sinks)) {
+              val = lds128_at<0>(at);
+              if (!(bf2_nonfinite(val.x) | bf2_nonfinite(val.y) | bf2_nonfinite(val.z) | bf2_nonfinite(val.w))) continue;
+              uint32_t* const parts[4] = {&val.x, &val.y, &val.z, &val.w};
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                if ((*parts[y] & 0x7F80u) == 0x7F80u) *parts[y] &= 0xFFFF0000u;
+                if ((*parts[y] & 0x7F800000u) == 0x7F800000u) *parts[y] &= 0xFFFFu;
+              }
+              odd = true;
+            }
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(val.x), "r"(val.y), "r"(val.z), "r"(val.w)
+                         : "memory");
+          }
+          if (odd) sh.odd[item & 3] = item + 1;
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&sh.vscan[vs]);
+        if (++vs == ST) vs = 0, vph ^= 1;
+      }
       ++item;
       if (u < u1) w.next(c);
     }
@@ -581,13 +640,16 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     const float scale = c.a.scale_log2;
     auto both_halves = [&] { asm volatile("bar.sync %0, 256;" ::"r"(1 + q) : "memory"); };
     uint32_t sph = 0, oph = 0, it = 0, item = 0;  // S tiles seen, items stored, tiles and items of the run
-    Walk<HD>& sw = sh.walk[warp];
+    Walk<HD>& sw = sh.walk[warp];  // lane 0 walks
     if (lane == 0) sw = w;
-    __syncwarp();
-    int64_t u = u0;
-    int t = first_tile;
-    while (u < u1) {
-      const int n = static_cast<int>(min(static_cast<int64_t>(sw.r.count() - t), u1 - u));
+    while (true) {
+      int more = 0;
+      if (lane == 0) more = sw.take(c, u, u1, x, t, n);
+      more = __shfl_sync(0xffffffffu, more, 0);
+      t = __shfl_sync(0xffffffffu, t, 0);
+      n = __shfl_sync(0xffffffffu, n, 0);
+      if (!more) break;
+      __syncwarp();
       const int tok0 = (sw.pair * NQ + q) * c.tpt, tok = tok0 + row / c.a.group;
       const bool active = q == 0 || tok0 < sw.s.qlen;
       const bool real = row < c.tpt * c.a.group && tok < sw.s.qlen;
@@ -598,42 +660,13 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (int i = 0; active && i < n; ++i) {
         const int j0 = sw.r.slice(t + i) * BN;
-        const uint32_t buf = C::kSB == 2 ? (i & 1) : 0, k = it + i;
+        const uint32_t buf = C::kSB == 2 ? (i & 1) : 0;
         wait(&sh.sfull[q][buf], C::kSB == 2 ? (sph >> buf) & 1 : sph & 1);
         __syncwarp();
         if (C::kSB == 2) sph ^= 1u << buf;
         else ++sph;
         tc_fence_after();
-        // A row's p is 0 where it does not see, but 0 * inf is not: zero the v
-        // rows no one sees and the values that are not finite (the rows that
-        // see those take them in the end).
         const bool whole = j0 <= all_hi && (j0 > all_lo || j0 <= all_sink);
-        if (q == 0 && !whole) {
-          wait(&sh.vfull[k % ST], (k / ST) & 1);
-          const uint32_t vs = v_sm + (k % ST) * C::kKV;
-          bool odd = false;
-          for (int e = half * kChunkRows + row; e < BN * (HD / 8); e += 2 * kChunkRows) {
-            const int r = e % BN, ch = e / BN, j = j0 + r;
-            const uint32_t at = vs + (ch / 8) * (BN * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4);
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (j < sw.r.hi && (j >= sw.r.lo || j < c.a.sinks)) {
-              x = lds128_at<0>(at);
-              uint32_t* const xs[4] = {&x.x, &x.y, &x.z, &x.w};
-              bool here = false;
-#pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                if ((*xs[y] & 0x7F80u) == 0x7F80u) *xs[y] &= 0xFFFF0000u, here = true;
-                if ((*xs[y] & 0x7F800000u) == 0x7F800000u) *xs[y] &= 0xFFFFu, here = true;
-              }
-              if (!here) continue;
-              odd = true;
-            }
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
-          }
-          if (odd) sh.odd[item & 1] = item + 1;
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
         const uint32_t s_addr = lane_addr + C::kSCol + (q + buf) * BN + half * HB;
         uint32_t sa[32], sb[32];
         tmem_ld32(s_addr, sa);
@@ -713,12 +746,11 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         const bool part = t > 0 || n < sw.r.count();
         const int head = sw.kvh * c.a.group + row % c.a.group;
         uint16_t* dst = c.a.out + static_cast<int64_t>(sw.s.q0 + tok) * c.a.o_tok + head * c.a.o_head + half * (HD / 2);
-        float* pd = c.parts + ((static_cast<int64_t>(blockIdx.x) * 2 + (t > 0 ? 0 : 1)) * NQ * kChunkRows + q * kChunkRows +
-                               row) * (HD + 2);
-        const bool odd = sh.odd[item & 1] == item + 1;
+        float* pd = part_of(c, blockIdx.x, t > 0 ? 0 : 1, NQ * kChunkRows * (HD + 2)) + q * kChunkRows * (HD + 2);
+        const bool odd = sh.odd[item & 3] == item + 1;
         const float inv = m == -INFINITY ? 0.f : 1.f / l;  // a row that sees nothing gives zeros
-        if (part && real && half == 0) pd[0] = m, pd[1] = l;
-        pd += 2 + half * (HD / 2);
+        if (part && half == 0) pd[row] = m, pd[kChunkRows + row] = l;
+        pd += 2 * kChunkRows + half * (HD / 2) * kChunkRows;
 #pragma unroll 1
         for (int e = 0; e < HD / 2; e += 32) {
           uint32_t o[32];
@@ -726,18 +758,18 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
           tmem_ld32(o_addr + e, o);
           tmem_wait_ld();
           if (odd) add_odd<HD>(c, sw, t, t + n, pos, half * (HD / 2) + e, o);
-          if (real && part) {
+          if (part) {  // [dims / 4][row][4]: a warp writes 512 bytes in a row
 #pragma unroll
-            for (int x = 0; x < 32; x += 2)
-              *reinterpret_cast<float2*>(pd + e + x) = make_float2(__uint_as_float(o[x]), __uint_as_float(o[x + 1]));
+            for (int y = 0; y < 32; y += 4)
+              *reinterpret_cast<uint4*>(pd + (e + y) * kChunkRows + row * 4) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
           } else if (real) {
 #pragma unroll
-            for (int x = 0; x < 32; x += 8) {
+            for (int y = 0; y < 32; y += 8) {
               uint32_t p[4];
 #pragma unroll
-              for (int y = 0; y < 4; ++y)
-                p[y] = pack_bf2_rn(__uint_as_float(o[x + 2 * y]) * inv, __uint_as_float(o[x + 2 * y + 1]) * inv);
-              *reinterpret_cast<uint4*>(dst + e + x) = make_uint4(p[0], p[1], p[2], p[3]);
+              for (int z = 0; z < 4; ++z)
+                p[z] = pack_bf2_rn(__uint_as_float(o[y + 2 * z]) * inv, __uint_as_float(o[y + 2 * z + 1]) * inv);
+              *reinterpret_cast<uint4*>(dst + e + y) = make_uint4(p[0], p[1], p[2], p[3]);
             }
           }
         }
@@ -745,8 +777,6 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         tc_fence_before();
       }
       it += n;
-      u += n;
-      t = 0;
       ++item;
       __syncwarp();
       if (lane == 0 && u < u1) sw.next(c);
@@ -762,60 +792,71 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
 }
 
 // Join the parts of items cut between CTAs: block (c, y) joins rows 32 y ..
-// 32 y + 31 of the item that cut c is the first inside, a warp per row.
+// 32 y + 31 (a lane each) of the item that cut c is the first inside; warps
+// take the dims in fours.
 template <int HD>
 __global__ void __launch_bounds__(256) paged_join_kernel(const ChunkArgs c, int grid) {
   using C = Chunk<HD>;
+  constexpr int kFloats = C::kNQ * kChunkRows * (HD + 2), G = HD / 32;  // G: groups of four dims per warp
   pdl_wait();
   const int cut = blockIdx.x + 1;
   const int4 it = c.cuts[cut];
   if (it.x < 0) return;
   const int64_t total = *c.total;
-  int64_t g = (total + kMinUnits - 1) / kMinUnits;
-  if (g > grid) g = grid;
+  const int g = runs_of(total, grid);
   if (cut >= g) return;
-  const int64_t at = total * cut / g, g0 = at - it.w;  // the item's first unit
-  if (total * (cut - 1) / g > g0) return;              // an earlier cut is inside the item
   Walk<HD> w{};
-  w.b = it.x;
-  w.kvh = it.y;
-  w.pair = it.z;
-  w.s = seq_span(c.a.c, w.b);
-  w.load(c);
-  const int64_t g1 = g0 + w.r.count();
-  const int lane = threadIdx.x & 31;
-  for (int r = blockIdx.y * 32 + (threadIdx.x >> 5); r < min(C::kNQ * kChunkRows, static_cast<int>(blockIdx.y) * 32 + 32); r += 8) {
-    const int q = r / kChunkRows, row = r % kChunkRows;
-    const int tok = (w.pair * C::kNQ + q) * c.tpt + row / c.a.group;
-    if (row >= c.tpt * c.a.group || tok >= w.s.qlen) continue;
-    auto part = [&](int cta) {  // the CTA's part: its last run's (slot 1) where the item starts, else its first
-      return c.parts + ((static_cast<int64_t>(cta) * 2 + (cta < cut ? 1 : 0)) * C::kNQ * kChunkRows + r) * (HD + 2);
-    };
-    float m = -INFINITY, l = 0.f, o[HD / 32] = {};
-    for (int cta = cut - 1; cta < g && total * cta / g < g1; ++cta) {
-      const float* p = part(cta);
-      const float pm = p[0], mn = fmaxf(m, pm), base = mn == -INFINITY ? 0.f : mn;
-      const float f0 = exp2_fast(m - base), f1 = exp2_fast(pm - base);
-      l = l * f0 + p[1] * f1;
+  w.at(c, static_cast<int64_t>(it.x) * c.max_pairs + it.y);
+  w.kvh = it.z;
+  const int64_t first = mul_div(total, cut, g) - it.w + kExtra;  // the item's first tile
+  const int c0 = run_of(first, total, g), c1 = run_of(first + w.r.count() - 1, total, g);
+  if (c0 + 1 != cut) return;  // an earlier cut is inside the item
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int q = blockIdx.y / 4, row = blockIdx.y % 4 * 32 + lane;
+  const int tok = (w.pair * C::kNQ + q) * c.tpt + row / c.a.group;
+  const bool real = row < c.tpt * c.a.group && tok < w.s.qlen;
+  if (!__any_sync(0xffffffffu, real)) return;
+  float m = -INFINITY, l = 0.f;
+  float4 o[G];
 #pragma unroll
-      for (int e = 0; e < HD / 32; ++e) o[e] = o[e] * f0 + p[2 + lane + 32 * e] * f1;
-      m = mn;
+  for (int i = 0; i < G; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int cta = c0; cta <= c1; ++cta) {
+    const float* p = part_of(c, cta, cta == c0 ? 1 : 0, kFloats) + q * kChunkRows * (HD + 2);
+    const float pm = p[row], pl = p[kChunkRows + row];
+    float4 v[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+      v[i] = *reinterpret_cast<const float4*>(p + 2 * kChunkRows + ((warp + 8 * i) * kChunkRows + row) * 4);
+    const float mn = fmaxf(m, pm), base = mn == -INFINITY ? 0.f : mn;
+    const float f0 = exp2_fast(m - base), f1 = exp2_fast(pm - base);
+    l = l * f0 + pl * f1;
+    m = mn;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      o[i].x = o[i].x * f0 + v[i].x * f1;
+      o[i].y = o[i].y * f0 + v[i].y * f1;
+      o[i].z = o[i].z * f0 + v[i].z * f1;
+      o[i].w = o[i].w * f0 + v[i].w * f1;
     }
-    const float inv = m == -INFINITY ? 0.f : 1.f / l;
-    const int head = w.kvh * c.a.group + row % c.a.group;
-    uint16_t* dst = c.a.out + static_cast<int64_t>(w.s.q0 + tok) * c.a.o_tok + head * c.a.o_head;
-#pragma unroll
-    for (int e = 0; e < HD / 32; ++e) dst[lane + 32 * e] = bf16_bits_rn(o[e] * inv);
   }
+  if (!real) return;
+  const float inv = m == -INFINITY ? 0.f : 1.f / l;
+  const int head = w.kvh * c.a.group + row % c.a.group;
+  uint16_t* dst = c.a.out + static_cast<int64_t>(w.s.q0 + tok) * c.a.o_tok + head * c.a.o_head;
+#pragma unroll
+  for (int i = 0; i < G; ++i)
+    *reinterpret_cast<uint2*>(dst + (warp + 8 * i) * 4) =
+        make_uint2(pack_bf2_rn(o[i].x * inv, o[i].y * inv), pack_bf2_rn(o[i].z * inv, o[i].w * inv));
 }
 
 template <int HD>
-int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int row_min, cudaStream_t st) {
+int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int max_q_len, int row_min, cudaStream_t st) {
   using C = Chunk<HD>;
   ChunkArgs c{};
   c.a = a;
   c.tpt = kChunkRows / a.group;
   c.row_min = row_min;
+  c.max_pairs = (max_q_len + C::kNQ * c.tpt - 1) / (C::kNQ * c.tpt);
   c.box = box_rows(a.c.page_size, C::kBN);
   CUtensorMap qmap, kmap, vmap;
   {
@@ -838,7 +879,7 @@ int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int row_min, cudaStream_t st
   if ((rc = prepare_kernel(ctx, k, C::kBytes))) return rc;
   if ((rc = launch_ex(ctx, k, dim3(grid), dim3(C::kThreads), C::kBytes, st, false, qmap, kmap, vmap, c))) return rc;
   if (grid < 2) return ALV_OK;
-  return launch_ex(ctx, paged_join_kernel<HD>, dim3(grid - 1, C::kNQ * kChunkRows / 32), dim3(256), 0, st, true, c, grid);
+  return launch_ex(ctx, paged_join_kernel<HD>, dim3(grid - 1, C::kNQ * 4), dim3(256), 0, st, true, c, grid);
 }
 
 }  // namespace
@@ -864,11 +905,11 @@ bool chunk_takes(const AttnArgs& a) {
          a.q_head < kMaxMapStride;
 }
 
-int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int row_min, cudaStream_t st) {
+int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int max_q_len, int row_min, cudaStream_t st) {
   switch (hd) {
-    case 64: return launch_chunk_t<64>(ctx, a, row_min, st);
-    case 128: return launch_chunk_t<128>(ctx, a, row_min, st);
-    default: return launch_chunk_t<256>(ctx, a, row_min, st);
+    case 64: return launch_chunk_t<64>(ctx, a, max_q_len, row_min, st);
+    case 128: return launch_chunk_t<128>(ctx, a, max_q_len, row_min, st);
+    default: return launch_chunk_t<256>(ctx, a, max_q_len, row_min, st);
   }
 }
 
