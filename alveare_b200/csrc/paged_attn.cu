@@ -9,6 +9,7 @@ namespace {
 struct RowArgs {
   AttnArgs a;
   int box, head_first;  // positions per tensor copy, order of the cache's maps
+  int early;            // wait for the kernel before at the end, not at the start
   float* parts;    // [2 * grid][kPart]: slot 0 where a run starts inside a block, 1 where it ends inside one
   uint32_t* done;  // [grid]: finished parts of the block that cut c is the first inside; zero between launches
 };
@@ -78,6 +79,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
   uint8_t* smem = smem_dyn + (((smem_u32(smem_dyn) + 1023u) & ~1023u) - smem_u32(smem_dyn));
   if (lane < NS) mbar_init(&full[warp][lane], 1);
   fence_mbar_init();
+  // Programmatic launch: inputs are touched once the kernel before is done.
+  // Beside a chunk kernel (which has waited itself, and triggered after that)
+  // nothing is shared, so only the end waits, for the join that follows.
+  if (!ra.early) pdl_wait();
+  pdl_trigger();
 
   // ---- this CTA's run [u0, u1) of the blocks laid end to end
   RowWalk<HD> w{};
@@ -104,7 +110,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
       total += sums[i];
     }
     G = static_cast<int>(min((total + R::kMinUnits - 1) / R::kMinUnits, static_cast<int64_t>(gridDim.x)));
-    if (blockIdx.x >= G) return;
+    if (blockIdx.x >= G) {
+      if (ra.early) pdl_wait();
+      return;
+    }
     u0 = mul_div(total, blockIdx.x, G);
     u1 = mul_div(total, blockIdx.x + 1, G);
     if (before <= u0 && u0 < before + mine) {
@@ -485,30 +494,42 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
       __syncthreads();
     }
   }
+  if (ra.early) pdl_wait();
 }
 
 template <int HD>
-int launch_rows(alv_ctx* ctx, const AttnArgs& a, cudaStream_t st) {
+int launch_rows_t(alv_ctx* ctx, const AttnArgs& a, size_t scratch, bool early, cudaStream_t st) {
   using R = RowRing<HD>;
   auto k = paged_rows_kernel<HD>;
   int rc = prepare_kernel(ctx, k, R::kBytes);
   if (rc) return rc;
-  const int grid = ctx->num_sms * 2;
-  if ((rc = ensure_scratch(ctx, static_cast<size_t>(grid) * 2 * R::kPart * 4))) return rc;
+  if ((rc = ensure_scratch(ctx, scratch + rows_scratch(ctx, HD)))) return rc;
   RowArgs ra{};
   ra.a = a;
   ra.a.c.status = status_ptr(ctx);
-  ra.parts = reinterpret_cast<float*>(work_ptr(ctx));
+  ra.parts = reinterpret_cast<float*>(work_ptr(ctx) + scratch);
   ra.done = counters_ptr(ctx);
+  ra.early = early;
   CUtensorMap kmap, vmap;
   ra.box = box_rows(a.c.page_size, R::kSlice);
   if ((rc = encode_cache(ctx, a.c, HD, ra.box, &kmap, &vmap, &ra.head_first))) return rc;
-  k<<<grid, kRowWarps * 32, R::kBytes, st>>>(kmap, vmap, ra);
-  ALV_CUDA(ctx, cudaGetLastError());
-  return ALV_OK;
+  return launch_ex(ctx, k, dim3(ctx->num_sms * 2), dim3(kRowWarps * 32), R::kBytes, st, true, kmap, vmap, ra);
 }
 
 }  // namespace
+
+size_t rows_scratch(alv_ctx* ctx, int hd) {
+  return static_cast<size_t>(ctx->num_sms) * 2 * 2 * kRowsPerBlock * (hd + 2) * 4;
+}
+
+int launch_rows(alv_ctx* ctx, const AttnArgs& a, int hd, size_t scratch, bool early, cudaStream_t st) {
+  switch (hd) {
+    case 64: return launch_rows_t<64>(ctx, a, scratch, early, st);
+    case 128: return launch_rows_t<128>(ctx, a, scratch, early, st);
+    default: return launch_rows_t<256>(ctx, a, scratch, early, st);
+  }
+}
+
 }  // namespace alv
 
 using namespace alv;
@@ -545,13 +566,9 @@ extern "C" int alv_paged_attention(alv_ctx* ctx, const alv_paged* cache, const a
   a.row_max = INT_MAX;
   if (static_cast<int64_t>(args->max_q_len) * a.group > kRowsPerBlock && chunk_takes(a)) {
     a.row_max = kRowsPerBlock;
-    if ((rc = launch_chunk(ctx, a, cache->head_dim, args->max_q_len, kRowsPerBlock + 1, st))) return rc;
     // all sequences as long as the longest: none is left for the row blocks
-    if (static_cast<int64_t>(cache->batch) * args->max_q_len == cache->tokens) return ALV_OK;
+    const bool mixed = static_cast<int64_t>(cache->batch) * args->max_q_len != cache->tokens;
+    return launch_chunk(ctx, a, cache->head_dim, args->max_q_len, kRowsPerBlock + 1, mixed, st);
   }
-  switch (cache->head_dim) {
-    case 64: return launch_rows<64>(ctx, a, st);
-    case 128: return launch_rows<128>(ctx, a, st);
-    default: return launch_rows<256>(ctx, a, st);
-  }
+  return launch_rows(ctx, a, cache->head_dim, 0, false, st);
 }

@@ -45,9 +45,15 @@ struct AttnArgs {
 };
 
 // The tensor-core form for chunks (paged_chunk.cu): sequences with at least
-// row_min rows (new tokens x heads of a kv group).
+// row_min rows (new tokens x heads of a kv group).  mixed: the row-block
+// kernel for the others is launched between it and its join.
 bool chunk_takes(const AttnArgs& a);
-int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int max_q_len, int row_min, cudaStream_t st);
+int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int max_q_len, int row_min, bool mixed, cudaStream_t st);
+// The row-block kernel (paged_attn.cu); its scratch starts at byte `scratch`
+// of the context's work area.  early: it does not wait for the kernel before
+// it, only ends after it.
+size_t rows_scratch(alv_ctx* ctx, int hd);
+int launch_rows(alv_ctx* ctx, const AttnArgs& a, int hd, size_t scratch, bool early, cudaStream_t st);
 
 constexpr int kRowsPerBlock = 16;
 constexpr int kRowWarps = 4;

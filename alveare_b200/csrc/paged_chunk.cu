@@ -342,7 +342,6 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
   const uint32_t q_sm = base, k_sm = base + NQ * C::kQTile, v_sm = k_sm + ST * C::kKV;
-  pdl_trigger();
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
@@ -372,6 +371,9 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     *reinterpret_cast<uint4*>(smem_dyn + (base - smem_u32(smem_dyn)) + i * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
 
+  // The row-block kernel of a mixed batch may start where this one's CTAs end.
+  pdl_wait();
+  pdl_trigger();
   // ---- the CTA's run: thread t adds up the lengths of its sequences and
   // pairs, a scan over the threads finds where the run starts
   Walk<HD> w{};
@@ -438,52 +440,75 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
   };
 
   if (warp == C::kSoftWarps) {
-    // ---- copies: lane i fetches box i of a tile's k and v
+    // ---- copies: lane i fetches box i of a tile's k and v.  Tile by tile: k,
+    // then v of the tile before (the order the products need them in); the
+    // next tile's page is looked up meanwhile.
     const int boxes = BN / c.box;
     uint32_t it = 0, item = 0;
-    while (w.take(c, u, u1, x, t, n)) {
-      const int tok = w.pair * NQ * c.tpt;
-      if (item > 0) wait(&sh.qempty, (item - 1) & 1);
-      const int nq = NQ == 2 && tok + c.tpt < w.s.qlen ? 2 : 1;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&sh.qfull, nq * c.tpt * c.a.group * HD * 2);
-        for (int q = 0; q < nq; ++q)
-          for (int d = 0; d < HD / 64; ++d)
-            tma_load_3d(q_sm + q * C::kQTile + d * (kChunkRows * 128), &qmap, d * 64, w.kvh * c.a.group,
-                        w.s.q0 + tok + q * c.tpt, smem_u32(&sh.qfull));
+    int i = -1;
+    // the tile to come: its first position here, whether some row sees this
+    // box (others are not fetched, their pages may be gone), its page
+    int j = 0, raw = -1;
+    bool live = false;
+    auto step = [&]() -> bool {
+      if (++i >= n) {
+        if (item > 0 && u < u1) w.next(c);
+        if (!w.take(c, u, u1, x, t, n)) return false;
+        i = 0;
+        ++item;
       }
-      for (int i = 0; i < n; ++i, ++it) {
-        const int j = w.r.slice(t + i) * BN + lane * c.box;
-        // boxes that no row sees are not fetched (their pages may be gone)
-        const bool live = lane < boxes && j < w.r.hi && (j + c.box > w.r.lo || j < c.a.sinks);
-        int page = c.a.c.pages;  // past the end: the copy reads zeros
-        if (live) {
-          const int p = page_of(c.a.c, w.b, j);
-          if (p >= 0) page = p;
-        }
-        const uint32_t n_live = __popc(__ballot_sync(0xffffffffu, live));
-        const int row = j % c.a.c.page_size;
-        const uint32_t stage = it % ST, ph = (it / ST) & 1;
-        for (int kv = 0; kv < 2; ++kv) {
-          uint64_t* full = kv ? &sh.vfull[stage] : &sh.kfull[stage];
-          if (it >= ST) wait(kv ? &sh.vempty[stage] : &sh.kempty[stage], ph ^ 1);
-          __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(full, n_live * c.box * HD * 2);
-          __syncwarp();
-          if (live) {
-            const uint32_t dst = (kv ? v_sm : k_sm) + stage * C::kKV + lane * c.box * 128;
-            const CUtensorMap* map = kv ? &vmap : &kmap;
-            for (int d = 0; d < HD / 64; ++d) {
-              if (c.head_first) tma_load_4d(dst + d * (BN * 128), map, d * 64, w.kvh, row, page, smem_u32(full));
-              else tma_load_4d(dst + d * (BN * 128), map, d * 64, row, w.kvh, page, smem_u32(full));
-            }
-          }
-          __syncwarp();
+      j = w.r.slice(t + i) * BN + lane * c.box;
+      live = lane < boxes && j < w.r.hi && (j + c.box > w.r.lo || j < c.a.sinks);
+      raw = live ? c.a.c.table[static_cast<int64_t>(w.b) * c.a.c.table_stride + j / c.a.c.page_size] : -1;
+      return true;
+    };
+    auto fetch = [&](uint32_t k, bool v, uint32_t n_live, bool mine, int page, int row, int kvh) {
+      const uint32_t stage = k % ST;
+      if (k >= ST) wait(v ? &sh.vempty[stage] : &sh.kempty[stage], ((k / ST) & 1) ^ 1);
+      __syncwarp();
+      const uint32_t full = smem_u32(v ? &sh.vfull[stage] : &sh.kfull[stage]);
+      if (lane == 0) mbar_arrive_expect_tx_s(full, n_live * c.box * HD * 2);
+      __syncwarp();
+      if (mine) {
+        const uint32_t dst = (v ? v_sm : k_sm) + stage * C::kKV + lane * c.box * 128;
+        const CUtensorMap* map = v ? &vmap : &kmap;
+        for (int d = 0; d < HD / 64; ++d) {
+          if (c.head_first) tma_load_4d(dst + d * (BN * 128), map, d * 64, kvh, row, page, full);
+          else tma_load_4d(dst + d * (BN * 128), map, d * 64, row, kvh, page, full);
         }
       }
-      ++item;
-      if (u < u1) w.next(c);
+      __syncwarp();
+    };
+    uint32_t v_live = 0;
+    bool v_mine = false;
+    int v_page = 0, v_row = 0, v_kvh = 0;
+    while (step()) {
+      if (i == 0) {  // the item's query tiles
+        const int tok = w.pair * NQ * c.tpt, nq = NQ == 2 && tok + c.tpt < w.s.qlen ? 2 : 1;
+        if (item > 1) wait(&sh.qempty, item & 1);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sh.qfull, nq * c.tpt * c.a.group * HD * 2);
+          for (int q = 0; q < nq; ++q)
+            for (int d = 0; d < HD / 64; ++d)
+              tma_load_3d(q_sm + q * C::kQTile + d * (kChunkRows * 128), &qmap, d * 64, w.kvh * c.a.group,
+                          w.s.q0 + tok + q * c.tpt, smem_u32(&sh.qfull));
+        }
+      }
+      const bool mine = live;
+      const uint32_t n_live = __popc(__ballot_sync(0xffffffffu, mine));
+      const int row = j % c.a.c.page_size, kvh = w.kvh;
+      int page = raw;
+      if (page < 0 || page >= c.a.c.pages) {
+        if (mine) atomicOr(c.a.c.status, kStatusBadIndex);
+        page = c.a.c.pages;  // past the end: the copy reads zeros
+      }
+      fetch(it, false, n_live, mine, page, row, kvh);
+      if (it > 0) fetch(it - 1, true, v_live, v_mine, v_page, v_row, v_kvh);
+      ++it;
+      v_live = n_live, v_mine = mine, v_page = page, v_row = row, v_kvh = kvh;
     }
+    if (it > 0) fetch(it - 1, true, v_live, v_mine, v_page, v_row, v_kvh);
     // every armed stage lands before the CTA may exit
     for (uint32_t k = it > ST ? it - ST : 0; k < it; ++k) {
       mbar_wait_bounded_s(smem_u32(&sh.kfull[k % ST]), (k / ST) & 1);
@@ -850,7 +875,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const ChunkArgs c, int 
 }
 
 template <int HD>
-int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int max_q_len, int row_min, cudaStream_t st) {
+int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int max_q_len, int row_min, bool mixed, cudaStream_t st) {
   using C = Chunk<HD>;
   ChunkArgs c{};
   c.a = a;
@@ -869,7 +894,8 @@ int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int max_q_len, int row_min, 
   if (const int rc = encode_cache(ctx, a.c, HD, c.box, &kmap, &vmap, &c.head_first)) return rc;
   const int grid = ctx->num_sms;
   const size_t o_cuts = 256, o_parts = o_cuts + align_up(static_cast<size_t>(grid) * sizeof(int4), 256);
-  int rc = ensure_scratch(ctx, o_parts + static_cast<size_t>(grid) * 2 * C::kNQ * kChunkRows * (HD + 2) * 4);
+  const size_t o_rows = align_up(o_parts + static_cast<size_t>(grid) * 2 * C::kNQ * kChunkRows * (HD + 2) * 4, 256);
+  int rc = ensure_scratch(ctx, o_rows + (mixed ? rows_scratch(ctx, HD) : 0));
   if (rc) return rc;
   c.total = reinterpret_cast<int64_t*>(work_ptr(ctx));
   c.cuts = reinterpret_cast<int4*>(work_ptr(ctx) + o_cuts);
@@ -877,7 +903,8 @@ int launch_chunk_t(alv_ctx* ctx, const AttnArgs& a, int max_q_len, int row_min, 
   c.a.c.status = status_ptr(ctx);
   auto k = paged_chunk_kernel<HD>;
   if ((rc = prepare_kernel(ctx, k, C::kBytes))) return rc;
-  if ((rc = launch_ex(ctx, k, dim3(grid), dim3(C::kThreads), C::kBytes, st, false, qmap, kmap, vmap, c))) return rc;
+  if ((rc = launch_ex(ctx, k, dim3(grid), dim3(C::kThreads), C::kBytes, st, true, qmap, kmap, vmap, c))) return rc;
+  if (mixed && (rc = launch_rows(ctx, a, HD, o_rows, true, st))) return rc;
   if (grid < 2) return ALV_OK;
   return launch_ex(ctx, paged_join_kernel<HD>, dim3(grid - 1, C::kNQ * 4), dim3(256), 0, st, true, c, grid);
 }
@@ -905,11 +932,11 @@ bool chunk_takes(const AttnArgs& a) {
          a.q_head < kMaxMapStride;
 }
 
-int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int max_q_len, int row_min, cudaStream_t st) {
+int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int max_q_len, int row_min, bool mixed, cudaStream_t st) {
   switch (hd) {
-    case 64: return launch_chunk_t<64>(ctx, a, max_q_len, row_min, st);
-    case 128: return launch_chunk_t<128>(ctx, a, max_q_len, row_min, st);
-    default: return launch_chunk_t<256>(ctx, a, max_q_len, row_min, st);
+    case 64: return launch_chunk_t<64>(ctx, a, max_q_len, row_min, mixed, st);
+    case 128: return launch_chunk_t<128>(ctx, a, max_q_len, row_min, mixed, st);
+    default: return launch_chunk_t<256>(ctx, a, max_q_len, row_min, mixed, st);
   }
 }
 
