@@ -483,6 +483,17 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     bool v_mine = false;
     int v_page = 0, v_row = 0, v_kvh = 0;
     while (step()) {
+      const bool mine = live;
+      const uint32_t n_live = __popc(__ballot_sync(0xffffffffu, mine));
+      const int row = j % c.a.c.page_size, kvh = w.kvh;
+      int page = raw;
+      if (page < 0 || page >= c.a.c.pages) {
+        if (mine) atomicOr(c.a.c.status, kStatusBadIndex);
+        page = c.a.c.pages;  // past the end: the copy reads zeros
+      }
+      fetch(it, false, n_live, mine, page, row, kvh);
+      if (it > 0) fetch(it - 1, true, v_live, v_mine, v_page, v_row, v_kvh);
+      ++it;
       if (i == 0) {  // the item's query tiles
         const int tok = w.pair * NQ * c.tpt, nq = NQ == 2 && tok + c.tpt < w.s.qlen ? 2 : 1;
         if (item > 1) wait(&sh.qempty, item & 1);
@@ -495,17 +506,6 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
                           w.s.q0 + tok + q * c.tpt, smem_u32(&sh.qfull));
         }
       }
-      const bool mine = live;
-      const uint32_t n_live = __popc(__ballot_sync(0xffffffffu, mine));
-      const int row = j % c.a.c.page_size, kvh = w.kvh;
-      int page = raw;
-      if (page < 0 || page >= c.a.c.pages) {
-        if (mine) atomicOr(c.a.c.status, kStatusBadIndex);
-        page = c.a.c.pages;  // past the end: the copy reads zeros
-      }
-      fetch(it, false, n_live, mine, page, row, kvh);
-      if (it > 0) fetch(it - 1, true, v_live, v_mine, v_page, v_row, v_kvh);
-      ++it;
       v_live = n_live, v_mine = mine, v_page = page, v_row = row, v_kvh = kvh;
     }
     if (it > 0) fetch(it - 1, true, v_live, v_mine, v_page, v_row, v_kvh);
@@ -627,24 +627,35 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         if (!sees_all(c.a, w, j0)) {
           const uint32_t v = v_sm + vs * C::kKV;
           bool odd = false;
-          // 64 threads: 64 rows of one 16-byte column at a time
-          for (int e = threadIdx.x - (C::kSoftWarps + 2) * 32; e < BN * (HD / 8); e += 64) {
-            const int r = e % BN, ch = e / BN, j = j0 + r;
-            const uint32_t at = v + (ch / 8) * (BN * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4);
-            uint4 val = make_uint4(0, 0, 0, 0);
-            if (j < w.r.hi && (j >= w.r.lo || j < c.a.sinks)) {
-              val = lds128_at<0>(at);
-              if (!(bf2_nonfinite(val.x) | bf2_nonfinite(val.y) | bf2_nonfinite(val.z) | bf2_nonfinite(val.w))) continue;
-              uint32_t* const parts[4] = {&val.x, &val.y, &val.z, &val.w};
+          for (int r = threadIdx.x - (C::kSoftWarps + 2) * 32; r < BN; r += 64) {  // a thread per row
+            const int j = j0 + r;
+            auto at = [&](int ch) { return v + (ch / 8) * (BN * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4); };
+            if (j >= w.r.hi || (j < w.r.lo && j >= c.a.sinks)) {
+#pragma unroll 8
+              for (int ch = 0; ch < HD / 8; ++ch)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at(ch)), "r"(0) : "memory");
+              continue;
+            }
+            uint32_t any = 0;  // an exponent of all ones carries into the sign's place
+#pragma unroll 8
+            for (int ch = 0; ch < HD / 8; ++ch) {
+              const uint4 val = lds128_at<0>(at(ch));
+              any |= ((val.x & 0x7F807F80u) + 0x00800080u) | ((val.y & 0x7F807F80u) + 0x00800080u) |
+                     ((val.z & 0x7F807F80u) + 0x00800080u) | ((val.w & 0x7F807F80u) + 0x00800080u);
+            }
+            if (!(any & 0x80008000u)) continue;
+            odd = true;
+            for (int ch = 0; ch < HD / 8; ++ch) {
+              const uint4 val = lds128_at<0>(at(ch));
+              uint32_t x4[4] = {val.x, val.y, val.z, val.w};
 #pragma unroll
               for (int y = 0; y < 4; ++y) {
-                if ((*parts[y] & 0x7F80u) == 0x7F80u) *parts[y] &= 0xFFFF0000u;
-                if ((*parts[y] & 0x7F800000u) == 0x7F800000u) *parts[y] &= 0xFFFFu;
+                if ((x4[y] & 0x7F80u) == 0x7F80u) x4[y] &= 0xFFFF0000u;
+                if ((x4[y] & 0x7F800000u) == 0x7F800000u) x4[y] &= 0xFFFFu;
               }
-              odd = true;
+              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at(ch)), "r"(x4[0]), "r"(x4[1]), "r"(x4[2]), "r"(x4[3])
+                           : "memory");
             }
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(val.x), "r"(val.y), "r"(val.z), "r"(val.w)
-                         : "memory");
           }
           if (odd) sh.odd[item & 3] = item + 1;
           fence_proxy_async_smem();
