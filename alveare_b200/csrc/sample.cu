@@ -6,19 +6,18 @@
 //   min-p: of those, w_i >= min_p;
 //   token: the first, in index order, whose running mass passes floor(u * total).
 //
-// The masses are integers (a vocabulary of 2^20 sums to at most 2^60), so sums
+// The masses are integers (a vocabulary of 2^19 sums to at most 2^59), so sums
 // of any order and atomics give one result.
 //
 // A cluster of CTAs takes a row and keeps it in its shared memory, so the
 // logits are read once; the CTAs exchange sums and histograms through
 // distributed shared memory.  The end of a prefix is found by a histogram over
-// max - s (2048 even bins; counts for top-k, masses for top-p), the bin where
-// the k-th element (or the wanted mass) falls, and then among that bin's
-// elements, gathered in one CTA, by comparing each with each; a bin with too
-// many elements is cut again by the bits of s.  Elements equal to the last one
-// kept enter in index order.  For top-p only elements that can be in the
-// prefix enter the histogram: those below e = (1 - p) total / (2 n) weigh less
-// than (1 - p) total together.
+// max - s (2048 even bins; counts for top-k, masses for top-p, whose bins also
+// add up to the mass that p is a share of), the bin where the k-th element (or
+// the wanted mass) falls, and then among that bin's elements, gathered in one
+// CTA, by comparing each with each; a bin with too many elements is cut again
+// by the bits of s.  Elements equal to the last one kept enter in index order.
+// Where top-k leaves few elements, that CTA finishes the row by itself.
 #include <cooperative_groups.h>
 
 #include "internal.h"
@@ -34,6 +33,7 @@ constexpr int kBins = 2048;
 constexpr int kCand = kSampleThreads;  // elements of the last bin compared each with each
 constexpr int kMaxCluster = 8;
 constexpr float kMaxDist = 27.75f;     // exp(-27.75) < 2^-40: no mass beyond
+constexpr int kMaxSlice = 65536;       // elements per CTA: 65,536 16-bit digits add up below 2^32
 typedef unsigned long long u64;
 
 struct SampleArgs {
@@ -72,7 +72,7 @@ struct Cut {  // kept: s > last, and the first `ties` (in index order) of s == l
 };
 
 struct SampleShared {
-  uint32_t lo[kBins], hi[kBins];  // counts, or masses in two words
+  uint32_t bins[3][kBins];  // counts in the first, or masses as three 16-bit digits' sums
   uint32_t ckey[kCand], cidx[kCand];
   u64 cmass[kCand];
   uint32_t n_cand;
@@ -81,7 +81,7 @@ struct SampleShared {
   u64 sum[5];
   uint32_t best_key, best_idx, kmin, kmax;
   // what a CTA tells all
-  struct { int bin; u64 before; uint32_t last_key, ties, of; } found;
+  struct { int bin; u64 before, in, want; uint32_t last_key, ties, of; } found;
   uint32_t wties[kSampleWarps];
   u64 wmass[kSampleWarps];
 };
@@ -158,116 +158,145 @@ struct Row {
   }
 };
 
-// Sum over the cluster of v (a thread's share), through slot `slot`.
-__device__ __forceinline__ u64 cluster_sum(cg::cluster_group& cl, SampleShared& sh, u64 v, int slot) {
+// The histogram's crossing: with `bin_of(s)` (-1: not in question) of every
+// element, the bin in which the count (MASS: the mass) starting from `acc`
+// reaches the wanted one, what lies before it and what it holds (found.*, in
+// every CTA).  `want_of(total)` gives the wanted one from the sum of all bins;
+// 0 or more than there is: found.bin = -1.
+template <bool MASS, bool BF16, bool RES, class B, class W>
+__device__ __forceinline__ void crossing(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, float top,
+                                         u64 acc, int slot, B bin_of, W want_of) {
+  const unsigned rank = cl.block_rank(), nb = cl.num_blocks();
+  for (int b = threadIdx.x; b < kBins * (MASS ? 3 : 1); b += kSampleThreads) (&sh.bins[0][0])[b] = 0;
+  if (threadIdx.x == 0) {
+    sh.n_cand = 0;
+    sh.kmin = 0xFFFFFFFFu;
+    sh.kmax = 0;
+    sh.found.bin = -1;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
+    const float s = row.at(i);
+    const int b = bin_of(s);
+    if (b < 0) continue;
+    if (MASS) {
+      const u64 m = mass_of(expf(s - top));
+      const uint32_t m0 = static_cast<uint32_t>(m) & 0xFFFFu, m1 = static_cast<uint32_t>(m >> 16) & 0xFFFFu,
+                     m2 = static_cast<uint32_t>(m >> 32);
+      atomicAdd(&sh.bins[0][b], m0);
+      if (m1) atomicAdd(&sh.bins[1][b], m1);
+      if (m2) atomicAdd(&sh.bins[2][b], m2);
+    } else {
+      atomicAdd(&sh.bins[0][b], 1u);
+    }
+  }
+  cl.sync();
+  // CTA r adds up bins [r, r + 1) * kBins / nb of all CTAs
+  const int per = kBins / nb, tp = (per + kSampleThreads - 1) / kSampleThreads;
+  u64 bins[kBins / kSampleThreads] = {}, mine = 0;
+#pragma unroll
+  for (int e = 0; e < kBins / kSampleThreads; ++e) {
+    const int b = threadIdx.x * tp + e;
+    if (e < tp && b < per)
+      for (unsigned r = 0; r < nb; ++r) {
+        const SampleShared* o = cl.map_shared_rank(&sh, r);
+        bins[e] += o->bins[0][rank * per + b];
+        if (MASS)
+          bins[e] += (static_cast<u64>(o->bins[1][rank * per + b]) << 16) + (static_cast<u64>(o->bins[2][rank * per + b]) << 32);
+      }
+    mine += bins[e];
+  }
   u64 t;
-  cta_scan(v, &t, sh.scan);
+  u64 upto = cta_scan(mine, &t, sh.scan) - mine;
   if (threadIdx.x == 0) sh.sum[slot] = t;
   cl.sync();
-  u64 all = 0;
-  for (unsigned r = 0; r < cl.num_blocks(); ++r) all += cl.map_shared_rank(&sh, r)->sum[slot];
-  return all;
+  u64 before = acc, all = 0;
+  for (unsigned r = 0; r < nb; ++r) {
+    const u64 x = cl.map_shared_rank(&sh, r)->sum[slot];
+    if (r < rank) before += x;
+    all += x;
+  }
+  const u64 want = want_of(all);
+  upto += before;
+#pragma unroll
+  for (int e = 0; e < kBins / kSampleThreads; ++e) {
+    if (e < tp && upto < want && want <= upto + bins[e])
+      for (unsigned r = 0; r < nb; ++r) {
+        SampleShared* o = cl.map_shared_rank(&sh, r);
+        o->found.bin = static_cast<int>(rank) * per + threadIdx.x * tp + e;
+        o->found.before = upto;
+        o->found.in = bins[e];
+        o->found.want = want;
+      }
+    upto += bins[e];
+  }
+  cl.sync();
+}
+
+// Bins of max - s, even up to kMaxDist.
+__device__ __forceinline__ int even_bin(float top, float s) {
+  const float d = top - s;
+  if (!(d <= kMaxDist)) return -1;
+  return min(static_cast<int>(__float_as_uint(__fmaf_rz(d, kBins / kMaxDist, 8388608.0f)) & 0x7FFFFFu), kBins - 1);
+}
+
+// Put the elements with in(s) into CTA 0's list (and their keys' range there).
+template <bool BF16, bool RES, class F>
+__device__ __forceinline__ void gather(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, F in) {
+  SampleShared* lead = cl.map_shared_rank(&sh, 0);
+  uint32_t lo = 0xFFFFFFFFu, hi = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
+    const float s = row.at(i);
+    if (!in(s)) continue;
+    const uint32_t k = key_of(s), at = atomicAdd(&lead->n_cand, 1u);
+    lo = min(lo, k);
+    hi = max(hi, k);
+    if (at < kCand) {
+      lead->ckey[at] = k;
+      lead->cidx[at] = row.first + i;
+    }
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if ((threadIdx.x & 31) == 0 && hi >= lo) {
+    atomicMin(&lead->kmin, lo);
+    atomicMax(&lead->kmax, hi);
+  }
+  cl.sync();
 }
 
 // The prefix of the row, in (s descending, index ascending) order, that ends
-// with the element where the count (or, MASS, the mass) reaches `want`; the
-// elements are those with top - s <= dist and s >= floor_s, and they reach it.
+// with the element where the count (MASS: the mass) reaches the wanted one:
+// called once the histogram over even bins has found the bin (found.*).
 template <bool MASS, bool BF16, bool RES>
-__device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, float top, float dist,
-                      float floor_s, u64 want) {
+__device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, float top, float floor_s) {
   const unsigned rank = cl.block_rank(), nb = cl.num_blocks();
-  const float scale = static_cast<float>(kBins) / dist;
   uint32_t kmin = 0, kmax = 0;  // after the first round: the keys of the bin that is cut again
   int shift = 0;
-  u64 acc = 0;
+  const u64 want = sh.found.want;
   for (int round = 0;; ++round) {
-    auto bin_of = [&](float s) -> int {  // -1: not in question
-      if (round == 0) {
-        const float d = top - s;
-        return d <= dist && s >= floor_s ? min(static_cast<int>(d * scale), kBins - 1) : -1;
-      }
+    auto bin_of = [&](float s) -> int {
+      if (round == 0) return s >= floor_s ? even_bin(top, s) : -1;
       const uint32_t k = key_of(s);
       return k >= kmin && k <= kmax ? static_cast<int>((kmax - k) >> shift) : -1;
     };
-    for (int b = threadIdx.x; b < kBins; b += kSampleThreads) sh.lo[b] = sh.hi[b] = 0;
-    if (threadIdx.x == 0) {
-      sh.n_cand = 0;
-      sh.kmin = 0xFFFFFFFFu;
-      sh.kmax = 0;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
-      const float s = row.at(i);
-      const int b = bin_of(s);
-      if (b < 0) continue;
-      if (MASS) {
-        const u64 m = mass_of(expf(s - top));
-        const uint32_t ml = static_cast<uint32_t>(m), old = atomicAdd(&sh.lo[b], ml);
-        const uint32_t mh = static_cast<uint32_t>(m >> 32) + (old + ml < old);
-        if (mh) atomicAdd(&sh.hi[b], mh);
-      } else {
-        atomicAdd(&sh.lo[b], 1u);
-      }
-    }
-    cl.sync();
-    // CTA r adds up bins [r, r + 1) * kBins / nb of all CTAs
-    const int per = kBins / nb, tp = (per + kSampleThreads - 1) / kSampleThreads;
-    u64 bins[kBins / kSampleThreads] = {}, mine = 0;
-    for (int e = 0; e < tp; ++e) {
-      const int b = threadIdx.x * tp + e;
-      if (b < per)
-        for (unsigned r = 0; r < nb; ++r) {
-          const SampleShared* o = cl.map_shared_rank(&sh, r);
-          bins[e] += o->lo[rank * per + b] + (static_cast<u64>(o->hi[rank * per + b]) << 32);
-        }
-      mine += bins[e];
-    }
-    u64 t;
-    u64 upto = cta_scan(mine, &t, sh.scan) - mine;
-    if (threadIdx.x == 0) sh.sum[round & 1] = t;
-    cl.sync();
-    u64 before = acc;
-    for (unsigned r = 0; r < rank; ++r) before += cl.map_shared_rank(&sh, r)->sum[round & 1];
-    upto += before;
-    for (int e = 0; e < tp; ++e) {
-      if (upto < want && want <= upto + bins[e])
-        for (unsigned r = 0; r < nb; ++r) {
-          SampleShared* o = cl.map_shared_rank(&sh, r);
-          o->found.bin = static_cast<int>(rank) * per + threadIdx.x * tp + e;
-          o->found.before = upto;
-        }
-      upto += bins[e];
-    }
-    cl.sync();
     const int bin = sh.found.bin;
-    acc = sh.found.before;
-    // gather the bin's elements in CTA 0
+    const u64 acc = sh.found.before;
+    if (round > 0) {
+      crossing<MASS>(cl, sh, row, top, acc, round & 1, bin_of, [&](u64) { return want; });
+    }
+    const int at = round > 0 ? sh.found.bin : bin;
+    const u64 pre0 = round > 0 ? sh.found.before : acc;
+    gather(cl, sh, row, [&](float s) { return bin_of(s) == at; });
     SampleShared* lead = cl.map_shared_rank(&sh, 0);
-    uint32_t lo = 0xFFFFFFFFu, hi = 0;
-    for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
-      const float s = row.at(i);
-      if (bin_of(s) != bin) continue;
-      const uint32_t k = key_of(s), at = atomicAdd(&lead->n_cand, 1u);
-      lo = min(lo, k);
-      hi = max(hi, k);
-      if (at < kCand) {
-        lead->ckey[at] = k;
-        lead->cidx[at] = row.first + i;
-      }
-    }
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    if ((threadIdx.x & 31) == 0 && hi >= lo) {
-      atomicMin(&lead->kmin, lo);
-      atomicMax(&lead->kmax, hi);
-    }
-    cl.sync();
     const uint32_t n = lead->n_cand;
     kmin = lead->kmin;
     kmax = lead->kmax;
     if (kmin == kmax) {  // all equal
       const u64 each = MASS ? mass_of(expf(key_value(kmin) - top)) : 1;
-      const u64 need = (want - acc + each - 1) / each;
+      const u64 need = (want - pre0 + each - 1) / each;
       cl.sync();  // CTA 0 stays until its words are read
       return {key_value(kmin), static_cast<uint32_t>(need), n};
     }
@@ -284,7 +313,7 @@ __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, R
         }
         __syncthreads();
         if (i < n) {
-          u64 pre = acc;
+          u64 pre = pre0;
           uint32_t ties = 1, of = 0;
           for (uint32_t j = 0; j < n; ++j) {
             const uint32_t kj = sh.ckey[j];
@@ -308,6 +337,59 @@ __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, R
     shift = 0;
     while (((kmax - kmin) >> shift) >= kBins) ++shift;
     cl.sync();  // CTA 0's words are read before the next round clears them
+  }
+}
+
+// The rest of a row whose top k are among CTA 0's list: ranks by comparing each
+// with each, then top-p over the ranks, min-p, and the draw in index order.
+__device__ void finish_few(SampleShared& sh, const SampleArgs& a, int r, uint32_t n, uint32_t k, float p, float min_p,
+                           float top) {
+  const uint32_t i = threadIdx.x;
+  uint32_t key = 0, idx = 0, rank = 0xFFFFFFFFu;
+  u64 m = 0;
+  float w = 0.f;
+  if (i < n) {
+    key = sh.ckey[i];
+    idx = sh.cidx[i];
+    rank = 0;
+    for (uint32_t j = 0; j < n; ++j) {
+      const uint32_t kj = sh.ckey[j];
+      rank += kj > key || (kj == key && sh.cidx[j] < idx);
+    }
+    if (rank < k) {
+      w = expf(key_value(key) - top);
+      m = mass_of(w);
+    }
+  }
+  sh.cmass[i] = 0;
+  __syncthreads();
+  if (i < n) sh.cmass[rank] = m;  // by rank
+  __syncthreads();
+  u64 total;
+  const u64 upto = cta_scan(sh.cmass[i], &total, sh.scan);
+  uint32_t last = k;  // ranks below are kept
+  if (p < 1.f) {
+    const double x = ceil(static_cast<double>(total) * static_cast<double>(p));
+    const u64 goal = x >= 1.0 ? static_cast<u64>(x) : 1;
+    if (upto >= goal && upto - sh.cmass[i] < goal) sh.found.last_key = i + 1;
+    __syncthreads();
+    last = sh.found.last_key;
+  }
+  __syncthreads();
+  const bool keep = i < n && rank < last && rank < k && w >= min_p;
+  sh.cmass[i] = keep ? m : 0;  // by place in the list
+  __syncthreads();
+  u64 before = 0, kept = 0;
+  for (uint32_t j = 0; j < n; ++j) {
+    const u64 mj = sh.cmass[j];
+    kept += mj;
+    if (i < n && sh.cidx[j] < idx) before += mj;
+  }
+  const u64 x = static_cast<u64>(fmax(floor(static_cast<double>(a.u[r]) * static_cast<double>(kept)), 0.0));
+  const u64 goal = x < kept ? x : kept - 1;
+  if (keep && before <= goal && goal < before + m) {
+    a.tokens[r] = static_cast<int>(idx);
+    if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(m) / static_cast<double>(kept)));
   }
 }
 
@@ -370,30 +452,34 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   // ---- where the kept prefix ends
   Cut cut{-INFINITY, 0, 0};
   bool all = true;
-  uint32_t n_kept = a.vocab;
   if (k > 0 && k < a.vocab) {
     // elements without mass do not matter: if fewer than k have some, all do
-    u64 n = 0;
-    for (int i = threadIdx.x; i < row.n; i += kSampleThreads) n += top - row.at(i) <= kMaxDist;
-    n = cluster_sum(cl, sh, n, 2);
-    if (n > static_cast<u64>(k)) {
-      cut = select<false>(cl, sh, row, top, kMaxDist, -INFINITY, static_cast<u64>(k));
+    crossing<false>(cl, sh, row, top, 0, 2, [&](float s) { return even_bin(top, s); },
+                    [&](u64 n) { return n > static_cast<u64>(k) ? static_cast<u64>(k) : 0; });
+    const int bin = sh.found.bin;
+    if (bin >= 0 && sh.found.before + sh.found.in <= kCand) {
+      gather(cl, sh, row, [&](float s) {
+        const int b = even_bin(top, s);
+        return b >= 0 && b <= bin;
+      });
+      if (rank == 0) finish_few(sh, a, r, sh.n_cand, static_cast<uint32_t>(k), p, min_p, top);
+      return;  // CTA 0's words are its own from here
+    }
+    if (bin >= 0) {
+      cut = select<false>(cl, sh, row, top, -INFINITY);
       all = false;
     }
-    n_kept = k;
   }
   if (p < 1.f) {
-    u64 m = 0;
-    for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
-      const float s = row.at(i);
-      if (all || s > cut.last) m += mass_of(expf(s - top));
-    }
-    m = cluster_sum(cl, sh, m, 3);
-    if (!all) m += cut.ties * mass_of(expf(cut.last - top));
-    const double goal = ceil(static_cast<double>(m) * static_cast<double>(p));
-    const double eps = 0.5 * (1.0 - static_cast<double>(p)) * (static_cast<double>(m) / 1099511627776.0) / n_kept;
-    const float dist = fminf(0.01f - logf(fmaxf(static_cast<float>(eps), 1e-30f)), kMaxDist);
-    cut = select<true>(cl, sh, row, top, fmaxf(dist, 0.01f), cut.last, goal >= 1.0 ? static_cast<u64>(goal) : 1);
+    // the mass that p is a share of: all of it, or the k largest (of the
+    // elements equal to the last one only some)
+    const u64 each = all ? 0 : mass_of(expf(cut.last - top));
+    const u64 beyond = all ? 0 : (cut.of - cut.ties) * each;
+    crossing<true>(cl, sh, row, top, 0, 3, [&](float s) { return s >= cut.last ? even_bin(top, s) : -1; }, [&](u64 m) {
+      const double goal = ceil(static_cast<double>(m - beyond) * static_cast<double>(p));
+      return goal >= 1.0 ? static_cast<u64>(goal) : static_cast<u64>(1);
+    });
+    cut = select<true>(cl, sh, row, top, cut.last);
     all = false;
   }
 
@@ -499,7 +585,7 @@ extern "C" int alv_sample(alv_ctx* ctx, const alv_sample_args* s, void* stream) 
   if (s->rows < 0 || s->vocab < 1 || !valid_dtype(s->logits_dtype) || (s->rows && (!s->logits || !s->u || !s->tokens)) ||
       s->logits_stride < s->vocab)
     return fail(ctx, ALV_ERR_ARG, "sample: bad argument");
-  if (s->vocab > 1 << 20) return fail(ctx, ALV_ERR_UNSUPPORTED, "sample: at most 1,048,576 tokens");
+  if (s->vocab > kMaxCluster * kMaxSlice) return fail(ctx, ALV_ERR_UNSUPPORTED, "sample: at most 524,288 tokens");
   if (reinterpret_cast<uintptr_t>(s->logits) & (s->logits_dtype == ALV_F32 ? 3 : 1))
     return fail(ctx, ALV_ERR_ARG, "sample: logits must be aligned to their type");
   if ((!s->temperature_rows && !(s->temperature >= 0.f)) || (!s->top_p_rows && !(s->top_p >= 0.f)) ||

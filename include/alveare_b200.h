@@ -422,7 +422,7 @@ int alv_pages_compact(alv_ctx* ctx, const alv_pages* p, int32_t* table_out, int3
  * Masses are summed as integers, so the result does not depend on any order.
  * Per-row parameters are device arrays where the pointer is given, else the
  * scalar applies to all.  temperature 0: the largest logit (lowest index).
- * NaN counts as -inf.  A row with nothing above -inf gives token -1.  logprobs
+ * NaN counts as -inf.  At most 524,288 tokens.  A row with nothing above -inf gives token -1.  logprobs
  * (fp32, may be NULL): log of the token's share of the kept mass. */
 typedef struct {
   const void* logits;
