@@ -158,6 +158,21 @@ struct Row {
   }
 };
 
+// sum[slot] of the CTAs before this one and of all, in every thread (a lane
+// reads a CTA's).
+__device__ __forceinline__ void cluster_sums(cg::cluster_group& cl, SampleShared& sh, int slot, u64* before, u64* all) {
+  const unsigned lane = threadIdx.x & 31, nb = cl.num_blocks();
+  const u64 v = lane < nb ? cl.map_shared_rank(&sh, lane)->sum[slot] : 0;
+  u64 x = v, y = lane < cl.block_rank() ? v : 0;
+#pragma unroll
+  for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
+    x += __shfl_xor_sync(0xffffffffu, x, o);
+    y += __shfl_xor_sync(0xffffffffu, y, o);
+  }
+  *all = __shfl_sync(0xffffffffu, x, 0);
+  *before = __shfl_sync(0xffffffffu, y, 0);
+}
+
 // The histogram's crossing: with `bin_of(s)` (-1: not in question) of every
 // element, the bin in which the count (MASS: the mass) starting from `acc`
 // reaches the wanted one, what lies before it and what it holds (found.*, in
@@ -198,25 +213,28 @@ __device__ __forceinline__ void crossing(cg::cluster_group& cl, SampleShared& sh
 #pragma unroll
   for (int e = 0; e < kBins / kSampleThreads; ++e) {
     const int b = threadIdx.x * tp + e;
-    if (e < tp && b < per)
-      for (unsigned r = 0; r < nb; ++r) {
-        const SampleShared* o = cl.map_shared_rank(&sh, r);
-        bins[e] += o->bins[0][rank * per + b];
-        if (MASS)
-          bins[e] += (static_cast<u64>(o->bins[1][rank * per + b]) << 16) + (static_cast<u64>(o->bins[2][rank * per + b]) << 32);
+    if (e < tp && b < per) {
+      uint32_t w[MASS ? 3 : 1][kMaxCluster];  // all in flight at once
+#pragma unroll
+      for (unsigned r = 0; r < kMaxCluster; ++r) {
+        const SampleShared* o = cl.map_shared_rank(&sh, r < nb ? r : 0);
+#pragma unroll
+        for (int x = 0; x < (MASS ? 3 : 1); ++x) w[x][r] = r < nb ? o->bins[x][rank * per + b] : 0;
       }
+#pragma unroll
+      for (unsigned r = 0; r < kMaxCluster; ++r)
+#pragma unroll
+        for (int x = 0; x < (MASS ? 3 : 1); ++x) bins[e] += static_cast<u64>(w[x][r]) << (16 * x);
+    }
     mine += bins[e];
   }
   u64 t;
   u64 upto = cta_scan(mine, &t, sh.scan) - mine;
   if (threadIdx.x == 0) sh.sum[slot] = t;
   cl.sync();
-  u64 before = acc, all = 0;
-  for (unsigned r = 0; r < nb; ++r) {
-    const u64 x = cl.map_shared_rank(&sh, r)->sum[slot];
-    if (r < rank) before += x;
-    all += x;
-  }
+  u64 before, all;
+  cluster_sums(cl, sh, slot, &before, &all);
+  before += acc;
   const u64 want = want_of(all);
   upto += before;
 #pragma unroll
@@ -241,28 +259,19 @@ __device__ __forceinline__ int even_bin(float top, float s) {
   return min(static_cast<int>(__float_as_uint(__fmaf_rz(d, kBins / kMaxDist, 8388608.0f)) & 0x7FFFFFu), kBins - 1);
 }
 
-// Put the elements with in(s) into CTA 0's list (and their keys' range there).
+// Put the elements with in(s) into CTA 0's list (as many as it holds).
 template <bool BF16, bool RES, class F>
 __device__ __forceinline__ void gather(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, F in) {
   SampleShared* lead = cl.map_shared_rank(&sh, 0);
-  uint32_t lo = 0xFFFFFFFFu, hi = 0;
 #pragma unroll 4
   for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
     const float s = row.at(i);
     if (!in(s)) continue;
-    const uint32_t k = key_of(s), at = atomicAdd(&lead->n_cand, 1u);
-    lo = min(lo, k);
-    hi = max(hi, k);
+    const uint32_t at = atomicAdd(&lead->n_cand, 1u);
     if (at < kCand) {
-      lead->ckey[at] = k;
+      lead->ckey[at] = key_of(s);
       lead->cidx[at] = row.first + i;
     }
-  }
-  lo = __reduce_min_sync(0xffffffffu, lo);
-  hi = __reduce_max_sync(0xffffffffu, hi);
-  if ((threadIdx.x & 31) == 0 && hi >= lo) {
-    atomicMin(&lead->kmin, lo);
-    atomicMax(&lead->kmax, hi);
   }
   cl.sync();
 }
@@ -292,14 +301,6 @@ __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, R
     gather(cl, sh, row, [&](float s) { return bin_of(s) == at; });
     SampleShared* lead = cl.map_shared_rank(&sh, 0);
     const uint32_t n = lead->n_cand;
-    kmin = lead->kmin;
-    kmax = lead->kmax;
-    if (kmin == kmax) {  // all equal
-      const u64 each = MASS ? mass_of(expf(key_value(kmin) - top)) : 1;
-      const u64 need = (want - pre0 + each - 1) / each;
-      cl.sync();  // CTA 0 stays until its words are read
-      return {key_value(kmin), static_cast<uint32_t>(need), n};
-    }
     if (n <= kCand) {
       if (rank == 0) {
         const int i = threadIdx.x;
@@ -333,6 +334,29 @@ __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, R
       }
       cl.sync();
       return {key_value(sh.found.last_key), sh.found.ties, sh.found.of};
+    }
+    // too many: the range of their keys, to cut it again
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
+      const float s = row.at(i);
+      if (bin_of(s) != at) continue;
+      lo = min(lo, key_of(s));
+      hi = max(hi, key_of(s));
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if ((threadIdx.x & 31) == 0 && hi >= lo) {
+      atomicMin(&lead->kmin, lo);
+      atomicMax(&lead->kmax, hi);
+    }
+    cl.sync();
+    kmin = lead->kmin;
+    kmax = lead->kmax;
+    if (kmin == kmax) {  // all equal
+      const u64 each = MASS ? mass_of(expf(key_value(kmin) - top)) : 1;
+      const u64 need = (want - pre0 + each - 1) / each;
+      cl.sync();  // CTA 0 stays until its words are read
+      return {key_value(kmin), static_cast<uint32_t>(need), n};
     }
     shift = 0;
     while (((kmax - kmin) >> shift) >= kBins) ++shift;
@@ -431,11 +455,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     }
     if (threadIdx.x == 0) sh.best_key = bk, sh.best_idx = idx;
     cl.sync();
-    for (unsigned o = 0; o < nb; ++o) {
-      const SampleShared* q = cl.map_shared_rank(&sh, o);
-      const uint32_t x = q->best_key, y = q->best_idx;
-      if (x > bk || (x == bk && y < idx)) bk = x, idx = y;
-    }
+    const SampleShared* q = cl.map_shared_rank(&sh, lane < static_cast<int>(nb) ? lane : 0);
+    const uint32_t x = q->best_key, y = q->best_idx;
+    bk = __reduce_max_sync(0xffffffffu, x);
+    idx = __reduce_min_sync(0xffffffffu, x == bk ? y : 0xFFFFFFFFu);
   }
   float top = key_value(bk);
   if (row.greedy || top == -INFINITY) {  // the same in every CTA of the cluster
@@ -524,18 +547,42 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     sh.sum[4] = t;
   }
   cl.sync();
-  u64 total = 0, before = 0;
-  for (unsigned o = 0; o < nb; ++o) {
-    const u64 t = cl.map_shared_rank(&sh, o)->sum[4];
-    if (o < rank) before += t;
-    total += t;
-  }
+  u64 total, before;
+  cluster_sums(cl, sh, 4, &before, &total);
+  cl.barrier_arrive();  // its words are read; no CTA leaves before all have read
   for (int w = 0; w < warp; ++w) before += sh.wmass[w];
   const u64 x = static_cast<u64>(fmax(floor(static_cast<double>(a.u[r]) * static_cast<double>(total)), 0.0));
   const u64 goal = x < total ? x : total - 1;
   if (before <= goal && goal < before + m) {  // this warp's run holds the token
+    int b = i0;
     ties = tie0;
-    for (int b = i0; b < i1; b += 32) {
+    if (!ranked) {  // 32 blocks of the run at a time: a lane adds up a block, then the right block is taken apart
+      for (; b < i1; b += 1024) {
+        u64 e = 0;
+        for (int j = 0; j < 32; ++j) {  // rotated, so that the lanes use different banks
+          const int i = b + 32 * lane + ((j + lane) & 31);
+          const float s = i < i1 ? row.at(i) : -INFINITY;
+          if (i >= i1 || !(all || s >= cut.last)) continue;
+          const float w = expf(s - top);
+          if (w >= min_p) e += mass_of(w);
+        }
+        u64 upto = e;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += y;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + upto > goal);
+        if (past) {
+          const int blk = __ffs(past) - 1;
+          before += __shfl_sync(0xffffffffu, upto - e, blk);
+          b += 32 * blk;
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    for (; b < i1; b += 32) {
       const u64 e = kept_mass(b + lane);
       u64 upto = e;
 #pragma unroll
@@ -551,7 +598,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       if (before > goal) break;
     }
   }
-  cl.sync();  // no CTA leaves while another reads its words
+  cl.barrier_wait();
 }
 
 template <bool BF16, bool RES>
