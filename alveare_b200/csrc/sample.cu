@@ -116,7 +116,8 @@ struct Row {
   float* vals;
   int n, first;      // elements of the slice, index of its first
   float temp;
-  bool greedy, infinite;  // infinite: the largest value is +inf, only those count
+  bool greedy;
+  bool infinite;  // without a copy: +inf is the largest value and reads as 0, the rest as -inf
   __device__ __forceinline__ float value(float x) const {
     if (!greedy && temp != 1.0f) x = __fdiv_rn(x, temp);
     if (x != x) x = -INFINITY;
@@ -126,9 +127,27 @@ struct Row {
     return BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(base)[i]) : static_cast<const float*>(base)[i];
   }
   __device__ __forceinline__ float at(int i) const {
-    float x = RES ? vals[i] : value(raw(i));
-    if (infinite) x = x == INFINITY ? 0.f : -INFINITY;
-    return x;
+    if (RES) return vals[i];
+    const float x = value(raw(i));
+    return !infinite ? x : x == INFINITY ? 0.f : -INFINITY;
+  }
+  // f(i, value) for i in [i0, i1) (i0 a multiple of 4), `step` threads from
+  // `first`, four values at a time; in shared memory -inf may follow past i1.
+  template <class F>
+  __device__ __forceinline__ void each(int i0, int i1, int first, int step, F f) const {
+    if (RES) {
+#pragma unroll 2
+      for (int i = i0 + 4 * first; i < i1; i += 4 * step) {
+        const float4 v = *reinterpret_cast<const float4*>(vals + i);
+        f(i, v.x);
+        f(i + 1, v.y);
+        f(i + 2, v.z);
+        f(i + 3, v.w);
+      }
+    } else {
+#pragma unroll 4
+      for (int i = i0 + first; i < i1; i += step) f(i, at(i));
+    }
   }
   // f(i, value) for every element of the slice, 16-byte loads where aligned.
   template <class F>
@@ -190,11 +209,9 @@ __device__ __forceinline__ void crossing(cg::cluster_group& cl, SampleShared& sh
     sh.found.bin = -1;
   }
   __syncthreads();
-#pragma unroll 4
-  for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
-    const float s = row.at(i);
+  row.each(0, row.n, threadIdx.x, kSampleThreads, [&](int, float s) {
     const int b = bin_of(s);
-    if (b < 0) continue;
+    if (b < 0) return;
     if (MASS) {
       const u64 m = mass_of(expf(s - top));
       const uint32_t m0 = static_cast<uint32_t>(m) & 0xFFFFu, m1 = static_cast<uint32_t>(m >> 16) & 0xFFFFu,
@@ -205,7 +222,7 @@ __device__ __forceinline__ void crossing(cg::cluster_group& cl, SampleShared& sh
     } else {
       atomicAdd(&sh.bins[0][b], 1u);
     }
-  }
+  });
   cl.sync();
   // CTA r adds up bins [r, r + 1) * kBins / nb of all CTAs
   const int per = kBins / nb, tp = (per + kSampleThreads - 1) / kSampleThreads;
@@ -263,16 +280,14 @@ __device__ __forceinline__ int even_bin(float top, float s) {
 template <bool BF16, bool RES, class F>
 __device__ __forceinline__ void gather(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, F in) {
   SampleShared* lead = cl.map_shared_rank(&sh, 0);
-#pragma unroll 4
-  for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
-    const float s = row.at(i);
-    if (!in(s)) continue;
+  row.each(0, row.n, threadIdx.x, kSampleThreads, [&](int i, float s) {
+    if (!in(s)) return;
     const uint32_t at = atomicAdd(&lead->n_cand, 1u);
     if (at < kCand) {
       lead->ckey[at] = key_of(s);
       lead->cidx[at] = row.first + i;
     }
-  }
+  });
   cl.sync();
 }
 
@@ -298,7 +313,8 @@ __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, R
     }
     const int at = round > 0 ? sh.found.bin : bin;
     const u64 pre0 = round > 0 ? sh.found.before : acc;
-    gather(cl, sh, row, [&](float s) { return bin_of(s) == at; });
+    if (round == 0) gather(cl, sh, row, [&](float s) { return even_bin(top, s) == at && s >= floor_s; });
+    else gather(cl, sh, row, [&](float s) { return bin_of(s) == at; });
     SampleShared* lead = cl.map_shared_rank(&sh, 0);
     const uint32_t n = lead->n_cand;
     if (n <= kCand) {
@@ -337,12 +353,11 @@ __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, R
     }
     // too many: the range of their keys, to cut it again
     uint32_t lo = 0xFFFFFFFFu, hi = 0;
-    for (int i = threadIdx.x; i < row.n; i += kSampleThreads) {
-      const float s = row.at(i);
-      if (bin_of(s) != at) continue;
+    row.each(0, row.n, threadIdx.x, kSampleThreads, [&](int, float s) {
+      if (bin_of(s) != at) return;
       lo = min(lo, key_of(s));
       hi = max(hi, key_of(s));
-    }
+    });
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
     if ((threadIdx.x & 31) == 0 && hi >= lo) {
@@ -442,6 +457,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     if (RES) row.vals[i] = s;
     if (s > best || (s == best && i < bi)) best = s, bi = i;
   });
+  if (RES && threadIdx.x < 4 && (row.n & 3) && threadIdx.x >= (row.n & 3)) row.vals[(row.n & ~3) + threadIdx.x] = -INFINITY;
   uint32_t bk = key_of(best), idx = bi == INT_MAX ? 0xFFFFFFFFu : static_cast<uint32_t>(row.first + bi);
   {
     const uint32_t wk = __reduce_max_sync(0xffffffffu, bk);
@@ -469,8 +485,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     cl.sync();  // no CTA leaves while another reads its words
     return;
   }
-  row.infinite = top == INFINITY;
-  if (row.infinite) top = 0.f;
+  if (top == INFINITY) {  // only the infinite ones count, all alike: as 0 among -inf
+    row.infinite = true;
+    top = 0.f;
+    if (RES) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < row.n; i += kSampleThreads) row.vals[i] = row.vals[i] == INFINITY ? 0.f : -INFINITY;
+    }
+  }
+  __syncthreads();
 
   // ---- where the kept prefix ends
   Cut cut{-INFINITY, 0, 0};
@@ -507,7 +530,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   }
 
   // ---- the kept mass of every warp's run of the slice, then the token
-  const int seg = (row.n + kSampleWarps * 32 - 1) / (kSampleWarps * 32) * 32;
+  const int seg = (row.n + kSampleWarps * 128 - 1) / (kSampleWarps * 128) * 128;
   const int i0 = min(warp * seg, row.n), i1 = min(i0 + seg, row.n);
   const bool ranked = !all && cut.ties < cut.of;  // only some of the equals are kept
   uint32_t tie0 = 0;
@@ -536,7 +559,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     return w >= min_p ? mass_of(w) : 0;
   };
   u64 m = 0;
-  for (int b = i0; b < i1; b += 32) m += kept_mass(b + lane);
+  const float least = all ? -INFINITY : cut.last;
+  if (ranked) {
+    for (int b = i0; b < i1; b += 32) m += kept_mass(b + lane);
+  } else {
+    row.each(i0, i1, lane, 32, [&](int, float s) {
+      if (!(s >= least)) return;
+      const float w = expf(s - top);
+      if (w >= min_p) m += mass_of(w);
+    });
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
   if (lane == 0) sh.wmass[warp] = m;
