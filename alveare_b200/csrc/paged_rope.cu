@@ -15,6 +15,7 @@ namespace alv {
 namespace {
 
 constexpr int kRopeThreads = 256;
+constexpr int kRopeTokens = 8;  // tokens of a CTA at most
 
 struct RopeArgs {
   PagedView c;
@@ -23,7 +24,7 @@ struct RopeArgs {
   uint16_t* q_out;
   int64_t q_tok, q_head;   // elements
   const void* table;       // [max_pos][2 rot]: cos (rot) | sin (rot)
-  int max_pos, rot, nq, hd;
+  int max_pos, rot, nq, tokens_per_cta;
   const float *qw, *kw;
   float eps;
 };
@@ -64,74 +65,120 @@ __device__ __forceinline__ int seq_of(const PagedView& c, int t) {
   return lo;
 }
 
-// One (token, head) per group of hd / 16 lanes.  Each lane holds two groups of
-// eight values: a rotation pair's two halves, or 16 that pass through.
-template <bool F32, bool TF32>
+// A CTA takes `tokens_per_cta` tokens: first their sequences, positions and
+// cache slots (a thread each), then all their heads, one per group of HD / 16
+// lanes.  Each lane holds two groups of eight values: a rotation pair's two
+// halves, or 16 that pass through.  Two units are loaded before either is
+// worked on.
+template <int HD, bool F32, bool TF32>
 __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeArgs a) {
+  constexpr int LPH = HD / 16;
+  __shared__ int pos_of[kRopeTokens];          // -1: skipped
+  __shared__ int64_t slot_of[kRopeTokens];     // element of the cache, -1: no page
   const PagedView& c = a.c;
-  const int heads = a.nq + 2 * c.nkv, lph = a.hd / 16;
-  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kRopeThreads + threadIdx.x) / lph;
-  const int l = threadIdx.x % lph;
-  const int t = static_cast<int>(unit / heads), head = static_cast<int>(unit % heads);
-  const bool real = t < c.tokens;
-  const bool is_q = head < a.nq, is_k = !is_q && head < a.nq + c.nkv;
-  const int pairs = a.rot / 16;
-  const bool turn = l < pairs && !(!is_q && !is_k);
+  const int t0 = blockIdx.x * a.tokens_per_cta, nt = min(a.tokens_per_cta, c.tokens - t0);
+  pdl_wait();
+  pdl_trigger();
+  if (threadIdx.x < nt) {
+    const int t = t0 + threadIdx.x, b = seq_of(c, t);
+    const SeqSpan s = seq_span(c, b);
+    int pos = s.kv - s.qlen + (t - s.q0);
+    int64_t slot = -1;
+    if (t < s.q0 || t >= s.q0 + s.qlen || pos < 0 || pos >= a.max_pos) {
+      atomicOr(c.status, kStatusBadIndex);
+      pos = -1;
+    } else {
+      const int page = page_of(c, b, pos);
+      if (page >= 0) slot = page * c.page_stride + (pos % c.page_size) * c.row_stride;
+    }
+    pos_of[threadIdx.x] = pos;
+    slot_of[threadIdx.x] = slot;
+  }
+  __syncthreads();
+  const int lanes = (a.nq + 2 * c.nkv) * LPH, total = nt * lanes;  // lanes of a token, of the CTA
+  const int l = threadIdx.x % LPH, pairs = a.rot / 16;
   const int d0 = l < pairs ? 8 * l : a.rot + 16 * (l - pairs);
   const int d1 = l < pairs ? a.rot / 2 + 8 * l : d0 + 8;
-  float x0[8] = {}, x1[8] = {};
-  if (real) {
-    const int64_t at = t * a.qkv_stride + static_cast<int64_t>(head) * a.hd;
-    load8<F32>(a.qkv, at + d0, x0);
-    load8<F32>(a.qkv, at + d1, x1);
-  }
-  const float* w = is_q ? a.qw : (is_k ? a.kw : nullptr);
-  float ss = 0.f;
+  // this thread's unit and the token and place in it, moved on by kRopeThreads at a time
+  int u = threadIdx.x, i = u / lanes, v = u - i * lanes;
+  auto next = [&] {
+    u += kRopeThreads;
+    v += kRopeThreads;
+    while (v >= lanes) v -= lanes, ++i;
+  };
+  while (u - static_cast<int>(threadIdx.x & 31) < total) {  // warps stay whole
+    float x0[2][8] = {}, x1[2][8] = {};
+    int ti[2], hd_[2];
+    bool real[2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ss += x0[i] * x0[i] + x1[i] * x1[i];
-  for (int o = lph / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (!real) return;
-  if (w) {
-    const float inv = 1.0f / sqrtf(ss / static_cast<float>(a.hd) + a.eps);
-    float w0[8], w1[8];
-    load8<true>(w, d0, w0);
-    load8<true>(w, d1, w1);
+    for (int k = 0; k < 2; ++k) {
+      real[k] = u < total;
+      ti[k] = i;
+      hd_[k] = v / LPH;
+      if (real[k]) {
+        const int64_t at = static_cast<int64_t>(t0 + i) * a.qkv_stride + hd_[k] * HD;
+        load8<F32>(a.qkv, at + d0, x0[k]);
+        load8<F32>(a.qkv, at + d1, x1[k]);
+      }
+      next();
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x0[i] = x0[i] * inv * w0[i];
-      x1[i] = x1[i] * inv * w1[i];
+    for (int k = 0; k < 2; ++k) {
+      const int head = hd_[k];
+      const bool is_q = head < a.nq, is_k = !is_q && head < a.nq + c.nkv;
+      const float* w = is_q ? a.qw : (is_k ? a.kw : nullptr);
+      if (a.qw || a.kw) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += x0[k][e] * x0[k][e] + x1[k][e] * x1[k][e];
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (w && real[k]) {
+          const float inv = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
+          float w0[8], w1[8];
+          load8<true>(w, d0, w0);
+          load8<true>(w, d1, w1);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x0[k][e] = x0[k][e] * inv * w0[e];
+            x1[k][e] = x1[k][e] * inv * w1[e];
+          }
+        }
+      }
+      if (!real[k]) continue;
+      const int pos = pos_of[ti[k]];
+      if (pos < 0) continue;
+      if (l < pairs && (is_q || is_k)) {
+        float cs[8], sn[8];
+        const int64_t at = static_cast<int64_t>(pos) * 2 * a.rot + d0;
+        load8<TF32>(a.table, at, cs);
+        load8<TF32>(a.table, at + a.rot, sn);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y0 = x0[k][e] * cs[e] - x1[k][e] * sn[e], y1 = x1[k][e] * cs[e] + x0[k][e] * sn[e];
+          x0[k][e] = y0;
+          x1[k][e] = y1;
+        }
+      }
+      uint16_t* dst;
+      if (is_q) {
+        dst = a.q_out + static_cast<int64_t>(t0 + ti[k]) * a.q_tok + head * a.q_head;
+      } else {
+        if (slot_of[ti[k]] < 0) continue;
+        dst = (is_k ? c.k : c.v) + slot_of[ti[k]] + (head - a.nq - (is_k ? 0 : c.nkv)) * c.head_stride;
+      }
+      store8(dst + d0, x0[k]);
+      store8(dst + d1, x1[k]);
     }
   }
-  const int b = seq_of(c, t);
-  const SeqSpan s = seq_span(c, b);
-  const int pos = s.kv - s.qlen + (t - s.q0);
-  if (t < s.q0 || t >= s.q0 + s.qlen || pos < 0 || pos >= a.max_pos) {
-    atomicOr(c.status, kStatusBadIndex);
-    return;
-  }
-  if (turn) {
-    float cs[8], sn[8];
-    const int64_t at = static_cast<int64_t>(pos) * 2 * a.rot + d0;
-    load8<TF32>(a.table, at, cs);
-    load8<TF32>(a.table, at + a.rot, sn);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y0 = x0[i] * cs[i] - x1[i] * sn[i], y1 = x1[i] * cs[i] + x0[i] * sn[i];
-      x0[i] = y0;
-      x1[i] = y1;
-    }
-  }
-  uint16_t* dst;
-  if (is_q) {
-    dst = a.q_out + t * a.q_tok + head * a.q_head;
-  } else {
-    const int page = page_of(c, b, pos);
-    if (page < 0) return;
-    const int kvh = head - a.nq - (is_k ? 0 : c.nkv);
-    dst = (is_k ? c.k : c.v) + page * c.page_stride + kvh * c.head_stride + (pos % c.page_size) * c.row_stride;
-  }
-  store8(dst + d0, x0);
-  store8(dst + d1, x1);
+}
+
+template <int HD>
+int launch_rope(alv_ctx* ctx, const RopeArgs& a, bool xf, bool tf, cudaStream_t st) {
+  auto k = xf ? (tf ? qk_norm_rope_kernel<HD, true, true> : qk_norm_rope_kernel<HD, true, false>)
+              : (tf ? qk_norm_rope_kernel<HD, false, true> : qk_norm_rope_kernel<HD, false, false>);
+  const unsigned grid = static_cast<unsigned>((a.c.tokens + a.tokens_per_cta - 1) / a.tokens_per_cta);
+  return launch_ex(ctx, k, dim3(grid), dim3(kRopeThreads), 0, st, true, a);
 }
 
 }  // namespace
@@ -191,19 +238,18 @@ extern "C" int alv_qk_norm_rope(alv_ctx* ctx, const alv_paged* cache, const alv_
   a.max_pos = args->max_pos;
   a.rot = args->rot;
   a.nq = args->heads;
-  a.hd = hd;
   a.qw = args->q_weight;
   a.kw = args->k_weight;
   a.eps = args->eps;
-  const int64_t threads = static_cast<int64_t>(cache->tokens) * heads * (hd / 16);
-  const int64_t grid = (threads + kRopeThreads - 1) / kRopeThreads;
-  if (grid == 0 || cache->batch == 0) return ALV_OK;
-  if (grid > INT_MAX) return fail(ctx, ALV_ERR_UNSUPPORTED, "qk_norm_rope: too many tokens for one call");
+  if (cache->tokens == 0 || cache->batch == 0) return ALV_OK;
+  // a token per CTA while that leaves SMs idle, then up to 8: the look-up of a
+  // CTA's tokens is shared
+  a.tokens_per_cta = std::max(1, std::min(kRopeTokens, cache->tokens / (ctx->num_sms * 4)));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool xf = args->qkv_dtype == ALV_F32, tf = args->rope_dtype == ALV_F32;
-  auto k = xf ? (tf ? qk_norm_rope_kernel<true, true> : qk_norm_rope_kernel<true, false>)
-              : (tf ? qk_norm_rope_kernel<false, true> : qk_norm_rope_kernel<false, false>);
-  k<<<static_cast<unsigned>(grid), kRopeThreads, 0, st>>>(a);
-  ALV_CUDA(ctx, cudaGetLastError());
-  return ALV_OK;
+  switch (hd) {
+    case 64: return launch_rope<64>(ctx, a, xf, tf, st);
+    case 128: return launch_rope<128>(ctx, a, xf, tf, st);
+    default: return launch_rope<256>(ctx, a, xf, tf, st);
+  }
 }

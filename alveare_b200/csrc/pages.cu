@@ -73,25 +73,26 @@ __device__ __forceinline__ void count(const PagesArgs& a, int page, int by) {
   else if (page >= a.pages) atomicOr(a.status, kStatusBadIndex);
 }
 
-// Whether ids[0 .. n) (stride apart) repeat a slot, by a bitmap in shared
-// memory; with `others`, also whether one of those is among them.
-__device__ bool ids_clash(const PagesArgs& a, uint32_t* bits, const int* ids, int n, int stride, const int* others) {
-  if (n < 2) return false;
-  for (int i = threadIdx.x; i < (a.slots + 31) / 32; i += blockDim.x) bits[i] = 0;
-  __syncthreads();
+// Which lists name a slot twice (bit 0: free, bit 1: fork, as a child or as a
+// child that is another pair's parent, bit 2: extend), by three bitmaps in
+// shared memory.
+__device__ int lists_clash(const PagesArgs& a, uint32_t* bits) {
+  const int words = (a.slots + 31) / 32;
   int clash = 0;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int s = ids[static_cast<int64_t>(i) * stride];
-    if (s < 0 || s >= a.slots) continue;
-    clash |= (atomicOr(bits + s / 32, 1u << (s % 32)) >> (s % 32)) & 1;
-  }
+  auto mark = [&](uint32_t* set, int slot, int bit) {
+    if (slot >= 0 && slot < a.slots && (atomicOr(set + slot / 32, 1u << (slot % 32)) >> (slot % 32) & 1)) clash |= bit;
+  };
+  for (int i = threadIdx.x; i < 3 * words; i += blockDim.x) bits[i] = 0;
   __syncthreads();
-  if (others)
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const int s = others[static_cast<int64_t>(i) * stride];
-      if (s >= 0 && s < a.slots && s != ids[static_cast<int64_t>(i) * stride]) clash |= (bits[s / 32] >> (s % 32)) & 1;
-    }
-  return __syncthreads_or(clash);
+  for (int i = threadIdx.x; i < a.n_free; i += blockDim.x) mark(bits, a.free_ids[i], 1);
+  for (int i = threadIdx.x; i < a.n_fork; i += blockDim.x) mark(bits + words, a.fork[2 * i + 1], 2);
+  for (int i = threadIdx.x; i < a.n_extend; i += blockDim.x) mark(bits + 2 * words, a.extend[2 * i], 4);
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.n_fork; i += blockDim.x) {
+    const int par = a.fork[2 * i];
+    if (par >= 0 && par < a.slots && par != a.fork[2 * i + 1] && (bits[words + par / 32] >> (par % 32) & 1)) clash |= 2;
+  }
+  return __syncthreads_or(clash & 1) * 1 | (__syncthreads_or(clash & 2) ? 2 : 0) | (__syncthreads_or(clash & 4) ? 4 : 0);
 }
 
 // Slots free_ids[i0 .. i1): one warp per slot.
@@ -159,75 +160,80 @@ __device__ __forceinline__ Need need_of(const PagesArgs& a, int i) {
 // Extends i0 .. i1 (no slot twice).  Returns the index of the first that does
 // not fit, or i1.  `used` and `moves` accumulate the call's totals.
 __device__ int extend_slots(const PagesArgs& a, int i0, int i1, int64_t* used, int* moves, int64_t* sh) {
-  // pages wanted by the whole list (an entry past the table's width ends it);
+  __shared__ int first_bad;
+  __shared__ int64_t given;
+  // pages wanted by the whole list, up to an entry past the table's width;
   // which last pages are shared is decided before any count changes
-  int64_t total = 0, t;
-  int stop = i1;
+  if (threadIdx.x == 0) first_bad = INT_MAX;
+  __syncthreads();
+  Need n{-1, 0, 0, 0, -1, true};  // the entry of the last round: the only one of a list of up to 1024
+  int64_t total = 0, t, mine = 0;
   for (int base = i0; base < i1; base += blockDim.x) {
     const int i = base + threadIdx.x;
-    int64_t want = 0;
-    int bad = INT_MAX;
     if (i < i1) {
-      const Need n = need_of(a, i);
-      if (!n.ok) bad = i;
-      else want = n.slot < 0 ? 0 : n.want - n.have + (n.cow >= 0);
+      n = need_of(a, i);
+      if (!n.ok) atomicMin(&first_bad, i);
+      else mine += n.slot < 0 ? 0 : n.want - n.have + (n.cow >= 0);
       a.cow[i] = n.cow;
     }
-    cta_scan(want, &t, sh);
-    total += t;
-    bad = __reduce_min_sync(0xffffffffu, bad);
-    __shared__ int first_bad;
-    if (threadIdx.x == 0) first_bad = INT_MAX;
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0 && bad != INT_MAX) atomicMin(&first_bad, bad);
-    __syncthreads();
-    if (first_bad < stop) stop = first_bad;
-    __syncthreads();
   }
+  cta_scan(mine, &total, sh);  // (of entries past first_bad too: more pages are listed than handed out)
+  const int stop = min(i1, first_bad);
   // free pages in ascending order, as many as wanted
   int64_t have = 0;
-  for (int base = 0; base < a.pages; base += blockDim.x) {
-    const int p = base + threadIdx.x;
-    const bool is_free = p < a.pages && a.refs[p] == 0;
-    const int64_t r = have + cta_scan(is_free ? 1 : 0, &t, sh);
-    if (is_free && r < total) a.avail[r] = p;
+  for (int base = 0; base < a.pages; base += 4 * blockDim.x) {
+    int is_free[4], c = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int p = base + 4 * threadIdx.x + e;
+      is_free[e] = p < a.pages && a.refs[p] == 0;
+      c += is_free[e];
+    }
+    int64_t r = have + cta_scan(c, &t, sh);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (is_free[e]) {
+        if (r < total) a.avail[r] = base + 4 * threadIdx.x + e;
+        ++r;
+      }
     have += t;
   }
   __syncthreads();
   // hand them out in list order
+  const bool kept = i1 - i0 <= static_cast<int>(blockDim.x);
   int64_t at = 0;
   int n_moves = *moves;
   int fail = stop;
   for (int base = i0; base < stop; base += blockDim.x) {
     const int i = base + threadIdx.x;
-    Need n{-1, 0, 0, 0, -1, true};
-    int64_t want = 0;
-    if (i < stop) {
-      n = need_of(a, i);
-      n.cow = a.cow[i];
-      want = n.slot < 0 ? 0 : n.want - n.have + (n.cow >= 0);
+    if (!kept) {
+      n = Need{-1, 0, 0, 0, -1, true};
+      if (i < stop) {
+        n = need_of(a, i);
+        n.cow = a.cow[i];
+      }
     }
-    const int64_t first = at + cta_scan(want, &t, sh);
+    const int64_t want = i < stop && n.slot >= 0 ? n.want - n.have + (n.cow >= 0) : 0;
+    // pages and copies in one sum: copies in the high part
+    const int64_t both = cta_scan(want + (i < stop && n.slot >= 0 && n.cow >= 0 ? int64_t{1} << 44 : 0), &t, sh);
+    const int64_t first = at + (both & ((int64_t{1} << 44) - 1));
     const bool fits = i < stop && first + want <= have;
-    __shared__ int first_fail;
-    __shared__ int64_t given;
     if (threadIdx.x == 0) {
-      first_fail = INT_MAX;
+      first_bad = INT_MAX;
       given = at;
     }
     __syncthreads();
-    if (i < stop && !fits) atomicMin(&first_fail, i);
+    if (i < stop && !fits) atomicMin(&first_bad, i);
     __syncthreads();
-    const bool apply = fits && i < first_fail && n.slot >= 0;
-    if (apply) atomicMax(reinterpret_cast<unsigned long long*>(&given), static_cast<unsigned long long>(first + want));
-    int64_t moved;
-    const int64_t mv = n_moves + cta_scan(apply && n.cow >= 0 ? 1 : 0, &moved, sh);
+    const int unmet = first_bad;
+    const bool apply = fits && i < unmet && n.slot >= 0;
     if (apply) {
+      if (unmet != INT_MAX) atomicMax(reinterpret_cast<unsigned long long*>(&given), static_cast<unsigned long long>(first + want));
       int* row = a.table + n.slot * a.table_stride;
       int64_t next = first;
       if (n.cow >= 0) {
         const int dst = a.avail[next++];
-        a.moves[mv] = make_int2(n.cow, dst);
+        a.moves[n_moves + static_cast<int>(both >> 44)] = make_int2(n.cow, dst);
         atomicSub(a.refs + n.cow, 1);
         a.refs[dst] = 1;
         row[n.have - 1] = dst;
@@ -239,15 +245,14 @@ __device__ int extend_slots(const PagesArgs& a, int i0, int i1, int64_t* used, i
       }
       a.lens[n.slot] = n.len + a.extend[2 * i + 1];
     }
-    __syncthreads();
-    n_moves += static_cast<int>(moved);
-    at = given;
-    const int ff = first_fail;
-    __syncthreads();
-    if (ff != INT_MAX) {
-      fail = ff;
+    if (unmet != INT_MAX) {
+      n_moves += __syncthreads_count(apply && n.cow >= 0);
+      at = given;
+      fail = unmet;
       break;
     }
+    n_moves += static_cast<int>(t >> 44);
+    at += t & ((int64_t{1} << 44) - 1);
   }
   *moves = n_moves;
   *used += at;
@@ -257,19 +262,21 @@ __device__ int extend_slots(const PagesArgs& a, int i0, int i1, int64_t* used, i
 __global__ void __launch_bounds__(kPageThreads, 1) pages_update_kernel(const PagesArgs a) {
   extern __shared__ uint32_t bits[];
   __shared__ int64_t sh[32];
+  pdl_wait();
   pdl_trigger();
   // A list that names a slot twice is taken one entry at a time.
-  bool one = ids_clash(a, bits, a.free_ids, a.n_free, 1, nullptr);
+  const int clash = lists_clash(a, bits);
+  bool one = clash & 1;
   for (int i = 0; i < a.n_free; i = one ? i + 1 : a.n_free) {
     drop_slots(a, i, one ? i + 1 : a.n_free);
     __syncthreads();
   }
-  one = ids_clash(a, bits, a.fork + 1, a.n_fork, 2, a.fork);
+  one = clash & 2;
   for (int i = 0; i < a.n_fork; i = one ? i + 1 : a.n_fork) {
     fork_slots(a, i, one ? i + 1 : a.n_fork);
     __syncthreads();
   }
-  one = ids_clash(a, bits, a.extend, a.n_extend, 2, nullptr);
+  one = clash & 4;
   int moves = 0, done = 0;
   int64_t used = 0;
   while (done < a.n_extend) {
@@ -307,6 +314,7 @@ struct CompactArgs {
 
 __global__ void __launch_bounds__(kPageThreads, 1) pages_compact_kernel(const CompactArgs a) {
   __shared__ int64_t sh[32];
+  pdl_wait();
   pdl_trigger();
   int64_t t, n = 0;
   for (int p = threadIdx.x; p < a.pages; p += blockDim.x) n += a.refs[p] > 0;
@@ -412,7 +420,7 @@ int check_pages(alv_ctx* ctx, const char* who, const alv_pages* p) {
   if (p->page_bytes % 16 || p->page_stride % 16 || p->layer_stride % 16 || p->page_stride < p->page_bytes ||
       p->layer_stride < 0 || ((reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v)) & 15))
     return fail(ctx, ALV_ERR_ARG, w + ": pages must be 16-byte aligned blocks of whole 16 bytes");
-  if (p->slots > 1 << 20) return fail(ctx, ALV_ERR_UNSUPPORTED, w + ": at most 1,048,576 slots");
+  if (p->slots > 1 << 19) return fail(ctx, ALV_ERR_UNSUPPORTED, w + ": at most 524,288 slots");
   return ALV_OK;
 }
 
@@ -471,10 +479,10 @@ extern "C" int alv_pages_update(alv_ctx* ctx, const alv_pages* p, const int32_t*
   a.moves = reinterpret_cast<int2*>(ws + o_moves);
   a.cow = reinterpret_cast<int*>(ws + o_cow);
   a.avail = reinterpret_cast<int*>(ws + o_avail);
-  const size_t smem = static_cast<size_t>((p->slots + 31) / 32) * 4;
+  const size_t smem = static_cast<size_t>((p->slots + 31) / 32) * 12;  // three bitmaps
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if ((rc = prepare_kernel(ctx, pages_update_kernel, smem))) return rc;
-  if ((rc = launch_ex(ctx, pages_update_kernel, dim3(1), dim3(kPageThreads), smem, st, false, a))) return rc;
+  if ((rc = launch_ex(ctx, pages_update_kernel, dim3(1), dim3(kPageThreads), smem, st, true, a))) return rc;
   if (n_extend == 0) return ALV_OK;
   CopyArgs c = copy_args(ctx, p);
   c.n_moves = a.n_moves;
@@ -504,7 +512,7 @@ extern "C" int alv_pages_compact(alv_ctx* ctx, const alv_pages* p, int32_t* tabl
   a.to = reinterpret_cast<int*>(ws + o_to);
   a.holes = reinterpret_cast<int*>(ws + o_holes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if ((rc = launch_ex(ctx, pages_compact_kernel, dim3(1), dim3(kPageThreads), 0, st, false, a))) return rc;
+  if ((rc = launch_ex(ctx, pages_compact_kernel, dim3(1), dim3(kPageThreads), 0, st, true, a))) return rc;
   CopyArgs c = copy_args(ctx, p);
   c.n_moves = a.n_moves;
   c.moves = a.moves;

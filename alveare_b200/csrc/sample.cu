@@ -20,6 +20,7 @@
 // Where top-k leaves few elements, that CTA finishes the row by itself.
 #include <cooperative_groups.h>
 
+#include "common.cuh"
 #include "internal.h"
 
 namespace alv {
@@ -440,6 +441,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   const unsigned rank = cl.block_rank(), nb = cl.num_blocks();
   const int r = blockIdx.x / nb, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Row<BF16, RES> row;
+  pdl_wait();
+  pdl_trigger();
   row.first = min(static_cast<int>(rank) * a.slice, a.vocab);
   row.n = min(a.slice, a.vocab - row.first);
   row.base = static_cast<const char*>(a.logits) + (r * a.stride + row.first) * (BF16 ? 2 : 4);
@@ -644,12 +647,14 @@ int launch_sample(alv_ctx* ctx, const SampleArgs& a, int rows, int cluster, cuda
   cfg.blockDim = dim3(kSampleThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   ALV_CUDA(ctx, cudaLaunchKernelEx(&cfg, k, a));
   return ALV_OK;
 }
