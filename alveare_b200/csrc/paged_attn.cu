@@ -28,10 +28,11 @@ struct RowWalk {
     return rows > a.row_max ? 0 : static_cast<int>((rows + kRowsPerBlock - 1) / kRowsPerBlock);
   }
   __device__ __forceinline__ void load(const AttnArgs& a) {
-    const int64_t r0 = static_cast<int64_t>(blk) * kRowsPerBlock;
-    nrow = static_cast<int>(min(static_cast<int64_t>(kRowsPerBlock), static_cast<int64_t>(s.qlen) * a.group - r0));
-    p0 = s.kv - s.qlen + static_cast<int>(r0 / a.group);
-    p1 = s.kv - s.qlen + static_cast<int>((r0 + nrow - 1) / a.group);
+    // (rows of one kv head fit 31 bits: q itself would be larger than memory)
+    const int r0 = blk * kRowsPerBlock;
+    nrow = min(kRowsPerBlock, s.qlen * a.group - r0);
+    p0 = s.kv - s.qlen + r0 / a.group;
+    p1 = s.kv - s.qlen + (r0 + nrow - 1) / a.group;
     r = slice_range<R::kSlice>(p0, p1, a.window, a.sinks);
   }
   // A block that sees nothing still has one (empty) unit: it writes zeros.
@@ -72,12 +73,17 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
   extern __shared__ uint8_t smem_dyn[];
   __shared__ __align__(8) uint64_t full[kRowWarps][NS];
   __shared__ int64_t sums[kRowWarps];
-  __shared__ int64_t start_before;
-  __shared__ int start_b;
+  __shared__ int longest[kRowWarps], shortest[kRowWarps];  // blocks
+  __shared__ RowWalk<HD> start;                              // where the run starts, at its sequence's first block
+  __shared__ int64_t start_rest, start_head;                 // how far into the sequence; the length of a kv head's blocks
   __shared__ uint32_t arrived;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* smem = smem_dyn + (((smem_u32(smem_dyn) + 1023u) & ~1023u) - smem_u32(smem_dyn));
   if (lane < NS) mbar_init(&full[warp][lane], 1);
+  if (threadIdx.x == 0) {
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
+  }
   fence_mbar_init();
   // Programmatic launch: inputs are touched once the kernel before is done.
   // Beside a chunk kernel (which has waited itself, and triggered after that)
@@ -89,18 +95,33 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
   RowWalk<HD> w{};
   int64_t total, u0, u1;
   int G;  // CTAs that get a run
+  bool cut = true;
   {
     const int per = (a.c.batch + kRowWarps * 32 - 1) / (kRowWarps * 32);
     const int b0 = threadIdx.x * per, b1 = min(b0 + per, a.c.batch);
     int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += w.length_of(a, seq_span(a.c, b)) * a.c.nkv;
+    int most = 0, least = INT_MAX;
+    for (int b = b0; b < b1; ++b) {
+      const int64_t len = w.length_of(a, seq_span(a.c, b));
+      mine += len * a.c.nkv;
+      if (len) {
+        most = max(most, w.length());
+        least = min(least, w.length());
+      }
+    }
     int64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += y;
     }
-    if (lane == 31) sums[warp] = incl;
+    most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (lane == 31) {
+      sums[warp] = incl;
+      longest[warp] = most;
+      shortest[warp] = least;
+    }
     __syncthreads();
     int64_t before = incl - mine;
     total = 0;
@@ -108,6 +129,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
     for (int i = 0; i < kRowWarps; ++i) {
       if (i < warp) before += sums[i];
       total += sums[i];
+      most = max(most, longest[i]);
+      least = min(least, shortest[i]);
     }
     G = static_cast<int>(min((total + R::kMinUnits - 1) / R::kMinUnits, static_cast<int64_t>(gridDim.x)));
     if (blockIdx.x >= G) {
@@ -116,13 +139,22 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
     }
     u0 = mul_div(total, blockIdx.x, G);
     u1 = mul_div(total, blockIdx.x + 1, G);
+    // Blocks all about as long as a run: one each is as even as cutting, and
+    // nothing is joined.  (A sequence's last block stands for its others.)
+    const int64_t run = total / G;
+    if (8 * static_cast<int64_t>(least) >= 7 * run && 4 * static_cast<int64_t>(most) <= 5 * run) cut = false;
     if (before <= u0 && u0 < before + mine) {
       int64_t at = before;
       for (int b = b0; b < b1; ++b) {
-        const int64_t u = w.length_of(a, seq_span(a.c, b)) * a.c.nkv;
+        const int64_t head = w.length_of(a, seq_span(a.c, b)), u = head * a.c.nkv;
         if (u0 < at + u) {
-          start_b = b;
-          start_before = at;
+          w.b = b;
+          w.blks = w.blocks_of(a, w.s);
+          w.blk = w.kvh = 0;
+          w.load(a);
+          start = w;
+          start_rest = u0 - at;
+          start_head = head;
           break;
         }
         at += u;
@@ -130,20 +162,14 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
     }
     __syncthreads();
   }
+  w = start;
   int x;  // where the run is inside the current block
   {
-    const SeqSpan q = seq_span(a.c, start_b);
-    const int64_t per_head = w.length_of(a, q);
-    int64_t rem = u0 - start_before;
-    w.b = start_b;
-    w.blks = w.blocks_of(a, q);
-    w.kvh = 0;
-    if (rem >= per_head) {
-      w.kvh = static_cast<int>(mul_div(rem, 1, static_cast<int>(min(per_head, static_cast<int64_t>(INT_MAX)))));
-      rem -= w.kvh * per_head;
+    int64_t rem = start_rest;
+    if (rem >= start_head) {
+      w.kvh = static_cast<int>(mul_div(rem, 1, static_cast<int>(min(start_head, static_cast<int64_t>(INT_MAX)))));
+      rem -= w.kvh * start_head;
     }
-    w.blk = 0;
-    w.load(a);
     while (rem >= w.length()) {
       rem -= w.length();
       ++w.blk;
@@ -163,7 +189,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
     const SeqSpan& s = w.s;
     const int units = w.units(), r0 = w.blk * kRowsPerBlock, nrow = w.nrow;
     int t0 = 0, t1 = units;  // units of this block that are this run's
-    if (units <= R::kWhole) {
+    if (!cut || units <= R::kWhole) {
       if (x > 0) t1 = 0;  // a block that is not cut belongs to the run it begins in
     } else {
       t0 = max(0, x - R::kExtra);
@@ -314,57 +340,79 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
       const uint32_t vs = ring + use * R::kSlotBytes;
       // positions no row sees hold anything: their v counts as zero
       const bool edge = j0 + SL > w.r.hi || (j0 < w.r.lo && j0 + SL > a.sinks);
-      const bool mixed = !whole && !one_token;
+      uint32_t pa[SL / 16][4], live[SL / 16][2];
 #pragma unroll
       for (int k = 0; k < SL / 16; ++k) {
-        uint32_t pa[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pa[e] = pack_bf2_rn(sc[2 * k + (e >> 1)][2 * (e & 1)], sc[2 * k + (e >> 1)][2 * (e & 1) + 1]);
-        uint32_t live[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
-        if (edge) {
+        for (int e = 0; e < 4; ++e)
+          pa[k][e] = pack_bf2_rn(sc[2 * k + (e >> 1)][2 * (e & 1)], sc[2 * k + (e >> 1)][2 * (e & 1) + 1]);
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            const int j = j0 + 16 * k + 8 * hh + 2 * t;
-            live[hh] = (j < w.r.hi && (j >= w.r.lo || j < a.sinks) ? 0xFFFFu : 0u) |
-                       (j + 1 < w.r.hi && (j + 1 >= w.r.lo || j + 1 < a.sinks) ? 0xFFFF0000u : 0u);
-          }
+        for (int hh = 0; hh < 2; ++hh) {
+          const int j = j0 + 16 * k + 8 * hh + 2 * t;
+          live[k][hh] = !edge ? 0xFFFFFFFFu
+                              : (j < w.r.hi && (j >= w.r.lo || j < a.sinks) ? 0xFFFFu : 0u) |
+                                    (j + 1 < w.r.hi && (j + 1 >= w.r.lo || j + 1 < a.sinks) ? 0xFFFF0000u : 0u);
         }
+      }
+      auto v_at = [&](int k, int n) {
+        return vs + (n / 4) * (SL * 128) + (16 * k + lrow) * 128 + (((2 * (n % 4) + lhi) ^ (lrow & 7)) << 4);
+      };
+      // A value that is not finite must not reach the rows that do not see its
+      // position (0 * inf): then each token's rows take their own product.
+      bool odd = false;
+      if (!whole && !one_token) {
+        uint32_t any = 0;
+#pragma unroll 1
+        for (int k = 0; k < SL / 16; ++k)
+#pragma unroll 4
+          for (int n = 0; n < HD / 16; ++n) {
+            uint32_t vb[4];
+            ldsm4_t(v_at(k, n), vb);
 #pragma unroll
-        for (int n = 0; n < HD / 16; ++n) {
-          uint32_t vb[4];
-          ldsm4_t(vs + (n / 4) * (SL * 128) + (16 * k + lrow) * 128 + (((2 * (n % 4) + lhi) ^ (lrow & 7)) << 4), vb);
-          if (edge) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vb[e] &= live[e & 1];
+            for (int e = 0; e < 4; ++e) any |= bf2_nonfinite(vb[e] & live[k][e & 1]);
           }
-          // A value that is not finite must not reach the rows that do not see
-          // its position (0 * inf): then each token's rows take their own product.
-          if (mixed && __any_sync(0xffffffffu, bf2_nonfinite(vb[0]) | bf2_nonfinite(vb[1]) | bf2_nonfinite(vb[2]) |
-                                                   bf2_nonfinite(vb[3]))) {
-            for (int pt = p0; pt <= p1; ++pt) {
-              uint32_t mk[2];
+        odd = __any_sync(0xffffffffu, any);
+      }
+      if (!odd) {
+#pragma unroll
+        for (int k = 0; k < SL / 16; ++k)
+#pragma unroll
+          for (int n = 0; n < HD / 16; ++n) {
+            uint32_t vb[4];
+            ldsm4_t(v_at(k, n), vb);
+            if (edge) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) vb[e] &= live[k][e & 1];
+            }
+            mma_16816(o[2 * n], pa[k][0], pa[k][1], pa[k][2], pa[k][3], vb[0], vb[1]);
+            mma_16816(o[2 * n + 1], pa[k][0], pa[k][1], pa[k][2], pa[k][3], vb[2], vb[3]);
+          }
+      } else {
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n)
+          for (int pt = p0; pt <= p1; ++pt)
+#pragma unroll
+            for (int k = 0; k < SL / 16; ++k) {
+              uint32_t vb[4];
+              ldsm4_t(v_at(k, n), vb);
 #pragma unroll
               for (int hh = 0; hh < 2; ++hh) {
-                const int j = j0 + 16 * k + 8 * hh + 2 * t;
-                mk[hh] = (sees(j, pt, a.window, a.sinks) ? 0xFFFFu : 0u) |
-                         (sees(j + 1, pt, a.window, a.sinks) ? 0xFFFF0000u : 0u);
-              }
+                uint32_t mk[2];
 #pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
+                for (int y = 0; y < 2; ++y) {
+                  const int j = j0 + 16 * k + 8 * y + 2 * t;
+                  mk[y] = (sees(j, pt, a.window, a.sinks) ? 0xFFFFu : 0u) |
+                          (sees(j + 1, pt, a.window, a.sinks) ? 0xFFFF0000u : 0u);
+                }
                 float tmp[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) tmp[e] = o[2 * n + hh][e];
-                mma_16816(tmp, pa[0], pa[1], pa[2], pa[3], vb[2 * hh] & mk[0], vb[2 * hh + 1] & mk[1]);
+                mma_16816(tmp, pa[k][0], pa[k][1], pa[k][2], pa[k][3], vb[2 * hh] & mk[0], vb[2 * hh + 1] & mk[1]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                   if (pr[e >> 1] == pt) o[2 * n + hh][e] = tmp[e];
               }
             }
-          } else {
-            mma_16816(o[2 * n], pa[0], pa[1], pa[2], pa[3], vb[0], vb[1]);
-            mma_16816(o[2 * n + 1], pa[0], pa[1], pa[2], pa[3], vb[2], vb[3]);
-          }
-        }
       }
       release();
     }

@@ -42,7 +42,7 @@ __device__ __forceinline__ void load8(const void* base, int64_t at, float (&v)[8
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v[2 * i] = bf16_bits_to_f32(w[i] & 0xFFFFu);
-      v[2 * i + 1] = bf16_bits_to_f32(w[i] >> 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
   }
 }
@@ -68,10 +68,12 @@ __device__ __forceinline__ int seq_of(const PagedView& c, int t) {
 // A CTA takes `tokens_per_cta` tokens: first their sequences, positions and
 // cache slots (a thread each), then all their heads, one per group of HD / 16
 // lanes.  Each lane holds two groups of eight values: a rotation pair's two
-// halves, or 16 that pass through.  Two units are loaded before either is
-// worked on.
+// halves, or 16 that pass through.  A thread works on one unit at a time, in 40
+// registers: six CTAs to an SM hide the loads better than more units in flight
+// per thread (4,096 tokens of 48 heads of 128 with norm: 40 us; two units per
+// thread at three CTAs: 45 us, four: 53 us).
 template <int HD, bool F32, bool TF32>
-__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads, 6) qk_norm_rope_kernel(const RopeArgs a) {
   constexpr int LPH = HD / 16;
   __shared__ int pos_of[kRopeTokens];          // -1: skipped
   __shared__ int64_t slot_of[kRopeTokens];     // element of the cache, -1: no page
@@ -107,69 +109,59 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeAr
     while (v >= lanes) v -= lanes, ++i;
   };
   while (u - static_cast<int>(threadIdx.x & 31) < total) {  // warps stay whole
-    float x0[2][8] = {}, x1[2][8] = {};
-    int ti[2], hd_[2];
-    bool real[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      real[k] = u < total;
-      ti[k] = i;
-      hd_[k] = v / LPH;
-      if (real[k]) {
-        const int64_t at = static_cast<int64_t>(t0 + i) * a.qkv_stride + hd_[k] * HD;
-        load8<F32>(a.qkv, at + d0, x0[k]);
-        load8<F32>(a.qkv, at + d1, x1[k]);
-      }
-      next();
+    const bool real = u < total;
+    const int ti = i, head = v / LPH;
+    float x0[8] = {}, x1[8] = {};
+    if (real) {
+      const int64_t at = static_cast<int64_t>(t0 + i) * a.qkv_stride + head * HD;
+      load8<F32>(a.qkv, at + d0, x0);
+      load8<F32>(a.qkv, at + d1, x1);
     }
+    next();
+    const bool is_q = head < a.nq, is_k = !is_q && head < a.nq + c.nkv;
+    const float* w = is_q ? a.qw : (is_k ? a.kw : nullptr);
+    if (a.qw || a.kw) {
+      float ss = 0.f;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int head = hd_[k];
-      const bool is_q = head < a.nq, is_k = !is_q && head < a.nq + c.nkv;
-      const float* w = is_q ? a.qw : (is_k ? a.kw : nullptr);
-      if (a.qw || a.kw) {
-        float ss = 0.f;
+      for (int e = 0; e < 8; ++e) ss += x0[e] * x0[e] + x1[e] * x1[e];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x0[k][e] * x0[k][e] + x1[k][e] * x1[k][e];
-#pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (w && real[k]) {
-          const float inv = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
-          float w0[8], w1[8];
-          load8<true>(w, d0, w0);
-          load8<true>(w, d1, w1);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x0[k][e] = x0[k][e] * inv * w0[e];
-            x1[k][e] = x1[k][e] * inv * w1[e];
-          }
-        }
-      }
-      if (!real[k]) continue;
-      const int pos = pos_of[ti[k]];
-      if (pos < 0) continue;
-      if (l < pairs && (is_q || is_k)) {
-        float cs[8], sn[8];
-        const int64_t at = static_cast<int64_t>(pos) * 2 * a.rot + d0;
-        load8<TF32>(a.table, at, cs);
-        load8<TF32>(a.table, at + a.rot, sn);
+      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (w && real) {
+        const float inv = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
+        float w0[8], w1[8];
+        load8<true>(w, d0, w0);
+        load8<true>(w, d1, w1);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float y0 = x0[k][e] * cs[e] - x1[k][e] * sn[e], y1 = x1[k][e] * cs[e] + x0[k][e] * sn[e];
-          x0[k][e] = y0;
-          x1[k][e] = y1;
+          x0[e] = x0[e] * inv * w0[e];
+          x1[e] = x1[e] * inv * w1[e];
         }
       }
-      uint16_t* dst;
-      if (is_q) {
-        dst = a.q_out + static_cast<int64_t>(t0 + ti[k]) * a.q_tok + head * a.q_head;
-      } else {
-        if (slot_of[ti[k]] < 0) continue;
-        dst = (is_k ? c.k : c.v) + slot_of[ti[k]] + (head - a.nq - (is_k ? 0 : c.nkv)) * c.head_stride;
-      }
-      store8(dst + d0, x0[k]);
-      store8(dst + d1, x1[k]);
     }
+    if (!real) continue;
+    const int pos = pos_of[ti];
+    if (pos < 0) continue;
+    if (l < pairs && (is_q || is_k)) {
+      float cs[8], sn[8];
+      const int64_t at = static_cast<int64_t>(pos) * 2 * a.rot + d0;
+      load8<TF32>(a.table, at, cs);
+      load8<TF32>(a.table, at + a.rot, sn);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y0 = x0[e] * cs[e] - x1[e] * sn[e], y1 = x1[e] * cs[e] + x0[e] * sn[e];
+        x0[e] = y0;
+        x1[e] = y1;
+      }
+    }
+    uint16_t* dst;
+    if (is_q) {
+      dst = a.q_out + static_cast<int64_t>(t0 + ti) * a.q_tok + head * a.q_head;
+    } else {
+      if (slot_of[ti] < 0) continue;
+      dst = (is_k ? c.k : c.v) + slot_of[ti] + (head - a.nq - (is_k ? 0 : c.nkv)) * c.head_stride;
+    }
+    store8(dst + d0, x0);
+    store8(dst + d1, x1);
   }
 }
 
