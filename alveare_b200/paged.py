@@ -366,7 +366,18 @@ class PagedKVCache:
         keys = ("free_pages", "handed_out", "copied", "first_unmet")
         return dict(zip(keys, self.info.tolist()))
 
+    def snapshot(self):
+        """Copies of the tables, lengths and counts, for :meth:`restore`."""
+        return self.table.clone(), self.lens.clone(), self.refs.clone()
+
+    def restore(self, state) -> None:
+        """Undo the updates since a :meth:`snapshot` (the pages themselves keep
+        what was written; those in use then are untouched by updates)."""
+        for t, old in zip((self.table, self.lens, self.refs), state):
+            t.copy_(old)
+
     def compact(self) -> None:
+        """:func:`compact_pages` on this pool, in place."""
         compact_pages(self.k, self.v, self.table, self.refs, self.table, self.refs)
 
     def batch(self, slots, q_lens) -> dict:
