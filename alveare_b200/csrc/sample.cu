@@ -72,16 +72,19 @@ struct Cut {  // kept: s > last, and the first `ties` (in index order) of s == l
   uint32_t ties, of;  // of: how many equal `last`
 };
 
+constexpr int kCoarse = 64;  // runs of 32 bins
+
 struct SampleShared {
   uint32_t bins[3][kBins];  // counts in the first, or masses as three 16-bit digits' sums
+  u64 coarse[4][kCoarse];   // their sums over runs of bins, one slot per use
+  u64 tmp[kMaxCluster][kCoarse];
+  // this CTA's elements of the bin in question, then the cluster's
+  uint32_t lkey[kCand], lidx[kCand], n_list;
   uint32_t ckey[kCand], cidx[kCand];
   u64 cmass[kCand];
-  uint32_t n_cand;
   u64 scan[32];
-  // what this CTA shows the others, one slot per use
-  u64 sum[5];
+  u64 sum;  // kept mass
   uint32_t best_key, best_idx, kmin, kmax;
-  // what a CTA tells all
   struct { int bin; u64 before, in, want; uint32_t last_key, ties, of; } found;
   uint32_t wties[kSampleWarps];
   u64 wmass[kSampleWarps];
@@ -178,11 +181,11 @@ struct Row {
   }
 };
 
-// sum[slot] of the CTAs before this one and of all, in every thread (a lane
+// Sums over the CTAs before this one and over all, in every thread (a lane
 // reads a CTA's).
-__device__ __forceinline__ void cluster_sums(cg::cluster_group& cl, SampleShared& sh, int slot, u64* before, u64* all) {
+__device__ __forceinline__ void cluster_sums(cg::cluster_group& cl, SampleShared& sh, u64* before, u64* all) {
   const unsigned lane = threadIdx.x & 31, nb = cl.num_blocks();
-  const u64 v = lane < nb ? cl.map_shared_rank(&sh, lane)->sum[slot] : 0;
+  const u64 v = lane < nb ? cl.map_shared_rank(&sh, lane)->sum : 0;
   u64 x = v, y = lane < cl.block_rank() ? v : 0;
 #pragma unroll
   for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
@@ -193,22 +196,29 @@ __device__ __forceinline__ void cluster_sums(cg::cluster_group& cl, SampleShared
   *before = __shfl_sync(0xffffffffu, y, 0);
 }
 
+__device__ __forceinline__ u64 lane_scan(u64 v) {  // inclusive
+  const unsigned lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+
 // The histogram's crossing: with `bin_of(s)` (-1: not in question) of every
 // element, the bin in which the count (MASS: the mass) starting from `acc`
-// reaches the wanted one, what lies before it and what it holds (found.*, in
-// every CTA).  `want_of(total)` gives the wanted one from the sum of all bins;
-// 0 or more than there is: found.bin = -1.
+// reaches the wanted one, what lies before it and what it holds (found.*).
+// `want_of(total)` gives the wanted one from the sum of all bins; 0: found.bin
+// = -1.  Every CTA shows the sums of its runs of 32 bins; each then finds the
+// run and adds up that run's bins itself, so the cluster meets once.  Leaves the
+// list empty for a gather (by the meeting, every CTA has read the last one's).
 template <bool MASS, bool BF16, bool RES, class B, class W>
 __device__ __forceinline__ void crossing(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, float top,
                                          u64 acc, int slot, B bin_of, W want_of) {
-  const unsigned rank = cl.block_rank(), nb = cl.num_blocks();
+  const unsigned nb = cl.num_blocks();
+  const int lane = threadIdx.x & 31;
   for (int b = threadIdx.x; b < kBins * (MASS ? 3 : 1); b += kSampleThreads) (&sh.bins[0][0])[b] = 0;
-  if (threadIdx.x == 0) {
-    sh.n_cand = 0;
-    sh.kmin = 0xFFFFFFFFu;
-    sh.kmax = 0;
-    sh.found.bin = -1;
-  }
   __syncthreads();
   row.each(0, row.n, threadIdx.x, kSampleThreads, [&](int, float s) {
     const int b = bin_of(s);
@@ -224,50 +234,65 @@ __device__ __forceinline__ void crossing(cg::cluster_group& cl, SampleShared& sh
       atomicAdd(&sh.bins[0][b], 1u);
     }
   });
-  cl.sync();
-  // CTA r adds up bins [r, r + 1) * kBins / nb of all CTAs
-  const int per = kBins / nb, tp = (per + kSampleThreads - 1) / kSampleThreads;
-  u64 bins[kBins / kSampleThreads] = {}, mine = 0;
+  __syncthreads();
+  {
+    constexpr int kPer = kBins / kSampleThreads, kLanes = 32 / kPer;  // bins per thread, threads per run
+    u64 v = 0;
 #pragma unroll
-  for (int e = 0; e < kBins / kSampleThreads; ++e) {
-    const int b = threadIdx.x * tp + e;
-    if (e < tp && b < per) {
+    for (int x = 0; x < (MASS ? 3 : 1); ++x) {
+      const uint4 q = *reinterpret_cast<const uint4*>(&sh.bins[x][threadIdx.x * kPer]);
+      v += (static_cast<u64>(q.x) + q.y + q.z + q.w) << (16 * x);
+    }
+    static_assert(kPer == 4, "four bins per thread");
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (threadIdx.x % kLanes == 0) sh.coarse[slot][threadIdx.x / kLanes] = v;
+  }
+  cl.sync();
+  if (threadIdx.x == 0) sh.n_list = 0;
+  for (unsigned i = threadIdx.x; i < nb * kCoarse; i += kSampleThreads)
+    sh.tmp[i / kCoarse][i % kCoarse] = cl.map_shared_rank(&sh, i / kCoarse)->coarse[slot][i % kCoarse];
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    u64 v0 = 0, v1 = 0;  // runs 2 lane, 2 lane + 1
+#pragma unroll
+    for (unsigned r = 0; r < kMaxCluster; ++r)
+      if (r < nb) {
+        v0 += sh.tmp[r][2 * lane];
+        v1 += sh.tmp[r][2 * lane + 1];
+      }
+    const u64 upto = lane_scan(v0 + v1);
+    const u64 want = want_of(__shfl_sync(0xffffffffu, upto, 31));
+    const u64 b0 = acc + upto - v0 - v1, b1 = b0 + v0, b2 = b1 + v1;
+    const int here = want == 0 ? -1 : b0 < want && want <= b1 ? 2 * lane : b1 < want && want <= b2 ? 2 * lane + 1 : -1;
+    const uint32_t who = __ballot_sync(0xffffffffu, here >= 0);
+    if (lane == 0) sh.found.bin = -1;
+    __syncwarp();
+    if (who) {
+      const int src = __ffs(who) - 1, run = __shfl_sync(0xffffffffu, here, src);
+      u64 before = __shfl_sync(0xffffffffu, here & 1 ? b1 : b0, src);
       uint32_t w[MASS ? 3 : 1][kMaxCluster];  // all in flight at once
 #pragma unroll
       for (unsigned r = 0; r < kMaxCluster; ++r) {
         const SampleShared* o = cl.map_shared_rank(&sh, r < nb ? r : 0);
 #pragma unroll
-        for (int x = 0; x < (MASS ? 3 : 1); ++x) w[x][r] = r < nb ? o->bins[x][rank * per + b] : 0;
+        for (int x = 0; x < (MASS ? 3 : 1); ++x) w[x][r] = r < nb ? o->bins[x][run * 32 + lane] : 0;
       }
+      u64 v = 0;
 #pragma unroll
       for (unsigned r = 0; r < kMaxCluster; ++r)
 #pragma unroll
-        for (int x = 0; x < (MASS ? 3 : 1); ++x) bins[e] += static_cast<u64>(w[x][r]) << (16 * x);
-    }
-    mine += bins[e];
-  }
-  u64 t;
-  u64 upto = cta_scan(mine, &t, sh.scan) - mine;
-  if (threadIdx.x == 0) sh.sum[slot] = t;
-  cl.sync();
-  u64 before, all;
-  cluster_sums(cl, sh, slot, &before, &all);
-  before += acc;
-  const u64 want = want_of(all);
-  upto += before;
-#pragma unroll
-  for (int e = 0; e < kBins / kSampleThreads; ++e) {
-    if (e < tp && upto < want && want <= upto + bins[e])
-      for (unsigned r = 0; r < nb; ++r) {
-        SampleShared* o = cl.map_shared_rank(&sh, r);
-        o->found.bin = static_cast<int>(rank) * per + threadIdx.x * tp + e;
-        o->found.before = upto;
-        o->found.in = bins[e];
-        o->found.want = want;
+        for (int x = 0; x < (MASS ? 3 : 1); ++x) v += static_cast<u64>(w[x][r]) << (16 * x);
+      before += lane_scan(v) - v;
+      if (before < want && want <= before + v) {
+        sh.found.bin = run * 32 + lane;
+        sh.found.before = before;
+        sh.found.in = v;
+        sh.found.want = want;
       }
-    upto += bins[e];
+    }
   }
-  cl.sync();
+  __syncthreads();
 }
 
 // Bins of max - s, even up to kMaxDist.
@@ -277,106 +302,127 @@ __device__ __forceinline__ int even_bin(float top, float s) {
   return min(static_cast<int>(__float_as_uint(__fmaf_rz(d, kBins / kMaxDist, 8388608.0f)) & 0x7FFFFFu), kBins - 1);
 }
 
-// Put the elements with in(s) into CTA 0's list (as many as it holds).
+// Put the elements with in(s) into this CTA's list; once the cluster has met,
+// how many there are (more than kCand: the lists are cut off), and in lane r's
+// *n_mine how many of CTA r.
 template <bool BF16, bool RES, class F>
-__device__ __forceinline__ void gather(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, F in) {
-  SampleShared* lead = cl.map_shared_rank(&sh, 0);
+__device__ __forceinline__ uint32_t gather(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row,
+                                           uint32_t* n_mine, F in) {
   row.each(0, row.n, threadIdx.x, kSampleThreads, [&](int i, float s) {
     if (!in(s)) return;
-    const uint32_t at = atomicAdd(&lead->n_cand, 1u);
+    const uint32_t at = atomicAdd(&sh.n_list, 1u);
     if (at < kCand) {
-      lead->ckey[at] = key_of(s);
-      lead->cidx[at] = row.first + i;
+      sh.lkey[at] = key_of(s);
+      sh.lidx[at] = row.first + i;
     }
   });
   cl.sync();
+  const unsigned lane = threadIdx.x & 31;
+  *n_mine = lane < cl.num_blocks() ? cl.map_shared_rank(&sh, lane)->n_list : 0;
+  return __reduce_add_sync(0xffffffffu, *n_mine);
+}
+
+// The cluster's lists (n <= kCand elements, n_mine of them in the CTA whose
+// rank is this lane's) into ckey / cidx of this CTA.
+__device__ __forceinline__ void pull(cg::cluster_group& cl, SampleShared& sh, uint32_t n, uint32_t n_mine) {
+  const uint32_t i = threadIdx.x;
+  uint32_t at = 0, from = 0, skip = 0;
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; ++r) {  // the list that element i is in
+    const uint32_t m = __shfl_sync(0xffffffffu, n_mine, r);
+    if (i >= at && i < at + m) from = r, skip = at;
+    at += m;
+  }
+  if (i < n) {
+    const SampleShared* o = cl.map_shared_rank(&sh, from);
+    sh.ckey[i] = o->lkey[i - skip];
+    sh.cidx[i] = o->lidx[i - skip];
+  }
+  __syncthreads();
 }
 
 // The prefix of the row, in (s descending, index ascending) order, that ends
 // with the element where the count (MASS: the mass) reaches the wanted one:
-// called once the histogram over even bins has found the bin (found.*).
+// called once the histogram over even bins has found the bin (found.*).  Every
+// CTA compares the bin's elements by itself, so nothing is told around.
 template <bool MASS, bool BF16, bool RES>
 __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, float top, float floor_s) {
-  const unsigned rank = cl.block_rank(), nb = cl.num_blocks();
+  const unsigned nb = cl.num_blocks();
+  const int lane = threadIdx.x & 31;
+  const u64 want = sh.found.want;
   uint32_t kmin = 0, kmax = 0;  // after the first round: the keys of the bin that is cut again
   int shift = 0;
-  const u64 want = sh.found.want;
   for (int round = 0;; ++round) {
     auto bin_of = [&](float s) -> int {
       if (round == 0) return s >= floor_s ? even_bin(top, s) : -1;
       const uint32_t k = key_of(s);
       return k >= kmin && k <= kmax ? static_cast<int>((kmax - k) >> shift) : -1;
     };
+    if (round > 0) crossing<MASS>(cl, sh, row, top, sh.found.before, round & 1, bin_of, [&](u64) { return want; });
     const int bin = sh.found.bin;
-    const u64 acc = sh.found.before;
-    if (round > 0) {
-      crossing<MASS>(cl, sh, row, top, acc, round & 1, bin_of, [&](u64) { return want; });
-    }
-    const int at = round > 0 ? sh.found.bin : bin;
-    const u64 pre0 = round > 0 ? sh.found.before : acc;
-    if (round == 0) gather(cl, sh, row, [&](float s) { return even_bin(top, s) == at && s >= floor_s; });
-    else gather(cl, sh, row, [&](float s) { return bin_of(s) == at; });
-    SampleShared* lead = cl.map_shared_rank(&sh, 0);
-    const uint32_t n = lead->n_cand;
+    const u64 pre0 = sh.found.before;
+    uint32_t n_mine;
+    const uint32_t n = round == 0 ? gather(cl, sh, row, &n_mine, [&](float s) { return even_bin(top, s) == bin && s >= floor_s; })
+                                  : gather(cl, sh, row, &n_mine, [&](float s) { return bin_of(s) == bin; });
     if (n <= kCand) {
-      if (rank == 0) {
-        const int i = threadIdx.x;
-        uint32_t k = 0, idx = 0;
-        u64 m = 0;
-        if (i < n) {
-          k = sh.ckey[i];
-          idx = sh.cidx[i];
-          m = MASS ? mass_of(expf(key_value(k) - top)) : 1;
-          sh.cmass[i] = m;
+      pull(cl, sh, n, n_mine);
+      const uint32_t i = threadIdx.x;
+      uint32_t k = 0, idx = 0;
+      u64 m = 0;
+      if (i < n) {
+        k = sh.ckey[i];
+        idx = sh.cidx[i];
+        m = MASS ? mass_of(expf(key_value(k) - top)) : 1;
+        sh.cmass[i] = m;
+      }
+      __syncthreads();
+      if (i < n) {
+        u64 pre = pre0;
+        uint32_t ties = 1, of = 0;
+        for (uint32_t j = 0; j < n; ++j) {
+          const uint32_t kj = sh.ckey[j];
+          const bool earlier = kj == k && sh.cidx[j] < idx;
+          if (kj > k || earlier) pre += sh.cmass[j];
+          ties += earlier;
+          of += kj == k;
         }
-        __syncthreads();
-        if (i < n) {
-          u64 pre = pre0;
-          uint32_t ties = 1, of = 0;
-          for (uint32_t j = 0; j < n; ++j) {
-            const uint32_t kj = sh.ckey[j];
-            const bool earlier = kj == k && sh.cidx[j] < idx;
-            if (kj > k || earlier) pre += sh.cmass[j];
-            ties += earlier;
-            of += kj == k;
-          }
-          if (pre < want && want <= pre + m)
-            for (unsigned r = 0; r < nb; ++r) {
-              SampleShared* o = cl.map_shared_rank(&sh, r);
-              o->found.last_key = k;
-              o->found.ties = ties;
-              o->found.of = of;
-            }
+        if (pre < want && want <= pre + m) {
+          sh.found.last_key = k;
+          sh.found.ties = ties;
+          sh.found.of = of;
         }
       }
-      cl.sync();
+      __syncthreads();
       return {key_value(sh.found.last_key), sh.found.ties, sh.found.of};
     }
     // too many: the range of their keys, to cut it again
+    if (threadIdx.x == 0) {
+      sh.kmin = 0xFFFFFFFFu;
+      sh.kmax = 0;
+    }
+    __syncthreads();
     uint32_t lo = 0xFFFFFFFFu, hi = 0;
     row.each(0, row.n, threadIdx.x, kSampleThreads, [&](int, float s) {
-      if (bin_of(s) != at) return;
+      if (bin_of(s) != bin) return;
       lo = min(lo, key_of(s));
       hi = max(hi, key_of(s));
     });
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
-    if ((threadIdx.x & 31) == 0 && hi >= lo) {
-      atomicMin(&lead->kmin, lo);
-      atomicMax(&lead->kmax, hi);
+    if (lane == 0 && hi >= lo) {
+      atomicMin(&sh.kmin, lo);
+      atomicMax(&sh.kmax, hi);
     }
     cl.sync();
-    kmin = lead->kmin;
-    kmax = lead->kmax;
+    const SampleShared* o = cl.map_shared_rank(&sh, lane < static_cast<int>(nb) ? lane : 0);
+    kmin = __reduce_min_sync(0xffffffffu, o->kmin);
+    kmax = __reduce_max_sync(0xffffffffu, o->kmax);
     if (kmin == kmax) {  // all equal
       const u64 each = MASS ? mass_of(expf(key_value(kmin) - top)) : 1;
-      const u64 need = (want - pre0 + each - 1) / each;
-      cl.sync();  // CTA 0 stays until its words are read
-      return {key_value(kmin), static_cast<uint32_t>(need), n};
+      return {key_value(kmin), static_cast<uint32_t>((want - pre0 + each - 1) / each), n};
     }
     shift = 0;
     while (((kmax - kmin) >> shift) >= kBins) ++shift;
-    cl.sync();  // CTA 0's words are read before the next round clears them
   }
 }
 
@@ -507,12 +553,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                     [&](u64 n) { return n > static_cast<u64>(k) ? static_cast<u64>(k) : 0; });
     const int bin = sh.found.bin;
     if (bin >= 0 && sh.found.before + sh.found.in <= kCand) {
-      gather(cl, sh, row, [&](float s) {
+      uint32_t n_mine;
+      const uint32_t n = gather(cl, sh, row, &n_mine, [&](float s) {
         const int b = even_bin(top, s);
         return b >= 0 && b <= bin;
       });
-      if (rank == 0) finish_few(sh, a, r, sh.n_cand, static_cast<uint32_t>(k), p, min_p, top);
-      return;  // CTA 0's words are its own from here
+      if (rank == 0) pull(cl, sh, n, n_mine);
+      cl.barrier_arrive();  // the lists are read
+      if (rank == 0) finish_few(sh, a, r, n, static_cast<uint32_t>(k), p, min_p, top);
+      cl.barrier_wait();
+      return;
     }
     if (bin >= 0) {
       cut = select<false>(cl, sh, row, top, -INFINITY);
@@ -579,11 +629,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   if (threadIdx.x == 0) {
     u64 t = 0;
     for (int w = 0; w < kSampleWarps; ++w) t += sh.wmass[w];
-    sh.sum[4] = t;
+    sh.sum = t;
   }
   cl.sync();
   u64 total, before;
-  cluster_sums(cl, sh, 4, &before, &total);
+  cluster_sums(cl, sh, &before, &total);
   cl.barrier_arrive();  // its words are read; no CTA leaves before all have read
   for (int w = 0; w < warp; ++w) before += sh.wmass[w];
   const u64 x = static_cast<u64>(fmax(floor(static_cast<double>(a.u[r]) * static_cast<double>(total)), 0.0));
