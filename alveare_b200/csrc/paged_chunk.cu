@@ -48,8 +48,6 @@ int encode(alv_ctx* ctx, CUtensorMap* map, uint32_t rank, const void* p, const c
 }
 
 constexpr int kChunkRows = 128;
-constexpr int kMinRun = 4;  // a CTA's run at least, in tiles: a part costs about as much as two
-constexpr int kExtra = 2;   // tiles an item counts for its start and end (query tile, first scores, store)
 
 template <int HD>
 struct Chunk {
@@ -61,6 +59,9 @@ struct Chunk {
   static constexpr uint32_t kKV = kBN * HD * 2;
   static constexpr uint32_t kBytes = kNQ * kQTile + 2 * kStages * kKV + 1024;
   static constexpr int kHalf = kBN / 2;            // columns of S a softmax thread takes
+  // a CTA's run at least (a part costs about as much as 256 positions), and what
+  // an item counts for its start and end (query tile, first scores, store)
+  static constexpr int kMinRun = 512 / kBN, kExtra = 256 / kBN;
   static constexpr int kSoftWarps = 8 * kNQ;
   static constexpr int kThreads = (kSoftWarps + 4) * 32;  // + copy, issue and two scan warps
   static constexpr uint32_t kSCol = 0;      // S (and P) of tile q, buffer b: (q + b) * kBN
@@ -238,7 +239,7 @@ struct Walk {
     load(c);
     return true;
   }
-  __device__ __forceinline__ int length() const { return r.count() + kExtra; }
+  __device__ __forceinline__ int length() const { return r.count() + C::kExtra; }
   __device__ __forceinline__ void next(const ChunkArgs& c) {
     if (++kvh < c.a.c.nkv) return;
     kvh = 0;
@@ -258,8 +259,8 @@ struct Walk {
   __device__ __forceinline__ bool take(const ChunkArgs& c, int64_t& u, int64_t u1, int& x, int& t, int& n) {
     while (u < u1) {
       const int len = length();
-      t = max(0, x - kExtra);
-      n = max(0, static_cast<int>(min(static_cast<int64_t>(len), x + (u1 - u))) - kExtra) - t;
+      t = max(0, x - C::kExtra);
+      n = max(0, static_cast<int>(min(static_cast<int64_t>(len), x + (u1 - u))) - C::kExtra) - t;
       u += len - x;
       x = 0;
       if (n > 0) return true;
@@ -269,8 +270,8 @@ struct Walk {
   }
 };
 // CTAs that get a run, and the run that holds a place: the last c with total * c / g <= place.
-__device__ __forceinline__ int runs_of(int64_t total, int grid) {
-  return static_cast<int>(min((total + kMinRun - 1) / kMinRun, static_cast<int64_t>(grid)));
+__device__ __forceinline__ int runs_of(int64_t total, int min_run, int grid) {
+  return static_cast<int>(min((total + min_run - 1) / min_run, static_cast<int64_t>(grid)));
 }
 __device__ __forceinline__ int run_of(int64_t place, int64_t total, int g) {
   return static_cast<int>(((place + 1) * g - 1) / total);
@@ -400,7 +401,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     if (i < warp) before += sh.sums[i];
     total += sh.sums[i];
   }
-  const int g = runs_of(total, gridDim.x);
+  const int g = runs_of(total, C::kMinRun, gridDim.x);
   const int64_t u0 = static_cast<int>(blockIdx.x) < g ? mul_div(total, blockIdx.x, g) : total;
   const int64_t u1 = static_cast<int>(blockIdx.x) < g ? mul_div(total, blockIdx.x + 1, g) : total;
   if (blockIdx.x == 0 && threadIdx.x == 0) *c.total = total;
@@ -429,12 +430,12 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     x0 = static_cast<int>(sh.start_rest) - w.kvh * w.length();
   }
   if (threadIdx.x == 0)
-    c.cuts[blockIdx.x] = x0 > kExtra ? make_int4(w.b, w.pair, w.kvh, x0) : make_int4(-1, 0, 0, 0);
+    c.cuts[blockIdx.x] = x0 > C::kExtra ? make_int4(w.b, w.pair, w.kvh, x0) : make_int4(-1, 0, 0, 0);
   int64_t u = u0;
   int x = x0, t = 0, n = 0;
 
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (sh.failed || mbar_wait_bounded_s(smem_u32(bar), parity)) return;
+    if (mbar_try_wait_s(smem_u32(bar), parity) || sh.failed || mbar_wait_bounded_slow(smem_u32(bar), parity)) return;
     atomicOr(c.a.c.status, kStatusMbarTimeout);
     sh.failed = 1;
   };
@@ -588,10 +589,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
           if (q >= nq) break;
           const int buf = C::kSB == 2 ? i & 1 : 0;
           wait(&sh.pfull[q][buf], pph >> (2 * q + buf) & 1);
-          if (q == 0) {
-            wait(&sh.vfull[vs], vph);
-            wait(&sh.vscan[vs], vph);
-          }
+          if (q == 0) wait(&sh.vscan[vs], vph);  // (it follows the copy's arrival)
           pph ^= 1u << (2 * q + buf);
           tc_fence_after();
           pv(q, buf, i > 0);
@@ -839,12 +837,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const ChunkArgs c, int 
   const int4 it = c.cuts[cut];
   if (it.x < 0) return;
   const int64_t total = *c.total;
-  const int g = runs_of(total, grid);
+  const int g = runs_of(total, C::kMinRun, grid);
   if (cut >= g) return;
   Walk<HD> w{};
   w.at(c, static_cast<int64_t>(it.x) * c.max_pairs + it.y);
   w.kvh = it.z;
-  const int64_t first = mul_div(total, cut, g) - it.w + kExtra;  // the item's first tile
+  const int64_t first = mul_div(total, cut, g) - it.w + C::kExtra;  // the item's first tile
   const int c0 = run_of(first, total, g), c1 = run_of(first + w.r.count() - 1, total, g);
   if (c0 + 1 != cut) return;  // an earlier cut is inside the item
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
