@@ -123,9 +123,12 @@ struct Row {
   bool greedy;
   bool infinite;  // without a copy: +inf is the largest value and reads as 0, the rest as -inf
   __device__ __forceinline__ float value(float x) const {
-    if (!greedy && temp != 1.0f) x = __fdiv_rn(x, temp);
-    if (x != x) x = -INFINITY;
-    return x == 0.0f ? 0.0f : x;  // -0 counts as +0
+    return !greedy && temp != 1.0f ? scaled<true>(x) : scaled<false>(x);
+  }
+  template <bool DIV>
+  __device__ __forceinline__ float scaled(float x) const {
+    if (DIV) x = __fdiv_rn(x, temp);
+    return fmaxf(x + 0.0f, -INFINITY);  // -0 counts as +0, NaN as -inf
   }
   __device__ __forceinline__ float raw(int i) const {
     return BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(base)[i]) : static_cast<const float*>(base)[i];
@@ -153,10 +156,13 @@ struct Row {
       for (int i = i0 + first; i < i1; i += step) f(i, at(i));
     }
   }
-  // f(i, value) for every element of the slice, 16-byte loads where aligned.
-  template <class F>
-  __device__ __forceinline__ void load(F f) const {
+  // Reads the slice (RES: into vals), 16 bytes a load where aligned; this
+  // thread's largest value.
+  __device__ __forceinline__ float load() const { return !greedy && temp != 1.0f ? load_t<true>() : load_t<false>(); }
+  template <bool DIV>
+  __device__ __forceinline__ float load_t() const {
     constexpr int V = BF16 ? 8 : 4;
+    float best = -INFINITY;
     int i0 = 0;
     if ((reinterpret_cast<uintptr_t>(base) & 15) == 0) {
       const uint4* p = static_cast<const uint4*>(base);
@@ -165,19 +171,24 @@ struct Row {
       for (int c = threadIdx.x; c < nv; c += kSampleThreads) {
         const uint4 x = p[c];
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        float v[V];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (BF16) {
-            f(c * V + 2 * e, value(bf16_bits_to_f32(w[e] & 0xFFFFu)));
-            f(c * V + 2 * e + 1, value(bf16_bits_to_f32(w[e] >> 16)));
-          } else {
-            f(c * V + e, value(__uint_as_float(w[e])));
-          }
+        for (int e = 0; e < V; ++e) {
+          v[e] = scaled<DIV>(BF16 ? bf16_bits_to_f32(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu) : __uint_as_float(w[e & 3]));
+          best = fmaxf(best, v[e]);
         }
+#pragma unroll
+        for (int e = 0; e < V; e += 4)
+          if (RES) *reinterpret_cast<float4*>(vals + c * V + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
       }
       i0 = nv * V;
     }
-    for (int i = i0 + threadIdx.x; i < n; i += kSampleThreads) f(i, value(raw(i)));
+    for (int i = i0 + threadIdx.x; i < n; i += kSampleThreads) {
+      const float v = scaled<DIV>(raw(i));
+      best = fmaxf(best, v);
+      if (RES) vals[i] = v;
+    }
+    return best;
   }
 };
 
@@ -299,8 +310,16 @@ __device__ __forceinline__ void crossing(cg::cluster_group& cl, SampleShared& sh
 __device__ __forceinline__ int even_bin(float top, float s) {
   const float d = top - s;
   if (!(d <= kMaxDist)) return -1;
-  return min(static_cast<int>(__float_as_uint(__fmaf_rz(d, kBins / kMaxDist, 8388608.0f)) & 0x7FFFFFu), kBins - 1);
+  return static_cast<int>(__float_as_uint(__fmaf_rz(d, kBins / kMaxDist * 0.99999f, 8388608.0f)) & 0x7FFFFFu);
 }
+// A range of s around bins b0 .. b1 with a bin to spare on either side: two
+// comparisons that spare most elements the bin.
+struct Near {
+  float lo, hi;
+  __device__ __forceinline__ Near(float top, int b0, int b1)
+      : lo(top - (b1 + 2) * (kMaxDist / kBins)), hi(top - (b0 - 1) * (kMaxDist / kBins)) {}
+  __device__ __forceinline__ bool has(float s) const { return s >= lo && s <= hi; }
+};
 
 // Put the elements with in(s) into this CTA's list; once the cluster has met,
 // how many there are (more than kCand: the lists are cut off), and in lane r's
@@ -362,7 +381,10 @@ __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, R
     const int bin = sh.found.bin;
     const u64 pre0 = sh.found.before;
     uint32_t n_mine;
-    const uint32_t n = round == 0 ? gather(cl, sh, row, &n_mine, [&](float s) { return even_bin(top, s) == bin && s >= floor_s; })
+    const Near near(top, bin, bin);
+    const uint32_t n = round == 0 ? gather(cl, sh, row, &n_mine, [&](float s) {
+      return near.has(s) && even_bin(top, s) == bin && s >= floor_s;
+    })
                                   : gather(cl, sh, row, &n_mine, [&](float s) { return bin_of(s) == bin; });
     if (n <= kCand) {
       pull(cl, sh, n, n_mine);
@@ -499,37 +521,32 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   const int k = a.k_rows ? a.k_rows[r] : a.k;
   const float p = a.p_rows ? a.p_rows[r] : a.p, min_p = fminf(a.m_rows ? a.m_rows[r] : a.m, 1.f);
 
-  // ---- the row into shared memory; its largest value and that one's first index
-  float best = -INFINITY;
-  int bi = INT_MAX;
-  row.load([&](int i, float s) {
-    if (RES) row.vals[i] = s;
-    if (s > best || (s == best && i < bi)) best = s, bi = i;
-  });
+  // ---- the row into shared memory; its largest value
+  const float best = row.load();
   if (RES && threadIdx.x < 4 && (row.n & 3) && threadIdx.x >= (row.n & 3)) row.vals[(row.n & ~3) + threadIdx.x] = -INFINITY;
-  uint32_t bk = key_of(best), idx = bi == INT_MAX ? 0xFFFFFFFFu : static_cast<uint32_t>(row.first + bi);
   {
-    const uint32_t wk = __reduce_max_sync(0xffffffffu, bk);
-    idx = __reduce_min_sync(0xffffffffu, bk == wk ? idx : 0xFFFFFFFFu);
-    if (lane == 0) sh.wties[warp] = wk, sh.wmass[warp] = idx;
+    uint32_t bk = __reduce_max_sync(0xffffffffu, key_of(best));
+    if (lane == 0) sh.wties[warp] = bk;
     __syncthreads();
-    bk = 0;
-    for (int w = 0; w < kSampleWarps; ++w) {
-      const uint32_t x = sh.wties[w], y = static_cast<uint32_t>(sh.wmass[w]);
-      if (x > bk || (x == bk && y < idx)) bk = x, idx = y;
-    }
-    if (threadIdx.x == 0) sh.best_key = bk, sh.best_idx = idx;
-    cl.sync();
-    const SampleShared* q = cl.map_shared_rank(&sh, lane < static_cast<int>(nb) ? lane : 0);
-    const uint32_t x = q->best_key, y = q->best_idx;
-    bk = __reduce_max_sync(0xffffffffu, x);
-    idx = __reduce_min_sync(0xffffffffu, x == bk ? y : 0xFFFFFFFFu);
+    bk = __reduce_max_sync(0xffffffffu, sh.wties[lane % kSampleWarps]);
+    if (threadIdx.x == 0) sh.best_key = bk, sh.best_idx = 0xFFFFFFFFu;
   }
-  float top = key_value(bk);
+  cl.sync();
+  float top = key_value(__reduce_max_sync(0xffffffffu, cl.map_shared_rank(&sh, lane < static_cast<int>(nb) ? lane : 0)->best_key));
   if (row.greedy || top == -INFINITY) {  // the same in every CTA of the cluster
-    if (rank == 0 && threadIdx.x == 0) {
-      a.tokens[r] = top == -INFINITY ? -1 : static_cast<int>(idx);
-      if (a.logprobs) a.logprobs[r] = top == -INFINITY ? -INFINITY : 0.f;
+    uint32_t idx = 0xFFFFFFFFu;  // the first index of the largest
+    row.each(0, row.n, threadIdx.x, kSampleThreads, [&](int i, float s) {
+      if (s == top) idx = min(idx, static_cast<uint32_t>(row.first + i));
+    });
+    idx = __reduce_min_sync(0xffffffffu, idx);
+    if (lane == 0 && idx != 0xFFFFFFFFu) atomicMin(&sh.best_idx, idx);
+    cl.sync();
+    if (rank == 0 && warp == 0) {
+      idx = __reduce_min_sync(0xffffffffu, cl.map_shared_rank(&sh, lane < static_cast<int>(nb) ? lane : 0)->best_idx);
+      if (lane == 0) {
+        a.tokens[r] = top == -INFINITY ? -1 : static_cast<int>(idx);
+        if (a.logprobs) a.logprobs[r] = top == -INFINITY ? -INFINITY : 0.f;
+      }
     }
     cl.sync();  // no CTA leaves while another reads its words
     return;
@@ -554,7 +571,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const int bin = sh.found.bin;
     if (bin >= 0 && sh.found.before + sh.found.in <= kCand) {
       uint32_t n_mine;
+      const Near near(top, 0, bin);
       const uint32_t n = gather(cl, sh, row, &n_mine, [&](float s) {
+        if (!near.has(s)) return false;
         const int b = even_bin(top, s);
         return b >= 0 && b <= bin;
       });
