@@ -35,6 +35,7 @@ constexpr int kCand = kSampleThreads;  // elements of the last bin compared each
 constexpr int kMaxCluster = 8;
 constexpr float kMaxDist = 27.75f;     // exp(-27.75) < 2^-40: no mass beyond
 constexpr int kMaxSlice = 65536;       // elements per CTA: 65,536 16-bit digits add up below 2^32
+constexpr int kSlice18 = 16384;        // up to here 18-bit digits do: most masses are then one digit long
 typedef unsigned long long u64;
 
 struct SampleArgs {
@@ -58,13 +59,18 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// floor(w 2^40) for w in [0, 1], by two additions that round down: at 8 a
-// float's step is 2^-20, at 2^-17 it is 2^-40.
+// floor(w 2^40) for w in [0, 1], by two additions that round down: at 2 a
+// float's step is 2^-22, at 2^-17 it is 2^-40.  hi 2^18 + lo, lo < 2^18.
+__device__ __forceinline__ void mass_digits(float w, uint32_t* hi, uint32_t* lo) {
+  const float a = __fadd_rz(w, 2.0f);
+  const float b = __fadd_rz(__fsub_rn(w, __fsub_rn(a, 2.0f)), 7.62939453125e-06f);
+  *hi = __float_as_uint(a) - 0x40000000u;
+  *lo = __float_as_uint(b) & 0x3FFFFu;
+}
 __device__ __forceinline__ u64 mass_of(float w) {
-  const float a = __fadd_rz(w, 8.0f);
-  const float rest = __fsub_rn(w, __fsub_rn(a, 8.0f));
-  const float b = __fadd_rz(rest, 7.62939453125e-06f);
-  return (static_cast<u64>(__float_as_uint(a) - 0x41000000u) << 20) + (__float_as_uint(b) - 0x37000000u);
+  uint32_t hi, lo;
+  mass_digits(w, &hi, &lo);
+  return (static_cast<u64>(hi) << 18) + lo;
 }
 
 struct Cut {  // kept: s > last, and the first `ties` (in index order) of s == last
@@ -75,7 +81,7 @@ struct Cut {  // kept: s > last, and the first `ties` (in index order) of s == l
 constexpr int kCoarse = 64;  // runs of 32 bins
 
 struct SampleShared {
-  uint32_t bins[3][kBins];  // counts in the first, or masses as three 16-bit digits' sums
+  uint32_t bins[3][kBins];  // counts in the first, or masses as three digits' sums
   u64 coarse[4][kCoarse];   // their sums over runs of bins, one slot per use
   u64 tmp[kMaxCluster][kCoarse];
   // this CTA's elements of the bin in question, then the cluster's
@@ -84,6 +90,7 @@ struct SampleShared {
   u64 cmass[kCand];
   u64 scan[32];
   u64 sum;  // kept mass
+  u64 few_all, few_before, few_own;  // of a last bin's elements: kept mass, that before this CTA's slice, in it
   uint32_t best_key, best_idx, kmin, kmax;
   struct { int bin; u64 before, in, want; uint32_t last_key, ties, of; } found;
   uint32_t wties[kSampleWarps];
@@ -119,6 +126,7 @@ struct Row {
   const void* base;  // this CTA's slice
   float* vals;
   int n, first;      // elements of the slice, index of its first
+  int slice;         // elements of a full slice
   float temp;
   bool greedy;
   bool infinite;  // without a copy: +inf is the largest value and reads as 0, the rest as -inf
@@ -207,6 +215,11 @@ __device__ __forceinline__ void cluster_sums(cg::cluster_group& cl, SampleShared
   *before = __shfl_sync(0xffffffffu, y, 0);
 }
 
+__device__ __forceinline__ u64 lane_sum(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 __device__ __forceinline__ u64 lane_scan(u64 v) {  // inclusive
   const unsigned lane = threadIdx.x & 31;
 #pragma unroll
@@ -229,22 +242,34 @@ __device__ __forceinline__ void crossing(cg::cluster_group& cl, SampleShared& sh
                                          u64 acc, int slot, B bin_of, W want_of) {
   const unsigned nb = cl.num_blocks();
   const int lane = threadIdx.x & 31;
+  const int digit = row.slice <= kSlice18 ? 18 : 16;
   for (int b = threadIdx.x; b < kBins * (MASS ? 3 : 1); b += kSampleThreads) (&sh.bins[0][0])[b] = 0;
   __syncthreads();
-  row.each(0, row.n, threadIdx.x, kSampleThreads, [&](int, float s) {
-    const int b = bin_of(s);
-    if (b < 0) return;
-    if (MASS) {
+  auto add = [&](int b, uint32_t m0, uint32_t m1, uint32_t m2) {
+    if (m0) atomicAdd(&sh.bins[0][b], m0);
+    if (m1) atomicAdd(&sh.bins[1][b], m1);
+    if (m2) atomicAdd(&sh.bins[2][b], m2);
+  };
+  if (!MASS) {
+    row.each(0, row.n, threadIdx.x, kSampleThreads, [&](int, float s) {
+      const int b = bin_of(s);
+      if (b >= 0) atomicAdd(&sh.bins[0][b], 1u);
+    });
+  } else if (digit == 18) {
+    row.each(0, row.n, threadIdx.x, kSampleThreads, [&](int, float s) {
+      const int b = bin_of(s);
+      uint32_t hi, lo;  // an element not in question has no mass
+      mass_digits(b < 0 ? 0.f : expf(s - top), &hi, &lo);
+      add(b, lo, hi & 0x3FFFFu, hi >> 18);
+    });
+  } else {
+    row.each(0, row.n, threadIdx.x, kSampleThreads, [&](int, float s) {
+      const int b = bin_of(s);
+      if (b < 0) return;
       const u64 m = mass_of(expf(s - top));
-      const uint32_t m0 = static_cast<uint32_t>(m) & 0xFFFFu, m1 = static_cast<uint32_t>(m >> 16) & 0xFFFFu,
-                     m2 = static_cast<uint32_t>(m >> 32);
-      atomicAdd(&sh.bins[0][b], m0);
-      if (m1) atomicAdd(&sh.bins[1][b], m1);
-      if (m2) atomicAdd(&sh.bins[2][b], m2);
-    } else {
-      atomicAdd(&sh.bins[0][b], 1u);
-    }
-  });
+      add(b, static_cast<uint32_t>(m) & 0xFFFFu, static_cast<uint32_t>(m >> 16) & 0xFFFFu, static_cast<uint32_t>(m >> 32));
+    });
+  }
   __syncthreads();
   {
     constexpr int kPer = kBins / kSampleThreads, kLanes = 32 / kPer;  // bins per thread, threads per run
@@ -252,7 +277,7 @@ __device__ __forceinline__ void crossing(cg::cluster_group& cl, SampleShared& sh
 #pragma unroll
     for (int x = 0; x < (MASS ? 3 : 1); ++x) {
       const uint4 q = *reinterpret_cast<const uint4*>(&sh.bins[x][threadIdx.x * kPer]);
-      v += (static_cast<u64>(q.x) + q.y + q.z + q.w) << (16 * x);
+      v += (static_cast<u64>(q.x) + q.y + q.z + q.w) << (digit * x);
     }
     static_assert(kPer == 4, "four bins per thread");
 #pragma unroll
@@ -260,7 +285,7 @@ __device__ __forceinline__ void crossing(cg::cluster_group& cl, SampleShared& sh
     if (threadIdx.x % kLanes == 0) sh.coarse[slot][threadIdx.x / kLanes] = v;
   }
   cl.sync();
-  if (threadIdx.x == 0) sh.n_list = 0;
+  if (threadIdx.x == 0) sh.n_list = 0, sh.few_all = 0, sh.few_before = 0, sh.few_own = 0;
   for (unsigned i = threadIdx.x; i < nb * kCoarse; i += kSampleThreads)
     sh.tmp[i / kCoarse][i % kCoarse] = cl.map_shared_rank(&sh, i / kCoarse)->coarse[slot][i % kCoarse];
   __syncthreads();
@@ -293,13 +318,24 @@ __device__ __forceinline__ void crossing(cg::cluster_group& cl, SampleShared& sh
 #pragma unroll
       for (unsigned r = 0; r < kMaxCluster; ++r)
 #pragma unroll
-        for (int x = 0; x < (MASS ? 3 : 1); ++x) v += static_cast<u64>(w[x][r]) << (16 * x);
+        for (int x = 0; x < (MASS ? 3 : 1); ++x) v += static_cast<u64>(w[x][r]) << (digit * x);
       before += lane_scan(v) - v;
       if (before < want && want <= before + v) {
         sh.found.bin = run * 32 + lane;
         sh.found.before = before;
         sh.found.in = v;
         sh.found.want = want;
+      }
+      if (MASS) {  // this CTA's mass before the bin
+        const int bin = run * 32 + __ffs(__ballot_sync(0xffffffffu, before < want && want <= before + v)) - 1;
+        u64 own = 0;
+        if (2 * lane < run) own += sh.coarse[slot][2 * lane];
+        if (2 * lane + 1 < run) own += sh.coarse[slot][2 * lane + 1];
+        if (run * 32 + lane < bin)
+#pragma unroll
+          for (int x = 0; x < (MASS ? 3 : 1); ++x) own += static_cast<u64>(sh.bins[x][run * 32 + lane]) << (digit * x);
+        own = lane_sum(own);
+        if (lane == 0) sh.sum = own;
       }
     }
   }
@@ -341,6 +377,13 @@ __device__ __forceinline__ uint32_t gather(cg::cluster_group& cl, SampleShared& 
   return __reduce_add_sync(0xffffffffu, *n_mine);
 }
 
+// The kept mass, found along with the end of the prefix.
+struct Sums {
+  bool known;
+  u64 total, before, own;  // of the row, before this CTA's slice, of the slice
+  uint32_t listed;    // elements in ckey / cidx
+};
+
 // The cluster's lists (n <= kCand elements, n_mine of them in the CTA whose
 // rank is this lane's) into ckey / cidx of this CTA.
 __device__ __forceinline__ void pull(cg::cluster_group& cl, SampleShared& sh, uint32_t n, uint32_t n_mine) {
@@ -363,9 +406,12 @@ __device__ __forceinline__ void pull(cg::cluster_group& cl, SampleShared& sh, ui
 // The prefix of the row, in (s descending, index ascending) order, that ends
 // with the element where the count (MASS: the mass) reaches the wanted one:
 // called once the histogram over even bins has found the bin (found.*).  Every
-// CTA compares the bin's elements by itself, so nothing is told around.
+// CTA compares the bin's elements by itself, so nothing is told around.  MASS:
+// with what the histogram says of the bins before, that gives the kept mass of
+// every CTA too, unless min-p takes some of it away.
 template <bool MASS, bool BF16, bool RES>
-__device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, float top, float floor_s) {
+__device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, RES>& row, float top, float floor_s,
+                      float min_p, Sums* sums) {
   const unsigned nb = cl.num_blocks();
   const int lane = threadIdx.x & 31;
   const u64 want = sh.found.want;
@@ -387,9 +433,10 @@ __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, R
     })
                                   : gather(cl, sh, row, &n_mine, [&](float s) { return bin_of(s) == bin; });
     if (n <= kCand) {
+      if (MASS && round == 0) cluster_sums(cl, sh, &sums->before, &sums->total);
       pull(cl, sh, n, n_mine);
       const uint32_t i = threadIdx.x;
-      uint32_t k = 0, idx = 0;
+      uint32_t k = 0, idx = 0, ties = 1, of = 0;
       u64 m = 0;
       if (i < n) {
         k = sh.ckey[i];
@@ -400,7 +447,6 @@ __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, R
       __syncthreads();
       if (i < n) {
         u64 pre = pre0;
-        uint32_t ties = 1, of = 0;
         for (uint32_t j = 0; j < n; ++j) {
           const uint32_t kj = sh.ckey[j];
           const bool earlier = kj == k && sh.cidx[j] < idx;
@@ -415,7 +461,27 @@ __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, R
         }
       }
       __syncthreads();
-      return {key_value(sh.found.last_key), sh.found.ties, sh.found.of};
+      const uint32_t last = sh.found.last_key;
+      if (MASS && round == 0 && expf(key_value(last) - top) >= min_p) {
+        if ((i & ~31u) < n) {
+          const bool keep = i < n && (k > last || (k == last && ties <= sh.found.ties));
+          const u64 all = lane_sum(keep ? m : 0);
+          const u64 pre = lane_sum(keep && idx < static_cast<uint32_t>(row.first) ? m : 0);
+          const u64 own = lane_sum(keep && idx - row.first < static_cast<uint32_t>(row.n) ? m : 0);
+          if (lane == 0) {
+            atomicAdd(&sh.few_all, all);
+            atomicAdd(&sh.few_before, pre);
+            atomicAdd(&sh.few_own, own);
+          }
+        }
+        __syncthreads();
+        sums->before += sh.few_before;
+        sums->total += sh.few_all;
+        sums->own = sh.sum + sh.few_own;
+        sums->known = true;
+        sums->listed = n;
+      }
+      return {key_value(last), sh.found.ties, sh.found.of};
     }
     // too many: the range of their keys, to cut it again
     if (threadIdx.x == 0) {
@@ -512,6 +578,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   pdl_wait();
   pdl_trigger();
   row.first = min(static_cast<int>(rank) * a.slice, a.vocab);
+  row.slice = a.slice;
   row.n = min(a.slice, a.vocab - row.first);
   row.base = static_cast<const char*>(a.logits) + (r * a.stride + row.first) * (BF16 ? 2 : 4);
   row.vals = reinterpret_cast<float*>(dyn + (sizeof(SampleShared) + 15) / 16 * 16);
@@ -564,6 +631,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   // ---- where the kept prefix ends
   Cut cut{-INFINITY, 0, 0};
   bool all = true;
+  Sums sums{};
   if (k > 0 && k < a.vocab) {
     // elements without mass do not matter: if fewer than k have some, all do
     crossing<false>(cl, sh, row, top, 0, 2, [&](float s) { return even_bin(top, s); },
@@ -584,7 +652,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       return;
     }
     if (bin >= 0) {
-      cut = select<false>(cl, sh, row, top, -INFINITY);
+      cut = select<false>(cl, sh, row, top, -INFINITY, min_p, nullptr);
       all = false;
     }
   }
@@ -597,28 +665,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       const double goal = ceil(static_cast<double>(m - beyond) * static_cast<double>(p));
       return goal >= 1.0 ? static_cast<u64>(goal) : static_cast<u64>(1);
     });
-    cut = select<true>(cl, sh, row, top, cut.last);
+    cut = select<true>(cl, sh, row, top, cut.last, min_p, &sums);
     all = false;
   }
 
-  // ---- the kept mass of every warp's run of the slice, then the token
-  const int seg = (row.n + kSampleWarps * 128 - 1) / (kSampleWarps * 128) * 128;
-  const int i0 = min(warp * seg, row.n), i1 = min(i0 + seg, row.n);
+  // ---- the CTA whose slice holds the token
   const bool ranked = !all && cut.ties < cut.of;  // only some of the equals are kept
-  uint32_t tie0 = 0;
-  if (ranked) {
-    uint32_t n = 0;
-    for (int i = i0 + lane; i < i1; i += 32) n += row.at(i) == cut.last;
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) sh.wties[warp] = n;
-    cl.sync();
-    for (unsigned o = 0; o <= rank; ++o) {
-      const SampleShared* q = cl.map_shared_rank(&sh, o);
-      for (int w = 0; w < (o == rank ? warp : kSampleWarps); ++w) tie0 += q->wties[w];
-    }
-  }
-  uint32_t ties = tie0;
-  auto kept_mass = [&](int i) -> u64 {  // lanes take consecutive elements; `ties` counts the equals so far
+  const int seg = (row.n + kSampleWarps * 128 - 1) / (kSampleWarps * 128) * 128;  // a warp's run of the slice
+  const int i0 = min(warp * seg, row.n), i1 = min(i0 + seg, row.n);
+  uint32_t tie0 = 0, ties;  // equals of the last one before this warp's run, and so far
+  auto kept_mass = [&](int i) -> u64 {  // lanes take consecutive elements
     const float s = i < i1 ? row.at(i) : -INFINITY;
     bool keep = i < i1 && (all || s >= cut.last);
     if (ranked) {
@@ -630,33 +686,63 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const float w = expf(s - top);
     return w >= min_p ? mass_of(w) : 0;
   };
+  auto run_mass = [&] {  // of this warp's run
+    u64 m = 0;
+    ties = tie0;
+    if (ranked) {
+      for (int b = i0; b < i1; b += 32) m += kept_mass(b + lane);
+    } else {
+      const float least = all ? -INFINITY : cut.last;
+      row.each(i0, i1, lane, 32, [&](int, float s) {
+        if (!(s >= least)) return;
+        const float w = expf(s - top);
+        if (w >= min_p) m += mass_of(w);
+      });
+    }
+    m = lane_sum(m);
+    if (lane == 0) sh.wmass[warp] = m;
+    __syncthreads();
+    return m;
+  };
   u64 m = 0;
-  const float least = all ? -INFINITY : cut.last;
-  if (ranked) {
-    for (int b = i0; b < i1; b += 32) m += kept_mass(b + lane);
-  } else {
-    row.each(i0, i1, lane, 32, [&](int, float s) {
-      if (!(s >= least)) return;
-      const float w = expf(s - top);
-      if (w >= min_p) m += mass_of(w);
-    });
+  if (!sums.known) {
+    if (ranked) {
+      uint32_t n = 0;
+      for (int i = i0 + lane; i < i1; i += 32) n += row.at(i) == cut.last;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0) sh.wties[warp] = n;
+      cl.sync();
+      for (unsigned o = 0; o <= rank; ++o) {
+        const SampleShared* q = cl.map_shared_rank(&sh, o);
+        for (int w = 0; w < (o == rank ? warp : kSampleWarps); ++w) tie0 += q->wties[w];
+      }
+    }
+    m = run_mass();
+    for (int w = 0; w < kSampleWarps; ++w) sums.own += sh.wmass[w];
+    if (threadIdx.x == 0) sh.sum = sums.own;
+    cl.sync();
+    cluster_sums(cl, sh, &sums.before, &sums.total);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-  if (lane == 0) sh.wmass[warp] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    u64 t = 0;
-    for (int w = 0; w < kSampleWarps; ++w) t += sh.wmass[w];
-    sh.sum = t;
-  }
-  cl.sync();
-  u64 total, before;
-  cluster_sums(cl, sh, &before, &total);
   cl.barrier_arrive();  // its words are read; no CTA leaves before all have read
-  for (int w = 0; w < warp; ++w) before += sh.wmass[w];
+  const u64 total = sums.total;
   const u64 x = static_cast<u64>(fmax(floor(static_cast<double>(a.u[r]) * static_cast<double>(total)), 0.0));
   const u64 goal = x < total ? x : total - 1;
+  u64 before = sums.before;
+  if (goal < before || goal >= before + sums.own) {
+    cl.barrier_wait();
+    return;
+  }
+
+  // ---- the warp whose run does, and there the token
+  if (sums.known) {
+    if (ranked) {  // the equals are all among the last bin's elements
+      const uint32_t key = key_of(cut.last), first = static_cast<uint32_t>(row.first + i0);
+      for (uint32_t j = lane; j < sums.listed; j += 32) tie0 += sh.ckey[j] == key && sh.cidx[j] < first;
+      tie0 = __reduce_add_sync(0xffffffffu, tie0);
+    }
+    m = run_mass();
+  }
+  for (int w = 0; w < warp; ++w) before += sh.wmass[w];
   if (before <= goal && goal < before + m) {  // this warp's run holds the token
     int b = i0;
     ties = tie0;
