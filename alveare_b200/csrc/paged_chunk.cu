@@ -345,6 +345,9 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
   const uint32_t q_sm = base, k_sm = base + NQ * C::kQTile, v_sm = k_sm + ST * C::kKV;
 
   if (threadIdx.x == 0) {
+    prefetch_map(&qmap);
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&sh.kfull[i], 1);
       mbar_init(&sh.kempty[i], 1);
@@ -779,7 +782,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         tc_fence_after();
         const bool part = t > 0 || n < sw.r.count();
         const int head = sw.kvh * c.a.group + row % c.a.group;
-        uint16_t* dst = c.a.out + static_cast<int64_t>(sw.s.q0 + tok) * c.a.o_tok + head * c.a.o_head + half * (HD / 2);
+        uint16_t* dst = !real ? nullptr : c.a.out + static_cast<int64_t>(sw.s.q0 + tok) * c.a.o_tok + head * c.a.o_head + half * (HD / 2);
         float* pd = part_of(c, blockIdx.x, t > 0 ? 0 : 1, NQ * kChunkRows * (HD + 2)) + q * kChunkRows * (HD + 2);
         const bool odd = sh.odd[item & 3] == item + 1;
         const float inv = m == -INFINITY ? 0.f : 1.f / l;  // a row that sees nothing gives zeros
@@ -796,14 +799,30 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
 #pragma unroll
             for (int y = 0; y < 32; y += 4)
               *reinterpret_cast<uint4*>(pd + (e + y) * kChunkRows + row * 4) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
-          } else if (real) {
+          } else {
+            // four lanes exchange the 16-byte quarters of their rows: a store
+            // then writes 64 bytes in a row of eight rows, not 16 of 32
+            uint32_t p[16];
 #pragma unroll
-            for (int y = 0; y < 32; y += 8) {
-              uint32_t p[4];
+            for (int y = 0; y < 16; ++y)
+              p[y] = pack_bf2_rn(__uint_as_float(o[2 * y]) * inv, __uint_as_float(o[2 * y + 1]) * inv);
 #pragma unroll
-              for (int z = 0; z < 4; ++z)
-                p[z] = pack_bf2_rn(__uint_as_float(o[y + 2 * z]) * inv, __uint_as_float(o[y + 2 * z + 1]) * inv);
-              *reinterpret_cast<uint4*>(dst + e + y) = make_uint4(p[0], p[1], p[2], p[3]);
+            for (int b = 1; b < 4; b *= 2)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (k & b) continue;
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                  uint32_t &lo = p[4 * k + z], &hi = p[4 * (k | b) + z];
+                  const uint32_t got = __shfl_xor_sync(0xffffffffu, lane & b ? lo : hi, b);
+                  if (lane & b) lo = got;
+                  else hi = got;
+                }
+              }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint16_t* d = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), (lane & 28) + k));
+              if (d) *reinterpret_cast<uint4*>(d + e + 8 * (lane & 3)) = make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]);
             }
           }
         }
