@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
   const AttnArgs& a = ra.a;
   extern __shared__ uint8_t smem_dyn[];
   __shared__ __align__(8) uint64_t full[kRowWarps][NS];
-  __shared__ int64_t sums[kRowWarps];
+  __shared__ int64_t sums[kRowWarps], few[kRowWarps];
   __shared__ int longest[kRowWarps], shortest[kRowWarps];  // blocks
   __shared__ RowWalk<HD> start;                              // where the run starts, at its sequence's first block
   __shared__ int64_t start_rest, start_head;                 // how far into the sequence; the length of a kv head's blocks
@@ -99,10 +99,14 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
   {
     const int per = (a.c.batch + kRowWarps * 32 - 1) / (kRowWarps * 32);
     const int b0 = threadIdx.x * per, b1 = min(b0 + per, a.c.batch);
-    int64_t mine = 0;
+    int64_t mine = 0, theirs = 0;  // theirs: as items of the chunk kernel
     int most = 0, least = INT_MAX;
     for (int b = b0; b < b1; ++b) {
       const int64_t len = w.length_of(a, seq_span(a.c, b));
+      if (ra.early && len) {
+        const SliceRange r = slice_range<ChunkTile<HD>::kBN>(w.s.kv - w.s.qlen, w.s.kv - 1, a.window, a.sinks);
+        theirs += static_cast<int64_t>(max(r.count(), 1) + ChunkTile<HD>::kExtra) * a.c.nkv;
+      }
       mine += len * a.c.nkv;
       if (len) {
         most = max(most, w.length());
@@ -117,6 +121,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
     }
     most = __reduce_max_sync(0xffffffffu, most);
     least = __reduce_min_sync(0xffffffffu, least);
+    if (ra.early) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) theirs += __shfl_xor_sync(0xffffffffu, theirs, o);
+      if (lane == 0) few[warp] = theirs;
+    }
     if (lane == 31) {
       sums[warp] = incl;
       longest[warp] = most;
@@ -131,6 +140,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
       total += sums[i];
       most = max(most, longest[i]);
       least = min(least, shortest[i]);
+    }
+    if (ra.early) {
+      int64_t all = 0;
+#pragma unroll
+      for (int i = 0; i < kRowWarps; ++i) all += few[i];
+      if (chunk_takes_few(all, gridDim.x / 2)) total = 0;  // (two CTAs per SM here, one there)
     }
     G = static_cast<int>(min((total + R::kMinUnits - 1) / R::kMinUnits, static_cast<int64_t>(gridDim.x)));
     if (blockIdx.x >= G) {

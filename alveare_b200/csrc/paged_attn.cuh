@@ -51,6 +51,18 @@ struct AttnArgs {
   int row_max;            // row-block kernel: sequences with more rows are not its
 };
 
+// The tensor-core form's tile, and what an item counts beyond its tiles.
+template <int HD>
+struct ChunkTile {
+  static constexpr int kBN = HD == 256 ? 64 : 128, kExtra = 256 / kBN;
+};
+// Whether it takes a mixed batch's short sequences too (`length`: of their
+// items, one per kv head): up to six tiles per CTA, 6 to 8 us, where the
+// row-block kernel beside it adds some 15 us for however little (start, one
+// fetch from memory, join).  13 sequences of 1 to 517 new tokens, three of them
+// single: 98 us with both kernels, 86 with one.
+__device__ __forceinline__ bool chunk_takes_few(int64_t length, int ctas) { return length <= 6ll * ctas; }
+
 // The tensor-core form for chunks (paged_chunk.cu): sequences with at least
 // row_min rows (new tokens x heads of a kv group).  mixed: the row-block
 // kernel for the others is launched between it and its join.

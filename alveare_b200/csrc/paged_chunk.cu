@@ -77,6 +77,7 @@ struct Chunk {
   // a CTA's run at least (a part costs about as much as 256 positions), and what
   // an item counts for its start and end (query tile, first scores, store)
   static constexpr int kMinRun = 512 / kBN, kExtra = 256 / kBN;
+  static_assert(kBN == ChunkTile<HD>::kBN && kExtra == ChunkTile<HD>::kExtra, "the row-block kernel counts the same");
   static constexpr int kSoftWarps = 8 * kNQ;
   static constexpr int kThreads = (kSoftWarps + 4) * 32;  // + copy, issue and two scan warps
   static constexpr uint32_t kSCol = 0;      // S (and P) of tile q, buffer b: (q + b) * kBN
@@ -88,10 +89,10 @@ struct ChunkArgs {
   int tpt;        // tokens per query tile: 128 / group
   int box;        // positions per tensor copy
   int head_first; // cache tensor map order: (hd, head, row, page) instead of (hd, row, head, page)
-  int row_min;    // sequences with at least this many rows are this kernel's
+  int row_min;    // sequences with at least this many rows are this kernel's in any case
   float* parts;   // [2 * grid][kNQ * 128][HD + 2]
   int4* cuts;     // [grid]: item (b, pair, kvh) that the run starts inside, and where (x = -1: none)
-  int64_t* total; // [1] length of all items
+  int64_t* total; // [2] length of all items; rows of the shortest sequence taken
   int max_pairs;  // query-tile pairs of the longest sequence
 };
 
@@ -230,6 +231,7 @@ struct Walk {
   SeqSpan s;
   SliceRange r;      // tiles of the current item
   int p0, p1;        // positions of the item's first and last new token
+  int row_min;       // sequences of fewer rows are left out
 
   __device__ __forceinline__ void load(const ChunkArgs& c) {
     p0 = s.kv - s.qlen + pair * C::kNQ * c.tpt;
@@ -239,7 +241,7 @@ struct Walk {
     if (r.count() == 0) r.n_main = 1;
   }
   __device__ __forceinline__ int pairs_of(const ChunkArgs& c) const {
-    if (s.qlen <= 0 || static_cast<int64_t>(s.qlen) * c.a.group < c.row_min) return 0;
+    if (s.qlen <= 0 || static_cast<int64_t>(s.qlen) * c.a.group < row_min) return 0;
     return min((s.qlen + C::kNQ * c.tpt - 1) / (C::kNQ * c.tpt), c.max_pairs);
   }
   // Sequence and pair number e of batch x max_pairs; false where there is none.
@@ -307,7 +309,7 @@ struct ChunkShared {
   // ahead of an item's store)
   volatile uint32_t odd[4];
   // the CTA's run
-  int64_t sums[C::kThreads / 32 + 1];
+  int64_t sums[C::kThreads / 32], few[C::kThreads / 32];
   int64_t u0, u1;
   int64_t start_e;     // batch x pair number the run starts in
   int64_t start_rest;  // and how far into its kv heads' items
@@ -396,33 +398,42 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
   // ---- the CTA's run: thread t adds up the lengths of its sequences and
   // pairs, a scan over the threads finds where the run starts
   Walk<HD> w{};
+  w.row_min = 1;
   const int64_t n_e = static_cast<int64_t>(c.a.c.batch) * c.max_pairs, per = (n_e + C::kThreads - 1) / C::kThreads;
   const int64_t e0 = threadIdx.x * per, e1 = min(e0 + per, n_e);
-  int64_t mine = 0;
+  int64_t mine = 0, few = 0;  // few: of the sequences short enough for row blocks
   for (int64_t e = e0; e < e1; ++e)
-    if (w.at(c, e)) mine += static_cast<int64_t>(w.length()) * c.a.c.nkv;
-  int64_t incl = mine;
+    if (w.at(c, e)) (w.s.qlen * static_cast<int64_t>(c.a.group) < c.row_min ? few : mine) += static_cast<int64_t>(w.length()) * c.a.c.nkv;
+  int64_t incl = mine, incl_few = few;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o), z = __shfl_up_sync(0xffffffffu, incl_few, o);
+    if (lane >= o) incl += y, incl_few += z;
   }
-  if (lane == 31) sh.sums[warp] = incl;
+  if (lane == 31) sh.sums[warp] = incl, sh.few[warp] = incl_few;
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   __syncthreads();
-  int64_t before = incl - mine, total = 0;
+  int64_t before = incl - mine, total = 0, before_few = incl_few - few, total_few = 0;
   for (int i = 0; i < C::kThreads / 32; ++i) {
-    if (i < warp) before += sh.sums[i];
+    if (i < warp) before += sh.sums[i], before_few += sh.few[i];
     total += sh.sums[i];
+    total_few += sh.few[i];
+  }
+  w.row_min = c.row_min;
+  if (chunk_takes_few(total_few, gridDim.x)) {
+    w.row_min = 1;
+    mine += few;
+    before += before_few;
+    total += total_few;
   }
   const int g = runs_of(total, C::kMinRun, gridDim.x);
   const int64_t u0 = static_cast<int>(blockIdx.x) < g ? mul_div(total, blockIdx.x, g) : total;
   const int64_t u1 = static_cast<int>(blockIdx.x) < g ? mul_div(total, blockIdx.x + 1, g) : total;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *c.total = total;
+  if (blockIdx.x == 0 && threadIdx.x == 0) c.total[0] = total, c.total[1] = w.row_min;
   if (u0 < u1 && before <= u0 && u0 < before + mine) {  // this thread's range holds the start
     int64_t at = before;
     for (int64_t e = e0; e < e1; ++e) {
@@ -874,6 +885,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const ChunkArgs c, int 
   const int g = runs_of(total, C::kMinRun, grid);
   if (cut >= g) return;
   Walk<HD> w{};
+  w.row_min = static_cast<int>(c.total[1]);
   w.at(c, static_cast<int64_t>(it.x) * c.max_pairs + it.y);
   w.kvh = it.z;
   const int64_t first = mul_div(total, cut, g) - it.w + C::kExtra;  // the item's first tile

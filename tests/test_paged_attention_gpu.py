@@ -109,6 +109,18 @@ def test_many_sequences(hd):
 
 
 @pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("singles, window, sinks", [(30, 0, 0), (300, 0, 0), (40, 60, 3), (400, 60, 3)])
+def test_few_and_many_single_tokens_beside_chunks(hd, singles, window, sinks):
+    """A few single tokens beside chunks are taken by the chunks' kernel, many by
+    the row blocks'."""
+    r = np.random.default_rng(singles)
+    q = [1] * singles + [70, 0, 3, 129]
+    kv = r.integers(1, 400, singles).tolist() + [300, 0, 500, 129]
+    at = r.permutation(len(q))
+    check([q[i] for i in at], [kv[i] for i in at], 4, 2, hd, 16, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("q_len", [2, 6, 200])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
 def test_unseen_values_do_not_matter(hd, q_len, value):
