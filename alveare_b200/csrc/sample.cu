@@ -26,7 +26,8 @@
 // us: a row's cluster is busy 23 us, of them 5 loading, 7 in the exponentials
 // and atomics of the histogram, and most of the rest in four meetings of the
 // cluster; two CTAs per SM cover for each other.  One row of 128,256 bf16
-// values with top-k 40 and top-p: 15.6 us, of it about 10 in launch and
+// values with top-k 40 and top-p: 14.5 us, of it 4.4 until the row is loaded, 3
+// in the one CTA that finishes it, the rest in passes of a few instructions and
 // meetings.
 #include <cooperative_groups.h>
 
@@ -525,23 +526,30 @@ __device__ Cut select(cg::cluster_group& cl, SampleShared& sh, const Row<BF16, R
 }
 
 // The rest of a row whose top k are among CTA 0's list: ranks by comparing each
-// with each, then top-p over the ranks, min-p, and the draw in index order.
+// with each (a warp an element: this CTA is alone by now, and 40 elements take 3
+// us of it, 5.3 with a thread for each), then top-p over the ranks, min-p, and
+// the draw in index order.
 __device__ void finish_few(SampleShared& sh, const SampleArgs& a, int r, uint32_t n, uint32_t k, float p, float min_p,
                            float top) {
-  const uint32_t i = threadIdx.x;
-  uint32_t key = 0, idx = 0, rank = 0xFFFFFFFFu;
+  const uint32_t i = threadIdx.x, lane = i & 31;
+  for (uint32_t e = i / 32; e < n; e += kSampleWarps) {  // a warp compares element e with all
+    const uint32_t ke = sh.ckey[e], ie = sh.cidx[e];
+    uint32_t before = 0;
+    for (uint32_t j = lane; j < n; j += 32) {
+      const uint32_t kj = sh.ckey[j];
+      before += kj > ke || (kj == ke && sh.cidx[j] < ie);
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0) sh.lkey[e] = before;  // (the CTA's own list is read)
+  }
+  __syncthreads();
+  uint32_t rank = 0xFFFFFFFFu;
   u64 m = 0;
   float w = 0.f;
   if (i < n) {
-    key = sh.ckey[i];
-    idx = sh.cidx[i];
-    rank = 0;
-    for (uint32_t j = 0; j < n; ++j) {
-      const uint32_t kj = sh.ckey[j];
-      rank += kj > key || (kj == key && sh.cidx[j] < idx);
-    }
+    rank = sh.lkey[i];
     if (rank < k) {
-      w = expf(key_value(key) - top);
+      w = expf(key_value(sh.ckey[i]) - top);
       m = mass_of(w);
     }
   }
@@ -563,17 +571,23 @@ __device__ void finish_few(SampleShared& sh, const SampleArgs& a, int r, uint32_
   const bool keep = i < n && rank < last && rank < k && w >= min_p;
   sh.cmass[i] = keep ? m : 0;  // by place in the list
   __syncthreads();
-  u64 before = 0, kept = 0;
-  for (uint32_t j = 0; j < n; ++j) {
-    const u64 mj = sh.cmass[j];
-    kept += mj;
-    if (i < n && sh.cidx[j] < idx) before += mj;
-  }
+  u64 kept = 0;
+  for (uint32_t j = lane; j < n; j += 32) kept += sh.cmass[j];
+  kept = lane_sum(kept);
   const u64 x = static_cast<u64>(fmax(floor(static_cast<double>(a.u[r]) * static_cast<double>(kept)), 0.0));
   const u64 goal = x < kept ? x : kept - 1;
-  if (keep && before <= goal && goal < before + m) {
-    a.tokens[r] = static_cast<int>(idx);
-    if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(m) / static_cast<double>(kept)));
+  for (uint32_t e = i / 32; e < n; e += kSampleWarps) {
+    const u64 me = sh.cmass[e];
+    if (me == 0) continue;
+    const uint32_t ie = sh.cidx[e];
+    u64 before = 0;
+    for (uint32_t j = lane; j < n; j += 32)
+      if (sh.cidx[j] < ie) before += sh.cmass[j];
+    before = lane_sum(before);
+    if (lane == 0 && before <= goal && goal < before + me) {
+      a.tokens[r] = static_cast<int>(ie);
+      if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(me) / static_cast<double>(kept)));
+    }
   }
 }
 
