@@ -79,6 +79,28 @@ def test_tokens_match_the_integers(dtype, vocab, setting):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [360449, 400001, 524288])
+def test_vocabularies_too_long_to_keep_on_chip(dtype, vocab):
+    logits, u = rand(3, vocab, dtype, seed=vocab)
+    for kw in (dict(), dict(top_p=0.9), dict(top_k=40, top_p=0.95), dict(top_k=5000, top_p=0.8, min_p=0.001),
+               dict(temperature=0.0)):
+        same(logits, u, **kw)
+
+
+@pytest.mark.parametrize("step", [0.0, 0.01, 0.25])
+@pytest.mark.parametrize("top_k", [0, 600, 3000])
+@pytest.mark.parametrize("top_p", [0.2, 0.7, 0.97])
+@pytest.mark.parametrize("min_p", [0.0, 1e-4, 0.03, 0.4])
+def test_prefixes_and_floor_together(step, top_k, top_p, min_p):
+    """Prefixes that end in ties of any length (logits on a grid), with a floor
+    above, inside and below them."""
+    logits, u = rand(4, 40000, seed=int(1000 * step) + top_k)
+    if step:
+        logits = (logits / step).round() * step
+    same(logits, u, top_k=top_k, top_p=top_p, min_p=min_p)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_ties_keep_the_lowest_indices(dtype):
     logits = torch.zeros(6, 5000, dtype=dtype, device="cuda")
     u = torch.linspace(0, 0.999, 6).cuda()
