@@ -228,8 +228,8 @@ int make_paged_view(alv_ctx* ctx, const char* who, const alv_paged* p, PagedView
   const std::string w(who);
   if (!p || p->batch < 0 || p->tokens < 0 || !p->k || !p->v || !p->table || !p->q_start || !p->kv_lens)
     return fail(ctx, ALV_ERR_ARG, w + ": null pointer or negative size in the paged cache");
-  if (p->pages < 1 || p->kv_heads < 1 || p->page_size < 1 || p->table_width < 1 || p->table_stride < p->table_width)
-    return fail(ctx, ALV_ERR_ARG, w + ": pages, kv_heads, page_size and table_width must be positive");
+  if (p->pages < 1 || p->kv_heads < 1 || p->page_size < 1 || p->table_width < 1 || p->table_stride < 0)
+    return fail(ctx, ALV_ERR_ARG, w + ": pages, kv_heads, page_size and table_width must be positive, table_stride not negative");
   if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
     return fail(ctx, ALV_ERR_SHAPE, w + ": head_dim must be 64, 128 or 256");
   if (p->page_size % 16) return fail(ctx, ALV_ERR_SHAPE, w + ": page_size must be a multiple of 16");
@@ -258,13 +258,13 @@ extern "C" int alv_qk_norm_rope(alv_ctx* ctx, const alv_paged* cache, const alv_
   if (rc) return rc;
   RopeArgs a{};
   if ((rc = make_paged_view(ctx, "qk_norm_rope", cache, &a.c))) return rc;
-  const int hd = cache->head_dim, heads = args->heads + 2 * cache->kv_heads;
+  const int hd = cache->head_dim;
   if ((cache->tokens && (!args->qkv || !args->q_out)) || !args->rope || !valid_dtype(args->qkv_dtype) || !valid_dtype(args->rope_dtype) ||
       args->heads < 1 || args->max_pos < 1 || !(args->eps >= 0.f))
     return fail(ctx, ALV_ERR_ARG, "qk_norm_rope: bad argument");
   if (args->rot < 16 || args->rot > hd || args->rot % 16)
     return fail(ctx, ALV_ERR_SHAPE, "qk_norm_rope: the rotated dims must be a multiple of 16, at most head_dim");
-  if (args->qkv_stride < static_cast<int64_t>(heads) * hd || args->qkv_stride % 8 || args->q_token_stride % 8 ||
+  if (args->qkv_stride < 0 || args->qkv_stride % 8 || args->q_token_stride % 8 ||
       args->q_head_stride % 8 || args->q_token_stride < 0 || args->q_head_stride < 0 ||
       ((reinterpret_cast<uintptr_t>(args->qkv) | reinterpret_cast<uintptr_t>(args->q_out) |
         reinterpret_cast<uintptr_t>(args->rope) | reinterpret_cast<uintptr_t>(args->q_weight) |

@@ -846,7 +846,7 @@ using namespace alv;
 extern "C" int alv_sample(alv_ctx* ctx, const alv_sample_args* s, void* stream) {
   if (!ctx || !s) return fail(ctx, ALV_ERR_ARG, "sample: bad argument");
   if (s->rows < 0 || s->vocab < 1 || !valid_dtype(s->logits_dtype) || (s->rows && (!s->logits || !s->u || !s->tokens)) ||
-      s->logits_stride < s->vocab)
+      s->logits_stride < 0)
     return fail(ctx, ALV_ERR_ARG, "sample: bad argument");
   if (s->vocab > kMaxCluster * kMaxSlice) return fail(ctx, ALV_ERR_UNSUPPORTED, "sample: at most 524,288 tokens");
   if (reinterpret_cast<uintptr_t>(s->logits) & (s->logits_dtype == ALV_F32 ? 3 : 1))

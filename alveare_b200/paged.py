@@ -89,6 +89,12 @@ def _vector(t, name: str, device: int, dtype, n: int) -> int:
     return t.data_ptr()
 
 
+def _step(stride: int, rows: int, width: int) -> int:
+    """Elements between a matrix's rows: its own stride (0 where one row is
+    broadcast); of a single row, whose stride may be anything, its width."""
+    return stride if rows > 1 else width
+
+
 def _stream(device: int) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -117,7 +123,7 @@ def _paged(device: int, k_pages, v_pages, page_table, q_start, kv_lens, tokens: 
         raise ValueError("pages and page_table must be contiguous in their last dimension, q_start and kv_lens whole")
     pages, heads, ps, hd = shape
     return _PAGED.pack(k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], strides[2], pages, heads, ps, hd,
-                       page_table.data_ptr(), max(ts[0], width), q_start.data_ptr(), kv_lens.data_ptr(), width, batch,
+                       page_table.data_ptr(), _step(ts[0], rows, width), q_start.data_ptr(), kv_lens.data_ptr(), width, batch,
                        tokens, 0), heads, hd
 
 
@@ -157,7 +163,7 @@ def qk_norm_rope(qkv, q_out, k_pages, v_pages, page_table, q_start, kv_lens, rop
         raise ValueError("qkv and q_out must be contiguous in their last dimension")
     qw = 0 if q_weight is None else _vector(q_weight, "q_weight", device, torch.float32, hd)
     kw = 0 if k_weight is None else _vector(k_weight, "k_weight", device, torch.float32, hd)
-    a = _NORM_ROPE.pack(qkv.data_ptr(), max(xs[0], cols), q_out.data_ptr(), qs[0], qs[1], rope.data_ptr(), qw, kw, qd,
+    a = _NORM_ROPE.pack(qkv.data_ptr(), _step(xs[0], tokens, cols), q_out.data_ptr(), qs[0], qs[1], rope.data_ptr(), qw, kw, qd,
                         rd, heads, width // 2, max_pos, eps)
     ctx = context(device)
     rc = ctx.lib.alv_qk_norm_rope(ctx.ptr, c, a, _stream(device))
@@ -213,9 +219,12 @@ def _pool(device: int, k_pool, v_pool, page_table, lens, refs) -> bytes:
     if st[2:] != (ps * hd, hd, 1) or ts[1] != 1:
         raise ValueError("a page must be contiguous, and page_table in its last dimension")
     slots, width = page_table.shape
+    step = _step(ts[0], slots, width)
+    if step < width:
+        raise ValueError("page_table's rows must not overlap (it is written)")
     lp = 0 if lens is None else _vector(lens, "lens", device, torch.int32, slots)
     return _PAGES.pack(k_pool.data_ptr(), v_pool.data_ptr(), st[0] * 2, st[1] * 2, nkv * ps * hd * 2,
-                       page_table.data_ptr(), lp, _vector(refs, "refs", device, torch.int32, pages), max(ts[0], width),
+                       page_table.data_ptr(), lp, _vector(refs, "refs", device, torch.int32, pages), step,
                        layers, pages, ps, slots, width, 0)
 
 
@@ -320,7 +329,7 @@ def sample_tokens(logits, u, tokens, logprobs=None, *, temperature=1.0, top_k=0,
     k_rows, k = _param(top_k, "top_k", device, torch.int32, rows, 0)
     p_rows, p = _param(top_p, "top_p", device, torch.float32, rows, 1.0)
     m_rows, m = _param(min_p, "min_p", device, torch.float32, rows, 0.0)
-    a = _SAMPLE.pack(logits.data_ptr(), max(stride[0], vocab), up, tp, lp, t_rows, p_rows, m_rows, k_rows, ld, rows,
+    a = _SAMPLE.pack(logits.data_ptr(), _step(stride[0], rows, vocab), up, tp, lp, t_rows, p_rows, m_rows, k_rows, ld, rows,
                      vocab, max(0, min(k, vocab)), t, p, m, 0)
     ctx = context(device)
     rc = ctx.lib.alv_sample(ctx.ptr, a, _stream(device))

@@ -327,7 +327,8 @@ int alv_llama_info(alv_ctx* ctx, alv_handle model, int64_t* info);
  * sequence b's position j is row j % page_size of page table[b * table_stride
  * + j / page_size].  Its new tokens are rows q_start[b] .. q_start[b + 1] - 1
  * of the call's token tensors and the last positions of kv_lens[b] (which
- * counts them).  head_dim 64, 128 or 256; page_size a multiple of 16; k, v
+ * counts them).  Table rows may overlap or coincide (table_stride 0: one row
+ * for every sequence).  head_dim 64, 128 or 256; page_size a multiple of 16; k, v
  * 16-byte aligned and strides multiples of 8 elements. */
 typedef struct {
   uint16_t *k, *v;
@@ -345,7 +346,8 @@ typedef struct {
  * (heads + 2 kv_heads) * head_dim, ALV_F32 or ALV_BF16).  q_weight / k_weight
  * (head_dim fp32; NULL: no norm); rope: (max_pos, 2 * rot) rows of cos (rot) |
  * sin (rot), ALV_F32 or ALV_BF16 (the first rot / 2 of each are read); dims
- * past rot pass through unrotated.  fp32 arithmetic, one rounding to bf16. */
+ * past rot pass through unrotated.  Rows of qkv may overlap (qkv_stride 0: one
+ * row for every token).  fp32 arithmetic, one rounding to bf16. */
 typedef struct {
   const void* qkv;
   int64_t qkv_stride;
@@ -422,8 +424,10 @@ int alv_pages_compact(alv_ctx* ctx, const alv_pages* p, int32_t* table_out, int3
  * Masses are summed as integers, so the result does not depend on any order.
  * Per-row parameters are device arrays where the pointer is given, else the
  * scalar applies to all.  temperature 0: the largest logit (lowest index).
- * NaN counts as -inf.  At most 524,288 tokens.  A row with nothing above -inf gives token -1.  logprobs
- * (fp32, may be NULL): log of the token's share of the kept mass. */
+ * NaN counts as -inf.  At most 524,288 tokens.  A row with nothing above -inf
+ * gives token -1.  logprobs (fp32, may be NULL): log of the token's share of
+ * the kept mass.  Rows of logits may overlap (logits_stride 0: one row, drawn
+ * from `rows` times). */
 typedef struct {
   const void* logits;
   int64_t logits_stride; /* elements per row */
