@@ -629,9 +629,11 @@ extern "C" int alv_paged_attention(alv_ctx* ctx, const alv_paged* cache, const a
   a.row_max = INT_MAX;
   if (static_cast<int64_t>(args->max_q_len) * a.group > kRowsPerBlock && chunk_takes(a)) {
     a.row_max = kRowsPerBlock;
-    // all sequences as long as the longest: none is left for the row blocks
+    // Room for max_q_len tokens of every sequence: a uniform batch, which leaves
+    // nothing for row blocks.  A captured one may be replayed with shorter
+    // sequences, so the tensor-core form, alone, takes those too.
     const bool mixed = static_cast<int64_t>(cache->batch) * args->max_q_len != cache->tokens;
-    return launch_chunk(ctx, a, cache->head_dim, args->max_q_len, kRowsPerBlock + 1, mixed, st);
+    return launch_chunk(ctx, a, cache->head_dim, args->max_q_len, mixed ? kRowsPerBlock + 1 : 1, mixed, st);
   }
   return launch_rows(ctx, a, cache->head_dim, 0, false, st);
 }

@@ -65,7 +65,8 @@ __device__ __forceinline__ bool chunk_takes_few(int64_t length, int ctas) { retu
 
 // The tensor-core form for chunks (paged_chunk.cu): sequences with at least
 // row_min rows (new tokens x heads of a kv group).  mixed: the row-block
-// kernel for the others is launched between it and its join.
+// kernel for the others is launched between it and its join (without it
+// row_min is 1: every sequence is somebody's).
 bool chunk_takes(const AttnArgs& a);
 int launch_chunk(alv_ctx* ctx, const AttnArgs& a, int hd, int max_q_len, int row_min, bool mixed, cudaStream_t st);
 // The row-block kernel (paged_attn.cu); its scratch starts at byte `scratch`

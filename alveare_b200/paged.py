@@ -139,7 +139,8 @@ def qk_norm_rope(qkv, q_out, k_pages, v_pages, page_table, q_start, kv_lens, rop
     q_out    (tokens, heads, head_dim) bfloat16
     k_pages, v_pages  (pages, kv_heads, page_size, head_dim) bfloat16, one layer
     page_table        (batch, width) int32: page of positions [i page_size, (i + 1) page_size)
-    q_start           (batch + 1,) int32: first token of each sequence, then the token count
+    q_start           (batch + 1,) int32: first token of each sequence, then one past the
+                      last (rows from there on are left alone)
     kv_lens           (batch,) int32: positions in the cache, the new tokens' included
     rope     (max_pos, 2 rot) float32 or bfloat16: cos (rot) | sin (rot) of each
              position (:func:`alveare_b200.llama.rope_table`); pairs are (i, i + rot / 2)

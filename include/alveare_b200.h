@@ -327,7 +327,9 @@ int alv_llama_info(alv_ctx* ctx, alv_handle model, int64_t* info);
  * sequence b's position j is row j % page_size of page table[b * table_stride
  * + j / page_size].  Its new tokens are rows q_start[b] .. q_start[b + 1] - 1
  * of the call's token tensors and the last positions of kv_lens[b] (which
- * counts them).  Table rows may overlap or coincide (table_stride 0: one row
+ * counts them).  The token tensors may have more rows than the sequences use
+ * (a captured step replayed with less): rows before q_start[0] and from
+ * q_start[batch] on belong to no sequence, and nothing is written for them.  Table rows may overlap or coincide (table_stride 0: one row
  * for every sequence).  head_dim 64, 128 or 256; page_size a multiple of 16; k, v
  * 16-byte aligned and strides multiples of 8 elements. */
 typedef struct {
