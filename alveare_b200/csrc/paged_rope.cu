@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(kRopeThreads, 3) qk_norm_rope_kernel(const Rop
     int pos = s.kv - s.qlen + (t - s.q0);
     int64_t slot = -1;
     if (t < s.q0 || t >= s.q0 + s.qlen || pos < 0 || pos >= a.max_pos) {
-      atomicOr(c.status, kStatusBadIndex);
+      // (a row before the first sequence or past the last is nobody's, and no error)
+      if (t >= c.q_start[0] && t < c.q_start[c.batch]) atomicOr(c.status, kStatusBadIndex);
       pos = -1;
     } else {
       const int page = page_of(c, b, pos);

@@ -61,3 +61,31 @@ def test_uniform_looking_batches(window, sinks):
         out = torch.full_like(q, 7.0)
         ab.paged_attention(q, out, k, v, table, starts(q_lens), ints(kv), max_q_len=5, window=window, sinks=sinks)
         check(out, q, rows, q_lens, kv, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("tokens", [9, 3000])
+def test_rows_past_the_last_sequence_are_not_an_error(tokens):
+    """Norm + rotation + append leaves them alone, as attention does."""
+    k, v, table, _ = make_cache([20, 5], 2, 64, 16, fill=0.0)
+    qkv = noise(tokens, 8 * 64).cuda()
+    rope = torch.rand(32, 128, generator=torch.Generator().manual_seed(2)).cuda()
+    got = []
+    for x, n in ((qkv, tokens), (qkv[:5], 5)):
+        kk, vv = k.clone(), v.clone()
+        out = torch.full((n, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        ab.qk_norm_rope(x, out, kk, vv, table, starts([3, 2]), ints([20, 5]), rope)
+        _lib.context(0).sync_status(torch.cuda.current_stream().cuda_stream)
+        got.append((out, kk, vv))
+    (a, ka, va), (b, kb, vb) = got
+    assert torch.equal(a[:5], b) and (a[5:] == 7).all()
+    assert torch.equal(ka, kb) and torch.equal(va, vb)
+    # the first sequence may start past row 0
+    out = torch.full((tokens, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    ab.qk_norm_rope(qkv, out, k.clone(), v.clone(), table, ints([2, 5, 7]), ints([20, 5]), rope)
+    _lib.context(0).sync_status(torch.cuda.current_stream().cuda_stream)
+    assert (out[:2] == 7).all() and (out[7:] == 7).all() and (out[2:7] != 7).any(-1).all()
+    # starts that are out of order or past the rows still are
+    for st in ([0, 3, 2], [0, 3, tokens + 1], [-1, 3, 5]):
+        ab.qk_norm_rope(qkv, out, k.clone(), v.clone(), table, ints(st), ints([20, 5]), rope)
+        with pytest.raises(_lib.AlvError):
+            _lib.context(0).sync_status(torch.cuda.current_stream().cuda_stream)
