@@ -366,6 +366,12 @@ class PagedKVCache:
         t = torch.tensor(v, dtype=torch.int32).to(torch.device("cuda", self.device))
         return t.reshape(-1, 2) if pairs else t
 
+    def check_slots(self, slots) -> None:
+        """ValueError unless all of these (host numbers) are slots of this pool."""
+        n = self.lens.shape[0]
+        if not all(0 <= s < n for s in slots):
+            raise ValueError(f"slots must be in [0, {n})")
+
     def update(self, free=None, fork=None, extend=None) -> None:
         """:func:`update_pages` on this pool; lists of ids (or pairs) or int32 CUDA tensors."""
         update_pages(self.k, self.v, self.table, self.lens, self.refs, free=self._ids(free, False),
@@ -394,9 +400,13 @@ class PagedKVCache:
         """Tensors of a step in which ``slots[i]`` gets ``q_lens[i]`` new tokens
         (already reserved by :meth:`update`): page_table, q_start, kv_lens."""
         dev = torch.device("cuda", self.device)
-        idx = torch.tensor(list(slots), dtype=torch.int64).to(dev)
+        slots, q_lens = [int(s) for s in slots], [int(n) for n in q_lens]
+        self.check_slots(slots)
+        if len(slots) != len(q_lens) or min(q_lens, default=0) < 0:
+            raise ValueError("batch: every slot needs a number of new tokens")
+        idx = torch.tensor(slots, dtype=torch.int64).to(dev)
         start = [0]
         for n in q_lens:
-            start.append(start[-1] + int(n))
+            start.append(start[-1] + n)
         return dict(page_table=self.table[idx], q_start=torch.tensor(start, dtype=torch.int32).to(dev),
                     kv_lens=self.lens[idx])

@@ -78,8 +78,9 @@ class PagedLlama:
         token.  Raises RuntimeError (and appends nothing) when the cache has no
         room for all of them."""
         c = self.cfg
-        lens = [len(t) for t in tokens]
-        if min(lens, default=0) < 1 or len(set(slots)) != len(lens):
+        lens, slots = [len(t) for t in tokens], [int(s) for s in slots]
+        self.cache.check_slots(slots)
+        if min(lens, default=0) < 1 or not len(set(slots)) == len(slots) == len(lens):
             raise ValueError("step: every slot once, with at least one token")
         flat = torch.tensor([t for ts in tokens for t in ts], dtype=torch.int64)
         if int(flat.min()) < 0 or int(flat.max()) >= c.vocab:

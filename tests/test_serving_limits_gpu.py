@@ -1,0 +1,58 @@
+"""PagedLlama at its limits: positions past max_seq, slots that do not exist,
+prompts without tokens, sequences of others, steps that fail half way."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from alveare_b200 import PagedKVCache, _lib  # noqa: E402
+from alveare_b200.llama import LlamaConfig  # noqa: E402
+from alveare_b200.serving import PagedLlama  # noqa: E402
+from oracle import llama  # noqa: E402
+
+CFG = llama.Config(hidden=256, intermediate=512, heads=4, kv_heads=2, head_dim=64, layers=2, vocab=1000,
+                   vocab_padded=1024, max_seq=100)
+
+
+@pytest.fixture(scope="module")
+def weights():
+    return llama.synthetic_weights(CFG, seed=3)[0]
+
+
+def build(w, max_seq=100, **kw):
+    c = LlamaConfig(CFG.hidden, CFG.intermediate, CFG.heads, CFG.kv_heads, CFG.head_dim, CFG.layers, CFG.vocab, max_seq,
+                    1e-5, 0)
+    return PagedLlama(w, c, rope_theta=CFG.rope_theta, **{**dict(pages=64, page_size=16, slots=8), **kw})
+
+
+def state(m):
+    return [t.clone() for t in (m.cache.table, m.cache.lens, m.cache.refs)]
+
+
+def unchanged(m, before):
+    assert all(torch.equal(a, b) for a, b in zip(state(m), before))
+    _lib.context(0).sync_status(torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("slot", [-1, 8, 10 ** 6])
+def test_slots_that_do_not_exist(weights, slot):
+    m = build(weights)
+    m.step([7], [[1] * 20])
+    before = state(m)
+    with pytest.raises(ValueError, match="slot"):
+        m.step([0, slot], [[1], [2]])
+    unchanged(m, before)
+    with pytest.raises(ValueError, match="slot"):
+        m.step([0, 0, 1], [[1], [2]])
+    unchanged(m, before)
+    with pytest.raises(ValueError, match="slot"):
+        m.cache.batch([slot], [1])
+
+
+def test_batches_that_do_not_match():
+    c = PagedKVCache(1, 2, 64, 8, slots=4, max_len=64)
+    with pytest.raises(ValueError):
+        c.batch([0, 1], [1])
+    with pytest.raises(ValueError):
+        c.batch([0, 1], [1, -1])
