@@ -76,7 +76,7 @@ class PagedLlama:
         """Append ``tokens[i]`` (a list of ids) to sequence ``slots[i]``, all in
         one batch; the bfloat16 logits (len(slots), vocab) after each one's last
         token.  Raises RuntimeError (and appends nothing) when the cache has no
-        room for all of them."""
+        room for all of them or a sequence would pass ``max_seq`` tokens."""
         c = self.cfg
         lens, slots = [len(t) for t in tokens], [int(s) for s in slots]
         self.cache.check_slots(slots)
@@ -87,9 +87,11 @@ class PagedLlama:
             raise ValueError("step: token id out of range")
         before = self.cache.snapshot()
         self.cache.update(extend=list(zip(slots, lens)))
-        if self.cache.check()["first_unmet"] >= 0:
+        # (pages are whole: the last one may have room past max_seq)
+        first_unmet, *held = torch.cat((self.cache.info[3:], self.cache.lens)).tolist()
+        if first_unmet >= 0 or any(held[s] > c.max_seq for s in slots):
             self.cache.restore(before)
-            raise RuntimeError("step: the cache has no room for these tokens")
+            raise RuntimeError("step: the cache has no room for these tokens, or max_seq is passed")
         b = self.cache.batch(slots, lens)
         x = self.emb[flat.to(self.device)].bfloat16()
         rows, hd = x.shape[0], c.head_dim

@@ -56,3 +56,23 @@ def test_batches_that_do_not_match():
         c.batch([0, 1], [1])
     with pytest.raises(ValueError):
         c.batch([0, 1], [1, -1])
+
+
+@pytest.mark.parametrize("page_size", [16, 48])
+@pytest.mark.parametrize("max_seq", [96, 100])
+def test_max_seq(weights, max_seq, page_size):
+    """max_seq tokens fit, whatever the page size; one more appends nothing."""
+    m = build(weights, max_seq, page_size=page_size)
+    m.step([1, 3], [[5] * (max_seq - 1), [6] * 10])
+    assert torch.isfinite(m.step([1], [[7]]).float()).all()
+    before = state(m)
+    with pytest.raises(RuntimeError, match="room"):
+        m.step([3, 1], [[8], [9]])
+    unchanged(m, before)
+    with pytest.raises(RuntimeError, match="room"):
+        m.step([3], [[8] * (max_seq - 9)])
+    unchanged(m, before)
+    assert torch.isfinite(m.step([3], [[8] * (max_seq - 10)]).float()).all()
+    _lib.context(0).sync_status(torch.cuda.current_stream().cuda_stream)
+    with pytest.raises(RuntimeError, match="room"):   # prompt and answer together
+        build(weights, max_seq, page_size=page_size).generate([[1] * (max_seq - 2)], 4)
