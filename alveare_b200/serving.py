@@ -116,6 +116,10 @@ class PagedLlama:
         tokens (all sequences' chunks in one batch), their pages shared by the n
         branches, then sampled tokens.  Returns [prompt][branch][token]."""
         B = len(prompts)
+        if B < 1 or min(map(len, prompts)) < 1:
+            raise ValueError("generate: every prompt needs at least one token")
+        if n < 1 or chunk < 1:
+            raise ValueError("generate: n and chunk must be positive")
         if B * n > self.cache.table.shape[0]:
             raise ValueError(f"generate: {B * n} sequences need as many slots (there are {self.cache.table.shape[0]})")
         self.cache.update(free=list(range(B * n)))

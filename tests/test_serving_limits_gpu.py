@@ -76,3 +76,16 @@ def test_max_seq(weights, max_seq, page_size):
     _lib.context(0).sync_status(torch.cuda.current_stream().cuda_stream)
     with pytest.raises(RuntimeError, match="room"):   # prompt and answer together
         build(weights, max_seq, page_size=page_size).generate([[1] * (max_seq - 2)], 4)
+
+
+def test_prompts_without_tokens(weights):
+    m = build(weights)
+    for prompts in ([], [[]], [[1, 2], []]):
+        with pytest.raises(ValueError, match="prompt"):
+            m.generate(prompts, 3)
+    with pytest.raises(ValueError):
+        m.generate([[1, 2]], 3, chunk=-4)
+    with pytest.raises(ValueError):
+        m.generate([[1, 2]], 3, n=0)
+    assert m.generate([[1, 2]], 0) == [[[]]]
+    assert int(m.cache.refs.sum()) == 0
