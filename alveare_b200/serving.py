@@ -114,21 +114,24 @@ class PagedLlama:
                  top_k=0, top_p=1.0, min_p=0.0):
         """``n`` continuations of every prompt: prompts in chunks of ``chunk``
         tokens (all sequences' chunks in one batch), their pages shared by the n
-        branches, then sampled tokens.  Returns [prompt][branch][token]."""
+        branches, then sampled tokens.  Returns [prompt][branch][token].  Takes
+        slots that hold no tokens (ValueError if there are too few) and empties
+        them again; other sequences stay as they are."""
         B = len(prompts)
         if B < 1 or min(map(len, prompts)) < 1:
             raise ValueError("generate: every prompt needs at least one token")
         if n < 1 or chunk < 1:
             raise ValueError("generate: n and chunk must be positive")
-        if B * n > self.cache.table.shape[0]:
-            raise ValueError(f"generate: {B * n} sequences need as many slots (there are {self.cache.table.shape[0]})")
-        self.cache.update(free=list(range(B * n)))
+        slots = [s for s, held in enumerate(self.cache.lens.tolist()) if held == 0][:B * n]
+        if len(slots) < B * n:
+            raise ValueError(f"generate: {B * n} sequences need as many empty slots (there are {len(slots)})")
+        self.cache.update(free=slots)  # (pages that a shortened sequence left)
         logits = torch.empty(B, self.cfg.vocab, dtype=torch.bfloat16, device=self.device)
         for at in range(0, max(map(len, prompts)), chunk):
             rows = [i for i, p in enumerate(prompts) if at < len(p)]
-            logits[rows] = self.step([i * n for i in rows], [list(prompts[i][at:at + chunk]) for i in rows])
+            logits[rows] = self.step([slots[i * n] for i in rows], [list(prompts[i][at:at + chunk]) for i in rows])
         if n > 1:
-            self.cache.update(fork=[(i * n, i * n + j) for i in range(B) for j in range(1, n)])
+            self.cache.update(fork=[(slots[i * n], slots[i * n + j]) for i in range(B) for j in range(1, n)])
         logits = logits.repeat_interleave(n, 0)
         gen = torch.Generator(device=self.device).manual_seed(seed)
         tok = torch.empty(B * n, dtype=torch.int32, device=self.device)
@@ -138,6 +141,6 @@ class PagedLlama:
             sample_tokens(logits, u, tok, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
             out.append(tok.tolist())
             if i + 1 < max_new_tokens:
-                logits = self.step(list(range(B * n)), [[t] for t in out[-1]])
-        self.cache.update(free=list(range(B * n)))
+                logits = self.step(slots, [[t] for t in out[-1]])
+        self.cache.update(free=slots)
         return [[[row[i * n + j] for row in out] for j in range(n)] for i in range(B)]

@@ -89,3 +89,20 @@ def test_prompts_without_tokens(weights):
         m.generate([[1, 2]], 3, n=0)
     assert m.generate([[1, 2]], 0) == [[[]]]
     assert int(m.cache.refs.sum()) == 0
+
+
+def test_generate_leaves_other_sequences_alone(weights):
+    r = np.random.default_rng(1)
+    prompt, more = r.integers(0, CFG.vocab, 30).tolist(), [r.integers(0, CFG.vocab, 11).tolist() for _ in range(2)]
+    m = build(weights)
+    m.step([0, 2], [prompt, prompt[:9]])
+    kept = m.cache.lens.tolist()
+    a = m.generate(more, 4, n=2, temperature=0.0, seed=1)
+    assert m.cache.lens.tolist() == kept
+    after = m.step([0], [[17]])
+    alone = build(weights)
+    alone.step([0, 2], [prompt, prompt[:9]])
+    assert torch.equal(after, alone.step([0], [[17]]))
+    assert a == build(weights).generate(more, 4, n=2, temperature=0.0, seed=1)
+    with pytest.raises(ValueError, match="slots"):   # six are free
+        m.generate([[1]] * 7, 1)
