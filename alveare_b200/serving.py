@@ -126,21 +126,23 @@ class PagedLlama:
         if len(slots) < B * n:
             raise ValueError(f"generate: {B * n} sequences need as many empty slots (there are {len(slots)})")
         self.cache.update(free=slots)  # (pages that a shortened sequence left)
-        logits = torch.empty(B, self.cfg.vocab, dtype=torch.bfloat16, device=self.device)
-        for at in range(0, max(map(len, prompts)), chunk):
-            rows = [i for i, p in enumerate(prompts) if at < len(p)]
-            logits[rows] = self.step([slots[i * n] for i in rows], [list(prompts[i][at:at + chunk]) for i in rows])
-        if n > 1:
-            self.cache.update(fork=[(slots[i * n], slots[i * n + j]) for i in range(B) for j in range(1, n)])
-        logits = logits.repeat_interleave(n, 0)
-        gen = torch.Generator(device=self.device).manual_seed(seed)
-        tok = torch.empty(B * n, dtype=torch.int32, device=self.device)
-        out = []
-        for i in range(max_new_tokens):
-            u = torch.rand(B * n, generator=gen, device=self.device)
-            sample_tokens(logits, u, tok, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
-            out.append(tok.tolist())
-            if i + 1 < max_new_tokens:
-                logits = self.step(slots, [[t] for t in out[-1]])
-        self.cache.update(free=slots)
+        try:
+            logits = torch.empty(B, self.cfg.vocab, dtype=torch.bfloat16, device=self.device)
+            for at in range(0, max(map(len, prompts)), chunk):
+                rows = [i for i, p in enumerate(prompts) if at < len(p)]
+                logits[rows] = self.step([slots[i * n] for i in rows], [list(prompts[i][at:at + chunk]) for i in rows])
+            if n > 1:
+                self.cache.update(fork=[(slots[i * n], slots[i * n + j]) for i in range(B) for j in range(1, n)])
+            logits = logits.repeat_interleave(n, 0)
+            gen = torch.Generator(device=self.device).manual_seed(seed)
+            tok = torch.empty(B * n, dtype=torch.int32, device=self.device)
+            out = []
+            for i in range(max_new_tokens):
+                u = torch.rand(B * n, generator=gen, device=self.device)
+                sample_tokens(logits, u, tok, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+                out.append(tok.tolist())
+                if i + 1 < max_new_tokens:
+                    logits = self.step(slots, [[t] for t in out[-1]])
+        finally:  # also when a step finds no room half way
+            self.cache.update(free=slots)
         return [[[row[i * n + j] for row in out] for j in range(n)] for i in range(B)]

@@ -106,3 +106,13 @@ def test_generate_leaves_other_sequences_alone(weights):
     assert a == build(weights).generate(more, 4, n=2, temperature=0.0, seed=1)
     with pytest.raises(ValueError, match="slots"):   # six are free
         m.generate([[1]] * 7, 1)
+
+
+def test_generate_that_fails_gives_its_pages_back(weights):
+    m = build(weights, pages=8)
+    m.step([5], [[1] * 20])
+    before = state(m)
+    with pytest.raises(RuntimeError, match="room"):
+        m.generate([[1] * 60, [2] * 30], 40)
+    after = state(m)
+    assert torch.equal(after[1], before[1]) and torch.equal(after[2], before[2])
