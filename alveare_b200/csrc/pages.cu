@@ -30,7 +30,8 @@ struct PagesArgs {
   int* n_moves;
   int2* moves;
   int* avail;
-  int* cow;  // [n_extend] the shared last page an extend copies, or -1
+  int* cow;    // [n_extend] the shared last page an extend copies, or -1
+  int* drops;  // [pages] pages to drop at the end
 };
 
 // Exclusive prefix sum over the CTA; `total` in every thread.
@@ -60,11 +61,6 @@ __device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t* total, int64_t* 
 }
 
 __device__ __forceinline__ int pages_for(int64_t len, int ps) { return static_cast<int>((len + ps - 1) / ps); }
-
-// Entries of a slot's row that may hold pages.
-__device__ __forceinline__ int row_entries(const PagesArgs& a, int slot) {
-  return min(a.width, pages_for(max(a.lens[slot], 0), a.page_size));
-}
 
 __device__ __forceinline__ bool slot_ok(const PagesArgs& a, int slot) {
   if (slot >= 0 && slot < a.slots) return true;
@@ -99,40 +95,66 @@ __device__ int lists_clash(const PagesArgs& a, uint32_t* bits) {
   return __syncthreads_or(clash & 1) * 1 | (__syncthreads_or(clash & 2) ? 2 : 0) | (__syncthreads_or(clash & 4) ? 4 : 0);
 }
 
-// Slots free_ids[i0 .. i1): one warp per slot.
-__device__ void drop_slots(const PagesArgs& a, int i0, int i1) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  for (int i = i0 + warp; i < i1; i += nw) {
-    const int slot = a.free_ids[i];
-    if (!slot_ok(a, slot)) continue;
-    int* row = a.table + slot * a.table_stride;
-    const int n = row_entries(a, slot);
-    __syncwarp();
-    for (int e = lane; e < n; e += 32) {
-      count(a, row[e], -1);
-      row[e] = -1;
-    }
-    if (lane == 0) a.lens[slot] = 0;
+// Whole rows are dropped and forked: a caller may have lowered lens (rejected
+// tokens), and the entries past it still name pages.  A warp takes kRowPart
+// entries of a list's row at a time, their loads in flight together.
+constexpr int kRowLoads = 8, kRowPart = 32 * kRowLoads;
+
+// f(list entry, first table entry of the part) for every part of rows i0 .. i1.
+template <class F>
+__device__ __forceinline__ void each_part(const PagesArgs& a, int i0, int i1, F f) {
+  const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5, parts = (a.width + kRowPart - 1) / kRowPart;
+  int i = i0 + warp / parts, part = warp % parts;
+  while (i < i1) {
+    f(i, part * kRowPart);
+    for (part += nw; part >= parts; part -= parts) ++i;
+  }
+}
+__device__ __forceinline__ void load_part(const PagesArgs& a, const int* row, int e0, int (&page)[kRowLoads]) {
+#pragma unroll
+  for (int x = 0; x < kRowLoads; ++x) {
+    const int e = e0 + 32 * x + (threadIdx.x & 31);
+    page[x] = e < a.width ? row[e] : -1;
   }
 }
 
+// Slots free_ids[i0 .. i1).
+__device__ void drop_slots(const PagesArgs& a, int i0, int i1) {
+  const int lane = threadIdx.x & 31;
+  each_part(a, i0, i1, [&](int i, int e0) {
+    const int slot = a.free_ids[i];
+    if (!slot_ok(a, slot)) return;
+    int* row = a.table + slot * a.table_stride;
+    int page[kRowLoads];
+    load_part(a, row, e0, page);
+#pragma unroll
+    for (int x = 0; x < kRowLoads; ++x)
+      if (page[x] != -1) {
+        count(a, page[x], -1);
+        row[e0 + 32 * x + lane] = -1;
+      }
+    if (e0 == 0 && lane == 0) a.lens[slot] = 0;
+  });
+}
+
 __device__ void fork_slots(const PagesArgs& a, int i0, int i1) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  for (int i = i0 + warp; i < i1; i += nw) {
+  const int lane = threadIdx.x & 31;
+  each_part(a, i0, i1, [&](int i, int e0) {
     const int par = a.fork[2 * i], kid = a.fork[2 * i + 1];
-    if (!slot_ok(a, par) || !slot_ok(a, kid) || par == kid) continue;
-    const int* from = a.table + par * a.table_stride;
+    if (!slot_ok(a, par) || !slot_ok(a, kid) || par == kid) return;
     int* to = a.table + kid * a.table_stride;
-    const int np = row_entries(a, par), nk = row_entries(a, kid);
-    __syncwarp();
-    for (int e = lane; e < max(np, nk); e += 32) {
-      const int page = e < np ? from[e] : -1;
-      if (e < nk) count(a, to[e], -1);
-      count(a, page, 1);
-      to[e] = page;
-    }
-    if (lane == 0) a.lens[kid] = a.lens[par];
-  }
+    int page[kRowLoads], old[kRowLoads];
+    load_part(a, a.table + par * a.table_stride, e0, page);
+    load_part(a, to, e0, old);
+#pragma unroll
+    for (int x = 0; x < kRowLoads; ++x)
+      if (page[x] != old[x]) {
+        count(a, old[x], -1);
+        count(a, page[x], 1);
+        to[e0 + 32 * x + lane] = page[x];
+      }
+    if (e0 == 0 && lane == 0) a.lens[kid] = a.lens[par];
+  });
 }
 
 struct Need {
@@ -161,9 +183,18 @@ __device__ __forceinline__ Need need_of(const PagesArgs& a, int i) {
   return n;
 }
 
+// A page that an extend puts another in the place of: its count goes down when
+// all extends are done, so that no later one of the call is given the page
+// while a copy from it is still to be made.  (Never more than pages handed out.)
+__device__ __forceinline__ void drop_later(const PagesArgs& a, int page, int* n_drops) {
+  const int at = atomicAdd(n_drops, 1);
+  if (at < a.pages) a.drops[at] = page;
+}
+
 // Extends i0 .. i1 (no slot twice).  Returns the index of the first that does
-// not fit, or i1.  `used` and `moves` accumulate the call's totals.
-__device__ int extend_slots(const PagesArgs& a, int i0, int i1, int64_t* used, int* moves, int64_t* sh) {
+// not fit, or i1.  `used`, `moves` and `n_drops` (shared) accumulate the call's
+// totals.
+__device__ int extend_slots(const PagesArgs& a, int i0, int i1, int64_t* used, int* moves, int* n_drops, int64_t* sh) {
   __shared__ int first_bad;
   __shared__ int64_t given;
   // pages wanted by the whole list, up to an entry past the table's width;
@@ -243,7 +274,8 @@ __device__ int extend_slots(const PagesArgs& a, int i0, int i1, int64_t* used, i
         row[n.have - 1] = dst;
       }
       for (int e = n.have; e < n.want; ++e) {
-        const int page = a.avail[next++];
+        const int page = a.avail[next++], old = row[e];
+        if (old != -1) drop_later(a, old, n_drops);  // (left by a caller that lowered lens)
         a.refs[page] = 1;
         row[e] = page;
       }
@@ -266,6 +298,8 @@ __device__ int extend_slots(const PagesArgs& a, int i0, int i1, int64_t* used, i
 __global__ void __launch_bounds__(kPageThreads, 1) pages_update_kernel(const PagesArgs a) {
   extern __shared__ uint32_t bits[];
   __shared__ int64_t sh[32];
+  __shared__ int n_drops;
+  if (threadIdx.x == 0) n_drops = 0;
   pdl_wait();
   pdl_trigger();
   // A list that names a slot twice is taken one entry at a time.
@@ -285,10 +319,12 @@ __global__ void __launch_bounds__(kPageThreads, 1) pages_update_kernel(const Pag
   int64_t used = 0;
   while (done < a.n_extend) {
     const int end = one ? done + 1 : a.n_extend;
-    done = extend_slots(a, done, end, &used, &moves, sh);
+    done = extend_slots(a, done, end, &used, &moves, &n_drops, sh);
     __syncthreads();
     if (done < end) break;
   }
+  for (int i = threadIdx.x; i < min(n_drops, a.pages); i += blockDim.x) count(a, a.drops[i], -1);
+  __syncthreads();
   if (threadIdx.x == 0) {
     *a.n_moves = moves;
     if (a.info) {
@@ -459,8 +495,9 @@ extern "C" int alv_pages_update(alv_ctx* ctx, const alv_pages* p, const int32_t*
     return fail(ctx, ALV_ERR_ARG, "pages_update: a list is missing");
   if ((rc = set_device(ctx))) return rc;
   const size_t o_moves = 256, o_cow = o_moves + align_up(static_cast<size_t>(n_extend) * 8, 256),
-               o_avail = o_cow + align_up(static_cast<size_t>(n_extend) * 4, 256);
-  if ((rc = ensure_scratch(ctx, o_avail + static_cast<size_t>(p->pages) * 4))) return rc;
+               o_avail = o_cow + align_up(static_cast<size_t>(n_extend) * 4, 256),
+               o_drops = o_avail + align_up(static_cast<size_t>(p->pages) * 4, 256);
+  if ((rc = ensure_scratch(ctx, o_drops + static_cast<size_t>(p->pages) * 4))) return rc;
   uint8_t* ws = work_ptr(ctx);
   PagesArgs a{};
   a.table = p->table;
@@ -483,6 +520,7 @@ extern "C" int alv_pages_update(alv_ctx* ctx, const alv_pages* p, const int32_t*
   a.moves = reinterpret_cast<int2*>(ws + o_moves);
   a.cow = reinterpret_cast<int*>(ws + o_cow);
   a.avail = reinterpret_cast<int*>(ws + o_avail);
+  a.drops = reinterpret_cast<int*>(ws + o_drops);
   const size_t smem = static_cast<size_t>((p->slots + 31) / 32) * 12;  // three bitmaps
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if ((rc = prepare_kernel(ctx, pages_update_kernel, smem))) return rc;

@@ -253,7 +253,10 @@ def update_pages(k_pool, v_pool, page_table, lens, refs, *, free=None, fork=None
 
     k_pool, v_pool  (layers, pages, kv_heads, page_size, head_dim) bfloat16
     page_table      (slots, width) int32, -1 where a slot has no page
-    lens, refs      (slots,) positions held; (pages,) table entries naming the page
+    lens, refs      (slots,) positions held; (pages,) table entries naming the page.
+                    lens may be lowered between calls (rejected tokens): the pages
+                    past it are the slot's until it is dropped or forked onto, or an
+                    extend reaches their entries and drops them for new ones
     info            (4,) int32 or None: receives free pages left, pages handed
                     out, pages copied, index of the first extend that did not
                     fit (-1: all did)

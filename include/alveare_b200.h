@@ -400,7 +400,9 @@ typedef struct {
  * that others share is first copied to a page of the slot's own, in every
  * layer.  New pages are the free ones of lowest id, in list order.  The first
  * extend that does not fit (no free page, or past table_width) and all after
- * it change nothing.  Lists are device int32; info (4 int32 or NULL) receives
+ * it change nothing.  lens may be lowered between calls (rejected tokens): the
+ * pages past it stay the slot's until it is dropped or forked onto, or an
+ * extend reaches their entries, which drops them for new ones.  Lists are device int32; info (4 int32 or NULL) receives
  * free pages left, pages handed out, pages copied, and the index of the first
  * extend that did not fit or -1. */
 int alv_pages_update(alv_ctx* ctx, const alv_pages* p, const int32_t* free, int n_free, const int32_t* fork, int n_fork,
