@@ -152,9 +152,15 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// NaN if one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 // Two fp32 values in a register pair.
@@ -189,7 +195,7 @@ __device__ __forceinline__ void mask32(uint32_t (&s)[32], int hi, int lo, int si
 // 2^x of two values x >= -126 on the FMA pipe: x = n + f with n the nearest
 // integer (the low bits of x + 1.5 2^23), 2^f by the cubic of least relative
 // error on [-1/2, 1/2] (7.5e-5: a fiftieth of p's rounding to bf16), n added to
-// the exponent.
+// the exponent.  (Of NaN it gives any number: the row's maximum sees to that.)
 __device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
   const uint64_t magic = pack_f2(12582912.f, 12582912.f), minus_magic = pack_f2(-12582912.f, -12582912.f);
   const uint64_t r = add_f2(x, magic);
@@ -200,11 +206,6 @@ __device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
   const uint32_t lo = static_cast<uint32_t>(p) + (static_cast<uint32_t>(r) << 23);
   const uint32_t hi = static_cast<uint32_t>(p >> 32) + (static_cast<uint32_t>(r >> 32) << 23);
   return static_cast<uint64_t>(lo) | static_cast<uint64_t>(hi) << 32;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
 }
 // p = 2^(s scale - m) of 32 scores, added to the sums, as 16 packed bf16 pairs
 // in s[0 .. 16).  Where every score counts (POLY) a quarter of the
@@ -218,7 +219,7 @@ __device__ __forceinline__ void probs32(uint32_t (&s)[32], uint64_t scale2, uint
   for (int e = 0; e < 32; e += 2) {
     const uint64_t x = fma_f2(pack_f2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, sub2);
     uint64_t p;
-    if (POLY && e % 8 == 6) p = exp2_poly2(pack_f2(max_nan(lo_f2(x), -126.f), max_nan(hi_f2(x), -126.f)));
+    if (POLY && e % 8 == 6) p = exp2_poly2(pack_f2(fmaxf(lo_f2(x), -126.f), fmaxf(hi_f2(x), -126.f)));
     else p = pack_f2(exp2_fast(lo_f2(x)), exp2_fast(hi_f2(x)));
     sum[e / 2 & 1] = add_f2(sum[e / 2 & 1], p);
     s[e / 2] = pack_bf2_rn(lo_f2(p), hi_f2(p));
@@ -746,17 +747,19 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          mx[e / 2 & 1] = max3(mx[e / 2 & 1], __uint_as_float(sa[e]), __uint_as_float(sa[e + 1]));
-          if constexpr (HB == 64) mx[2 + (e / 2 & 1)] = max3(mx[2 + (e / 2 & 1)], __uint_as_float(sb[e]), __uint_as_float(sb[e + 1]));
+          mx[e / 2 & 1] = max3_nan(mx[e / 2 & 1], __uint_as_float(sa[e]), __uint_as_float(sa[e + 1]));
+          if constexpr (HB == 64) mx[2 + (e / 2 & 1)] = max3_nan(mx[2 + (e / 2 & 1)], __uint_as_float(sb[e]), __uint_as_float(sb[e + 1]));
         }
-        const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const float mine = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
         sh.mx[q][i & 1][half][row] = mine;
         both_halves();
-        const float mt = fmaxf(mine, sh.mx[q][i & 1][half ^ 1][row]) * scale;
-        const bool move = mt > m + 8.f;  // also from -inf
+        const float mt = max_nan(mine, sh.mx[q][i & 1][half ^ 1][row]) * scale;
+        // Also from -inf.  A score that is NaN or +inf leaves the row nothing
+        // defined: its maximum becomes NaN, and with it the sum and the output.
+        const bool move = !(mt <= m + 8.f);
         if (__any_sync(0xffffffffu, move)) {
           const float f = move ? (m == -INFINITY ? 0.f : exp2_fast(m - mt)) : 1.f;
-          if (move) m = mt;
+          if (move) m = mt == INFINITY ? NAN : mt;
           l *= f;
           if (i > 0) {
             if (NQ == 1) {  // O must hold the last product (with two tiles S's arrival says so)

@@ -1,0 +1,90 @@
+"""Attention where cached values are not finite: what a token sees of them
+gives what the formula gives, what it does not see changes nothing."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import alveare_b200 as ab  # noqa: E402
+from alveare_b200 import _lib  # noqa: E402
+from paged_util import attention_ref, attention_tol, ints, make_cache, starts  # noqa: E402
+
+NAN, INF = float("nan"), float("inf")
+
+
+def put(pages, table, rows, side, b, j, ps, value, dims=slice(None)):
+    """Position j of sequence b, in the pages and in the reference's copy."""
+    pages[int(table[b, j // ps]), :, j % ps, dims] = value
+    rows[b][side][:, j, dims] = value
+
+
+def queries(tokens, nq, hd, seed=1):
+    return torch.randn(tokens, nq, hd, generator=torch.Generator().manual_seed(seed)).bfloat16().cuda()
+
+
+def run(q, k, v, table, q_lens, kv_lens, **kw):
+    out = torch.full_like(q, 7.0)
+    ab.paged_attention(q, out, k, v, table, starts(q_lens), ints(kv_lens), max_q_len=max(q_lens), **kw)
+    _lib.context(0).sync_status(torch.cuda.current_stream().cuda_stream)
+    return out.double().cpu().numpy()
+
+
+def same(got, ref, mag):
+    """NaN and infinities where the formula has them, the rest within tolerance."""
+    assert np.array_equal(np.isnan(got), np.isnan(ref)), np.argwhere(np.isnan(got) != np.isnan(ref))[:4].tolist()
+    inf = np.isinf(ref)
+    assert np.array_equal(got[inf], ref[inf]) and not np.isinf(got[~inf]).any()
+    fin = np.isfinite(ref)
+    assert (np.abs(got[fin] - ref[fin]) <= attention_tol(ref[fin], mag[fin])).all()
+
+
+Q_LENS = [1, 3, 40, 200]  # row blocks, row blocks of several tokens, one and more query tiles
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("q_len", Q_LENS)
+def test_a_nan_key_that_every_token_sees(hd, q_len):
+    n, ps = 900, 32
+    for j in list(range(256, 264)) + [300, 415]:
+        k, v, table, rows = make_cache([n], 2, hd, ps, seed=j)
+        page = int(table[0, j // ps])
+        k[page, 0, j % ps, 5] = NAN   # one kv head: the other's query heads are as ever
+        rows[0][0][0, j, 5] = NAN
+        q = queries(q_len, 8, hd)
+        ref, mag = attention_ref(q, rows, [q_len], [n])
+        assert np.isnan(ref[:, :4]).all() and not np.isnan(ref[:, 4:]).any()
+        same(run(q, k, v, table, [q_len], [n]), ref, mag)
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("q_len", Q_LENS)
+@pytest.mark.parametrize("value", [INF, -INF])
+def test_infinite_scores(hd, q_len, value):
+    """A score of +inf leaves nothing defined, one of -inf a weight of zero."""
+    n, ps = 700, 16
+    for j in [128, 134, 263, n - 1]:
+        k, v, table, rows = make_cache([n], 2, hd, ps, seed=j)
+        put(k, table, rows, 0, 0, j, ps, value, 0)
+        q = queries(q_len, 8, hd)
+        q[:, :, 0] = q[:, :, 0].abs() + 0.5
+        ref, mag = attention_ref(q, rows, [q_len], [n])
+        same(run(q, k, v, table, [q_len], [n]), ref, mag)
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+def test_many_chunks_with_keys_that_are_not_finite(hd, value):
+    """As above in more chunks than there are SMs, most of them one CTA's alone;
+    the marked position of chunk b is 100 + b."""
+    batch, q_len, n, ps = 130, 40, 300, 32
+    k, v, table, rows = make_cache([n] * batch, 4, hd, ps)
+    for b in range(batch):
+        put(k, table, rows, 0, b, 100 + b, ps, value, 0)
+    q = queries(q_len * batch, 16, hd)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    ref, mag = attention_ref(q, rows, [q_len] * batch, [n] * batch)
+    same(run(q, k, v, table, [q_len] * batch, [n] * batch), ref, mag)
