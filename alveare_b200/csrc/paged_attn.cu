@@ -457,6 +457,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
     __syncthreads();
     const bool part = t0 > 0 || t1 < units;
     float* mypart = ra.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * R::kPart;
+    // (a row before the first position sees nothing and gives zeros; any other
+    // sees itself at least, and with no score above -inf it gives NaN)
+    auto share = [&](int r, float sum) { return pfirst + (r0 + r) / a.group < 0 ? 0.f : 1.f / sum; };
     auto store = [&](int r, int d, float x, float y) {  // two dims of a finished row
       const int tok = s.q0 + (r0 + r) / a.group, head = w.kvh * a.group + (r0 + r) % a.group;
       *reinterpret_cast<uint32_t*>(a.out + tok * a.o_tok + head * a.o_head + d) = pack_bf2_rn(x, y);
@@ -481,7 +484,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
         if (d == 0) mypart[r] = mm, mypart[kRowsPerBlock + r] = ll;
         *reinterpret_cast<float2*>(mypart + 2 * kRowsPerBlock + r * HD + d) = make_float2(x, y);
       } else {
-        const float inv = mm == -INFINITY ? 0.f : 1.f / ll;  // a row that sees nothing gives zeros
+        const float inv = share(r, ll);
         store(r, d, x * inv, y * inv);
       }
     }
@@ -546,7 +549,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2)
             x += f * v.x;
             y += f * v.y;
           }
-          const float inv = mm == -INFINITY ? 0.f : 1.f / ll;
+          const float inv = share(r, ll);
           store(r, d, x * inv, y * inv);
         }
       }

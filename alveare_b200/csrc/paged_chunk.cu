@@ -816,7 +816,9 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         uint16_t* dst = !real ? nullptr : c.a.out + static_cast<int64_t>(sw.s.q0 + tok) * c.a.o_tok + head * c.a.o_head + half * (HD / 2);
         float* pd = part_of(c, blockIdx.x, t > 0 ? 0 : 1, NQ * kChunkRows * (HD + 2)) + q * kChunkRows * (HD + 2);
         const bool odd = sh.odd[item & 3] == item + 1;
-        const float inv = m == -INFINITY ? 0.f : 1.f / l;  // a row that sees nothing gives zeros
+        // A row before the first position sees nothing and gives zeros; any other
+        // sees itself at least, and with no score above -inf it gives NaN.
+        const float inv = pos < 0 ? 0.f : 1.f / l;
         if (part && half == 0) pd[row] = m, pd[kChunkRows + row] = l;
         pd += 2 * kChunkRows + half * (HD / 2) * kChunkRows;
 #pragma unroll 1
@@ -925,7 +927,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const ChunkArgs c, int 
     }
   }
   if (!real) return;
-  const float inv = m == -INFINITY ? 0.f : 1.f / l;
+  const float inv = w.s.kv - w.s.qlen + tok < 0 ? 0.f : 1.f / l;
   const int head = w.kvh * c.a.group + row % c.a.group;
   uint16_t* dst = c.a.out + static_cast<int64_t>(w.s.q0 + tok) * c.a.o_tok + head * c.a.o_head;
 #pragma unroll

@@ -88,3 +88,22 @@ def test_many_chunks_with_keys_that_are_not_finite(hd, value):
     q[:, :, 0] = q[:, :, 0].abs() + 0.5
     ref, mag = attention_ref(q, rows, [q_len] * batch, [n] * batch)
     same(run(q, k, v, table, [q_len] * batch, [n] * batch), ref, mag)
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("q_len", [1, 2, 30])
+def test_nothing_but_scores_of_minus_infinity(hd, q_len):
+    """Undefined, unlike a row that sees no position, which gives zeros."""
+    n, ps = 40, 16
+    for kv in (n, q_len - 1):
+        if kv == 0:
+            continue
+        k, v, table, rows = make_cache([kv, n], 2, hd, ps)
+        for j in range(kv):
+            put(k, table, rows, 0, 0, j, ps, -INF, 3)
+        q = queries(q_len + 2, 8, hd)
+        q[:, :, 3] = 1.0
+        ref, mag = attention_ref(q, rows, [q_len, 2], [kv, n])
+        assert np.isnan(ref[max(0, q_len - kv):q_len]).all() and np.isfinite(ref[q_len:]).all()
+        same(run(q, k, v, table, [q_len, 2], [kv, n]), ref, mag)
