@@ -307,10 +307,11 @@ struct ChunkShared {
   float mx[C::kNQ][2][2][kChunkRows];  // a row's maximum over each half, two tiles deep
   float lx[C::kNQ][2][kChunkRows];
   Walk<HD> walk[C::kSoftWarps];  // each softmax warp's place (its registers hold scores)
-  // odd[i & 3] = i + 1: item i of the run has v values that are not finite in
-  // a tile that only some rows see whole (the scan is at most kStages items
-  // ahead of an item's store)
-  volatile uint32_t odd[4];
+  // i + 1 of the run's last item i so far with v values that are not finite in
+  // a tile that only some rows see whole; it never goes back.  An item's store
+  // adds such values if it is this item or an earlier one: the scan may be any
+  // number of items ahead of it, and an item without them has none to add.
+  uint32_t odd;
   // the CTA's run
   int64_t sums[C::kThreads / 32], few[C::kThreads / 32];
   int64_t u0, u1;
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
     mbar_init(&sh.pvdone, 1);
     fence_mbar_init();
     sh.failed = 0;
-    sh.odd[0] = sh.odd[1] = sh.odd[2] = sh.odd[3] = 0;
+    sh.odd = 0;
   }
   // query rows past tpt * group are never loaded: keep them zero
   for (uint32_t i = threadIdx.x; i < NQ * C::kQTile / 16; i += C::kThreads)
@@ -687,7 +688,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
                            : "memory");
             }
           }
-          if (odd) sh.odd[item & 3] = item + 1;
+          if (odd) atomicMax(&sh.odd, item + 1);
           fence_proxy_async_smem();
           __syncwarp();
         }
@@ -815,7 +816,7 @@ __global__ void __launch_bounds__(Chunk<HD>::kThreads, 1)
         const int head = sw.kvh * c.a.group + row % c.a.group;
         uint16_t* dst = !real ? nullptr : c.a.out + static_cast<int64_t>(sw.s.q0 + tok) * c.a.o_tok + head * c.a.o_head + half * (HD / 2);
         float* pd = part_of(c, blockIdx.x, t > 0 ? 0 : 1, NQ * kChunkRows * (HD + 2)) + q * kChunkRows * (HD + 2);
-        const bool odd = sh.odd[item & 3] == item + 1;
+        const bool odd = *const_cast<volatile uint32_t*>(&sh.odd) > item;
         // A row before the first position sees nothing and gives zeros; any other
         // sees itself at least, and with no score above -inf it gives NaN.
         const float inv = pos < 0 ? 0.f : 1.f / l;

@@ -107,3 +107,20 @@ def test_nothing_but_scores_of_minus_infinity(hd, q_len):
         ref, mag = attention_ref(q, rows, [q_len, 2], [kv, n])
         assert np.isnan(ref[max(0, q_len - kv):q_len]).all() and np.isfinite(ref[q_len:]).all()
         same(run(q, k, v, table, [q_len, 2], [kv, n]), ref, mag)
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_many_short_chunks_with_infinite_values(hd):
+    """Chunks of one and of two query tiles in turns, each with an infinite value
+    that its later tokens see, in more items than there are CTAs."""
+    r = np.random.default_rng(hd)
+    q_lens = [int(x) for x in np.where(np.arange(200) % 5 == 0, r.integers(33, 64, 200), r.integers(5, 30, 200))]
+    kv = [n + int(r.integers(0, 150)) for n in q_lens]
+    k, v, table, rows = make_cache(kv, 2, hd, 16)
+    for b, (ql, n) in enumerate(zip(q_lens, kv)):
+        if b % 3:
+            put(v, table, rows, 1, b, n - ql + ql // 2, 16, INF, slice(b % 7, hd, 11))
+    q = queries(sum(q_lens), 8, hd)
+    ref, mag = attention_ref(q, rows, q_lens, kv)
+    same(run(q, k, v, table, q_lens, kv), ref, mag)
