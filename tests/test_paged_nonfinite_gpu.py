@@ -124,3 +124,37 @@ def test_many_short_chunks_with_infinite_values(hd):
     q = queries(sum(q_lens), 8, hd)
     ref, mag = attention_ref(q, rows, q_lens, kv)
     same(run(q, k, v, table, q_lens, kv), ref, mag)
+
+
+# (new tokens, positions, window, first tokens, marked position relative to the first new token)
+SEEN_BY_SOME = [
+    (6, 306, 0, 0, 3), (6, 306, 150, 0, 2), (6, 306, 150, 0, 3 - 150), (2, 302, 150, 4, 1 - 150),
+    (40, 340, 0, 0, 20), (40, 340, 100, 4, 15 - 100), (40, 340, 100, 0, 39),
+    (200, 500, 0, 0, 100), (200, 500, 150, 0, 30), (200, 500, 150, 17, 64 - 150), (200, 500, 150, 0, 150 - 150),
+    (100, 6000, 0, 0, 50), (100, 6000, 2000, 0, 60 - 2000), (600, 600, 0, 0, 0), (600, 600, 130, 9, 300),
+]
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("case", range(len(SEEN_BY_SOME)))
+@pytest.mark.parametrize("side,value", [("k", NAN), ("k", INF), ("v", NAN), ("v", INF), ("v", -INF)])
+def test_a_position_that_only_some_tokens_see(hd, case, side, value):
+    """The tokens that see it get the formula's NaN or infinities, in the dims
+    that have them, the others what they would get without it."""
+    q_len, n, window, sinks, mark = SEEN_BY_SOME[case]
+    j, ps = n - q_len + mark, 16
+    k, v, table, rows = make_cache([n], 2, hd, ps, seed=case)
+    if side == "k":
+        put(k, table, rows, 0, 0, j, ps, value, 0)
+    else:
+        put(v, table, rows, 1, 0, j, ps, value, slice(0, hd, 3))
+        put(v, table, rows, 1, 0, j, ps, -value, slice(1, hd, 3))
+    q = queries(q_len, 8, hd, seed=case)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    ref, mag = attention_ref(q, rows, [q_len], [n], window=window, sinks=sinks)
+    pos = np.arange(n - q_len, n)
+    see = (j <= pos) & ((window == 0) | (j > pos - window) | (j < sinks))
+    assert case == 13 or 0 < see.sum() < q_len       # (case 13: position 0 of a whole prompt)
+    assert np.isfinite(ref[~see]).all() and not np.isfinite(ref[see]).all(-1).any()
+    same(run(q, k, v, table, [q_len], [n], window=window, sinks=sinks), ref, mag)
