@@ -227,7 +227,7 @@ int launch_rope(alv_ctx* ctx, const RopeArgs& a, bool xf, bool tf, cudaStream_t 
 
 int make_paged_view(alv_ctx* ctx, const char* who, const alv_paged* p, PagedView* out) {
   const std::string w(who);
-  if (!p || p->batch < 0 || p->tokens < 0 || !p->k || !p->v || !p->table || !p->q_start || !p->kv_lens)
+  if (!p || p->batch < 0 || p->tokens < 0 || !p->k || !p->v || (p->batch && (!p->table || !p->q_start || !p->kv_lens)))
     return fail(ctx, ALV_ERR_ARG, w + ": null pointer or negative size in the paged cache");
   if (p->pages < 1 || p->kv_heads < 1 || p->page_size < 1 || p->table_width < 1 || p->table_stride < 0)
     return fail(ctx, ALV_ERR_ARG, w + ": pages, kv_heads, page_size and table_width must be positive, table_stride not negative");
