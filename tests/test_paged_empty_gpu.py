@@ -22,6 +22,16 @@ def test_no_sequences():
     _lib.context(0).sync_status(torch.cuda.current_stream().cuda_stream)
 
 
+def test_empty_lists():
+    c = ab.PagedKVCache(1, 2, 64, 8, slots=4, max_len=64)
+    c.update(extend=[(1, 20)])
+    c.update(free=[], fork=[], extend=[])
+    c.update(fork=torch.empty(0, 2, dtype=torch.int32, device="cuda"))
+    assert c.lens.tolist() == [0, 20, 0, 0] and c.check()["free_pages"] == 6
+    with pytest.raises((RuntimeError, ValueError)):
+        c.update(extend=[1, 2, 3])
+
+
 def test_no_rows_to_sample():
     ab.sample_tokens(torch.empty(0, 50, device="cuda"), torch.empty(0, device="cuda"), ints([]), torch.empty(0, device="cuda"))
     _lib.context(0).sync_status()
