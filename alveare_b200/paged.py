@@ -95,6 +95,12 @@ def _step(stride: int, rows: int, width: int) -> int:
     return stride if rows > 1 else width
 
 
+def _apart(strides, tokens: int, heads: int, hd: int, name: str) -> None:
+    """An output's tokens and heads do not share memory."""
+    if (strides[0] < hd and tokens > 1) or (strides[1] < hd and heads > 1):
+        raise ValueError(f"{name}'s tokens and heads must not share memory (it is written)")
+
+
 def _stream(device: int) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -162,6 +168,7 @@ def qk_norm_rope(qkv, q_out, k_pages, v_pages, page_table, q_start, kv_lens, rop
     xs, qs = qkv.stride(), q_out.stride()
     if xs[1] != 1 or qs[2] != 1:
         raise ValueError("qkv and q_out must be contiguous in their last dimension")
+    _apart(qs, tokens, heads, hd, "q_out")
     qw = 0 if q_weight is None else _vector(q_weight, "q_weight", device, torch.float32, hd)
     kw = 0 if k_weight is None else _vector(k_weight, "k_weight", device, torch.float32, hd)
     a = _NORM_ROPE.pack(qkv.data_ptr(), _step(xs[0], tokens, cols), q_out.data_ptr(), qs[0], qs[1], rope.data_ptr(), qw, kw, qd,
@@ -196,6 +203,7 @@ def paged_attention(q, out, k_pages, v_pages, page_table, q_start, kv_lens, *, m
     qs, os = q.stride(), out.stride()
     if qs[2] != 1 or os[2] != 1:
         raise ValueError("q and out must be contiguous in their last dimension")
+    _apart(os, tokens, heads, hd, "out")
     if window < 0 or sinks < 0 or max_q_len < 0:
         raise ValueError("window, sinks and max_q_len must not be negative")
     a = _ATTENTION.pack(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], heads, min(max_q_len, tokens),
