@@ -30,8 +30,10 @@
 // Bound: the special-function unit and the tensor cores about alike.  A tile
 // pair of 256 rows x 128 positions of 128-wide heads is 1.1 us of products and
 // 0.85 of exponentials (a quarter of them on the FMA pipe) and takes 2.2 with
-// the power limit reached, 1.9 before; 2,048 tokens of 32 heads over 16,001
-// positions (503 GFLOP): 519 us back to back, 970 TFLOP/s, and 445 us, 1130
+// the power limit reached, 1.9 before: neither pipe is full (57 and 43 %), since
+// P V of a tile waits for all of its P and only the other query tile's work
+// fills the time.  2,048 tokens of 32 heads over 16,001 positions (503 GFLOP):
+// 517 to 534 us back to back by GPU, 944 to 972 TFLOP/s, and 445 us, 1130
 // TFLOP/s, when the GPU rests between calls.  64-wide heads do half the
 // products for the same exponentials: 1.55 us a pair.  256-wide: one query tile
 // of 128 rows, each 64 positions 1.35 us against 0.55 of products: nothing
@@ -194,7 +196,8 @@ __device__ __forceinline__ void mask32(uint32_t (&s)[32], int hi, int lo, int si
 }
 // 2^x of two values x >= -126 on the FMA pipe: x = n + f with n the nearest
 // integer (the low bits of x + 1.5 2^23), 2^f by the cubic of least relative
-// error on [-1/2, 1/2] (7.5e-5: a fiftieth of p's rounding to bf16), n added to
+// error on [-1/2, 1/2] (7.5e-5: a fiftieth of p's rounding to bf16; the fp32 sum
+// l adds the same p, so the output is off by no more than that), n added to
 // the exponent.  (Of NaN it gives any number: the row's maximum sees to that.)
 __device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
   const uint64_t magic = pack_f2(12582912.f, 12582912.f), minus_magic = pack_f2(-12582912.f, -12582912.f);

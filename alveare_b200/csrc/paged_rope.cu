@@ -11,8 +11,9 @@
 // Bound: HBM (each value of qkv is read once and written once).  A CTA takes up
 // to 8 tokens and looks up their sequence, page and table rows once for all
 // heads; one token per CTA for small batches, which wait for memory and not for
-// bytes.  7,000 tokens of 32 + 8 + 8 heads of 128 with norms (176 MB): 39.4 us,
-// 4.5 TB/s; a step of four tokens 8.9 us called from the host, 2.7 us in a CUDA
+// bytes.  7,000 tokens of 32 + 8 + 8 heads of 128 with norms (176 MB): 39 us,
+// 4.5 TB/s, 70 % of a copy's rate (what is in flight is one head ahead per
+// thread, in registers); a step of four tokens 8.9 us called from the host, 2.7 us in a CUDA
 // graph.
 #include "internal.h"
 #include "paged.cuh"

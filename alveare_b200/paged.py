@@ -16,11 +16,16 @@ runtime/cpp/src/model.cpp:196-216, 315-370, sampling in
 runtime/py/sampler.py:3-50.
 
 All tensors are torch CUDA tensors on one device; outputs are written in place
-and the work is stream-ordered on that device's current stream.  Lengths, page
-tables and counts are read on the device when a kernel runs, never on the
-host, so a step can be captured in a CUDA graph and replayed while they
-change.  A bad page, length or slot found there is skipped and reported by the
-next ``context(device).sync_status()``.
+and the work is ordered on that device's current stream.  Attention and page
+bookkeeping use one work area per device (as the Q4 products do), so calls on
+one device come from one thread at a time and must not overlap: before a call
+on another stream, or beside a replayed graph that holds such calls, make the
+stream wait (``wait_stream``, an event).  Lengths, page tables and counts are
+read on the device when a kernel runs, never on the host, so a step can be
+captured in a CUDA graph and replayed while they change; run it once before,
+since a call that needs a larger work area than any before it allocates, which
+a capture does not allow.  A bad page, length or slot found on the device is
+skipped and reported by the next ``context(device).sync_status()``.
 """
 from __future__ import annotations
 
