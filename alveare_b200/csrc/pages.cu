@@ -9,9 +9,9 @@
 // Dropping 56 branches of 8 sequences, forking 56 and extending all by a token,
 // with some 50 shared last pages of 32 KB (k and v) copied in each of 4 layers:
 // 16 to 17.5 us for both launches, launch latency and the passes.  Dropped and
-// forked rows are read whole by the one CTA: up to 256 entries (4,096 positions
-// of 16) that costs nothing, 56 drops and 56 forks of rows of 8,192 add some 75
-// us.  Compaction that moves 234 pages of 64 KB in each of 16 layers:
+// forked rows are read whole by the one CTA: 56 drops and 56 forks take 2 us more
+// with rows of 256 entries (4,096 positions of 16) than where only the entries in
+// use were read, 10 us more with 1,024 and 75 with 8,192.  Compaction that moves 234 pages of 64 KB in each of 16 layers:
 // 84 to 90 us, 5.4 to 5.8 TB/s.
 // Counts change by integer atomics, so their order does not matter.
 #include "internal.h"
